@@ -315,6 +315,46 @@ int gemm_graphsafe_cuda(const uint16_t* W, const uint16_t* X, uint16_t* Y, int M
 int pega_dense_w13_swiglu(const uint16_t* W13, const uint16_t* X, uint16_t* act, int inter, int N,
                           int K, hipStream_t stream);
 
+/* ---------------- residual add + norm ---------------- */
+
+/* No reference counterpart as one symbol: the residual add and the root-mean-square norm between
+ * two blocks, for rows [rows][hidden_dim]:
+ *   s = residual + x (x alone where residual is NULL); residual_out = bf16(s);
+ *   y = s * weight / sqrt(mean(s^2) + eps); normed = bf16(y); mxfp8_codes / mxfp8_scales = y in
+ *   MXFP8 (below).
+ * x is bf16, or fp32 with x_is_f32.  Each output may be NULL, not all of them; codes and scales go
+ * together.  An output may be the buffer of x or of residual (its first byte the input's); no two
+ * outputs may overlap.  The sums and products are in 64 bits, and every output is the formula's
+ * value rounded once.  A row's result does not depend on the other rows.  hidden_dim % 8 == 0
+ * (32 with MXFP8), at most 32768; 16-byte aligned buffers, scales 4-byte (801 otherwise). */
+int pega_add_rmsnorm(const void* x, bool x_is_f32, const uint16_t* residual,
+                     const uint16_t* weight, double eps, uint16_t* residual_out,
+                     uint16_t* normed, uint8_t* mxfp8_codes, uint8_t* mxfp8_scales, int rows,
+                     int hidden_dim, hipStream_t stream);
+
+/* ---------------- microscaled formats (MXFP8, MXFP4) ----------------
+ * 32 consecutive values of a row share a scale 2^s, stored as the byte s + 127 (255: NaN).
+ * format 0: E4M3 codes [rows][cols] bytes; format 1: E2M1 codes [rows][cols / 2] bytes, the even
+ * column in the low nibble; scales [rows][cols / 32] bytes.  Quantisation takes the smallest s >=
+ * -127 for which the block's largest magnitude rounds to a value of the format (at most 464 * 2^s
+ * in E4M3, below 7 * 2^s in E2M1) and rounds to nearest, ties to even; a block with an infinity or
+ * a NaN gets scale 255 and codes 0.  cols % 32 == 0; bf16 rows and codes 16-byte aligned, scales
+ * 4-byte (801 otherwise).  No reference counterpart. */
+
+/* bf16 rows [rows][cols] into codes and scales. */
+int pega_mx_quantize(const uint16_t* x, uint8_t* codes, uint8_t* scales, int format, int rows,
+                     int cols, hipStream_t stream);
+
+/* kimi_marlin_w13_swiglu_cuda's bf16 values (w13 [rows][2 intermediate_dim], gate then up) into
+ * codes and scales [rows][intermediate_dim], in one pass. */
+int pega_mx_swiglu_quantize(const uint16_t* w13, uint8_t* codes, uint8_t* scales, int format,
+                            int rows, int intermediate_dim, hipStream_t stream);
+
+/* The values that codes and scales stand for, as bf16 [rows][cols] (exact down to bf16's smallest
+ * numbers). */
+int pega_mx_dequantize(const uint8_t* codes, const uint8_t* scales, uint16_t* out, int format,
+                       int rows, int cols, hipStream_t stream);
+
 /* ---------------- routing select ---------------- */
 
 /* Replaces kimi_k2_router_noaux_tc_cuda, pegainfer-kernels/src/ffi/kimi.rs:52-66

@@ -16,6 +16,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _LL = ctypes.c_longlong
 _F = ctypes.c_float
+_D = ctypes.c_double
 _B = ctypes.c_bool
 
 
@@ -70,6 +71,10 @@ SIGNATURES = {
     "gemm_cuda": [_P, _P, _P, _I, _I, _I, _P],
     "gemm_graphsafe_cuda": [_P, _P, _P, _I, _I, _I, _P],
     "pega_dense_w13_swiglu": [_P, _P, _P, _I, _I, _I, _P],
+    "pega_add_rmsnorm": [_P, _B, _P, _P, _D, _P, _P, _P, _P, _I, _I, _P],
+    "pega_mx_quantize": [_P, _P, _P, _I, _I, _I, _P],
+    "pega_mx_swiglu_quantize": [_P, _P, _P, _I, _I, _I, _P],
+    "pega_mx_dequantize": [_P, _P, _P, _I, _I, _I, _P],
 }
 _RESTYPE = {"pegainfer_kernels_last_error": ctypes.c_char_p}
 

@@ -188,6 +188,13 @@ __device__ __forceinline__ u32x4_t rsrc_words(const void* base, uint32_t bytes) 
   return r;
 }
 
+// Whether two buffers share a byte (host-side checks of outputs against inputs).
+inline bool overlap(const void* a, long long na, const void* b, long long nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && na > 0 && nb > 0 && x < y + static_cast<uintptr_t>(nb) &&
+         y < x + static_cast<uintptr_t>(na);
+}
+
 __host__ __device__ constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 }  // namespace pega

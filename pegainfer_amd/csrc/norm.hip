@@ -1,0 +1,211 @@
+// Residual add + root-mean-square norm on MI355X (gfx950):
+//
+//   s = residual + x            residual_out = bf16(s)
+//   y = s * weight / sqrt(mean(s^2) + eps)
+//   normed = bf16(y)            codes, scales = MXFP8(y)   (either or both)
+//
+// One pass: a row's values stay in registers between the sum of squares and the outputs, so a
+// row is read once and each output written once; the bytes bound it.
+//
+// The sums and the products are in 64 bits: the values' squares are exact there, and a value's
+// E4M3 code and its block's scale follow the formula however near y lies to a rounding border
+// (in 32 bits about one value in 10^6 goes to the neighbouring code, and which ones depends on
+// the order of the sum).  y reaches 32 bits rounded to odd (the last bit set if anything was cut
+// off), after which one more rounding, to bf16 or to a code, is the rounding of y itself.  The
+// norm is of s itself, not of bf16(s).  The 64-bit work hides behind the memory.
+#include "common.h"
+#include "mx_format.h"
+#include "pega_moe.h"
+
+namespace pega {
+namespace {
+
+// y in fp32, rounded to odd: the low 29 mantissa bits cut off, and the last one kept set if any
+// of them was.  The cut value converts exactly (values below fp32's normal range aside, which
+// every output rounds to 0).
+__device__ __forceinline__ float to_odd(double y) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, y);
+  const uint32_t lo = static_cast<uint32_t>(b);
+  const uint64_t cut = (b & 0xffffffff00000000ull) | (lo & 0xe0000000u);
+  const float f = static_cast<float>(__builtin_bit_cast(double, cut));
+  const uint32_t u = __builtin_bit_cast(uint32_t, f);
+  // an infinite or NaN f keeps its bits
+  const bool sticky = (lo & 0x1fffffffu) != 0 && (u & 0x7f800000u) != 0x7f800000u;
+  return __builtin_bit_cast(float, sticky ? u | 1u : u);
+}
+
+__device__ __forceinline__ double shfl_xor_f64(double v, int mask) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __shfl_xor(static_cast<uint32_t>(b), mask);
+  const uint32_t hi = __shfl_xor(static_cast<uint32_t>(b >> 32), mask);
+  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+}
+
+// WPR waves take a row, CH vectors of 8 columns a lane; below four waves a row, a workgroup of
+// four waves takes 4 / WPR rows.  Every load of a row has returned before its first store (the
+// sum needs them all), so an output may be the buffer of an input.
+template <int WPR, int CH, bool kX32>
+__global__ __launch_bounds__(64 * (WPR < 4 ? 4 : WPR)) void add_rmsnorm_kernel(
+    const void* x, const uint16_t* residual, const uint16_t* __restrict__ weight, double eps,
+    uint16_t* residual_out, uint16_t* normed, uint8_t* codes, uint8_t* scales, int rows,
+    int hidden) {
+  constexpr int kWaves = WPR < 4 ? 4 : WPR;
+  constexpr int kLanes = 64 * WPR;
+  __shared__ double s_sum[kWaves];
+  const int wave = threadIdx.x >> 6;
+  const int row = blockIdx.x * (kWaves / WPR) + wave / WPR;
+  const int lane = static_cast<int>(threadIdx.x) % kLanes;  // within the row
+  const int vecs = hidden >> 3;
+  const bool in = row < rows;
+  const long long base = static_cast<long long>(row) * hidden;
+
+  uint4 xr[CH][kX32 ? 2 : 1], rr[CH], wr[CH];
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int v = lane + c * kLanes;
+    const bool ok = in && v < vecs;
+    const long long at = base + 8LL * v;
+    if constexpr (kX32) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(x) + at);
+      xr[c][0] = ok ? p[0] : zero;
+      xr[c][1] = ok ? p[1] : zero;
+    } else {
+      xr[c][0] = ok ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at) : zero;
+    }
+    rr[c] = ok && residual ? *reinterpret_cast<const uint4*>(residual + at) : zero;
+    wr[c] = v < vecs ? *reinterpret_cast<const uint4*>(weight + 8 * v) : zero;
+  }
+  double s[CH][8], sum = 0.0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t rw[4] = {rr[c].x, rr[c].y, rr[c].z, rr[c].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float xv;
+      if constexpr (kX32) {
+        const uint4 q = xr[c][i >> 2];
+        const uint32_t w = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+        xv = __builtin_bit_cast(float, w);
+      } else {
+        const uint4 q = xr[c][0];
+        const uint32_t w = (i >> 1) == 0 ? q.x : (i >> 1) == 1 ? q.y : (i >> 1) == 2 ? q.z : q.w;
+        xv = (i & 1) ? bf_hi(w) : bf_lo(w);
+      }
+      const float rv = (i & 1) ? bf_hi(rw[i >> 1]) : bf_lo(rw[i >> 1]);
+      s[c][i] = residual ? static_cast<double>(xv) + static_cast<double>(rv)
+                         : static_cast<double>(xv);
+      sum = __builtin_fma(s[c][i], s[c][i], sum);
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) sum += shfl_xor_f64(sum, m);
+  if constexpr (WPR > 1) {
+    if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    const int first = wave / WPR * WPR;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) sum += s_sum[first + w];
+  }
+  const double inv = 1.0 / __builtin_sqrt(sum / hidden + eps);
+
+  const bool whole = (hidden & 127) == 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int v = lane + c * kLanes;
+    const bool ok = in && v < vecs;
+    const long long at = base + 8LL * v;
+    const uint32_t ww[4] = {wr[c].x, wr[c].y, wr[c].z, wr[c].w};
+    if (residual_out && ok) {
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(to_odd(s[c][2 * i]), to_odd(s[c][2 * i + 1]));
+      *reinterpret_cast<uint4*>(residual_out + at) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w = (i & 1) ? bf_hi(ww[i >> 1]) : bf_lo(ww[i >> 1]);
+      y[i] = to_odd(s[c][i] * inv * static_cast<double>(w));
+    }
+    if (normed && ok)
+      *reinterpret_cast<uint4*>(normed + at) =
+          make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                     pack_bf16x2(y[6], y[7]));
+    if (codes) {
+      uint32_t w[2];
+      const uint32_t scale = mx_encode8<kMxE4M3>(y, w);
+      mx_store8<kMxE4M3>(codes + base, scales + (base >> 5), v, ok, whole, w, scale);
+    }
+  }
+}
+
+template <int WPR, int CH>
+void launch_norm(bool x32, const void* x, const uint16_t* residual, const uint16_t* weight,
+                 double eps, uint16_t* residual_out, uint16_t* normed, uint8_t* codes,
+                 uint8_t* scales, int rows, int hidden, hipStream_t stream) {
+  constexpr int kRows = WPR < 4 ? 4 / WPR : 1;
+  const dim3 grid(ceil_div(rows, kRows)), block(64 * (WPR < 4 ? 4 : WPR));
+  if (x32)
+    hipLaunchKernelGGL((add_rmsnorm_kernel<WPR, CH, true>), grid, block, 0, stream, x, residual,
+                       weight, eps, residual_out, normed, codes, scales, rows, hidden);
+  else
+    hipLaunchKernelGGL((add_rmsnorm_kernel<WPR, CH, false>), grid, block, 0, stream, x, residual,
+                       weight, eps, residual_out, normed, codes, scales, rows, hidden);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+}  // namespace pega
+
+using namespace pega;
+
+// No reference counterpart as one symbol: the add and the norm between two blocks.
+PEGA_API int pega_add_rmsnorm(const void* x, bool x_is_f32, const uint16_t* residual,
+                              const uint16_t* weight, double eps, uint16_t* residual_out,
+                              uint16_t* normed, uint8_t* mxfp8_codes, uint8_t* mxfp8_scales,
+                              int rows, int hidden_dim, hipStream_t stream) {
+  if (!x || !weight || rows < 0 || hidden_dim <= 0 || !(eps >= 0.0))
+    return fail(kInvalidValue, "add_rmsnorm: bad arguments (rows=%d hidden=%d)", rows, hidden_dim);
+  if (!residual_out && !normed && !mxfp8_codes)
+    return fail(kInvalidValue, "add_rmsnorm: no output");
+  if (!mxfp8_codes != !mxfp8_scales)
+    return fail(kInvalidValue, "add_rmsnorm: MXFP8 codes and scales go together");
+  if (hidden_dim % 8 != 0 || hidden_dim > 32768 || (mxfp8_codes && hidden_dim % kMxBlock != 0))
+    return fail(kNotSupported, "add_rmsnorm: hidden_dim %d (a multiple of 8, of 32 for MXFP8, at "
+                "most 32768)", hidden_dim);
+  if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(residual_out) ||
+      !aligned16(normed) || !aligned16(mxfp8_codes) || (reinterpret_cast<uintptr_t>(mxfp8_scales) & 3u))
+    return fail(kNotSupported, "add_rmsnorm: buffers must be 16-byte aligned (scales 4)");
+  if (rows == 0) return kSuccess;
+  // An output may be the bf16 buffer of x or of residual, row for row; any other overlap would
+  // let one row's stores meet another row's loads.
+  const long long n = static_cast<long long>(rows) * hidden_dim;
+  struct Span { const void* p; long long bytes; };
+  const Span outs[4] = {{residual_out, 2 * n}, {normed, 2 * n}, {mxfp8_codes, n}, {mxfp8_scales, n / kMxBlock}};
+  const Span ins[3] = {{x, (x_is_f32 ? 4 : 2) * n}, {residual, 2 * n}, {weight, 2LL * hidden_dim}};
+  for (int o = 0; o < 4; ++o) {
+    for (int i = 0; i < 3; ++i)
+      if (overlap(outs[o].p, outs[o].bytes, ins[i].p, ins[i].bytes) &&
+          !(o < 2 && i < 2 && outs[o].p == ins[i].p && ins[i].bytes == 2 * n))
+        return fail(kInvalidValue, "add_rmsnorm: an output overlaps an input");
+    for (int i = 0; i < o; ++i)
+      if (overlap(outs[o].p, outs[o].bytes, outs[i].p, outs[i].bytes))
+        return fail(kInvalidValue, "add_rmsnorm: two outputs overlap");
+  }
+  const int vecs = hidden_dim / 8;
+#define PEGA_NORM(WPR, CH) \
+  launch_norm<WPR, CH>(x_is_f32, x, residual, weight, eps, residual_out, normed, mxfp8_codes, \
+                       mxfp8_scales, rows, hidden_dim, stream)
+  if (vecs <= 64) PEGA_NORM(1, 1);
+  else if (vecs <= 128) PEGA_NORM(1, 2);
+  else if (vecs <= 256) PEGA_NORM(4, 1);
+  else if (vecs <= 512) PEGA_NORM(4, 2);
+  else if (vecs <= 1024) PEGA_NORM(4, 4);
+  else if (vecs <= 2048) PEGA_NORM(8, 4);
+  else PEGA_NORM(16, 4);
+#undef PEGA_NORM
+  return launch_status("add_rmsnorm");
+}

@@ -692,6 +692,140 @@ def dense_w13_swiglu(w13: torch.Tensor, x: torch.Tensor, act: torch.Tensor) -> N
 
 
 # --------------------------------------------------------------------------
+# Microscaled formats (no reference counterpart)
+# --------------------------------------------------------------------------
+MX_BLOCK = 32  # consecutive values of a row that share a scale
+
+
+class MxFormat(enum.Enum):
+    """Value formats of a microscaled tensor; the value is the C ABI's format number."""
+    Fp8E4M3 = 0
+    Fp4E2M1 = 1
+
+    def code_cols(self, cols: int) -> int:
+        """Bytes of codes that a row of `cols` values takes."""
+        return cols if self is MxFormat.Fp8E4M3 else cols // 2
+
+
+def _on_current_device(*tensors: torch.Tensor) -> None:
+    """The launches go to the current device's current stream: refuse another device's tensors."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None:
+            _ensure(t.is_cuda and t.device.index == here,
+                    f"tensor must live on the current GPU (cuda:{here}), got {t.device}")
+
+
+@dataclasses.dataclass
+class MxTensor:
+    """Rows in a microscaled format: `codes` uint8 [rows, cols] (E4M3) or [rows, cols / 2]
+    (E2M1, the even column in the low nibble), `scales` uint8 [rows, cols / 32] (the scale is
+    2^(byte - 127), 255 NaN).  Both contiguous."""
+    rows: int
+    cols: int
+    format: MxFormat
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        self.validate()
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, format: MxFormat, device="cuda") -> "MxTensor":
+        _ensure(rows >= 0 and cols > 0 and cols % MX_BLOCK == 0,
+                f"MX rows must have a multiple of {MX_BLOCK} columns, got {rows} x {cols}")
+        u8 = dict(dtype=torch.uint8, device=device)
+        return cls(rows, cols, format, torch.empty(rows, format.code_cols(cols), **u8),
+                   torch.empty(rows, cols // MX_BLOCK, **u8))
+
+    def head(self, rows: int) -> "MxTensor":
+        """The first `rows` rows, in place."""
+        _ensure(0 <= rows <= self.rows, f"{rows} rows of {self.rows}")
+        return MxTensor(rows, self.cols, self.format, self.codes[:rows], self.scales[:rows])
+
+    def validate(self) -> None:
+        _ensure(isinstance(self.format, MxFormat), "MX format must be an MxFormat")
+        _ensure(self.cols > 0 and self.cols % MX_BLOCK == 0,
+                f"MX rows must have a multiple of {MX_BLOCK} columns, got {self.cols}")
+        _ensure(self.codes.dtype == torch.uint8 and self.scales.dtype == torch.uint8,
+                "MX codes and scales must be uint8")
+        _ensure(tuple(self.codes.shape) == (self.rows, self.format.code_cols(self.cols)),
+                f"MX codes shape {tuple(self.codes.shape)} does not match {self.rows} x {self.cols}")
+        _ensure(tuple(self.scales.shape) == (self.rows, self.cols // MX_BLOCK),
+                f"MX scales shape {tuple(self.scales.shape)} does not match {self.rows} x {self.cols}")
+
+
+def _mx_rows(name: str, t: torch.Tensor, rows: int, cols: int) -> None:
+    _ensure(_is_bf16(t) and t.dim() == 2 and tuple(t.shape) == (rows, cols),
+            f"{name} must be bf16 [{rows}, {cols}], got {t.dtype} {tuple(t.shape)}")
+
+
+def mx_quantize(x: torch.Tensor, out: MxTensor) -> None:
+    """bf16 rows [rows, cols] into out's format: per 32 columns the smallest power-of-two scale
+    that holds the largest magnitude, codes rounded to nearest even."""
+    _mx_rows("x", x, out.rows, out.cols)
+    _on_current_device(x, out.codes, out.scales)
+    _lib.call("pega_mx_quantize", _ptr(x), _ptr(out.codes), _ptr(out.scales), out.format.value,
+              out.rows, out.cols, _stream())
+
+
+def mx_swiglu_quantize(w13: torch.Tensor, out: MxTensor) -> None:
+    """kimi_marlin_w13_swiglu then mx_quantize in one launch: w13 bf16 [rows, 2 cols], gate
+    columns first, out [rows, cols]; the same codes and scales as the two calls."""
+    _mx_rows("w13", w13, out.rows, 2 * out.cols)
+    _on_current_device(w13, out.codes, out.scales)
+    _lib.call("pega_mx_swiglu_quantize", _ptr(w13), _ptr(out.codes), _ptr(out.scales),
+              out.format.value, out.rows, out.cols, _stream())
+
+
+def mx_dequantize(x: MxTensor, out: torch.Tensor) -> None:
+    """The values that x stands for, as bf16 [rows, cols]."""
+    _mx_rows("out", out, x.rows, x.cols)
+    _on_current_device(out, x.codes, x.scales)
+    _lib.call("pega_mx_dequantize", _ptr(x.codes), _ptr(x.scales), _ptr(out), x.format.value,
+              x.rows, x.cols, _stream())
+
+
+# --------------------------------------------------------------------------
+# Residual add + norm (no reference counterpart as one op)
+# --------------------------------------------------------------------------
+def add_rmsnorm(x: torch.Tensor, residual, weight: torch.Tensor, eps: float, *,
+                residual_out: torch.Tensor = None, normed: torch.Tensor = None,
+                quantized: MxTensor = None) -> None:
+    """What stands between two blocks, in one launch, for rows [rows, hidden]:
+
+        s = residual + x                       (x alone where residual is None)
+        residual_out = bf16(s)
+        y = s * weight / sqrt(mean(s^2) + eps)
+        normed = bf16(y), quantized = y in MXFP8
+
+    x is bf16, or float32 (a routed sum); residual, weight and the outputs are bf16.  Outputs
+    left None are not formed (at least one is needed); an output may be x or residual itself,
+    and no two may share memory.  Every output is the formula's value rounded once."""
+    _ensure(x.dim() == 2, "x must be [rows, hidden]")
+    rows, hidden = x.shape
+    _ensure(x.dtype == torch.float32 or _is_bf16(x), "x must be bf16 or float32")
+    _ensure(_is_bf16(weight) and weight.numel() == hidden, f"weight must be bf16 [{hidden}]")
+    _ensure(residual_out is not None or normed is not None or quantized is not None,
+            "add_rmsnorm needs an output")
+    for name, t in (("residual", residual), ("residual_out", residual_out), ("normed", normed)):
+        if t is not None:
+            _mx_rows(name, t, rows, hidden)
+    codes = scales = None
+    if quantized is not None:
+        _ensure(quantized.format is MxFormat.Fp8E4M3, "add_rmsnorm quantizes into MXFP8")
+        _ensure((quantized.rows, quantized.cols) == (rows, hidden),
+                f"quantized must be [{rows}, {hidden}]")
+        codes, scales = quantized.codes, quantized.scales
+    _ensure(residual_out is None or normed is None or residual_out.data_ptr() != normed.data_ptr()
+            or rows == 0, "residual_out and normed must be different buffers")
+    _on_current_device(x, residual, weight, residual_out, normed, codes, scales)
+    _lib.call("pega_add_rmsnorm", _ptr(x), x.dtype == torch.float32, _ptr(residual), _ptr(weight),
+              float(eps), _ptr(residual_out), _ptr(normed), _ptr(codes), _ptr(scales), rows, hidden,
+              _stream())
+
+
+# --------------------------------------------------------------------------
 # Routing select
 # --------------------------------------------------------------------------
 ROUTE_ALIGN_MAX_ROUTES = 4096  # routes the fused select + permutation keeps in one workgroup

@@ -1,0 +1,145 @@
+"""The norm and microscaled operators without a GPU: their 64-bit references against torch's own
+conversions, and every refusal of the C entry points and of the Python wrappers."""
+import numpy as np
+import pytest
+import torch
+
+import mx_ref
+
+A = 0x10000  # addresses that no accepted call of these tests dereferences
+
+
+def _call(name, *args):
+    from pegainfer_amd import _lib
+    return getattr(_lib.lib(), name)(*args)
+
+
+def test_reference_codes_are_torch_casts():
+    g = np.random.default_rng(0)
+    v = np.concatenate([g.standard_normal((40, 64)) * 10.0 ** g.integers(-6, 6, (40, 1)),
+                        np.arange(-464, 464, 0.25)[:3712].reshape(58, 64)])
+    for fmt in ("fp8", "fp4"):
+        codes, sc = mx_ref.quantize(v, fmt)
+        u = (v.reshape(len(v), -1, 32) / 2.0 ** (sc[..., None].astype(float) - 127)).reshape(v.shape)
+        if fmt == "fp8":
+            want = torch.from_numpy(u).to(torch.float32).to(torch.float8_e4m3fn).view(torch.uint8)
+            assert np.array_equal(codes, want.numpy())
+        back = mx_ref.values(codes, sc, fmt)
+        # half a step of the value's binade, or of the smallest normal's
+        step = 2.0 ** -3 if fmt == "fp8" else 2.0 ** -1
+        low = 2.0 ** -6 if fmt == "fp8" else 1.0
+        unit = np.repeat(2.0 ** (sc.astype(float) - 127), 32, 1)
+        binade = 2.0 ** np.floor(np.log2(np.maximum(np.abs(v) / unit, low)))
+        assert (np.abs(back - v) <= binade * unit * step / 2).all()
+
+
+def test_reference_scale_is_the_smallest_that_holds():
+    for fmt, top in (("fp8", 464.0), ("fp4", 7.0)):
+        for s in (-126, -3, 0, 50, 110):
+            lim = top * 2.0 ** s
+            over = np.nextafter(lim, np.inf)
+            under = np.nextafter(lim, 0)
+            want = [s, s + 1, s] if fmt == "fp8" else [s + 1, s + 1, s]
+            got = mx_ref.scale_bytes([lim, over, under], fmt).astype(int) - 127
+            assert got.tolist() == want
+    assert mx_ref.scale_bytes([0.0, np.inf, 1e-45], "fp8").tolist() == [0, 255, 0]
+
+
+def test_reference_bf16_rounds_once():
+    one = 1.0
+    half = 2.0 ** -8  # half a bf16 step above 1
+    v = [one + half, one + half + 2.0 ** -40, one + 3 * half, -(one + half), 0.0, -0.0]
+    assert mx_ref.bf16_round(v).tolist() == [0x3F80, 0x3F81, 0x3F82, 0xBF80, 0, 0x8000]
+
+
+NORM = [A, False, A << 1, A << 2, 1e-6, A << 3, A << 4, A << 5, A << 6, 2, 64, None]
+
+
+@pytest.mark.parametrize("at,value,code", [
+    (0, None, 1), (3, None, 1), (9, -1, 1), (10, 0, 1), (10, -8, 1), (4, -1.0, 1),
+    (4, float("nan"), 1),
+    (7, None, 1), (8, None, 1),              # codes without scales, scales without codes
+    (10, 60, 801), (10, 40, 801),            # not a multiple of 8, of 32
+    (10, 32776, 801), (10, 65536, 801),      # past the registers
+    (0, A + 2, 801), (2, (A << 1) + 8, 801), (3, (A << 2) + 4, 801), (5, (A << 3) + 2, 801),
+    (6, (A << 4) + 8, 801), (7, (A << 5) + 8, 801), (8, (A << 6) + 2, 801),
+    (5, A << 4, 1), (5, (A << 4) + 16, 1),   # two outputs in one place
+    (5, A + 16, 1), (6, (A << 1) + 128, 1),  # an output across other rows of an input
+    (7, A, 1), (7, A << 1, 1), (8, A << 2, 1), (6, A << 2, 1),
+])
+def test_norm_refuses(at, value, code):
+    args = list(NORM)
+    args[at] = value
+    assert _call("pega_add_rmsnorm", *args) == code
+
+
+def test_norm_refuses_an_output_over_fp32_rows():
+    args = list(NORM)
+    args[1] = True
+    args[5] = A  # bf16 rows over fp32 rows: other rows' bytes
+    assert _call("pega_add_rmsnorm", *args) == 1
+
+
+def test_norm_needs_an_output_and_takes_no_rows():
+    args = list(NORM)
+    args[5] = args[6] = args[7] = args[8] = None
+    assert _call("pega_add_rmsnorm", *args) == 1
+    args = list(NORM)
+    args[9] = 0
+    assert _call("pega_add_rmsnorm", *args) == 0
+
+
+@pytest.mark.parametrize("name", ["pega_mx_quantize", "pega_mx_swiglu_quantize", "pega_mx_dequantize"])
+@pytest.mark.parametrize("at,value,code", [
+    (0, None, 1), (1, None, 1), (2, None, 1), (3, 2, 1), (3, -1, 1), (4, -1, 1), (5, 0, 1),
+    (5, -32, 1), (5, 48, 801), (0, A + 4, 801), (1, (A << 1) + 2, 801), (1, A, 1), (2, A + 16, 1),
+    (2, A << 1, 1),
+])
+def test_mx_refuses(name, at, value, code):
+    args = [A, A << 1, A << 2, 0, 2, 64, None]
+    args[at] = value
+    assert _call(name, *args) == code
+    args = [A, A << 1, A << 2, 1, 0, 64, None]
+    assert _call(name, *args) == 0  # no rows
+
+
+def test_mx_tensor_checks_its_shape():
+    from pegainfer_amd import ops
+    t = ops.MxTensor.empty(3, 64, ops.MxFormat.Fp4E2M1, device="cpu")
+    assert tuple(t.codes.shape) == (3, 32) and tuple(t.scales.shape) == (3, 2)
+    assert tuple(ops.MxTensor.empty(0, 32, ops.MxFormat.Fp8E4M3, device="cpu").codes.shape) == (0, 32)
+    assert t.head(2).rows == 2 and t.head(2).codes.data_ptr() == t.codes.data_ptr()
+    with pytest.raises(ValueError):
+        t.head(4)
+    with pytest.raises(ValueError):
+        ops.MxTensor.empty(3, 48, ops.MxFormat.Fp8E4M3, device="cpu")
+    with pytest.raises(ValueError):
+        ops.MxTensor(3, 64, ops.MxFormat.Fp8E4M3, t.codes, t.scales)
+    with pytest.raises(ValueError):
+        ops.MxTensor(3, 64, ops.MxFormat.Fp4E2M1, t.codes.int(), t.scales)
+    with pytest.raises(ValueError):
+        ops.MxTensor(3, 64, 1, t.codes, t.scales)
+
+
+def test_wrappers_refuse_shapes_and_types_before_the_device():
+    from pegainfer_amd import ops
+    bf = dict(dtype=torch.bfloat16)
+    x, w = torch.zeros(2, 64, **bf), torch.zeros(64, **bf)
+    q8 = ops.MxTensor.empty(2, 64, ops.MxFormat.Fp8E4M3, device="cpu")
+    q4 = ops.MxTensor.empty(2, 64, ops.MxFormat.Fp4E2M1, device="cpu")
+    out = torch.zeros(2, 64, **bf)
+    for bad in (lambda: ops.add_rmsnorm(x, None, w, 1e-6),
+                lambda: ops.add_rmsnorm(x.half(), None, w, 1e-6, normed=out),
+                lambda: ops.add_rmsnorm(x[0], None, w, 1e-6, normed=out),
+                lambda: ops.add_rmsnorm(x, x[:1], w, 1e-6, normed=out),
+                lambda: ops.add_rmsnorm(x, None, w[:32], 1e-6, normed=out),
+                lambda: ops.add_rmsnorm(x, None, w.float(), 1e-6, normed=out),
+                lambda: ops.add_rmsnorm(x, None, w, 1e-6, normed=out, residual_out=out),
+                lambda: ops.add_rmsnorm(x, None, w, 1e-6, normed=out.float()),
+                lambda: ops.add_rmsnorm(x, None, w, 1e-6, quantized=q4),
+                lambda: ops.add_rmsnorm(x, None, w, 1e-6, quantized=q8.head(1)),
+                lambda: ops.mx_quantize(x[:1], q8), lambda: ops.mx_quantize(x.float(), q8),
+                lambda: ops.mx_swiglu_quantize(x, q8),
+                lambda: ops.mx_dequantize(q8, out[:, :32])):
+        with pytest.raises(ValueError):
+            bad()
