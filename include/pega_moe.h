@@ -355,6 +355,29 @@ int pega_mx_swiglu_quantize(const uint16_t* w13, uint8_t* codes, uint8_t* scales
 int pega_mx_dequantize(const uint8_t* codes, const uint8_t* scales, uint16_t* out, int format,
                        int rows, int cols, hipStream_t stream);
 
+/* Y[n][m] = bf16(sum_k X[n][k] * W[m][k]): W [M][K] MXFP4, X [N][K] in x_format, Y [N][M] bf16,
+ * fp32 accumulation on the scaled matrix instructions (E4M3 products are aligned to the largest of
+ * 128 inside an instruction: about 2^-12 of it).  M % 16 == 0, K % 128 == 0, codes and Y 16-byte
+ * aligned, scales 4-byte (801 otherwise).  Never allocates.  A call's bits depend on its sizes and
+ * formats alone; a block of scale 255 makes its row's results NaN. */
+int pega_mx_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,
+                 const uint8_t* x_scales, int x_format, uint16_t* Y, int M, int N, int K,
+                 hipStream_t stream);
+
+/* pega_wna16_gemm on microscaled operands: for every block b < ntp / block size of expert e =
+ * expert_ids[b] in [0, local_experts) and every row sid of it below size_m * top_k,
+ *   output[sid] = bf16(X[sid / top_k] . W[e]^T)          W [local_experts][size_n][size_k] MXFP4
+ * times topk_weights[sid] before the rounding with mul_topk_weights (may be NULL otherwise).
+ * Other rows of output [size_m * top_k][size_n] are left as they are.  Block sizes 8, 16, 32, 48,
+ * 64; the shape and alignment rules of pega_mx_gemm; X under 2 GiB (801 otherwise). */
+int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scales, int x_format,
+                         uint16_t* output, const uint8_t* w_codes, const uint8_t* w_scales,
+                         const int32_t* sorted_token_ids, const int32_t* expert_ids,
+                         const int32_t* num_tokens_post_padded, const float* topk_weights,
+                         int sorted_token_ids_len, int moe_block_size, int top_k,
+                         bool mul_topk_weights, int size_m, int size_n, int size_k,
+                         int local_experts, hipStream_t stream);
+
 /* ---------------- routing select ---------------- */
 
 /* Replaces kimi_k2_router_noaux_tc_cuda, pegainfer-kernels/src/ffi/kimi.rs:52-66

@@ -1,0 +1,530 @@
+// Products of microscaled rows (mx_format.h) on MI355X (gfx950):
+//
+//   Y[n][m] = bf16( sum_k X[n][k] * W[m][k] ),   W [M][K] MXFP4, X [N][K] MXFP8 or MXFP4
+//
+// on v_mfma_scale_f32_16x16x128_f8f6f4, which takes codes and scale bytes as they are stored:
+// 16 features (operand A) by 16 rows (operand B) by 128 k.  Lane (c, g), c = lane % 16 and
+// g = lane / 16, holds row c of its operand: of E2M1 codes the 16 bytes of k 32 g .. 32 g + 31, of
+// E4M3 codes the 16 bytes from k 16 g on and those from k 64 + 16 g on; its scale byte is that of
+// the block k 32 g .. 32 g + 31 either way.  The lane's four sums are features 4 g .. 4 g + 3 of
+// row c of X.  Sums are fp32 from one instruction to the next; inside one, products of E4M3 codes
+// are aligned to the largest of the 128 and lose what lies about 2^-12 below it (measured: random
+// codes 3e-4 of the largest product, normal values 8e-6 of the sum of magnitudes; E2M1 with E2M1
+// products are exact to 2e-8), which is far below what the codes themselves keep.
+//
+// The grouped form takes its rows through the token -> expert permutation, as the INT4 GEMM does:
+//   for every block b < ntp / bs of expert e = expert_ids[b], row i: sid = sorted_token_ids[b bs + i]
+//   Y[sid] = X[sid / top_k] . W[e]   where sid < N top_k; other rows of Y stay as they are.
+//
+// Two kernels.  The streaming one serves few rows, where the weights' bytes bound the call: a
+// workgroup per 16 MR features and block of rows, whose waves share K.  The tiled one serves many
+// rows: both operands go straight to an LDS ring and each wave owns a part of the tile for all of K.
+#include <type_traits>
+
+#include "common.h"
+#include "mx_format.h"
+#include "pega_moe.h"
+
+namespace pega {
+namespace {
+
+typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8_t;
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4_t;
+
+constexpr uint32_t kOutOfRange = 0x80000000u;  // voffset that fails every range check
+
+struct MxArgs {
+  const uint8_t* wq;
+  const uint8_t* ws;
+  const uint8_t* xq;
+  const uint8_t* xs;
+  uint16_t* y;
+  int M, N, K;  // features, rows of X, columns
+  // grouped
+  const int32_t* sorted_ids;
+  const int32_t* expert_ids;
+  const int32_t* ntp;
+  const float* topk_w;
+  int sorted_len, bs, top_k, mul, experts;
+};
+
+template <int kXFormat>
+__device__ __forceinline__ floatx4_t mx_mfma(u32x4_t w, u32x4_t x0, u32x4_t x1, uint32_t sw,
+                                             uint32_t sx, floatx4_t c) {
+  i32x8_t a = {}, b = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[i] = static_cast<int>(w[i]);
+    b[i] = static_cast<int>(x0[i]);
+    if (kXFormat == kMxE4M3) b[4 + i] = static_cast<int>(x1[i]);
+  }
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      a, b, c, 4, kXFormat == kMxE4M3 ? 0 : 4, 0, static_cast<int>(sw), 0, static_cast<int>(sx));
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0),
+                                           static_cast<int>(bytes), 0x00020000);
+}
+
+__device__ __forceinline__ void store4(const MxArgs& p, long long row, int m, floatx4_t v, int sid) {
+  float w = 1.0f;
+  if (p.mul) w = p.topk_w[sid];
+  *reinterpret_cast<uint2*>(p.y + row * p.M + m) =
+      make_uint2(pack_bf16x2(v[0] * w, v[1] * w), pack_bf16x2(v[2] * w, v[3] * w));
+}
+
+// ---------------------------------------------------------------- few rows
+// One workgroup per (16 MR features, 16 RB rows); wave w of WV takes its share of K's steps of
+// 128.  A load's lanes read 64 contiguous bytes of a row per quad (fragment order would touch a
+// line per lane), and ds_bpermute hands every lane its fragment's 16 bytes.  Four steps' scales of
+// 16 rows are one word per lane.  D steps are in flight.
+template <int kXFormat, int MR, int RB>
+struct MxStep {
+  u32x4_t w[MR];
+  u32x4_t x[RB][kXFormat == kMxE4M3 ? 2 : 1];
+};
+
+template <int kXFormat, int WV, int MR, int RB, bool kGrouped>
+__global__ __launch_bounds__(64 * WV) void mx_stream_kernel(MxArgs p) {
+  constexpr int D = RB == 1 ? 8 : 4;
+  constexpr int kQuads = D / 4;
+  constexpr int kHalves = kXFormat == kMxE4M3 ? 2 : 1;
+  constexpr int kXStep = 64 * kHalves;  // bytes of a row of X per step
+  __shared__ __align__(16) floatx4_t s_red[WV][MR * RB][64];
+  __shared__ int s_sid[16 * RB];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int m0 = blockIdx.x * (16 * MR);
+  const int K = p.K, steps = K >> 7;
+  long long expert = 0;
+  int n0 = blockIdx.y * (16 * RB);
+  if constexpr (kGrouped) {
+    const int mb = blockIdx.y;
+    const int limit = p.N * p.top_k;
+    int sid = limit;
+    if (tid < p.bs && mb * p.bs + tid < p.sorted_len) sid = p.sorted_ids[mb * p.bs + tid];
+    const int e = __builtin_amdgcn_readfirstlane(p.expert_ids[mb]);
+    if (min(p.ntp[0], p.sorted_len) < (mb + 1) * p.bs || e < 0 || e >= p.experts) return;
+    expert = e;
+    if (tid < 16 * RB) s_sid[tid] = static_cast<unsigned>(sid) < static_cast<unsigned>(limit) ? sid : -1;
+    __syncthreads();
+    n0 = 0;
+  }
+  // the row of X (and of Y) of local row i; -1 where there is none
+  const auto sid_of = [&](int i) { return kGrouped ? s_sid[i] : (n0 + i < p.N ? n0 + i : -1); };
+  const auto x_row = [&](int i) {
+    const int sid = sid_of(i);
+    return static_cast<long long>(sid < 0 ? 0 : kGrouped ? sid / p.top_k : sid);
+  };
+
+  const uint32_t w_bytes = static_cast<uint32_t>(K) / 2u, s_bytes = static_cast<uint32_t>(K) / 32u;
+  const long long w_first = expert * p.M + m0;
+  const __amdgpu_buffer_rsrc_t wr = make_rsrc(p.wq + w_first * w_bytes, 16u * MR * w_bytes);
+  const __amdgpu_buffer_rsrc_t sr = make_rsrc(p.ws + w_first * s_bytes, 16u * MR * s_bytes);
+  const uint32_t lr = static_cast<uint32_t>(lane >> 2), lp = static_cast<uint32_t>(lane & 3);
+  const uint8_t *xp[RB], *xsp[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    xp[rb] = p.xq + x_row(16 * rb + static_cast<int>(lr)) * (w_bytes * kHalves) + 16u * lp;
+    xsp[rb] = p.xs + x_row(16 * rb + c) * s_bytes;
+  }
+  const int src = (4 * c + g) * 4;
+  const auto to_fragment = [&](u32x4_t v) {
+    u32x4_t f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      f[e] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(src, static_cast<int>(v[e])));
+    return f;
+  };
+
+  const int s0 = (steps * wave) / WV, s1 = (steps * (wave + 1)) / WV;
+  const auto load_step = [&](MxStep<kXFormat, MR, RB>& r, int s) {
+    s = min(s, steps - 1);  // past the share's end: fetched again, never used
+#pragma unroll
+    for (int mr = 0; mr < MR; ++mr)
+      r.w[mr] = __builtin_amdgcn_raw_buffer_load_b128(
+          wr, static_cast<int>((16u * mr + lr) * w_bytes + 16u * lp), s * 64, 0);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+        r.x[rb][h] = *reinterpret_cast<const u32x4_t*>(xp[rb] + static_cast<long long>(s) * kXStep + 64 * h);
+  };
+  // scales of steps s .. s + 3: lane (c, j) takes row c's word of step s + j
+  struct Scales {
+    uint32_t w[MR], x[RB];
+  };
+  const auto load_scales = [&](Scales& r, int s) {
+    const int at = 4 * min(s + g, steps - 1);
+#pragma unroll
+    for (int mr = 0; mr < MR; ++mr)
+      r.w[mr] = __builtin_amdgcn_raw_buffer_load_b32(
+          sr, static_cast<int>((16u * mr + c) * s_bytes) + at, 0, 0);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) r.x[rb] = *reinterpret_cast<const uint32_t*>(xsp[rb] + at);
+  };
+  floatx4_t acc[MR][RB] = {};
+  const auto compute = [&](const MxStep<kXFormat, MR, RB>& r, const Scales& sc, int j) {
+    const int from = (c + 16 * j) * 4;
+    uint32_t sx[RB];
+    u32x4_t x[RB][2];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      sx[rb] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from, static_cast<int>(sc.x[rb]))) >> (8 * g);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) x[rb][h] = to_fragment(r.x[rb][h]);
+      if (kHalves == 1) x[rb][1] = u32x4_t{};
+    }
+#pragma unroll
+    for (int mr = 0; mr < MR; ++mr) {
+      const uint32_t sw =
+          static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from, static_cast<int>(sc.w[mr]))) >> (8 * g);
+      const u32x4_t w = to_fragment(r.w[mr]);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        acc[mr][rb] = mx_mfma<kXFormat>(w, x[rb][0], x[rb][1], sw, sx[rb], acc[mr][rb]);
+    }
+  };
+
+  MxStep<kXFormat, MR, RB> slot[D];
+  Scales sc[kQuads];
+  if (s0 < s1) {
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) load_scales(sc[q], s0 + 4 * q);
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      load_step(slot[j], min(s0 + j, s1 - 1));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    int s = s0;
+    for (; s + D <= s1; s += D) {
+      Scales next[kQuads];
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) load_scales(next[q], s + D + 4 * q);
+#pragma unroll
+      for (int j = 0; j < D; ++j) {
+        compute(slot[j], sc[j / 4], j % 4);
+        load_step(slot[j], min(s + j + D, s1 - 1));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) sc[q] = next[q];
+    }
+#pragma unroll
+    for (int j = 0; j < D - 1; ++j)
+      if (s + j < s1) compute(slot[j], sc[j / 4], j % 4);
+  }
+  // the waves' sums in wave order
+#pragma unroll
+  for (int mr = 0; mr < MR; ++mr)
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) s_red[wave][mr * RB + rb][lane] = acc[mr][rb];
+  __syncthreads();
+  for (int t = wave; t < MR * RB; t += WV) {
+    floatx4_t sum = s_red[0][t][lane];
+#pragma unroll
+    for (int w = 1; w < WV; ++w) {
+      const floatx4_t v = s_red[w][t][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += v[e];
+    }
+    const int sid = sid_of(16 * (t % RB) + c);
+    if (sid >= 0) store4(p, sid, m0 + 16 * (t / RB) + 4 * g, sum, sid);
+  }
+}
+
+// ---------------------------------------------------------------- many rows
+// A workgroup owns BM features x BN rows, its WM x WN waves TM x TN blocks of 16 x 16 each for all
+// of K; a stage of the ring holds 128 k of both operands and their scales.  A load brings 1 KB:
+// 16 rows of 64 bytes (E2M1) or 8 of 128 (E4M3), the row's 16-byte pieces at slot piece ^ (row / 2
+// % 4) or piece ^ (row % 8), which spreads eight lanes' fragment reads over all banks; 64 rows'
+// scale words are one load.  One barrier a stage; the next stage's fragments are read while this
+// one's products run.
+template <int kXFormat_, int WM_, int WN_, int TM_, int TN_, int NS_>
+struct MxTile {
+  static constexpr int kXFormat = kXFormat_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, NS = NS_;
+  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int BM = 16 * WM * TM, BN = 16 * WN * TN;
+  static constexpr int kXRow = kXFormat == kMxE4M3 ? 128 : 64;  // bytes of a row of X in a stage
+  static constexpr int kXLoadRows = 1024 / kXRow;
+  static constexpr int kWLoads = BM / 16, kXLoads = BN / kXLoadRows;
+  static constexpr int kSLoads = (BM + BN) / 64;
+  static constexpr int PD = (kWLoads + kXLoads) / kWaves;  // data loads per wave and stage
+  static constexpr int PS = (kSLoads + kWaves - 1) / kWaves;
+  static constexpr int P = PD + PS;
+  static constexpr int kX = BM * 64, kS = kX + BN * kXRow, kStage = kS + (BM + BN) * 4;
+  static_assert(PD * kWaves == kWLoads + kXLoads && BM % 64 == 0 && BN % 64 == 0, "tile shape");
+  static_assert(NS >= 3 && NS * kStage <= 160 * 1024 && kStage % 16 == 0, "tile shape");
+};
+
+template <typename S, bool kGrouped>
+__global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
+  constexpr int BM = S::BM, BN = S::BN, NS = S::NS, TM = S::TM, TN = S::TN, P = S::P;
+  constexpr bool kF8 = S::kXFormat == kMxE4M3;
+  __shared__ __align__(1024) uint8_t smem[NS * S::kStage];
+  __shared__ int s_sid[kGrouped ? BN : 1];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % S::WM, wn = wave / S::WM;
+  const int c = lane & 15, g = lane >> 4;
+  const int m0 = blockIdx.x * BM;
+  int n0 = blockIdx.y * BN;
+  const int K = p.K, steps = K >> 7;
+  long long expert = 0;
+  if constexpr (kGrouped) {
+    const int mb = blockIdx.y;
+    const int limit = p.N * p.top_k;
+    const int e = __builtin_amdgcn_readfirstlane(p.expert_ids[mb]);
+    if (min(p.ntp[0], p.sorted_len) < (mb + 1) * p.bs || e < 0 || e >= p.experts) return;
+    expert = e;
+    for (int i = tid; i < BN; i += S::kThreads) {
+      int sid = limit;
+      if (i < p.bs && mb * p.bs + i < p.sorted_len) sid = p.sorted_ids[mb * p.bs + i];
+      s_sid[i] = static_cast<unsigned>(sid) < static_cast<unsigned>(limit) ? sid : -1;
+    }
+    __syncthreads();
+    n0 = 0;
+  }
+  const uint32_t w_bytes = static_cast<uint32_t>(K) / 2u, s_bytes = static_cast<uint32_t>(K) / 32u;
+  const uint32_t x_bytes = w_bytes * (S::kXRow / 64);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) uint8_t*)smem));
+  const long long w_first = expert * p.M + m0;
+  const int w_rows = min(BM, p.M - m0), x_rows = kGrouped ? p.N : min(BN, p.N - n0);
+
+  // This wave's loads of a stage.  Rows past the last feature or row are out of range: zeros.
+  u32x4_t rsrc[P];
+  uint32_t dst[P], voff[P], soff_step[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    if (j < S::PD) {
+      const int i = wave * S::PD + j;
+      const bool x = i >= S::kWLoads;
+      const int rows_per = x ? S::kXLoadRows : 16, pieces = 64 / rows_per;
+      const int r0 = (x ? i - S::kWLoads : i) * rows_per;
+      const int r = r0 + lane / pieces;
+      const int swz = pieces == 8 ? r & 7 : (r >> 1) & 3;
+      const uint32_t piece = static_cast<uint32_t>((lane % pieces) ^ swz);
+      const uint32_t row_bytes = x ? x_bytes : w_bytes;
+      const long long first = x ? n0 : w_first;
+      rsrc[j] = rsrc_words((x ? p.xq : p.wq) + first * row_bytes,
+                           static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
+                               static_cast<int>((x ? x_rows : w_rows) * row_bytes))));
+      dst[j] = lds0 + (x ? S::kX : 0) + 1024u * static_cast<uint32_t>(x ? i - S::kWLoads : i);
+      soff_step[j] = x ? S::kXRow : 64;
+      if (kGrouped && x) {
+        const int sid = s_sid[r];
+        voff[j] = sid < 0 ? kOutOfRange
+                          : static_cast<uint32_t>(sid / p.top_k) * row_bytes + 16u * piece;
+      } else {
+        voff[j] = static_cast<uint32_t>(r) * row_bytes + 16u * piece;
+      }
+    } else {
+      const int i = min(wave * S::PS + j - S::PD, S::kSLoads - 1);  // a repeat brings the same
+      const bool x = i >= BM / 64;
+      const int r = 64 * (x ? i - BM / 64 : i) + lane;
+      const long long first = x ? n0 : w_first;
+      rsrc[j] = rsrc_words((x ? p.xs : p.ws) + first * s_bytes,
+                           static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
+                               static_cast<int>((x ? x_rows : w_rows) * s_bytes))));
+      dst[j] = lds0 + S::kS + 256u * static_cast<uint32_t>(i);
+      soff_step[j] = 4;
+      if (kGrouped && x) {
+        const int sid = s_sid[r];
+        voff[j] = sid < 0 ? kOutOfRange : static_cast<uint32_t>(sid / p.top_k) * s_bytes;
+      } else {
+        voff[j] = static_cast<uint32_t>(r) * s_bytes;
+      }
+    }
+  }
+  const auto stage_in = [&](int step, int st) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const uint32_t at = dst[j] + static_cast<uint32_t>(st), so = soff_step[j] * static_cast<uint32_t>(step);
+      if (j < S::PD) dma_b128(rsrc[j], at, voff[j], so);
+      else dma_b32(rsrc[j], at, voff[j], so);
+    }
+  };
+  struct Frags {
+    u32x4_t w[TM], x[TN][kF8 ? 2 : 1];
+    uint32_t sw[TM], sx[TN];
+  };
+  const uint8_t* w_rd = smem + (wm * TM * 16 + c) * 64 + 16 * (g ^ ((c >> 1) & 3));
+  const uint8_t* x_rd = smem + S::kX + (wn * TN * 16 + c) * S::kXRow;
+  const int x_at0 = 16 * (kF8 ? g ^ (c & 7) : g ^ ((c >> 1) & 3));
+  const int x_at1 = 16 * ((4 + g) ^ (c & 7));
+  const uint8_t* sw_rd = smem + S::kS + (wm * TM * 16 + c) * 4 + g;
+  const uint8_t* sx_rd = smem + S::kS + (BM + wn * TN * 16 + c) * 4 + g;
+  const auto read = [&](Frags& f, int st) {
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+      f.w[t] = *reinterpret_cast<const u32x4_t*>(w_rd + st + 1024 * t);
+      f.sw[t] = sw_rd[st + 64 * t];
+    }
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      f.x[t][0] = *reinterpret_cast<const u32x4_t*>(x_rd + st + 16 * S::kXRow * t + x_at0);
+      if constexpr (kF8)
+        f.x[t][1] = *reinterpret_cast<const u32x4_t*>(x_rd + st + 16 * S::kXRow * t + x_at1);
+      f.sx[t] = sx_rd[st + 64 * t];
+    }
+  };
+  floatx4_t acc[TM][TN] = {};
+  const auto products = [&](const Frags& f) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int t = 0; t < TM; ++t)
+        acc[t][j] = mx_mfma<S::kXFormat>(f.w[t], f.x[j][0], f.x[j][kF8 ? 1 : 0], f.sw[t], f.sx[j],
+                                         acc[t][j]);
+  };
+
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (i < steps) stage_in(i, i * S::kStage);
+  if (steps >= NS - 1) vm_wait<(NS - 2) * P>(); else vm_wait<0>();
+  lds_barrier();
+  Frags f0, f1;
+  read(f0, 0);
+  int st_rd = S::kStage, st_in = (NS - 1) * S::kStage;
+  const auto next = [](int st) { return st + S::kStage == NS * S::kStage ? 0 : st + S::kStage; };
+  // Step s: stage s + 1 has landed (each wave waits for its own loads, the barrier for all);
+  // every wave has read stage s - 1, which the loads of stage s + NS - 1 then fill.
+  const auto step = [&](const Frags& cur, Frags& nxt, int s) {
+    if (s + NS - 2 < steps) vm_wait<(NS - 3) * P>(); else vm_wait<0>();
+    lds_barrier();
+    if (s + NS - 1 < steps) {
+      stage_in(s + NS - 1, st_in);
+      st_in = next(st_in);
+    }
+    if (s + 1 < steps) {
+      read(nxt, st_rd);
+      st_rd = next(st_rd);
+    }
+    products(cur);
+  };
+  for (int s = 0; s < steps; s += 2) {
+    step(f0, f1, s);
+    if (s + 1 < steps) step(f1, f0, s + 1);
+  }
+
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int i = (wn * TN + j) * 16 + c;
+    const int sid = kGrouped ? s_sid[i] : (n0 + i < p.N ? n0 + i : -1);
+    if (sid < 0) continue;
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+      const int m = m0 + (wm * TM + t) * 16 + 4 * g;
+      if (m < p.M) store4(p, sid, m, acc[t][j], sid);
+    }
+  }
+}
+
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int mx_gemm_checks(const char* name, const MxArgs& a, int x_format) {
+  if (!a.wq || !a.ws || !a.xq || !a.xs || !a.y) return fail(kInvalidValue, "%s: null pointer", name);
+  if (a.M <= 0 || a.N < 0 || a.K <= 0)
+    return fail(kInvalidValue, "%s: bad shape M=%d N=%d K=%d", name, a.M, a.N, a.K);
+  if (x_format != kMxE4M3 && x_format != kMxE2M1)
+    return fail(kInvalidValue, "%s: format %d (0 E4M3, 1 E2M1)", name, x_format);
+  if (a.M % 16 != 0 || a.K % 128 != 0)
+    return fail(kNotSupported, "%s: M %% 16 and K %% 128 must be 0 (M=%d K=%d)", name, a.M, a.K);
+  if (!aligned(a.wq, 16) || !aligned(a.xq, 16) || !aligned(a.y, 16) || !aligned(a.ws, 4) ||
+      !aligned(a.xs, 4))
+    return fail(kNotSupported, "%s: codes and output must be 16-byte aligned, scales 4-byte", name);
+  // a workgroup addresses up to 256 rows of either operand through one 32-bit range
+  if (256LL * a.K >= static_cast<long long>(kOutOfRange))
+    return fail(kNotSupported, "%s: K=%d is over 2^23", name, a.K);
+  return kSuccess;
+}
+
+template <int kXFormat, int WV, int MR, int RB, bool kGrouped>
+void launch_stream(const MxArgs& a, int row_blocks, hipStream_t stream) {
+  hipLaunchKernelGGL((mx_stream_kernel<kXFormat, WV, MR, RB, kGrouped>),
+                     dim3(a.M / (16 * MR), row_blocks), dim3(64 * WV), 0, stream, a);
+}
+
+template <typename S, bool kGrouped>
+void launch_tile(const MxArgs& a, int row_blocks, hipStream_t stream) {
+  hipLaunchKernelGGL((mx_tile_kernel<S, kGrouped>), dim3(ceil_div(a.M, S::BM), row_blocks),
+                     dim3(S::kThreads), 0, stream, a);
+}
+
+template <int kXFormat>
+int dense_launch(const MxArgs& a, hipStream_t stream, const char* name) {
+  if (a.N <= 16) launch_stream<kXFormat, 8, 1, 1, false>(a, 1, stream);
+  else if (a.N <= 32) launch_stream<kXFormat, 8, 1, 2, false>(a, 1, stream);
+  else if (a.N <= 64) launch_stream<kXFormat, 8, 1, 4, false>(a, 1, stream);
+  else {
+    using S = MxTile<kXFormat, 2, 2, 4, 4, 4>;
+    if (ceil_div(a.N, S::BN) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
+    launch_tile<S, false>(a, ceil_div(a.N, S::BN), stream);
+  }
+  return launch_status(name);
+}
+
+template <int kXFormat>
+int grouped_launch(const MxArgs& a, hipStream_t stream, const char* name) {
+  const int blocks = ceil_div(a.sorted_len, a.bs);
+  if (blocks > 65535) return fail(kNotSupported, "%s: too many blocks (%d)", name, blocks);
+  if (a.bs <= 16) launch_stream<kXFormat, 8, 1, 1, true>(a, blocks, stream);
+  else if (a.bs <= 32) launch_stream<kXFormat, 8, 1, 2, true>(a, blocks, stream);
+  else {
+    using S = MxTile<kXFormat, 4, 1, 4, 4, 4>;
+    launch_tile<S, true>(a, blocks, stream);
+  }
+  return launch_status(name);
+}
+
+}  // namespace
+}  // namespace pega
+
+using namespace pega;
+
+// No reference counterpart: Y = X . W^T of microscaled operands.
+PEGA_API int pega_mx_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,
+                          const uint8_t* x_scales, int x_format, uint16_t* Y, int M, int N, int K,
+                          hipStream_t stream) {
+  MxArgs a{w_codes, w_scales, x_codes, x_scales, Y, M, N, K, nullptr, nullptr, nullptr, nullptr, 0, 0, 1, 0, 1};
+  const int rc = mx_gemm_checks("mx_gemm", a, x_format);
+  if (rc != kSuccess) return rc;
+  if (N == 0) return kSuccess;
+  return x_format == kMxE4M3 ? dense_launch<kMxE4M3>(a, stream, "mx_gemm")
+                             : dense_launch<kMxE2M1>(a, stream, "mx_gemm");
+}
+
+// No reference counterpart: the grouped GEMM of pega_wna16_gemm on microscaled operands.
+PEGA_API int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scales, int x_format,
+                                  uint16_t* output, const uint8_t* w_codes, const uint8_t* w_scales,
+                                  const int32_t* sorted_token_ids, const int32_t* expert_ids,
+                                  const int32_t* num_tokens_post_padded, const float* topk_weights,
+                                  int sorted_token_ids_len, int moe_block_size, int top_k,
+                                  bool mul_topk_weights, int size_m, int size_n, int size_k,
+                                  int local_experts, hipStream_t stream) {
+  MxArgs a{w_codes, w_scales, x_codes, x_scales, output, size_n, size_m, size_k, sorted_token_ids,
+           expert_ids, num_tokens_post_padded, topk_weights, sorted_token_ids_len, moe_block_size,
+           top_k, mul_topk_weights ? 1 : 0, local_experts};
+  const int rc = mx_gemm_checks("mx_grouped_gemm", a, x_format);
+  if (rc != kSuccess) return rc;
+  if (!sorted_token_ids || !expert_ids || !num_tokens_post_padded || (mul_topk_weights && !topk_weights))
+    return fail(kInvalidValue, "mx_grouped_gemm: null pointer");
+  if (!(moe_block_size == 8 || (moe_block_size >= 16 && moe_block_size <= 64 && moe_block_size % 16 == 0)))
+    return fail(kInvalidValue, "mx_grouped_gemm: block size %d not in {8,16,32,48,64}", moe_block_size);
+  if (top_k <= 0 || local_experts <= 0 || sorted_token_ids_len < 0 ||
+      static_cast<long long>(size_m) * top_k >= (1LL << 31))
+    return fail(kInvalidValue, "mx_grouped_gemm: bad shape top_k=%d experts=%d sorted=%d", top_k,
+                local_experts, sorted_token_ids_len);
+  // the gathered rows are addressed through one 32-bit range
+  if (static_cast<long long>(size_m) * size_k >= static_cast<long long>(kOutOfRange))
+    return fail(kNotSupported, "mx_grouped_gemm: activations over 2 GiB (%d x %d)", size_m, size_k);
+  if (size_m == 0 || sorted_token_ids_len == 0) return kSuccess;
+  return x_format == kMxE4M3 ? grouped_launch<kMxE4M3>(a, stream, "mx_grouped_gemm")
+                             : grouped_launch<kMxE2M1>(a, stream, "mx_grouped_gemm");
+}

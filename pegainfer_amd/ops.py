@@ -786,6 +786,50 @@ def mx_dequantize(x: MxTensor, out: torch.Tensor) -> None:
               x.rows, x.cols, _stream())
 
 
+def _mx_weight(w: MxTensor) -> None:
+    _ensure(w.format is MxFormat.Fp4E2M1, "MX weights must be MXFP4")
+
+
+def mx_gemm(w: MxTensor, x: MxTensor, y: torch.Tensor) -> None:
+    """Y[n][m] = bf16(sum_k X[n][k] * W[m][k]) with fp32 accumulation: w [M, K] MXFP4, x [N, K]
+    MXFP8 or MXFP4, y [N, M] bf16 (gemm_graphsafe on microscaled operands)."""
+    _mx_weight(w)
+    _ensure(x.cols == w.cols, f"MX GEMM weight cols={w.cols} must match input dim {x.cols}")
+    _mx_rows("y", y, x.rows, w.rows)
+    _on_current_device(w.codes, w.scales, x.codes, x.scales, y)
+    _lib.call("pega_mx_gemm", _ptr(w.codes), _ptr(w.scales), _ptr(x.codes), _ptr(x.scales),
+              x.format.value, _ptr(y), w.rows, x.rows, w.cols, _stream())
+
+
+def mx_grouped_gemm(routing: KimiMarlinRouting, x: MxTensor, w: MxTensor, topk_weight,
+                    output: torch.Tensor, *, top_k: int, mul_topk_weights: bool,
+                    size_m: int) -> None:
+    """output[sorted_id] = bf16(X[sorted_id / top_k] . W[expert]^T), times topk_weight[sorted_id]
+    before the rounding with mul_topk_weights: wna16_gemm on microscaled operands.  w holds the
+    experts' weights one after another, [local_experts * N, K] MXFP4.  Rows not routed here are
+    left as they are."""
+    _mx_weight(w)
+    _ensure(w.rows % routing.local_experts == 0,
+            f"{w.rows} weight rows are not {routing.local_experts} experts' worth")
+    size_n = w.rows // routing.local_experts
+    _ensure(x.cols == w.cols, f"MX GEMM weight cols={w.cols} must match input dim {x.cols}")
+    _ensure(top_k > 0 and size_m >= 0, "top_k must be positive")
+    _ensure(x.rows >= size_m, "input too small")
+    _ensure(_is_bf16(output) and output.numel() >= size_m * top_k * size_n,
+            "output must be bf16 [size_m * top_k, N]")
+    if mul_topk_weights:
+        _ensure(topk_weight is not None and topk_weight.dtype == torch.float32
+                and topk_weight.numel() >= size_m * top_k,
+                "topk_weight must be float32 [size_m * top_k]")
+    _on_current_device(x.codes, x.scales, w.codes, w.scales, output, routing.sorted_token_ids)
+    _lib.call("pega_mx_grouped_gemm", _ptr(x.codes), _ptr(x.scales), x.format.value, _ptr(output),
+              _ptr(w.codes), _ptr(w.scales), _ptr(routing.sorted_token_ids),
+              _ptr(routing.expert_ids), _ptr(routing.num_tokens_post_padded),
+              _ptr(topk_weight) if mul_topk_weights else None, routing.max_padded_tokens,
+              routing.block_size, top_k, bool(mul_topk_weights), size_m, size_n, w.cols,
+              routing.local_experts, _stream())
+
+
 # --------------------------------------------------------------------------
 # Residual add + norm (no reference counterpart as one op)
 # --------------------------------------------------------------------------

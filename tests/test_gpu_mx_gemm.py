@@ -1,0 +1,184 @@
+"""Products of microscaled operands on the GPU against 64-bit products of the values that the codes
+stand for.
+
+Tolerance, element by element: half a bf16 step of the result (2^-8 of it), plus what the sums may
+lose.  An instruction adds 128 products in one go; E4M3 products are aligned to the largest of them
+and keep about 12 bits below it, so 2^-11 of the largest product of each 128 k is allowed (E2M1
+with E2M1: 2^-20); from instruction to instruction the sums are fp32: 2^-23 of the sum of
+magnitudes for each."""
+import numpy as np
+import pytest
+import torch
+
+import mx_ref
+from gpu_helpers import bf, dev, host
+
+pytestmark = pytest.mark.gpu
+FORMATS = {"fp8": 0, "fp4": 1}
+
+
+def _operand(g, rows, cols, name, spread=3):
+    """Codes and scales of normal rows with uneven blocks, on the GPU, and their values."""
+    from pegainfer_amd import ops
+    v = g.standard_normal((rows, cols)) * np.repeat(2.0 ** g.integers(-spread, spread + 1, (rows, cols // 32)), 32, 1)
+    codes, scales = mx_ref.quantize(v, name)
+    return (ops.MxTensor(rows, cols, ops.MxFormat(FORMATS[name]), dev(codes), dev(scales)),
+            mx_ref.values(codes, scales, name))
+
+
+def _bounds(x, w, name):
+    """want [N, M] and the tolerance."""
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a))  # noqa: E731
+    want = (t(x) @ t(w).T).numpy()
+    ax, aw = np.abs(x), np.abs(w)
+    peak = lambda a: a.reshape(len(a), -1, 128).max(-1)  # noqa: E731
+    steps = x.shape[1] // 128
+    lost = (2.0 ** -11 if name == "fp8" else 2.0 ** -20) * (t(peak(ax)) @ t(peak(aw)).T).numpy()
+    sums = steps * 2.0 ** -23 * (t(ax) @ t(aw).T).numpy()
+    return want, np.abs(want) * 2.0 ** -8 + lost + sums
+
+
+def _check(got, want, tol, what=""):
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (what, int(bad.sum()), np.argwhere(bad)[:4].tolist(), got[bad][:4], want[bad][:4])
+
+
+@pytest.mark.parametrize("name", ["fp8", "fp4"])
+@pytest.mark.parametrize("n,m,k", [
+    (1, 16, 128), (2, 48, 256), (3, 256, 384), (1, 9728, 2560), (15, 272, 512), (16, 64, 640),
+    (17, 80, 1152), (31, 512, 2048), (33, 1408, 128), (64, 4096, 1024), (48, 16, 7168),
+    (65, 16, 128), (100, 272, 256), (129, 640, 384), (300, 400, 2560), (128, 256, 640),
+    (257, 2816, 2048), (500, 32, 512), (1000, 1040, 128)])
+def test_dense(n, m, k, name):
+    from pegainfer_amd import ops
+    g = np.random.default_rng(n * 31 + m + k)
+    x, xv = _operand(g, n, k, name)
+    w, wv = _operand(g, m, k, "fp4")
+    y = torch.full((n + 1, m), 5.0, dtype=torch.bfloat16, device="cuda")
+    ops.mx_gemm(w, x, y[:n])
+    got = bf(host(y)).astype(np.float64)
+    assert (got[n] == 5).all()  # the row behind the last one
+    _check(got[:n], *_bounds(xv, wv, name))
+
+
+@pytest.mark.parametrize("name", ["fp8", "fp4"])
+@pytest.mark.parametrize("n", [3, 40, 200])
+def test_dense_extremes(n, name):
+    """Scales at the ends of their range, all-zero rows, and NaN scales, which stay in their own
+    row of X or W."""
+    from pegainfer_amd import ops
+    g = np.random.default_rng(n)
+    k, m = 512, 96
+    x, xv = _operand(g, n, k, name)
+    w, wv = _operand(g, m, k, "fp4")
+    xs, ws = host(x.scales), host(w.scales)
+    xs[0], ws[5] = 0, 10     # 2^-127 and 2^-117: below fp32's range together
+    xs[1], ws[7] = 254, 130  # 2^127: past bf16's range
+    xc = host(x.codes)
+    xc[2] = 0
+    x.codes.copy_(dev(xc)), x.scales.copy_(dev(xs)), w.scales.copy_(dev(ws))
+    xv, wv = mx_ref.values(xc, xs, name), mx_ref.values(host(w.codes), ws, "fp4")
+    y = torch.zeros(n, m, dtype=torch.bfloat16, device="cuda")
+    ops.mx_gemm(w, x, y)
+    got = bf(host(y)).astype(np.float64)
+    want, tol = _bounds(xv, wv, name)
+    tiny = np.abs(want) < 2.0 ** -100
+    assert (np.abs(got[tiny]) <= 2.0 ** -99).all()
+    rest = ~tiny & (np.abs(want) < 2.0 ** 120)
+    rest[1] = False
+    _check(got[rest], want[rest], tol[rest])
+    assert (got[2] == 0).all()
+    assert not np.isnan(got[[0] + list(range(2, n))]).any()
+    xs[n - 1, 3], ws[11, 15] = 255, 255
+    x.scales.copy_(dev(xs)), w.scales.copy_(dev(ws))
+    ops.mx_gemm(w, x, y)
+    again = bf(host(y)).astype(np.float64)
+    assert np.isnan(again[n - 1]).all() and np.isnan(again[:, 11]).all()
+    keep = np.ones((n, m), bool)
+    keep[n - 1], keep[:, 11], keep[1] = False, False, False
+    assert np.array_equal(again[keep], got[keep])
+
+
+def _route(tokens, topk, experts, local, start, bs, seed, lean=False):
+    from pegainfer_amd import ops
+    g = np.random.default_rng(seed)
+    if lean:  # every route to one or two experts
+        idx = np.stack([g.choice([start, start + local - 1, (start + local) % experts], topk, replace=False)
+                        for _ in range(tokens)])
+    else:
+        idx = np.stack([g.permutation(experts)[:topk] for _ in range(tokens)])
+    idx = idx.astype(np.int32)
+    ws = ops.KimiMarlinRouteWorkspace(tokens, bs, topk=topk, local_experts=local)
+    return idx, ops.moe_align_block_size(ws, dev(idx), tokens, tokens, start)
+
+
+@pytest.mark.parametrize("name", ["fp8", "fp4"])
+@pytest.mark.parametrize("tokens,topk,experts,local,start,bs,m,k", [
+    (1, 1, 4, 4, 0, 8, 16, 128), (1, 8, 384, 48, 48, 8, 256, 1024), (5, 2, 8, 4, 4, 8, 48, 384),
+    (64, 8, 96, 48, 48, 16, 512, 640), (64, 6, 64, 64, 0, 16, 80, 256), (33, 3, 16, 8, 8, 32, 272, 512),
+    (90, 4, 12, 6, 0, 48, 128, 384), (200, 6, 16, 16, 0, 64, 400, 2048), (300, 2, 6, 3, 3, 64, 16, 128),
+    (40, 2, 40, 3, 7, 64, 256, 256)])
+def test_grouped(tokens, topk, experts, local, start, bs, m, k, name):
+    """W13's use (top_k rows a token) and W2's (one row a route, the routing weight applied)."""
+    from pegainfer_amd import ops
+    g = np.random.default_rng(tokens + m + k)
+    idx, routing = _route(tokens, topk, experts, local, start, bs, tokens)
+    w, wv = _operand(g, local * m, k, "fp4")
+    wv = wv.reshape(local, m, k)
+    weights = g.random(tokens * topk).astype(np.float32)
+    flat = idx.reshape(-1) - start
+    for top_k, mul in ((topk, False), (1, True)):
+        rows = tokens if top_k == topk and not mul else tokens * topk
+        x, xv = _operand(g, rows, k, name)
+        y = torch.full((tokens * topk, m), 3.0, dtype=torch.bfloat16, device="cuda")
+        ops.mx_grouped_gemm(routing, x, w, dev(weights) if mul else None, y, top_k=top_k,
+                            mul_topk_weights=mul, size_m=rows)
+        got = bf(host(y)).astype(np.float64)
+        for e in range(local):
+            r = np.flatnonzero(flat == e)
+            if len(r):
+                want, tol = _bounds(xv[r // top_k], wv[e], name)
+                f = weights[r].astype(np.float64)[:, None] if mul else 1.0
+                # the factor's product rounds once more in fp32
+                _check(got[r], want * f, tol * f + np.abs(want * f) * 2.0 ** -23, f"expert {e}")
+        away = (flat < 0) | (flat >= local)
+        assert (got[away] == 3).all()
+
+
+def test_grouped_skewed_and_without_local_routes():
+    from pegainfer_amd import ops
+    g = np.random.default_rng(9)
+    w, wv = _operand(g, 4 * 64, 256, "fp4")
+    for bs in (8, 32, 64):
+        idx, routing = _route(150, 2, 16, 4, 8, bs, 1, lean=True)
+        x, xv = _operand(g, 150, 256, "fp8")
+        y = torch.zeros(300, 64, dtype=torch.bfloat16, device="cuda")
+        ops.mx_grouped_gemm(routing, x, w, None, y, top_k=2, mul_topk_weights=False, size_m=150)
+        got, flat = bf(host(y)).astype(np.float64), idx.reshape(-1) - 8
+        for e in (0, 3):
+            r = np.flatnonzero(flat == e)
+            _check(got[r], *_bounds(xv[r // 2], wv.reshape(4, 64, 256)[e], "fp8"))
+        assert (got[(flat < 0) | (flat > 3)] == 0).all()
+        # no route of this GPU at all: nothing is written
+        ws = ops.KimiMarlinRouteWorkspace(7, bs, topk=2, local_experts=4)
+        none = ops.moe_align_block_size(ws, dev(np.full((7, 2), 100, np.int32)), 7, 7, 0)
+        y.fill_(9.0)
+        ops.mx_grouped_gemm(none, x, w, None, y, top_k=2, mul_topk_weights=False, size_m=7)
+        assert (bf(host(y)) == 9).all()
+
+
+def test_repeat_and_graph_give_the_same_bits():
+    from pegainfer_amd import layer, ops
+    g = np.random.default_rng(2)
+    for n in (5, 200):
+        x, _ = _operand(g, n, 1024, "fp8")
+        w, _ = _operand(g, 512, 1024, "fp4")
+        y = torch.zeros(n, 512, dtype=torch.bfloat16, device="cuda")
+        ops.mx_gemm(w, x, y)
+        first = y.clone()
+        graph = layer.capture_graph(lambda: ops.mx_gemm(w, x, y))
+        for _ in range(3):
+            y.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, first)

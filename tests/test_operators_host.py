@@ -143,3 +143,66 @@ def test_wrappers_refuse_shapes_and_types_before_the_device():
                 lambda: ops.mx_dequantize(q8, out[:, :32])):
         with pytest.raises(ValueError):
             bad()
+
+
+GEMM = [A, A << 1, A << 2, A << 3, 0, A << 4, 32, 4, 256, None]
+
+
+@pytest.mark.parametrize("at,value,code", [
+    (0, None, 1), (1, None, 1), (2, None, 1), (3, None, 1), (5, None, 1), (4, 2, 1), (4, -1, 1),
+    (6, 0, 1), (7, -1, 1), (8, 0, 1), (6, 24, 801), (8, 96, 801), (8, 64, 801), (8, 1 << 23, 801),
+    (0, A + 8, 801), (2, (A << 2) + 4, 801), (5, (A << 4) + 8, 801), (1, (A << 1) + 2, 801),
+    (3, (A << 3) + 1, 801)])
+def test_mx_gemm_refuses(at, value, code):
+    args = list(GEMM)
+    args[at] = value
+    assert _call("pega_mx_gemm", *args) == code
+
+
+def test_mx_gemm_takes_no_rows():
+    args = list(GEMM)
+    args[7] = 0
+    assert _call("pega_mx_gemm", *args) == 0
+
+
+GROUPED = [A, A << 1, 0, A << 2, A << 3, A << 4, A << 5, A << 6, A << 7, A << 8, 64, 16, 2, True,
+           4, 32, 256, 3, None]
+
+
+@pytest.mark.parametrize("at,value,code", [
+    (0, None, 1), (1, None, 1), (3, None, 1), (4, None, 1), (5, None, 1), (6, None, 1),
+    (7, None, 1), (8, None, 1), (9, None, 1), (2, 2, 1), (10, -1, 1), (11, 24, 1), (11, 0, 1),
+    (11, 128, 1), (12, 0, 1), (12, 1 << 30, 1), (14, -1, 1), (15, 40, 801), (16, 192, 801),
+    (16, 0, 1), (17, 0, 1), (3, (A << 2) + 2, 801), (14, 1 << 24, 801)])
+def test_mx_grouped_gemm_refuses(at, value, code):
+    args = list(GROUPED)
+    args[at] = value
+    assert _call("pega_mx_grouped_gemm", *args) == code
+
+
+def test_mx_grouped_gemm_with_nothing_to_do():
+    for at in (10, 14):
+        args = list(GROUPED)
+        args[at] = 0
+        assert _call("pega_mx_grouped_gemm", *args) == 0
+
+
+def test_mx_gemm_wrappers_refuse_before_the_device():
+    from pegainfer_amd import ops
+    q = lambda r, c, f=ops.MxFormat.Fp4E2M1: ops.MxTensor.empty(r, c, f, device="cpu")  # noqa: E731
+    w, x = q(32, 256), q(4, 256, ops.MxFormat.Fp8E4M3)
+    y = torch.zeros(4, 32, dtype=torch.bfloat16)
+    i = torch.zeros(4, dtype=torch.int32)
+    routing = ops.KimiMarlinRouting(4, 4, 8, 0, 8, 64, 8, 2, 2, i, i, i)
+    g = lambda **kw: ops.mx_grouped_gemm(**{**dict(  # noqa: E731
+        routing=routing, x=x, w=w, topk_weight=None, output=torch.zeros(8, 16, dtype=torch.bfloat16),
+        top_k=2, mul_topk_weights=False, size_m=4), **kw})
+    for bad in (lambda: ops.mx_gemm(q(32, 256, ops.MxFormat.Fp8E4M3), x, y),
+                lambda: ops.mx_gemm(w, q(4, 128), y), lambda: ops.mx_gemm(w, x, y.float()),
+                lambda: ops.mx_gemm(w, x, y[:3]),
+                lambda: g(w=q(33, 256)), lambda: g(x=q(4, 128)), lambda: g(size_m=5),
+                lambda: g(output=torch.zeros(7, 16, dtype=torch.bfloat16)), lambda: g(top_k=0),
+                lambda: g(mul_topk_weights=True), lambda: g(mul_topk_weights=True, topk_weight=torch.zeros(7)),
+                lambda: g(output=torch.zeros(8, 16))):
+        with pytest.raises(ValueError):
+            bad()
