@@ -315,6 +315,56 @@ int gemm_graphsafe_cuda(const uint16_t* W, const uint16_t* X, uint16_t* Y, int M
 int pega_dense_w13_swiglu(const uint16_t* W13, const uint16_t* X, uint16_t* act, int inter, int N,
                           int K, hipStream_t stream);
 
+/* ---------------- a whole MoE layer for a few tokens ---------------- */
+
+enum { PEGA_SHARED_NONE = 0, PEGA_SHARED_BF16 = 1, PEGA_SHARED_INT4 = 2 };
+enum { PEGA_FEW_MAX_SPLITS = 8 };
+
+/* Arguments of pega_moe_few_tokens.  INT4 weights are device packages (the layout of
+ * pega_marlin_int4_*; W13 gate columns first).  Plain pointers and sizes; 208 bytes on LP64. */
+typedef struct pega_moe_few {
+    const uint16_t* x;           /* bf16 [tokens][hidden_dim], the normed rows */
+    const float* logits;         /* router logits [tokens][n_experts] */
+    const float* bias;           /* score correction [n_experts]; unused with softmax */
+    const uint8_t* w13;          /* [local_experts] INT4 gate and up */
+    const uint16_t* w13_scales;
+    const uint8_t* w2;           /* [local_experts] INT4 down */
+    const uint16_t* w2_scales;
+    const void* shared_w13;      /* bf16 [2 shared_inter][hidden_dim], or an INT4 package */
+    const uint16_t* shared_w13_scales; /* INT4 only */
+    const void* shared_w2;       /* bf16 [hidden_dim][shared_inter], or an INT4 package */
+    const uint16_t* shared_w2_scales;  /* INT4 only */
+    const uint16_t* residual;    /* bf16 [tokens][hidden_dim] or NULL */
+    uint16_t* out;               /* bf16 [tokens][hidden_dim]; may be residual's or x's buffer */
+    float* topk_weight;          /* out: [tokens][topk] */
+    int32_t* topk_idx;           /* out: [tokens][topk] */
+    uint16_t* act;               /* workspace: bf16 [min(tokens topk, local_experts)][tokens][inter] */
+    uint16_t* act_shared;        /* workspace: bf16 [tokens][shared_inter] */
+    int32_t* slots;              /* workspace: 1 + min(tokens topk, local_experts) */
+    float* partials;             /* workspace: PEGA_FEW_MAX_SPLITS * tokens * hidden_dim */
+    uint32_t* counters;          /* workspace: hidden_dim / 64, zero before the first call; every
+                                    call leaves them zero */
+    float route_scale;           /* of the sigmoid select (> 0); unused with softmax */
+    float routed_scale;          /* factor of the routed sum */
+    int softmax;                 /* 0: pega_kimi_router_select, 1: pega_dsv2_router_select */
+    int shared_kind;             /* PEGA_SHARED_* */
+    int tokens;                  /* 1 to 16 */
+    int hidden_dim, inter, shared_inter; /* multiples of 64 */
+    int n_experts, local_experts, global_start, topk;
+} pega_moe_few;
+
+/* No reference counterpart as one call: an MoE decode layer for a few tokens in two launches.
+ *   topk_idx, topk_weight = the select entry's, bit for bit;
+ *   out[t] = bf16(residual[t] + routed_scale * sum over t's local routes of weight *
+ *            (silu(x G_e^T) * (x U_e^T)) D_e^T + the shared expert's rows).
+ * INT4 weights count as (nibble - 8) * scale unrounded; the SwiGLU rows, times weight and
+ * routed_scale, are rounded to bf16 once, out once, and all sums are fp32, in an order that the
+ * sizes and the routing decide.  Experts without a route are not read.  Calls that share a
+ * workspace must not overlap (two captured graphs that may run at once need one each); nothing is
+ * kept in it from one call to the next but the zeroed counters.  At most 16 tokens, topk 32, 512
+ * local experts, 1024 experts, sizes multiples of 64, 16-byte aligned buffers (801 otherwise). */
+int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream);
+
 /* ---------------- residual add + norm ---------------- */
 
 /* No reference counterpart as one symbol: the residual add and the root-mean-square norm between

@@ -31,6 +31,17 @@ class Wna16Problem(ctypes.Structure):
                 ("local_experts", _I), ("group_size", _I)]
 
 
+class MoeFew(ctypes.Structure):
+    """pega_moe_few (include/pega_moe.h): the arguments of pega_moe_few_tokens."""
+    _fields_ = [(n, _P) for n in (
+        "x", "logits", "bias", "w13", "w13_scales", "w2", "w2_scales", "shared_w13",
+        "shared_w13_scales", "shared_w2", "shared_w2_scales", "residual", "out", "topk_weight",
+        "topk_idx", "act", "act_shared", "slots", "partials", "counters")] + [
+        ("route_scale", _F), ("routed_scale", _F)] + [(n, _I) for n in (
+            "softmax", "shared_kind", "tokens", "hidden_dim", "inter", "shared_inter", "n_experts",
+            "local_experts", "global_start", "topk")]
+
+
 # name -> argument types (return type is int unless listed in _RESTYPE)
 SIGNATURES = {
     "pegainfer_kernels_last_error": [],
@@ -75,6 +86,7 @@ SIGNATURES = {
     "pega_mx_quantize": [_P, _P, _P, _I, _I, _I, _P],
     "pega_mx_swiglu_quantize": [_P, _P, _P, _I, _I, _I, _P],
     "pega_mx_dequantize": [_P, _P, _P, _I, _I, _I, _P],
+    "pega_moe_few_tokens": [ctypes.POINTER(MoeFew), _P],
     "pega_mx_gemm": [_P] * 4 + [_I, _P] + [_I] * 3 + [_P],
     "pega_mx_grouped_gemm": [_P, _P, _I] + [_P] * 7 + [_I] * 3 + [_B] + [_I] * 4 + [_P],
 }

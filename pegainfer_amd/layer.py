@@ -266,16 +266,30 @@ def fused_route(tokens: int, topk: int, n_experts: int, softmax: bool = False) -
     return tokens * topk <= limit and n_experts <= 1024
 
 
+def few_workspace(routed: RoutedExperts, shared_inter: int, few_tokens: int, device):
+    """The two-launch form's workspace for batches of up to few_tokens, None for 0."""
+    if few_tokens == 0:
+        return None
+    return ops.FewTokensWorkspace(min(few_tokens, routed.max_tokens) if few_tokens > 0 else few_tokens,
+                                  routed.H, routed.I, topk=routed.topk, local_experts=routed.E,
+                                  shared_inter=shared_inter, device=device)
+
+
 class KimiMoeDecodeLayer:
     """One GPU's Kimi-K2 MoE decode layer (moe_nccl.rs:98-239 without the
     collectives): the shared expert on the normed input, the router select, the
     routed experts (fp32 combine of the local routes) and the residual join
-    out = bf16(routed * 2.827 + bf16(hidden + projected)) (kimi_experts.cu:25-39)."""
+    out = bf16(routed * 2.827 + bf16(hidden + projected)) (kimi_experts.cu:25-39).
+
+    few_tokens: batches of up to that many tokens (at most ops.FEW_TOKENS_MAX) take the
+    two-launch form instead, ops.moe_few_tokens, which rounds less in between (the INT4
+    weights' products, the routed rows and the joins stay fp32), so its bits differ."""
 
     def __init__(self, routed: RoutedExperts, shared: KimiSharedExpert, *, n_experts: int = 384,
-                 device="cuda"):
+                 device="cuda", few_tokens: int = 0):
         self.routed, self.shared = routed, shared
         T, H = routed.max_tokens, routed.H
+        self.few_ws = few_workspace(routed, shared.I, few_tokens, device)
         self.projected = torch.zeros(T, H, dtype=torch.bfloat16, device=device)
         self.routed_f32 = torch.zeros(T, H, dtype=torch.float32, device=device)
         self.topk_w = torch.zeros(T, routed.topk, dtype=torch.float32, device=device)
@@ -284,6 +298,13 @@ class KimiMoeDecodeLayer:
     def forward(self, hidden: torch.Tensor, normed: torch.Tensor, logits: torch.Tensor,
                 bias: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         T = hidden.shape[0]
+        if self.few_ws is not None and T <= self.few_ws.max_tokens:
+            ops.moe_few_tokens(self.few_ws, normed, logits, self.routed.w13, self.routed.w2,
+                               self.topk_w[:T], self.topk_idx[:T], out, bias=bias,
+                               routed_scale=ops.KIMI_K2_ROUTER_SCALE,
+                               global_start=self.routed.global_start, residual=hidden,
+                               shared=(self.shared.gate_up, self.shared.down))
+            return out
         projected, routed_f32 = self.projected[:T], self.routed_f32[:T]
         self.shared.forward(normed, projected)
         self.routed.forward_from_logits(normed, logits, bias, self.topk_w, self.topk_idx,
@@ -342,10 +363,10 @@ class Dsv2MoeLayer:
     in the fp32 combine, route order = expert id) plus a shared expert, joined
     as the reference rounds it: bf16(f(bf16(routed_f32)) + f(shared))
     (f32_to_bf16 at nccl_backend.rs:544-545, then the bf16 add at
-    runtime/moe.rs:656)."""
+    runtime/moe.rs:656).  few_tokens: as in KimiMoeDecodeLayer."""
 
     def __init__(self, routed: RoutedExperts, shared: ExpertFFN, device="cuda",
-                 overlap_shared: bool = True):
+                 overlap_shared: bool = True, few_tokens: int = 0):
         self.routed, self.shared = routed, shared
         T, H = routed.max_tokens, routed.H
         self.topk_w = torch.zeros(T, routed.topk, dtype=torch.float32, device=device)
@@ -353,6 +374,7 @@ class Dsv2MoeLayer:
         self.routed_f32 = torch.zeros(T, H, dtype=torch.float32, device=device)
         self.shared_out = torch.zeros(T, H, dtype=torch.bfloat16, device=device)
         self.overlap_shared = overlap_shared
+        self.few_ws = few_workspace(routed, shared.I, few_tokens, device)
         # prefill block sizes overlap in shared launches; the decode kernels use a
         # second stream (default priority, like every stream here), made on first use
         self.pair = (overlap_shared and routed.block_size > 16 and shared.up.block_size > 16
@@ -378,6 +400,12 @@ class Dsv2MoeLayer:
         stream that joins before the add.  Either way the kernels' bits are those
         of the serial order."""
         T = hidden.shape[0]
+        if self.few_ws is not None and T <= self.few_ws.max_tokens:
+            ops.moe_few_tokens(self.few_ws, hidden, logits, self.routed.w13, self.routed.w2,
+                               self.topk_w[:T], self.topk_idx[:T], out,
+                               global_start=self.routed.global_start,
+                               shared=(self.shared.up.w, self.shared.down.w))
+            return out
         if self.pair:
             companion = self.shared.pair_problems(hidden, self.shared_out[:T])
             routing = self._route(logits, T)

@@ -692,6 +692,105 @@ def dense_w13_swiglu(w13: torch.Tensor, x: torch.Tensor, act: torch.Tensor) -> N
 
 
 # --------------------------------------------------------------------------
+# A whole MoE layer for a few tokens (no reference counterpart as one op)
+# --------------------------------------------------------------------------
+FEW_TOKENS_MAX = 16        # rows of one matrix instruction
+FEW_TOKENS_MAX_TOPK = 32
+_FEW_MAX_SPLITS = 8        # PEGA_FEW_MAX_SPLITS
+_SHARED_NONE, _SHARED_BF16, _SHARED_INT4 = 0, 1, 2
+
+
+class FewTokensWorkspace:
+    """Buffers between moe_few_tokens' two launches, sized once for `max_tokens`.  Calls that
+    share one must not overlap: graphs that may replay at the same time need one each."""
+
+    def __init__(self, max_tokens: int, hidden: int, inter: int, *, topk: int, local_experts: int,
+                 shared_inter: int = 0, device="cuda"):
+        _ensure(0 < max_tokens <= FEW_TOKENS_MAX,
+                f"few-token batches have 1 to {FEW_TOKENS_MAX} tokens, got {max_tokens}")
+        _ensure(0 < topk <= FEW_TOKENS_MAX_TOPK and local_experts > 0,
+                f"few-token layers take top-1 to top-{FEW_TOKENS_MAX_TOPK}, got {topk}")
+        _ensure(hidden > 0 and inter > 0 and hidden % 64 == 0 and inter % 64 == 0
+                and shared_inter >= 0 and shared_inter % 64 == 0,
+                "hidden and intermediate sizes must be multiples of 64")
+        self.max_tokens, self.hidden, self.inter = max_tokens, hidden, inter
+        self.topk, self.local_experts, self.shared_inter = topk, local_experts, shared_inter
+        slots = min(max_tokens * topk, local_experts)
+        self.act = torch.empty(slots * max_tokens * inter, dtype=torch.bfloat16, device=device)
+        self.act_shared = torch.empty(max(1, max_tokens * shared_inter), dtype=torch.bfloat16,
+                                      device=device)
+        self.slots = torch.zeros(1 + slots, dtype=torch.int32, device=device)
+        self.partials = torch.empty(_FEW_MAX_SPLITS * max_tokens * hidden, dtype=torch.float32,
+                                    device=device)
+        self.counters = torch.zeros(hidden // 64, dtype=torch.int32, device=device)
+
+
+def moe_few_tokens(workspace: FewTokensWorkspace, x: torch.Tensor, logits: torch.Tensor,
+                   w13: MarlinInt4Weight, w2: MarlinInt4Weight, topk_weight: torch.Tensor,
+                   topk_idx: torch.Tensor, out: torch.Tensor, *, bias: torch.Tensor = None,
+                   route_scale: float = 1.0, routed_scale: float = 1.0, global_start: int = 0,
+                   residual: torch.Tensor = None, shared=None) -> None:
+    """An MoE decode layer for at most FEW_TOKENS_MAX tokens in two launches:
+
+        topk_idx, topk_weight = kimi_router_select (with `bias`) or dsv2_router_select (without)
+        out = bf16(residual + routed_scale * sum of the local routes' weighted experts + shared)
+
+    x: the normed rows, bf16 [T, hidden]; logits: f32 [T, n_experts]; w13, w2: the local experts'
+    INT4 packages; shared: None, a pair of bf16 matrices (gate-then-up [2 Is, hidden], down
+    [hidden, Is]) or a pair of one-expert INT4 packages.  out may be x or residual itself."""
+    ws = workspace
+    _ensure(x.dim() == 2 and _is_bf16(x), "x must be bf16 [tokens, hidden]")
+    T, H = x.shape
+    E, inter = w13.local_experts, w13.out_dim // 2
+    _ensure(0 < T <= ws.max_tokens, f"{T} tokens exceed the workspace's {ws.max_tokens}")
+    _ensure((H, inter, E) == (ws.hidden, ws.inter, ws.local_experts) and w13.in_dim == H
+            and (w2.local_experts, w2.in_dim, w2.out_dim) == (E, inter, H),
+            "the workspace and the experts' shapes differ")
+    w13.validate()
+    w2.validate()
+    _ensure(logits.dim() == 2 and logits.shape[0] == T, "logits must be f32 [tokens, n_experts]")
+    n_experts = logits.shape[1]
+    _ensure_router_inputs(logits, bias, T, n_experts)
+    _ensure(0 <= global_start <= n_experts - E, "global expert range exceeds the routed experts")
+    routes = T * ws.topk
+    _ensure(topk_weight.dtype == torch.float32 and topk_weight.numel() >= routes,
+            "topk_weight must be f32 covering tokens * topk")
+    _ensure(topk_idx.dtype == torch.int32 and topk_idx.numel() >= routes,
+            "topk_idx must be int32 covering tokens * topk")
+    _mx_rows("out", out, T, H)
+    if residual is not None:
+        _mx_rows("residual", residual, T, H)
+    kind, sw13, ss13, sw2, ss2 = _SHARED_NONE, None, None, None, None
+    if shared is not None:
+        up, down = shared
+        if isinstance(up, MarlinInt4Weight):
+            kind = _SHARED_INT4
+            _ensure((up.local_experts, up.in_dim, up.out_dim) == (1, H, 2 * ws.shared_inter)
+                    and (down.local_experts, down.in_dim, down.out_dim) == (1, ws.shared_inter, H),
+                    "the shared expert's shapes differ from the workspace's")
+            up.validate()
+            down.validate()
+            sw13, ss13 = up.weight_packed_uint4b8, up.weight_scale_permuted
+            sw2, ss2 = down.weight_packed_uint4b8, down.weight_scale_permuted
+        else:
+            kind = _SHARED_BF16
+            _mx_rows("shared gate/up", up, 2 * ws.shared_inter, H)
+            _mx_rows("shared down", down, H, ws.shared_inter)
+            sw13, sw2 = up, down
+    _on_current_device(x, logits, bias, w13.weight_packed_uint4b8, w2.weight_packed_uint4b8, sw13,
+                       sw2, residual, out, topk_weight, topk_idx, ws.act)
+    args = _lib.MoeFew(
+        _ptr(x), _ptr(logits), _ptr(bias), _ptr(w13.weight_packed_uint4b8),
+        _ptr(w13.weight_scale_permuted), _ptr(w2.weight_packed_uint4b8),
+        _ptr(w2.weight_scale_permuted), _ptr(sw13), _ptr(ss13), _ptr(sw2), _ptr(ss2),
+        _ptr(residual), _ptr(out), _ptr(topk_weight), _ptr(topk_idx), _ptr(ws.act),
+        _ptr(ws.act_shared), _ptr(ws.slots), _ptr(ws.partials), _ptr(ws.counters),
+        float(route_scale), float(routed_scale), int(bias is None), kind, T, H, inter,
+        ws.shared_inter if shared is not None else 0, n_experts, E, global_start, ws.topk)
+    _lib.call("pega_moe_few_tokens", ctypes.byref(args), _stream())
+
+
+# --------------------------------------------------------------------------
 # Microscaled formats (no reference counterpart)
 # --------------------------------------------------------------------------
 MX_BLOCK = 32  # consecutive values of a row that share a scale

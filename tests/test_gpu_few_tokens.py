@@ -1,0 +1,253 @@
+"""The two-launch MoE layer for a few tokens against the layer's formula in 64 bits, and its router
+outputs against the select stages bit for bit.
+
+Tolerance: the SwiGLU rows are rounded to bf16 (2^-8 of each at most, in the sum 2^-8 of the sum of
+magnitudes of their products), out once (2^-8 of it); fp32 sums add K * 2^-24 of the magnitudes in
+each product chain and silu's exponential a few ulp, 2^-12 of the magnitudes with room to spare."""
+import numpy as np
+import pytest
+import torch
+
+from gpu_helpers import bf, dev, host, pack_ckpt
+
+pytestmark = pytest.mark.gpu
+
+
+def _bits(v):
+    import mx_ref
+    return mx_ref.bf16_round(v)
+
+
+def _int4(g, e, out_dim, in_dim, scale=0.02):
+    """A checkpoint pair and its weights in float64: (nibble - 8) * scale."""
+    q = g.integers(-8, 8, (e, out_dim, in_dim)).astype(np.int8)
+    s = _bits(np.abs(g.standard_normal((e, out_dim, in_dim // 32))) * scale / 4 + 1e-4)
+    return (pack_ckpt(q), s), q * np.repeat(bf(s).astype(np.float64), 32, 2)
+
+
+def _silu(v):
+    with np.errstate(over="ignore"):
+        return v / (1 + np.exp(-v))
+
+
+class Case:
+    """A layer's weights on both sides."""
+
+    def __init__(self, h, i, e, n, topk, start, kind, seed, shared_i=None):
+        from pegainfer_amd import layer
+        g = self.g = np.random.default_rng(seed)
+        self.h, self.i, self.e, self.n, self.topk, self.start, self.kind = h, i, e, n, topk, start, kind
+        (gate, self.G), (up, self.U), (down, self.D) = (_int4(g, e, i, h), _int4(g, e, i, h), _int4(g, e, h, i))
+        self.w13, self.w2 = layer.package_w13(gate, up), layer.package_projection(*down)
+        si = self.si = shared_i or i
+        self.shared = None
+        if kind == "bf16":
+            gu, dn = _bits(g.standard_normal((2 * si, h)) * 0.02), _bits(g.standard_normal((h, si)) * 0.02)
+            self.shared = (dev(gu, bf16=True), dev(dn, bf16=True))
+            self.sG, self.sU, self.sD = (bf(v).astype(np.float64) for v in (gu[:si], gu[si:], dn))
+        elif kind == "int4":
+            (a, G), (b, U), (c, D) = (_int4(g, 1, si, h), _int4(g, 1, si, h), _int4(g, 1, h, si))
+            self.shared = (layer.package_w13(a, b), layer.package_projection(*c))
+            self.sG, self.sU, self.sD = G[0], U[0], D[0]
+
+    def workspace(self, tokens):
+        from pegainfer_amd import ops
+        return ops.FewTokensWorkspace(tokens, self.h, self.i, topk=self.topk, local_experts=self.e,
+                                      shared_inter=self.si if self.shared else 0)
+
+    def inputs(self, t, residual=True):
+        g = self.g
+        x = _bits(g.standard_normal((t, self.h)))
+        logits = g.standard_normal((t, self.n)).astype(np.float32)
+        bias = (g.standard_normal(self.n) * 0.05).astype(np.float32)
+        res = _bits(g.standard_normal((t, self.h))) if residual else None
+        return x, logits, bias, res
+
+    def run(self, ws, x, logits, bias, res, softmax, scale, out=None):
+        from pegainfer_amd import ops
+        t = len(x)
+        o = torch.full((t, self.h), 9.0, dtype=torch.bfloat16, device="cuda") if out is None else out
+        w = torch.zeros(t, self.topk, device="cuda")
+        idx = torch.zeros(t, self.topk, dtype=torch.int32, device="cuda")
+        ops.moe_few_tokens(ws, dev(x, bf16=True), dev(logits), self.w13, self.w2, w, idx, o,
+                           bias=None if softmax else dev(bias), routed_scale=scale,
+                           global_start=self.start, residual=None if res is None else dev(res, bf16=True),
+                           shared=self.shared)
+        return host(o), host(w), host(idx)
+
+    def want(self, x, idx, w, res, scale):
+        """The formula on the given routes, and the tolerance."""
+        xv = bf(x).astype(np.float64)
+        out, mag = np.zeros((len(x), self.h)), np.zeros((len(x), self.h))
+
+        def add(rows, G, U, D, f):
+            act = _silu(rows @ G.T) * (rows @ U.T) * f
+            room = np.abs(rows) @ np.abs(G).T * np.abs(rows @ U.T) + np.abs(rows @ G.T) * (np.abs(rows) @ np.abs(U).T)
+            return act @ D.T, (np.abs(act) * 2.0 ** -8 + room * np.abs(f) * 2.0 ** -19) @ np.abs(D).T
+        for t in range(len(x)):
+            for k in range(self.topk):
+                e = idx[t, k] - self.start
+                if 0 <= e < self.e:
+                    a, m = add(xv[t:t + 1], self.G[e], self.U[e], self.D[e], float(w[t, k]) * scale)
+                    out[t] += a[0]
+                    mag[t] += m[0]
+        if self.shared:
+            a, m = add(xv, self.sG, self.sU, self.sD, 1.0)
+            out, mag = out + a, mag + m
+        if res is not None:
+            out = out + bf(res)
+        return out, np.abs(out) * 2.0 ** -8 + mag * (1 + 2.0 ** -4)
+
+
+def _check(got, want, tol):
+    g = bf(got).astype(np.float64)
+    bad = ~(np.abs(g - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist(), g[bad][:4], want[bad][:4], tol[bad][:4])
+
+
+def _select(logits, bias, topk, softmax):
+    from pegainfer_amd import ops
+    t = len(logits)
+    w = torch.zeros(t, topk, device="cuda")
+    idx = torch.zeros(t, topk, dtype=torch.int32, device="cuda")
+    if softmax:
+        ops.dsv2_router_select(dev(logits), w, idx, t, topk)
+    else:
+        ops.kimi_router_select(dev(logits), dev(bias), w, idx, t, topk=topk)
+    return host(w), host(idx)
+
+
+SHAPES = [  # h, i, e, n, topk, start, shared kind, shared inter
+    (64, 64, 1, 1, 1, 0, "none", None), (128, 64, 4, 16, 2, 8, "bf16", 64),
+    (256, 192, 8, 8, 3, 0, "int4", 384), (512, 256, 48, 384, 8, 48, "bf16", 256),
+    (1024, 448, 16, 64, 6, 16, "int4", 64), (448, 128, 5, 100, 4, 95, "none", None),
+    (2048, 320, 12, 12, 6, 0, "int4", 640), (192, 64, 100, 700, 8, 300, "bf16", 128)]
+
+
+@pytest.mark.parametrize("h,i,e,n,topk,start,kind,si", SHAPES)
+@pytest.mark.parametrize("softmax", [False, True])
+def test_matches_the_formula(h, i, e, n, topk, start, kind, si, softmax):
+    c = Case(h, i, e, n, topk, start, kind, h + n, si)
+    ws = c.workspace(16)
+    for t in (1, 2, 3, 4, 5, 9, 16):
+        x, logits, bias, res = c.inputs(t, residual=t % 2 == 1)
+        out, w, idx = c.run(ws, x, logits, bias, res, softmax, 2.5)
+        sw, sidx = _select(logits, bias, topk, softmax)
+        assert np.array_equal(idx, sidx) and np.array_equal(w, sw)
+        _check(out, *c.want(x, idx, w, res, 2.5))
+    assert (host(ws.counters) == 0).all()
+
+
+def test_tokens_without_a_local_route_and_all_on_one_expert():
+    c = Case(256, 128, 4, 64, 4, 20, "bf16", 1)
+    ws = c.workspace(8)
+    x, logits, bias, res = c.inputs(8)
+    logits[:, 20:24] = -30.0  # nobody picks the local experts
+    bias[:] = 0
+    out, w, idx = c.run(ws, x, logits, bias, res, False, 1.0)
+    assert not ((idx >= 20) & (idx < 24)).any()
+    _check(out, *c.want(x, idx, w, res, 1.0))
+    logits[::2, 23] = 30.0  # every other token picks one
+    out, w, idx = c.run(ws, x, logits, bias, res, False, 1.0)
+    assert (idx[::2, 0] == 23).all()
+    _check(out, *c.want(x, idx, w, res, 1.0))
+
+
+def test_not_finite_rows_stay_their_own():
+    """A token with NaN, infinite or huge activations leaves the other tokens' bits alone, and
+    values past the quick form's range (16 times an activation over fp32's) are still exact."""
+    c = Case(256, 64, 6, 6, 2, 0, "bf16", 3)
+    ws = c.workspace(6)
+    x, logits, bias, res = c.inputs(6)
+    clean, w, idx = c.run(ws, x, logits, bias, res, True, 1.0)
+    for t, v in ((1, 0x7FC0), (3, 0x7F80)):
+        bad = x.copy()
+        bad[t, 17] = v
+        out, _, _ = c.run(ws, bad, logits, bias, res, True, 1.0)
+        assert np.isnan(bf(out)[t]).any()
+        keep = np.arange(6) != t
+        assert np.array_equal(out[keep], clean[keep])
+    # 2^125 in one place: 16 x overflows, (v - 8) * scale * x does not; SwiGLU's square would, so
+    # the up rows' weights there are zero-scaled and the gate alone is huge
+    from pegainfer_amd import layer
+    g = np.random.default_rng(8)
+    (gate, G), (up, U), (down, D) = (_int4(g, 6, 64, 256), _int4(g, 6, 64, 256), _int4(g, 6, 256, 64))
+    us = up[1].copy()
+    us[:, :, 0] = 0
+    U = U.copy()
+    U[:, :, :32] = 0
+    c.w13, c.w2, c.G, c.U, c.D = layer.package_w13(gate, (up[0], us)), layer.package_projection(*down), G, U, D
+    c.shared = None
+    ws = c.workspace(6)
+    big = x.copy()
+    big[2, 5] = _bits(np.array([2.0 ** 125]))[0]
+    out, w, idx = c.run(ws, big, logits, bias, None, True, 2.0 ** -100)
+    want, tol = c.want(big, idx, w, None, 2.0 ** -100)
+    assert np.isfinite(bf(out)).all()
+    _check(out, want, tol)
+
+
+def test_in_place_batches_of_any_size_and_stale_workspaces():
+    c = Case(512, 128, 8, 16, 4, 8, "int4", 5, 256)
+    ws = c.workspace(16)
+    for t in (ws.act, ws.act_shared, ws.partials):
+        t.fill_(float("nan"))
+    ws.slots.fill_(7)
+    for t in (16, 2, 11, 1):
+        x, logits, bias, res = c.inputs(t)
+        out, w, idx = c.run(ws, x, logits, bias, res, False, 1.5)
+        _check(out, *c.want(x, idx, w, res, 1.5))
+        again, _, _ = c.run(c.workspace(t), x, logits, bias, res, False, 1.5)
+        assert np.array_equal(again, out)
+        rd = dev(res, bf16=True)
+        from pegainfer_amd import ops
+        xd = dev(x, bf16=True)
+        wd, idxd = torch.zeros(t, 4, device="cuda"), torch.zeros(t, 4, dtype=torch.int32, device="cuda")
+        ops.moe_few_tokens(ws, xd, dev(logits), c.w13, c.w2, wd, idxd, rd, bias=dev(bias),
+                           routed_scale=1.5, global_start=8, residual=rd, shared=c.shared)
+        assert np.array_equal(host(rd), out)
+
+
+def test_kimi_sizes():
+    """The decode layer's real sizes, and the layer's own general path beside it."""
+    from pegainfer_amd import layer, ops
+    c = Case(7168, 2048, 4, 32, 8, 12, "bf16", 7)
+    routed = layer.RoutedExperts(c.w13, c.w2, max_tokens=8, topk=8, block_size=8, global_start=12, ep_size=8)
+    shared = layer.KimiSharedExpert(*c.shared, max_tokens=8)
+    few = layer.KimiMoeDecodeLayer(routed, shared, n_experts=32, few_tokens=6)
+    general = layer.KimiMoeDecodeLayer(routed, shared, n_experts=32)
+    for t in (1, 6, 8):  # 8: past few_tokens, the general path
+        x, logits, bias, res = c.inputs(t)
+        outs = []
+        for lay in (few, general):
+            out = torch.zeros(t, 7168, dtype=torch.bfloat16, device="cuda")
+            lay.forward(dev(res, bf16=True), dev(x, bf16=True), dev(logits), dev(bias), out)
+            outs.append(host(out))
+        idx, w = host(few.topk_idx[:t]), host(few.topk_w[:t])
+        assert np.array_equal(idx, host(general.topk_idx[:t]))
+        want, tol = c.want(x, idx, w, res, ops.KIMI_K2_ROUTER_SCALE)
+        if t <= 6:
+            _check(outs[0], want, tol)
+        else:
+            assert np.array_equal(outs[0], outs[1])
+        assert np.abs(bf(outs[0]) - bf(outs[1])).max() < 0.05 * np.abs(want).max()
+
+
+def test_dsv2_layer_graph_replays():
+    from pegainfer_amd import layer
+    c = Case(2048, 192, 16, 16, 6, 0, "int4", 9, 384)
+    routed = layer.RoutedExperts(c.w13, c.w2, max_tokens=4, topk=6, block_size=8)
+    shared = layer.ExpertFFN(*c.shared, max_rows=4)
+    moe = layer.Dsv2MoeLayer(routed, shared, few_tokens=4)
+    x, logits, _, _ = c.inputs(4)
+    xd, ld = dev(x, bf16=True), dev(logits)
+    out = torch.zeros(4, 2048, dtype=torch.bfloat16, device="cuda")
+    graph = layer.capture_graph(lambda: moe.forward(xd, ld, out))
+    for seed in range(3):
+        x, logits, _, _ = c.inputs(4)
+        xd.copy_(dev(x, bf16=True)), ld.copy_(dev(logits))
+        graph.replay()
+        got = host(out)
+        moe.forward(xd, ld, out)
+        assert np.array_equal(host(out), got)
+        _check(got, *c.want(x, host(moe.topk_idx), host(moe.topk_w), None, 1.0))

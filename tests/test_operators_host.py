@@ -206,3 +206,93 @@ def test_mx_gemm_wrappers_refuse_before_the_device():
                 lambda: g(output=torch.zeros(8, 16))):
         with pytest.raises(ValueError):
             bad()
+
+
+def _few(**kw):
+    from pegainfer_amd import _lib
+    a = _lib.MoeFew()
+    for i, (name, _) in enumerate(_lib.MoeFew._fields_[:20]):
+        setattr(a, name, A << i)
+    a.route_scale = a.routed_scale = 1.0
+    a.softmax, a.shared_kind, a.tokens, a.hidden_dim, a.inter, a.shared_inter = 0, 1, 4, 128, 64, 64
+    a.n_experts, a.local_experts, a.global_start, a.topk = 16, 4, 4, 2
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def _few_call(**kw):
+    import ctypes
+    return _call("pega_moe_few_tokens", ctypes.byref(_few(**kw)), None)
+
+
+@pytest.mark.parametrize("name", [
+    "x", "logits", "bias", "w13", "w13_scales", "w2", "w2_scales", "shared_w13", "shared_w2", "out",
+    "topk_weight", "topk_idx", "act", "act_shared", "slots", "partials", "counters"])
+def test_few_tokens_refuses_null(name):
+    assert _few_call(**{name: None}) == 1
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(tokens=0), 1), (dict(tokens=-1), 1), (dict(tokens=17), 801), (dict(hidden_dim=96), 801),
+    (dict(hidden_dim=0), 1), (dict(inter=32), 801), (dict(inter=0), 1), (dict(shared_inter=100), 801),
+    (dict(shared_inter=0), 1), (dict(n_experts=3), 1), (dict(global_start=13), 1),
+    (dict(global_start=-1), 1), (dict(topk=0), 1), (dict(topk=17), 1), (dict(topk=33, n_experts=64), 801),
+    (dict(local_experts=513, n_experts=1000), 801), (dict(n_experts=1025), 801),
+    (dict(local_experts=0), 1), (dict(shared_kind=3), 1), (dict(shared_kind=-1), 1),
+    (dict(shared_kind=2, shared_w13_scales=None), 1), (dict(shared_kind=2, shared_w2_scales=None), 1),
+    (dict(route_scale=0.0), 1), (dict(route_scale=float("nan")), 1), (dict(x=A + 8), 801),
+    (dict(w13=A + 4), 801), (dict(act=A + 2), 801), (dict(shared_w2=A + 2), 801),
+    (dict(hidden_dim=1 << 20, inter=1024), 801)])
+def test_few_tokens_refuses(kw, code):
+    assert _few_call(**kw) == code
+
+
+def test_few_tokens_struct_matches_the_header(tmp_path):
+    import ctypes
+    import os
+    import subprocess
+    from conftest import ROOT
+    from pegainfer_amd import _lib
+    src = tmp_path / "s.c"
+    fields = [n for n, _ in _lib.MoeFew._fields_]
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "pega_moe.h"\nint main(void) {\n'
+                   'printf("%zu", sizeof(pega_moe_few));\n'
+                   + "".join(f'printf(" %zu", offsetof(pega_moe_few, {n}));\n' for n in fields)
+                   + "return 0; }\n")
+    exe = tmp_path / "s"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got[0] == ctypes.sizeof(_lib.MoeFew) == 208
+    assert got[1:] == [getattr(_lib.MoeFew, n).offset for n in fields]
+
+
+def test_few_tokens_wrappers_refuse_before_the_device():
+    from pegainfer_amd import ops
+    ws = ops.FewTokensWorkspace(4, 128, 64, topk=2, local_experts=4, shared_inter=64, device="cpu")
+    assert ws.act.numel() == 4 * 4 * 64 and ws.counters.numel() == 2 and ws.slots.numel() == 5
+    for bad in (dict(max_tokens=17), dict(max_tokens=0), dict(hidden=96), dict(inter=100),
+                dict(topk=0), dict(topk=33), dict(shared_inter=32), dict(local_experts=0)):
+        kw = {**dict(max_tokens=4, hidden=128, inter=64, topk=2, local_experts=4, shared_inter=64), **bad}
+        with pytest.raises(ValueError):
+            ops.FewTokensWorkspace(kw.pop("max_tokens"), kw.pop("hidden"), kw.pop("inter"), device="cpu", **kw)
+
+    def pack(e, k, n):
+        return ops.MarlinInt4Weight(e, k, n, torch.zeros(e * k * n // 2, dtype=torch.uint8),
+                                    torch.zeros(e * n * (k // 32), dtype=torch.bfloat16))
+    bf = dict(dtype=torch.bfloat16)
+    good = dict(x=torch.zeros(3, 128, **bf), logits=torch.zeros(3, 16), w13=pack(4, 128, 128),
+                w2=pack(4, 64, 128), topk_weight=torch.zeros(3, 2),
+                topk_idx=torch.zeros(3, 2, dtype=torch.int32), out=torch.zeros(3, 128, **bf))
+    for bad in (dict(x=torch.zeros(3, 128)), dict(x=torch.zeros(5, 128, **bf)),
+                dict(x=torch.zeros(0, 128, **bf)), dict(x=torch.zeros(3, 64, **bf)),
+                dict(logits=torch.zeros(2, 16)), dict(logits=torch.zeros(3, 16, **bf)),
+                dict(w13=pack(3, 128, 128)), dict(w2=pack(4, 128, 128)), dict(w13=pack(4, 128, 256)),
+                dict(topk_weight=torch.zeros(3, 1)), dict(topk_idx=torch.zeros(3, 2)),
+                dict(out=torch.zeros(2, 128, **bf)), dict(residual=torch.zeros(3, 64, **bf)),
+                dict(bias=torch.zeros(15)), dict(global_start=13), dict(global_start=-1),
+                dict(shared=(torch.zeros(64, 128, **bf), torch.zeros(128, 64, **bf))),
+                dict(shared=(torch.zeros(128, 128, **bf), torch.zeros(128, 32, **bf))),
+                dict(shared=(pack(1, 128, 64), pack(1, 64, 128)))):
+        with pytest.raises(ValueError):
+            ops.moe_few_tokens(ws, **{**good, **bad})
