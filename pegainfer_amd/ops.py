@@ -691,6 +691,25 @@ def dense_w13_swiglu(w13: torch.Tensor, x: torch.Tensor, act: torch.Tensor) -> N
     _lib.call("pega_dense_w13_swiglu", _ptr(w13), _ptr(x), _ptr(act), two_i // 2, N, K, _stream())
 
 
+def _ptrs_here(*tensors):
+    """Device pointers of tensors (0 for None), which must be contiguous and on the current device,
+    whose current stream the launch goes to; then that stream.  Messages are only formed on
+    failure: at decode sizes a wrapper's host time is of the order of its kernel's."""
+    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    out = []
+    for t in tensors:
+        if t is None:
+            out.append(0)
+            continue
+        if t.get_device() != here:
+            raise ValueError(f"tensor must live on the current GPU, got {t.device}")
+        if not t.is_contiguous():
+            raise ValueError("tensor must be contiguous")
+        out.append(t.data_ptr())
+    out.append(torch._C._cuda_getCurrentRawStream(here))
+    return out
+
+
 # --------------------------------------------------------------------------
 # A whole MoE layer for a few tokens (no reference counterpart as one op)
 # --------------------------------------------------------------------------
@@ -739,55 +758,58 @@ def moe_few_tokens(workspace: FewTokensWorkspace, x: torch.Tensor, logits: torch
     INT4 packages; shared: None, a pair of bf16 matrices (gate-then-up [2 Is, hidden], down
     [hidden, Is]) or a pair of one-expert INT4 packages.  out may be x or residual itself."""
     ws = workspace
-    _ensure(x.dim() == 2 and _is_bf16(x), "x must be bf16 [tokens, hidden]")
+    if x.dim() != 2:
+        raise ValueError("x must be bf16 [tokens, hidden]")
     T, H = x.shape
     E, inter = w13.local_experts, w13.out_dim // 2
-    _ensure(0 < T <= ws.max_tokens, f"{T} tokens exceed the workspace's {ws.max_tokens}")
-    _ensure((H, inter, E) == (ws.hidden, ws.inter, ws.local_experts) and w13.in_dim == H
-            and (w2.local_experts, w2.in_dim, w2.out_dim) == (E, inter, H),
-            "the workspace and the experts' shapes differ")
+    if not 0 < T <= ws.max_tokens:
+        raise ValueError(f"{T} tokens exceed the workspace's {ws.max_tokens}")
+    if ((H, inter, E) != (ws.hidden, ws.inter, ws.local_experts) or w13.in_dim != H
+            or (w2.local_experts, w2.in_dim, w2.out_dim) != (E, inter, H)):
+        raise ValueError("the workspace and the experts' shapes differ")
     w13.validate()
     w2.validate()
-    _ensure(logits.dim() == 2 and logits.shape[0] == T, "logits must be f32 [tokens, n_experts]")
-    n_experts = logits.shape[1]
-    _ensure_router_inputs(logits, bias, T, n_experts)
-    _ensure(0 <= global_start <= n_experts - E, "global expert range exceeds the routed experts")
-    routes = T * ws.topk
-    _ensure(topk_weight.dtype == torch.float32 and topk_weight.numel() >= routes,
-            "topk_weight must be f32 covering tokens * topk")
-    _ensure(topk_idx.dtype == torch.int32 and topk_idx.numel() >= routes,
-            "topk_idx must be int32 covering tokens * topk")
+    _mx_rows("x", x, T, H)
     _mx_rows("out", out, T, H)
     if residual is not None:
         _mx_rows("residual", residual, T, H)
-    kind, sw13, ss13, sw2, ss2 = _SHARED_NONE, None, None, None, None
+    if logits.dim() != 2 or logits.shape[0] != T or logits.dtype != torch.float32:
+        raise ValueError("logits must be f32 [tokens, n_experts]")
+    n_experts = logits.shape[1]
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() < n_experts):
+        raise ValueError(f"bias must be f32 covering {n_experts} experts")
+    if not 0 <= global_start <= n_experts - E:
+        raise ValueError("global expert range exceeds the routed experts")
+    routes = T * ws.topk
+    if topk_weight.dtype != torch.float32 or topk_weight.numel() < routes:
+        raise ValueError("topk_weight must be f32 covering tokens * topk")
+    if topk_idx.dtype != torch.int32 or topk_idx.numel() < routes:
+        raise ValueError("topk_idx must be int32 covering tokens * topk")
+    kind, shared_inter, sw13, ss13, sw2, ss2 = _SHARED_NONE, 0, None, None, None, None
     if shared is not None:
         up, down = shared
+        shared_inter = ws.shared_inter
         if isinstance(up, MarlinInt4Weight):
             kind = _SHARED_INT4
-            _ensure((up.local_experts, up.in_dim, up.out_dim) == (1, H, 2 * ws.shared_inter)
-                    and (down.local_experts, down.in_dim, down.out_dim) == (1, ws.shared_inter, H),
-                    "the shared expert's shapes differ from the workspace's")
+            if ((up.local_experts, up.in_dim, up.out_dim) != (1, H, 2 * shared_inter)
+                    or (down.local_experts, down.in_dim, down.out_dim) != (1, shared_inter, H)):
+                raise ValueError("the shared expert's shapes differ from the workspace's")
             up.validate()
             down.validate()
             sw13, ss13 = up.weight_packed_uint4b8, up.weight_scale_permuted
             sw2, ss2 = down.weight_packed_uint4b8, down.weight_scale_permuted
         else:
             kind = _SHARED_BF16
-            _mx_rows("shared gate/up", up, 2 * ws.shared_inter, H)
-            _mx_rows("shared down", down, H, ws.shared_inter)
+            _mx_rows("shared gate/up", up, 2 * shared_inter, H)
+            _mx_rows("shared down", down, H, shared_inter)
             sw13, sw2 = up, down
-    _on_current_device(x, logits, bias, w13.weight_packed_uint4b8, w2.weight_packed_uint4b8, sw13,
-                       sw2, residual, out, topk_weight, topk_idx, ws.act)
-    args = _lib.MoeFew(
-        _ptr(x), _ptr(logits), _ptr(bias), _ptr(w13.weight_packed_uint4b8),
-        _ptr(w13.weight_scale_permuted), _ptr(w2.weight_packed_uint4b8),
-        _ptr(w2.weight_scale_permuted), _ptr(sw13), _ptr(ss13), _ptr(sw2), _ptr(ss2),
-        _ptr(residual), _ptr(out), _ptr(topk_weight), _ptr(topk_idx), _ptr(ws.act),
-        _ptr(ws.act_shared), _ptr(ws.slots), _ptr(ws.partials), _ptr(ws.counters),
-        float(route_scale), float(routed_scale), int(bias is None), kind, T, H, inter,
-        ws.shared_inter if shared is not None else 0, n_experts, E, global_start, ws.topk)
-    _lib.call("pega_moe_few_tokens", ctypes.byref(args), _stream())
+    *ptrs, stream = _ptrs_here(
+        x, logits, bias, w13.weight_packed_uint4b8, w13.weight_scale_permuted,
+        w2.weight_packed_uint4b8, w2.weight_scale_permuted, sw13, ss13, sw2, ss2, residual, out,
+        topk_weight, topk_idx, ws.act, ws.act_shared, ws.slots, ws.partials, ws.counters)
+    args = _lib.MoeFew(*ptrs, route_scale, routed_scale, bias is None, kind, T, H, inter,
+                       shared_inter, n_experts, E, global_start, ws.topk)
+    _lib.call("pega_moe_few_tokens", ctypes.byref(args), stream)
 
 
 # --------------------------------------------------------------------------
@@ -804,15 +826,6 @@ class MxFormat(enum.Enum):
     def code_cols(self, cols: int) -> int:
         """Bytes of codes that a row of `cols` values takes."""
         return cols if self is MxFormat.Fp8E4M3 else cols // 2
-
-
-def _on_current_device(*tensors: torch.Tensor) -> None:
-    """The launches go to the current device's current stream: refuse another device's tensors."""
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None:
-            _ensure(t.is_cuda and t.device.index == here,
-                    f"tensor must live on the current GPU (cuda:{here}), got {t.device}")
 
 
 @dataclasses.dataclass
@@ -855,49 +868,47 @@ class MxTensor:
 
 
 def _mx_rows(name: str, t: torch.Tensor, rows: int, cols: int) -> None:
-    _ensure(_is_bf16(t) and t.dim() == 2 and tuple(t.shape) == (rows, cols),
-            f"{name} must be bf16 [{rows}, {cols}], got {t.dtype} {tuple(t.shape)}")
+    if t.shape != (rows, cols) or not _is_bf16(t):
+        raise ValueError(f"{name} must be bf16 [{rows}, {cols}], got {t.dtype} {tuple(t.shape)}")
 
 
 def mx_quantize(x: torch.Tensor, out: MxTensor) -> None:
     """bf16 rows [rows, cols] into out's format: per 32 columns the smallest power-of-two scale
     that holds the largest magnitude, codes rounded to nearest even."""
     _mx_rows("x", x, out.rows, out.cols)
-    _on_current_device(x, out.codes, out.scales)
-    _lib.call("pega_mx_quantize", _ptr(x), _ptr(out.codes), _ptr(out.scales), out.format.value,
-              out.rows, out.cols, _stream())
+    px, pc, ps, stream = _ptrs_here(x, out.codes, out.scales)
+    _lib.call("pega_mx_quantize", px, pc, ps, out.format.value, out.rows, out.cols, stream)
 
 
 def mx_swiglu_quantize(w13: torch.Tensor, out: MxTensor) -> None:
     """kimi_marlin_w13_swiglu then mx_quantize in one launch: w13 bf16 [rows, 2 cols], gate
     columns first, out [rows, cols]; the same codes and scales as the two calls."""
     _mx_rows("w13", w13, out.rows, 2 * out.cols)
-    _on_current_device(w13, out.codes, out.scales)
-    _lib.call("pega_mx_swiglu_quantize", _ptr(w13), _ptr(out.codes), _ptr(out.scales),
-              out.format.value, out.rows, out.cols, _stream())
+    pw, pc, ps, stream = _ptrs_here(w13, out.codes, out.scales)
+    _lib.call("pega_mx_swiglu_quantize", pw, pc, ps, out.format.value, out.rows, out.cols, stream)
 
 
 def mx_dequantize(x: MxTensor, out: torch.Tensor) -> None:
     """The values that x stands for, as bf16 [rows, cols]."""
     _mx_rows("out", out, x.rows, x.cols)
-    _on_current_device(out, x.codes, x.scales)
-    _lib.call("pega_mx_dequantize", _ptr(x.codes), _ptr(x.scales), _ptr(out), x.format.value,
-              x.rows, x.cols, _stream())
+    pc, ps, po, stream = _ptrs_here(x.codes, x.scales, out)
+    _lib.call("pega_mx_dequantize", pc, ps, po, x.format.value, x.rows, x.cols, stream)
 
 
-def _mx_weight(w: MxTensor) -> None:
-    _ensure(w.format is MxFormat.Fp4E2M1, "MX weights must be MXFP4")
+def _mx_operands(w: MxTensor, x: MxTensor) -> None:
+    if w.format is not MxFormat.Fp4E2M1:
+        raise ValueError("MX weights must be MXFP4")
+    if x.cols != w.cols:
+        raise ValueError(f"MX GEMM weight cols={w.cols} must match input dim {x.cols}")
 
 
 def mx_gemm(w: MxTensor, x: MxTensor, y: torch.Tensor) -> None:
     """Y[n][m] = bf16(sum_k X[n][k] * W[m][k]) with fp32 accumulation: w [M, K] MXFP4, x [N, K]
     MXFP8 or MXFP4, y [N, M] bf16 (gemm_graphsafe on microscaled operands)."""
-    _mx_weight(w)
-    _ensure(x.cols == w.cols, f"MX GEMM weight cols={w.cols} must match input dim {x.cols}")
+    _mx_operands(w, x)
     _mx_rows("y", y, x.rows, w.rows)
-    _on_current_device(w.codes, w.scales, x.codes, x.scales, y)
-    _lib.call("pega_mx_gemm", _ptr(w.codes), _ptr(w.scales), _ptr(x.codes), _ptr(x.scales),
-              x.format.value, _ptr(y), w.rows, x.rows, w.cols, _stream())
+    wc, ws, xc, xs, py, stream = _ptrs_here(w.codes, w.scales, x.codes, x.scales, y)
+    _lib.call("pega_mx_gemm", wc, ws, xc, xs, x.format.value, py, w.rows, x.rows, w.cols, stream)
 
 
 def mx_grouped_gemm(routing: KimiMarlinRouting, x: MxTensor, w: MxTensor, topk_weight,
@@ -907,26 +918,24 @@ def mx_grouped_gemm(routing: KimiMarlinRouting, x: MxTensor, w: MxTensor, topk_w
     before the rounding with mul_topk_weights: wna16_gemm on microscaled operands.  w holds the
     experts' weights one after another, [local_experts * N, K] MXFP4.  Rows not routed here are
     left as they are."""
-    _mx_weight(w)
-    _ensure(w.rows % routing.local_experts == 0,
-            f"{w.rows} weight rows are not {routing.local_experts} experts' worth")
-    size_n = w.rows // routing.local_experts
-    _ensure(x.cols == w.cols, f"MX GEMM weight cols={w.cols} must match input dim {x.cols}")
-    _ensure(top_k > 0 and size_m >= 0, "top_k must be positive")
-    _ensure(x.rows >= size_m, "input too small")
-    _ensure(_is_bf16(output) and output.numel() >= size_m * top_k * size_n,
-            "output must be bf16 [size_m * top_k, N]")
-    if mul_topk_weights:
-        _ensure(topk_weight is not None and topk_weight.dtype == torch.float32
-                and topk_weight.numel() >= size_m * top_k,
-                "topk_weight must be float32 [size_m * top_k]")
-    _on_current_device(x.codes, x.scales, w.codes, w.scales, output, routing.sorted_token_ids)
-    _lib.call("pega_mx_grouped_gemm", _ptr(x.codes), _ptr(x.scales), x.format.value, _ptr(output),
-              _ptr(w.codes), _ptr(w.scales), _ptr(routing.sorted_token_ids),
-              _ptr(routing.expert_ids), _ptr(routing.num_tokens_post_padded),
-              _ptr(topk_weight) if mul_topk_weights else None, routing.max_padded_tokens,
-              routing.block_size, top_k, bool(mul_topk_weights), size_m, size_n, w.cols,
-              routing.local_experts, _stream())
+    _mx_operands(w, x)
+    experts = routing.local_experts
+    if w.rows % experts != 0:
+        raise ValueError(f"{w.rows} weight rows are not {experts} experts' worth")
+    size_n = w.rows // experts
+    if top_k <= 0 or size_m < 0 or x.rows < size_m:
+        raise ValueError(f"{x.rows} rows of input, top_k {top_k}, size_m {size_m}")
+    if not _is_bf16(output) or output.numel() < size_m * top_k * size_n:
+        raise ValueError("output must be bf16 [size_m * top_k, N]")
+    if mul_topk_weights and (topk_weight is None or topk_weight.dtype != torch.float32
+                             or topk_weight.numel() < size_m * top_k):
+        raise ValueError("topk_weight must be float32 [size_m * top_k]")
+    xc, xs, wc, ws, po, ids, eids, ntp, tw, stream = _ptrs_here(
+        x.codes, x.scales, w.codes, w.scales, output, routing.sorted_token_ids, routing.expert_ids,
+        routing.num_tokens_post_padded, topk_weight if mul_topk_weights else None)
+    _lib.call("pega_mx_grouped_gemm", xc, xs, x.format.value, po, wc, ws, ids, eids, ntp, tw,
+              routing.max_padded_tokens, routing.block_size, top_k, bool(mul_topk_weights), size_m,
+              size_n, w.cols, experts, stream)
 
 
 # --------------------------------------------------------------------------
@@ -945,27 +954,32 @@ def add_rmsnorm(x: torch.Tensor, residual, weight: torch.Tensor, eps: float, *,
     x is bf16, or float32 (a routed sum); residual, weight and the outputs are bf16.  Outputs
     left None are not formed (at least one is needed); an output may be x or residual itself,
     and no two may share memory.  Every output is the formula's value rounded once."""
-    _ensure(x.dim() == 2, "x must be [rows, hidden]")
+    if x.dim() != 2 or not (x.dtype == torch.float32 or _is_bf16(x)):
+        raise ValueError("x must be bf16 or float32 [rows, hidden]")
     rows, hidden = x.shape
-    _ensure(x.dtype == torch.float32 or _is_bf16(x), "x must be bf16 or float32")
-    _ensure(_is_bf16(weight) and weight.numel() == hidden, f"weight must be bf16 [{hidden}]")
-    _ensure(residual_out is not None or normed is not None or quantized is not None,
-            "add_rmsnorm needs an output")
-    for name, t in (("residual", residual), ("residual_out", residual_out), ("normed", normed)):
-        if t is not None:
-            _mx_rows(name, t, rows, hidden)
+    if not _is_bf16(weight) or weight.numel() != hidden:
+        raise ValueError(f"weight must be bf16 [{hidden}]")
+    if residual is not None:
+        _mx_rows("residual", residual, rows, hidden)
+    if residual_out is not None:
+        _mx_rows("residual_out", residual_out, rows, hidden)
+    if normed is not None:
+        _mx_rows("normed", normed, rows, hidden)
     codes = scales = None
     if quantized is not None:
-        _ensure(quantized.format is MxFormat.Fp8E4M3, "add_rmsnorm quantizes into MXFP8")
-        _ensure((quantized.rows, quantized.cols) == (rows, hidden),
-                f"quantized must be [{rows}, {hidden}]")
+        if quantized.format is not MxFormat.Fp8E4M3:
+            raise ValueError("add_rmsnorm quantizes into MXFP8")
+        if (quantized.rows, quantized.cols) != (rows, hidden):
+            raise ValueError(f"quantized must be [{rows}, {hidden}]")
         codes, scales = quantized.codes, quantized.scales
-    _ensure(residual_out is None or normed is None or residual_out.data_ptr() != normed.data_ptr()
-            or rows == 0, "residual_out and normed must be different buffers")
-    _on_current_device(x, residual, weight, residual_out, normed, codes, scales)
-    _lib.call("pega_add_rmsnorm", _ptr(x), x.dtype == torch.float32, _ptr(residual), _ptr(weight),
-              float(eps), _ptr(residual_out), _ptr(normed), _ptr(codes), _ptr(scales), rows, hidden,
-              _stream())
+    elif residual_out is None and normed is None:
+        raise ValueError("add_rmsnorm needs an output")
+    if residual_out is not None and residual_out is normed:
+        raise ValueError("residual_out and normed must be different buffers")
+    px, pr, pw, ps, pn, pc, psc, stream = _ptrs_here(x, residual, weight, residual_out, normed,
+                                                     codes, scales)
+    _lib.call("pega_add_rmsnorm", px, x.dtype == torch.float32, pr, pw, eps, ps, pn, pc, psc, rows,
+              hidden, stream)
 
 
 # --------------------------------------------------------------------------
