@@ -237,11 +237,10 @@ __global__ __launch_bounds__(64 * WV) void mx_stream_kernel(MxArgs p) {
 
 // ---------------------------------------------------------------- many rows
 // A workgroup owns BM features x BN rows, its WM x WN waves TM x TN blocks of 16 x 16 each for all
-// of K; a stage of the ring holds 128 k of both operands and their scales.  A load brings 1 KB:
+// of K; a stage of the ring holds 128 k of both operands.  A load brings 1 KB:
 // 16 rows of 64 bytes (E2M1) or 8 of 128 (E4M3), the row's 16-byte pieces at slot piece ^ (row / 2
 // % 4) or piece ^ (row % 8), which spreads eight lanes' fragment reads over all banks; 64 rows'
-// scale words are one load.  One barrier a stage; the next stage's fragments are read while this
-// one's products run.
+// scales of four steps are one load.  One barrier a stage.
 template <int kXFormat_, int WM_, int WN_, int TM_, int TN_, int NS_>
 struct MxTile {
   static constexpr int kXFormat = kXFormat_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, NS = NS_;
@@ -251,30 +250,47 @@ struct MxTile {
   static constexpr int kXLoadRows = 1024 / kXRow;
   static constexpr int kWLoads = BM / 16, kXLoads = BN / kXLoadRows;
   static constexpr int kSLoads = (BM + BN) / 64;
-  static constexpr int PD = (kWLoads + kXLoads) / kWaves;  // data loads per wave and stage
-  static constexpr int PS = (kSLoads + kWaves - 1) / kWaves;
-  static constexpr int P = PD + PS;
-  static constexpr int kX = BM * 64, kS = kX + BN * kXRow, kStage = kS + (BM + BN) * 4;
-  static_assert(PD * kWaves == kWLoads + kXLoads && BM % 64 == 0 && BN % 64 == 0, "tile shape");
-  static_assert(NS >= 3 && NS * kStage <= 160 * 1024 && kStage % 16 == 0, "tile shape");
+  static constexpr int P = (kWLoads + kXLoads) / kWaves;          // data loads per wave and stage
+  static constexpr int PS = (kSLoads + kWaves - 1) / kWaves;      // scale loads per wave and four
+  static constexpr int kX = BM * 64, kStage = kX + BN * kXRow;
+  static constexpr int kFour = (BM + BN) * 16;                    // four steps' scales
+  static constexpr int kS = NS * kStage, kLds = kS + 2 * kFour;
+  static_assert(P * kWaves == kWLoads + kXLoads && BM % 64 == 0 && BN % 64 == 0, "tile shape");
+  static_assert(NS >= 3 && kLds <= 160 * 1024, "tile shape");
 };
+
+// Workgroups go to the eight XCDs in turn; each XCD's are made to cover a compact part of the grid
+// of tiles (runs of the order that goes down panels four feature tiles wide), so that its L2 brings
+// in as few operand rows as it can.
+__device__ __forceinline__ void xcd_tile(int& tx, int& ty) {
+  const int gx = gridDim.x, gy = gridDim.y;
+  const int total = gx * gy, id = ty * gx + tx;
+  const int xcd = id & 7, each = total >> 3, more = total & 7;
+  const int at = xcd * each + min(xcd, more) + (id >> 3);
+  const int panel = at / (4 * gy), in = at - panel * 4 * gy;
+  const int wide = min(4, gx - 4 * panel);
+  ty = in / wide;
+  tx = 4 * panel + in - ty * wide;
+}
 
 template <typename S, bool kGrouped>
 __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
   constexpr int BM = S::BM, BN = S::BN, NS = S::NS, TM = S::TM, TN = S::TN, P = S::P;
   constexpr bool kF8 = S::kXFormat == kMxE4M3;
-  __shared__ __align__(1024) uint8_t smem[NS * S::kStage];
+  __shared__ __align__(1024) uint8_t smem[S::kLds];
   __shared__ int s_sid[kGrouped ? BN : 1];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % S::WM, wn = wave / S::WM;
   const int c = lane & 15, g = lane >> 4;
-  const int m0 = blockIdx.x * BM;
-  int n0 = blockIdx.y * BN;
+  int tx = blockIdx.x, ty = blockIdx.y;
+  if constexpr (!kGrouped) xcd_tile(tx, ty);
+  const int m0 = tx * BM;
+  int n0 = ty * BN;
   const int K = p.K, steps = K >> 7;
   long long expert = 0;
   if constexpr (kGrouped) {
-    const int mb = blockIdx.y;
+    const int mb = ty;
     const int limit = p.N * p.top_k;
     const int e = __builtin_amdgcn_readfirstlane(p.expert_ids[mb]);
     if (min(p.ntp[0], p.sorted_len) < (mb + 1) * p.bs || e < 0 || e >= p.experts) return;
@@ -294,121 +310,148 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
   const long long w_first = expert * p.M + m0;
   const int w_rows = min(BM, p.M - m0), x_rows = kGrouped ? p.N : min(BN, p.N - n0);
 
-  // This wave's loads of a stage.  Rows past the last feature or row are out of range: zeros.
+  // The offset of a row of the tile in its operand: rows past the last feature or row of X are past
+  // the operand's range, and so are grouped rows without a route; they bring zeros.
+  const auto row_off = [&](bool x, int r, uint32_t row_bytes) {
+    if (!kGrouped || !x) return static_cast<uint32_t>(r) * row_bytes;
+    const int sid = s_sid[r];
+    return sid < 0 ? kOutOfRange : static_cast<uint32_t>(sid / p.top_k) * row_bytes;
+  };
+  // This wave's loads of a stage.
   u32x4_t rsrc[P];
   uint32_t dst[P], voff[P], soff_step[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) {
-    if (j < S::PD) {
-      const int i = wave * S::PD + j;
-      const bool x = i >= S::kWLoads;
-      const int rows_per = x ? S::kXLoadRows : 16, pieces = 64 / rows_per;
-      const int r0 = (x ? i - S::kWLoads : i) * rows_per;
-      const int r = r0 + lane / pieces;
-      const int swz = pieces == 8 ? r & 7 : (r >> 1) & 3;
-      const uint32_t piece = static_cast<uint32_t>((lane % pieces) ^ swz);
-      const uint32_t row_bytes = x ? x_bytes : w_bytes;
-      const long long first = x ? n0 : w_first;
-      rsrc[j] = rsrc_words((x ? p.xq : p.wq) + first * row_bytes,
-                           static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
-                               static_cast<int>((x ? x_rows : w_rows) * row_bytes))));
-      dst[j] = lds0 + (x ? S::kX : 0) + 1024u * static_cast<uint32_t>(x ? i - S::kWLoads : i);
-      soff_step[j] = x ? S::kXRow : 64;
-      if (kGrouped && x) {
-        const int sid = s_sid[r];
-        voff[j] = sid < 0 ? kOutOfRange
-                          : static_cast<uint32_t>(sid / p.top_k) * row_bytes + 16u * piece;
-      } else {
-        voff[j] = static_cast<uint32_t>(r) * row_bytes + 16u * piece;
-      }
-    } else {
-      const int i = min(wave * S::PS + j - S::PD, S::kSLoads - 1);  // a repeat brings the same
-      const bool x = i >= BM / 64;
-      const int r = 64 * (x ? i - BM / 64 : i) + lane;
-      const long long first = x ? n0 : w_first;
-      rsrc[j] = rsrc_words((x ? p.xs : p.ws) + first * s_bytes,
+    const int i = wave * P + j;
+    const bool x = i >= S::kWLoads;
+    const int rows_per = x ? S::kXLoadRows : 16, pieces = 64 / rows_per;
+    const int r = (x ? i - S::kWLoads : i) * rows_per + lane / pieces;
+    const int swz = pieces == 8 ? r & 7 : (r >> 1) & 3;
+    const uint32_t piece = static_cast<uint32_t>((lane % pieces) ^ swz);
+    const uint32_t row_bytes = x ? x_bytes : w_bytes;
+    const long long first = x ? n0 : w_first;
+    rsrc[j] = rsrc_words((x ? p.xq : p.wq) + first * row_bytes,
+                         static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
+                             static_cast<int>((x ? x_rows : w_rows) * row_bytes))));
+    dst[j] = lds0 + (x ? S::kX : 0) + 1024u * static_cast<uint32_t>(x ? i - S::kWLoads : i);
+    soff_step[j] = x ? S::kXRow : 64;
+    voff[j] = row_off(x, r, row_bytes) + 16u * piece;
+  }
+  u32x4_t s_rsrc[S::PS];
+  uint32_t s_dst[S::PS], s_voff[S::PS];
+#pragma unroll
+  for (int j = 0; j < S::PS; ++j) {
+    const int i = min(wave * S::PS + j, S::kSLoads - 1);  // a repeat brings the same
+    const bool x = i >= BM / 64;
+    const long long first = x ? n0 : w_first;
+    s_rsrc[j] = rsrc_words((x ? p.xs : p.ws) + first * s_bytes,
                            static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
                                static_cast<int>((x ? x_rows : w_rows) * s_bytes))));
-      dst[j] = lds0 + S::kS + 256u * static_cast<uint32_t>(i);
-      soff_step[j] = 4;
-      if (kGrouped && x) {
-        const int sid = s_sid[r];
-        voff[j] = sid < 0 ? kOutOfRange : static_cast<uint32_t>(sid / p.top_k) * s_bytes;
-      } else {
-        voff[j] = static_cast<uint32_t>(r) * s_bytes;
-      }
-    }
+    s_dst[j] = lds0 + S::kS + 1024u * static_cast<uint32_t>(i);
+    s_voff[j] = row_off(x, 64 * (x ? i - BM / 64 : i) + lane, s_bytes);
   }
+  // Past the last step every lane is out of range and brings zeros that nothing reads: a branch
+  // there would cut the step in two, and the compiler moves products across it.
   const auto stage_in = [&](int step, int st) {
+    const uint32_t past = step < steps ? 0u : kOutOfRange;
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const uint32_t at = dst[j] + static_cast<uint32_t>(st), so = soff_step[j] * static_cast<uint32_t>(step);
-      if (j < S::PD) dma_b128(rsrc[j], at, voff[j], so);
-      else dma_b32(rsrc[j], at, voff[j], so);
-    }
+    for (int j = 0; j < P; ++j)
+      dma_b128(rsrc[j], dst[j] + static_cast<uint32_t>(st), voff[j] | past,
+               past ? 0u : soff_step[j] * static_cast<uint32_t>(step));
   };
-  struct Frags {
-    u32x4_t w[TM], x[TN][kF8 ? 2 : 1];
-    uint32_t sw[TM], sx[TN];
+  // Scales come for four steps at a time, 16 bytes a row (a word a step would touch as many lines
+  // four times as often: 4096 x 4096 x 7168 in MXFP4 84 us instead of 68 without scale loads); the
+  // last four are steps - 4 .. steps - 1, wherever that starts.
+  const auto four_first = [&](int four) { return min(4 * four, steps - 4); };
+  const auto scales_in = [&](int four, bool now) {
+#pragma unroll
+    for (int j = 0; j < S::PS; ++j)
+      dma_b128_if(now, s_rsrc[j], s_dst[j] + static_cast<uint32_t>((four & 1) * S::kFour), s_voff[j],
+                  4u * static_cast<uint32_t>(max(four_first(four), 0)));
+  };
+  struct WFrags {
+    u32x4_t w[TM];
+    uint32_t s[TM];
+  };
+  struct XFrag {
+    u32x4_t x[kF8 ? 2 : 1];
+    uint32_t s;
   };
   const uint8_t* w_rd = smem + (wm * TM * 16 + c) * 64 + 16 * (g ^ ((c >> 1) & 3));
   const uint8_t* x_rd = smem + S::kX + (wn * TN * 16 + c) * S::kXRow;
   const int x_at0 = 16 * (kF8 ? g ^ (c & 7) : g ^ ((c >> 1) & 3));
   const int x_at1 = 16 * ((4 + g) ^ (c & 7));
-  const uint8_t* sw_rd = smem + S::kS + (wm * TM * 16 + c) * 4 + g;
-  const uint8_t* sx_rd = smem + S::kS + (BM + wn * TN * 16 + c) * 4 + g;
-  const auto read = [&](Frags& f, int st) {
-#pragma unroll
-    for (int t = 0; t < TM; ++t) {
-      f.w[t] = *reinterpret_cast<const u32x4_t*>(w_rd + st + 1024 * t);
-      f.sw[t] = sw_rd[st + 64 * t];
-    }
-#pragma unroll
-    for (int t = 0; t < TN; ++t) {
-      f.x[t][0] = *reinterpret_cast<const u32x4_t*>(x_rd + st + 16 * S::kXRow * t + x_at0);
-      if constexpr (kF8)
-        f.x[t][1] = *reinterpret_cast<const u32x4_t*>(x_rd + st + 16 * S::kXRow * t + x_at1);
-      f.sx[t] = sx_rd[st + 64 * t];
-    }
+  const uint8_t* sw_rd = smem + S::kS + (wm * TM * 16 + c) * 16 + g;
+  const uint8_t* sx_rd = smem + S::kS + (BM + wn * TN * 16 + c) * 16 + g;
+  // where a step's scale bytes are
+  const auto scale_at = [&](int s) {
+    const int four = s >> 2;
+    return (four & 1) * S::kFour + 4 * (s - four_first(four));
+  };
+  const auto read_w = [&](WFrags& f, int t, int st, int sc) {
+    f.w[t] = *reinterpret_cast<const u32x4_t*>(w_rd + st + 1024 * t);
+    f.s[t] = sw_rd[sc + 256 * t];
+  };
+  const auto read_x = [&](XFrag& f, int j, int st, int sc) {
+    f.x[0] = *reinterpret_cast<const u32x4_t*>(x_rd + st + 16 * S::kXRow * j + x_at0);
+    if constexpr (kF8)
+      f.x[1] = *reinterpret_cast<const u32x4_t*>(x_rd + st + 16 * S::kXRow * j + x_at1);
+    f.s = sx_rd[sc + 256 * j];
   };
   floatx4_t acc[TM][TN] = {};
-  const auto products = [&](const Frags& f) {
+
+  scales_in(0, true);
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+  for (int i = 0; i < NS - 1; ++i) stage_in(i, i * S::kStage);
+  vm_wait<(NS - 2) * P>();
+  lds_barrier();
+  int st = 0, st_in = (NS - 1) * S::kStage;
+  const auto next = [](int at) { return at + S::kStage == NS * S::kStage ? 0 : at + S::kStage; };
+  // Step s multiplies the rows' fragments one after another, each read while the one before it is
+  // multiplied.  Half way the next stage has landed (each wave waits for its own loads, the barrier
+  // for all) and every wave is past stage s - 1, which the loads of stage s + NS - 1 then fill; in
+  // the second half the next stage's weight fragments and first row fragment are read.
+  constexpr int kMid = TN / 2, kPer = (TM + TN - kMid - 1) / (TN - kMid);
+  WFrags wa, wb;
+  XFrag x[2];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) read_w(wa, t, 0, 0);
+  read_x(x[0], 0, 0, 0);
+  const auto step = [&](const WFrags& w, WFrags& w_next, int s) {
+    // after the last step a stage that nothing uses
+    const int st_next = next(st), sc = scale_at(s), sc_next = scale_at(min(s + 1, steps - 1));
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      if (j == kMid) {
+        vm_wait<(NS - 3) * P>();
+        lds_barrier();
+        // the four steps after this one's four, whose place every wave has read to the end
+        scales_in((s >> 2) + 1, (s & 3) == 0 && s + 4 < steps);
+        stage_in(s + NS - 1, st_in);
+        st_in = next(st_in);
+      }
+      if (j + 1 < TN) read_x(x[(j + 1) & 1], j + 1, st, sc);
+      else read_x(x[0], 0, st_next, sc_next);
+      if (j >= kMid) {
+#pragma unroll
+        for (int t = (j - kMid) * kPer; t < (j - kMid + 1) * kPer && t < TM; ++t)
+          read_w(w_next, t, st_next, sc_next);
+      }
 #pragma unroll
       for (int t = 0; t < TM; ++t)
-        acc[t][j] = mx_mfma<S::kXFormat>(f.w[t], f.x[j][0], f.x[j][kF8 ? 1 : 0], f.sw[t], f.sx[j],
-                                         acc[t][j]);
-  };
-
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    if (i < steps) stage_in(i, i * S::kStage);
-  if (steps >= NS - 1) vm_wait<(NS - 2) * P>(); else vm_wait<0>();
-  lds_barrier();
-  Frags f0, f1;
-  read(f0, 0);
-  int st_rd = S::kStage, st_in = (NS - 1) * S::kStage;
-  const auto next = [](int st) { return st + S::kStage == NS * S::kStage ? 0 : st + S::kStage; };
-  // Step s: stage s + 1 has landed (each wave waits for its own loads, the barrier for all);
-  // every wave has read stage s - 1, which the loads of stage s + NS - 1 then fill.
-  const auto step = [&](const Frags& cur, Frags& nxt, int s) {
-    if (s + NS - 2 < steps) vm_wait<(NS - 3) * P>(); else vm_wait<0>();
-    lds_barrier();
-    if (s + NS - 1 < steps) {
-      stage_in(s + NS - 1, st_in);
-      st_in = next(st_in);
+        acc[t][j] = mx_mfma<S::kXFormat>(w.w[t], x[j & 1].x[0], x[j & 1].x[kF8 ? 1 : 0], w.s[t],
+                                         x[j & 1].s, acc[t][j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (s + 1 < steps) {
-      read(nxt, st_rd);
-      st_rd = next(st_rd);
-    }
-    products(cur);
+    st = st_next;
   };
-  for (int s = 0; s < steps; s += 2) {
-    step(f0, f1, s);
-    if (s + 1 < steps) step(f1, f0, s + 1);
+  static_assert(TN % 2 == 0, "the first row fragment of a stage takes slot 0");
+  int s = 0;
+  for (; s + 1 < steps; s += 2) {
+    step(wa, wb, s);
+    step(wb, wa, s + 1);
   }
+  if (s < steps) step(wa, wb, s);
 
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
@@ -457,14 +500,17 @@ void launch_tile(const MxArgs& a, int row_blocks, hipStream_t stream) {
                      dim3(S::kThreads), 0, stream, a);
 }
 
+// The tiled kernel's scales come four steps at a time.
+constexpr int kTileMinK = 512;
+
 template <int kXFormat>
 int dense_launch(const MxArgs& a, hipStream_t stream, const char* name) {
+  if (ceil_div(a.N, 64) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
   if (a.N <= 16) launch_stream<kXFormat, 8, 1, 1, false>(a, 1, stream);
   else if (a.N <= 32) launch_stream<kXFormat, 8, 1, 2, false>(a, 1, stream);
-  else if (a.N <= 64) launch_stream<kXFormat, 8, 1, 4, false>(a, 1, stream);
+  else if (a.N <= 64 || a.K < kTileMinK) launch_stream<kXFormat, 8, 1, 4, false>(a, ceil_div(a.N, 64), stream);
   else {
-    using S = MxTile<kXFormat, 2, 2, 4, 4, 4>;
-    if (ceil_div(a.N, S::BN) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
+    using S = MxTile<kXFormat, 2, 2, 4, 4, 3>;
     launch_tile<S, false>(a, ceil_div(a.N, S::BN), stream);
   }
   return launch_status(name);
@@ -476,10 +522,8 @@ int grouped_launch(const MxArgs& a, hipStream_t stream, const char* name) {
   if (blocks > 65535) return fail(kNotSupported, "%s: too many blocks (%d)", name, blocks);
   if (a.bs <= 16) launch_stream<kXFormat, 8, 1, 1, true>(a, blocks, stream);
   else if (a.bs <= 32) launch_stream<kXFormat, 8, 1, 2, true>(a, blocks, stream);
-  else {
-    using S = MxTile<kXFormat, 4, 1, 4, 4, 4>;
-    launch_tile<S, true>(a, blocks, stream);
-  }
+  else if (a.K < kTileMinK) launch_stream<kXFormat, 8, 1, 4, true>(a, blocks, stream);
+  else launch_tile<MxTile<kXFormat, 4, 1, 4, 4, 3>, true>(a, blocks, stream);
   return launch_status(name);
 }
 
