@@ -418,7 +418,9 @@ int pega_mx_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t*
  * expert_ids[b] in [0, local_experts) and every row sid of it below size_m * top_k,
  *   output[sid] = bf16(X[sid / top_k] . W[e]^T)          W [local_experts][size_n][size_k] MXFP4
  * times topk_weights[sid] before the rounding with mul_topk_weights (may be NULL otherwise).
- * Other rows of output [size_m * top_k][size_n] are left as they are.  Block sizes 8, 16, 32, 48,
+ * Other rows of output [size_m * top_k][size_n] are left as they are.  ep_size (at least 1): GPUs
+ * that the routes' experts are spread over, for the launch rules alone, which expect one route in
+ * ep_size to be local; they choose the order of the fp32 sums, nothing else.  Block sizes 8, 16, 32, 48,
  * 64; the shape and alignment rules of pega_mx_gemm; X under 2 GiB (801 otherwise). */
 int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scales, int x_format,
                          uint16_t* output, const uint8_t* w_codes, const uint8_t* w_scales,
@@ -426,7 +428,7 @@ int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scales, int x_
                          const int32_t* num_tokens_post_padded, const float* topk_weights,
                          int sorted_token_ids_len, int moe_block_size, int top_k,
                          bool mul_topk_weights, int size_m, int size_n, int size_k,
-                         int local_experts, hipStream_t stream);
+                         int local_experts, int ep_size, hipStream_t stream);
 
 /* ---------------- routing select ---------------- */
 

@@ -88,7 +88,7 @@ SIGNATURES = {
     "pega_mx_dequantize": [_P, _P, _P, _I, _I, _I, _P],
     "pega_moe_few_tokens": [ctypes.POINTER(MoeFew), _P],
     "pega_mx_gemm": [_P] * 4 + [_I, _P] + [_I] * 3 + [_P],
-    "pega_mx_grouped_gemm": [_P, _P, _I] + [_P] * 7 + [_I] * 3 + [_B] + [_I] * 4 + [_P],
+    "pega_mx_grouped_gemm": [_P, _P, _I] + [_P] * 7 + [_I] * 3 + [_B] + [_I] * 5 + [_P],
 }
 _RESTYPE = {"pegainfer_kernels_last_error": ctypes.c_char_p}
 

@@ -249,13 +249,13 @@ struct MxTile {
   static constexpr int kXRow = kXFormat == kMxE4M3 ? 128 : 64;  // bytes of a row of X in a stage
   static constexpr int kXLoadRows = 1024 / kXRow;
   static constexpr int kWLoads = BM / 16, kXLoads = BN / kXLoadRows;
-  static constexpr int kSLoads = (BM + BN) / 64;
-  static constexpr int P = (kWLoads + kXLoads) / kWaves;          // data loads per wave and stage
-  static constexpr int PS = (kSLoads + kWaves - 1) / kWaves;      // scale loads per wave and four
+  static constexpr int kLoads = kWLoads + kXLoads, kSLoads = BM / 64 + (BN + 63) / 64;
+  static constexpr int P = (kLoads + kWaves - 1) / kWaves;    // data loads per wave and stage
+  static constexpr int PS = (kSLoads + kWaves - 1) / kWaves;  // scale loads per wave and four
   static constexpr int kX = BM * 64, kStage = kX + BN * kXRow;
-  static constexpr int kFour = (BM + BN) * 16;                    // four steps' scales
+  static constexpr int kFour = kSLoads * 1024;                // four steps' scales
   static constexpr int kS = NS * kStage, kLds = kS + 2 * kFour;
-  static_assert(P * kWaves == kWLoads + kXLoads && BM % 64 == 0 && BN % 64 == 0, "tile shape");
+  static_assert(BM % 64 == 0 && BN % kXLoadRows == 0 && TN % 2 == 0, "tile shape");
   static_assert(NS >= 3 && kLds <= 160 * 1024, "tile shape");
 };
 
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
   // the operand's range, and so are grouped rows without a route; they bring zeros.
   const auto row_off = [&](bool x, int r, uint32_t row_bytes) {
     if (!kGrouped || !x) return static_cast<uint32_t>(r) * row_bytes;
-    const int sid = s_sid[r];
+    const int sid = s_sid[min(r, BN - 1)];
     return sid < 0 ? kOutOfRange : static_cast<uint32_t>(sid / p.top_k) * row_bytes;
   };
   // This wave's loads of a stage.
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
   uint32_t dst[P], voff[P], soff_step[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) {
-    const int i = wave * P + j;
+    const int i = min(wave * P + j, S::kLoads - 1);  // a repeat brings the same
     const bool x = i >= S::kWLoads;
     const int rows_per = x ? S::kXLoadRows : 16, pieces = 64 / rows_per;
     const int r = (x ? i - S::kWLoads : i) * rows_per + lane / pieces;
@@ -341,14 +341,15 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
   uint32_t s_dst[S::PS], s_voff[S::PS];
 #pragma unroll
   for (int j = 0; j < S::PS; ++j) {
-    const int i = min(wave * S::PS + j, S::kSLoads - 1);  // a repeat brings the same
+    const int i = min(wave * S::PS + j, S::kSLoads - 1);
     const bool x = i >= BM / 64;
     const long long first = x ? n0 : w_first;
     s_rsrc[j] = rsrc_words((x ? p.xs : p.ws) + first * s_bytes,
                            static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
                                static_cast<int>((x ? x_rows : w_rows) * s_bytes))));
     s_dst[j] = lds0 + S::kS + 1024u * static_cast<uint32_t>(i);
-    s_voff[j] = row_off(x, 64 * (x ? i - BM / 64 : i) + lane, s_bytes);
+    const int r = 64 * (x ? i - BM / 64 : i) + lane;
+    s_voff[j] = x && r >= BN ? kOutOfRange : row_off(x, r, s_bytes);
   }
   // Past the last step every lane is out of range and brings zeros that nothing reads: a branch
   // there would cut the step in two, and the compiler moves products across it.
@@ -445,7 +446,6 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
     }
     st = st_next;
   };
-  static_assert(TN % 2 == 0, "the first row fragment of a stage takes slot 0");
   int s = 0;
   for (; s + 1 < steps; s += 2) {
     step(wa, wb, s);
@@ -503,27 +503,104 @@ void launch_tile(const MxArgs& a, int row_blocks, hipStream_t stream) {
 // The tiled kernel's scales come four steps at a time.
 constexpr int kTileMinK = 512;
 
+// The tile shapes, smallest first, with what a step of 128 k costs a CU that has one tile, and each
+// of several, and what a tile costs besides its steps (its start, and its results, which the large
+// ones write while nothing else runs on their CU), in ns.  Measured with MXFP8 rows at K = 7168
+// and 2048 (64 x 64 to 256 x 256: 200 rows x 4096 x 7168 21 / 27 / 36 / 51 / 85 us, 4096 rows x 7168 x
+// 2048 117 / 85 / 89 / 75 / 67 us); MXFP4 rows are 5 to 30% faster everywhere and rank the shapes alike.
+// More stages where they fit: the loads' latency is what a step waits for (256 x 128 with three and
+// four stages, 4096 x 4096 x 7168: 121 and 101 us).
+template <int F> using Tile64 = MxTile<F, 2, 2, 2, 2, 5>;
+template <int F> using Tile128x64 = MxTile<F, 2, 2, 4, 2, 4>;
+template <int F> using Tile128 = MxTile<F, 2, 2, 4, 4, 4>;
+template <int F> using Tile256x128 = MxTile<F, 4, 2, 4, 4, 4>;
+template <int F> using Tile256 = MxTile<F, 4, 2, 4, 8, F == kMxE4M3 ? 3 : 4>;
+struct TileCost {
+  int m, n, alone, each, besides;
+};
+constexpr TileCost kTileCosts[] = {{64, 64, 370, 260, 200},
+                                   {128, 64, 480, 385, 400},
+                                   {128, 128, 630, 600, 700},
+                                   {256, 128, 900, 870, 4000},
+                                   {256, 256, 1450, 1450, 8000}};
+
+int best_tile(int M, int N, int K, int cu) {
+  int best = 0;
+  long long least = 0;
+  for (int i = 0; i < 5; ++i) {
+    const TileCost& c = kTileCosts[i];
+    const long long each = (static_cast<long long>(ceil_div(M, c.m)) * ceil_div(N, c.n) + cu - 1) / cu;
+    const long long t = each == 1 ? static_cast<long long>(K / 128) * c.alone + c.besides
+                                  : each * (static_cast<long long>(K / 128) * c.each + c.besides);
+    if (i == 0 || t < least) best = i, least = t;
+  }
+  return best;
+}
+
 template <int kXFormat>
 int dense_launch(const MxArgs& a, hipStream_t stream, const char* name) {
-  if (ceil_div(a.N, 64) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
-  if (a.N <= 16) launch_stream<kXFormat, 8, 1, 1, false>(a, 1, stream);
-  else if (a.N <= 32) launch_stream<kXFormat, 8, 1, 2, false>(a, 1, stream);
-  else if (a.N <= 64 || a.K < kTileMinK) launch_stream<kXFormat, 8, 1, 4, false>(a, ceil_div(a.N, 64), stream);
-  else {
-    using S = MxTile<kXFormat, 2, 2, 4, 4, 3>;
+  const int cu = current_cu_count();
+  if (cu <= 0) return fail(kInvalidValue, "%s: no device", name);
+  if (ceil_div(a.N, 32) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
+  const long long tiles64 = static_cast<long long>(ceil_div(a.M, 64)) * ceil_div(a.N, 64);
+  // The streaming kernel to 16 rows, and while 64 x 64 tiles would leave half of the CUs idle, since
+  // its waves share K (64 rows x 4096 x 7168, 64 tiles: 10.6 against 19.6 us; 128 rows, 128 tiles: 15.3
+  // and 21.6; 64 rows x 9728 x 2560, 152 tiles: 12.8 and 10.1).
+  if (a.N <= 16 || a.K < kTileMinK || tiles64 <= cu / 2) {
+    // To 16 rows as many workgroups as there are (9728 x 2560, 16 rows: 608 of 16 features 7.6 us,
+    // 304 of 32 8.4); beyond, more features a workgroup, which read X less often, as long as
+    // three quarters of the CUs have one (64 rows x 4096 x 7168 with 1 / 2 / 4 sets of 16: 15.7 / 10.6 /
+    // 14.5 us).
+    const int blocks = ceil_div(a.N, 32);
+    const auto enough = [&](int mr) {
+      return a.M % (16 * mr) == 0 && 4LL * (a.M / (16 * mr)) * blocks >= 3LL * cu;
+    };
+    if (a.N <= 16) launch_stream<kXFormat, 4, 1, 1, false>(a, 1, stream);
+    else if (a.N > 32 && enough(4)) launch_stream<kXFormat, 4, 4, 2, false>(a, blocks, stream);
+    else if (a.N > 32 && enough(2)) launch_stream<kXFormat, 4, 2, 2, false>(a, blocks, stream);
+    else launch_stream<kXFormat, 4, 1, 2, false>(a, blocks, stream);
+    return launch_status(name);
+  }
+  const auto go = [&](auto shape) {
+    using S = decltype(shape);
     launch_tile<S, false>(a, ceil_div(a.N, S::BN), stream);
+  };
+  switch (best_tile(a.M, a.N, a.K, cu)) {
+    case 0: go(Tile64<kXFormat>{}); break;
+    case 1: go(Tile128x64<kXFormat>{}); break;
+    case 2: go(Tile128<kXFormat>{}); break;
+    case 3: go(Tile256x128<kXFormat>{}); break;
+    default: go(Tile256<kXFormat>{}); break;
   }
   return launch_status(name);
 }
 
 template <int kXFormat>
-int grouped_launch(const MxArgs& a, hipStream_t stream, const char* name) {
+int grouped_launch(const MxArgs& a, int ep_size, hipStream_t stream, const char* name) {
+  const int cu = current_cu_count();
+  if (cu <= 0) return fail(kInvalidValue, "%s: no device", name);
   const int blocks = ceil_div(a.sorted_len, a.bs);
   if (blocks > 65535) return fail(kNotSupported, "%s: too many blocks (%d)", name, blocks);
-  if (a.bs <= 16) launch_stream<kXFormat, 8, 1, 1, true>(a, blocks, stream);
-  else if (a.bs <= 32) launch_stream<kXFormat, 8, 1, 2, true>(a, blocks, stream);
-  else if (a.K < kTileMinK) launch_stream<kXFormat, 8, 1, 4, true>(a, blocks, stream);
-  else launch_tile<MxTile<kXFormat, 4, 1, 4, 4, 3>, true>(a, blocks, stream);
+  // Workgroups of 128 features that will have rows: the blocks that the local routes (one in ep_size)
+  // fill, at least one for each expert that routes spread evenly would reach.
+  const double local = static_cast<double>(a.N) * a.top_k / ep_size;
+  const double reached = a.experts * (1.0 - __builtin_exp(local * __builtin_log1p(-1.0 / (a.experts + 1e-9))));
+  const double live = reached > local / a.bs ? reached : local / a.bs;
+  const double units = live * ceil_div(a.M, 128);
+  if (a.bs > 32) {
+    if (a.K < kTileMinK) launch_stream<kXFormat, 4, 1, 4, true>(a, blocks, stream);
+    else launch_tile<Tile128x64<kXFormat>, true>(a, blocks, stream);
+    return launch_status(name);
+  }
+  // Short blocks: tiles of 128 x 32 where they fill the CUs, and for long K several times over;
+  // else the streaming kernel, whose waves share K.  Streaming / tiled, MXFP8: 4096 x 7168 over 48 of
+  // 384 experts at 2, 8, 64, 160 tokens 7.8 / 16.8, 29.5 / 41.1, 113 / 115, 155 / 145 us; 7168 x 2048
+  // at 64 tokens 87 / 57; 2816 x 2048 over 64 experts at 3 tokens 17 / 12.5 us.
+  const bool tiled = a.K >= kTileMinK && units >= (a.K >= 4096 ? 5.0 * cu : 1.0 * cu);
+  if (tiled) launch_tile<MxTile<kXFormat, 4, 1, 2, 2, 6>, true>(a, blocks, stream);
+  else if (a.bs > 16) launch_stream<kXFormat, 4, 1, 2, true>(a, blocks, stream);
+  else if (kXFormat == kMxE4M3 && a.M % 32 == 0) launch_stream<kXFormat, 4, 2, 1, true>(a, blocks, stream);
+  else launch_stream<kXFormat, 4, 1, 1, true>(a, blocks, stream);
   return launch_status(name);
 }
 
@@ -551,7 +628,7 @@ PEGA_API int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scale
                                   const int32_t* num_tokens_post_padded, const float* topk_weights,
                                   int sorted_token_ids_len, int moe_block_size, int top_k,
                                   bool mul_topk_weights, int size_m, int size_n, int size_k,
-                                  int local_experts, hipStream_t stream) {
+                                  int local_experts, int ep_size, hipStream_t stream) {
   MxArgs a{w_codes, w_scales, x_codes, x_scales, output, size_n, size_m, size_k, sorted_token_ids,
            expert_ids, num_tokens_post_padded, topk_weights, sorted_token_ids_len, moe_block_size,
            top_k, mul_topk_weights ? 1 : 0, local_experts};
@@ -561,7 +638,7 @@ PEGA_API int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scale
     return fail(kInvalidValue, "mx_grouped_gemm: null pointer");
   if (!(moe_block_size == 8 || (moe_block_size >= 16 && moe_block_size <= 64 && moe_block_size % 16 == 0)))
     return fail(kInvalidValue, "mx_grouped_gemm: block size %d not in {8,16,32,48,64}", moe_block_size);
-  if (top_k <= 0 || local_experts <= 0 || sorted_token_ids_len < 0 ||
+  if (top_k <= 0 || local_experts <= 0 || ep_size <= 0 || sorted_token_ids_len < 0 ||
       static_cast<long long>(size_m) * top_k >= (1LL << 31))
     return fail(kInvalidValue, "mx_grouped_gemm: bad shape top_k=%d experts=%d sorted=%d", top_k,
                 local_experts, sorted_token_ids_len);
@@ -569,6 +646,6 @@ PEGA_API int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scale
   if (static_cast<long long>(size_m) * size_k >= static_cast<long long>(kOutOfRange))
     return fail(kNotSupported, "mx_grouped_gemm: activations over 2 GiB (%d x %d)", size_m, size_k);
   if (size_m == 0 || sorted_token_ids_len == 0) return kSuccess;
-  return x_format == kMxE4M3 ? grouped_launch<kMxE4M3>(a, stream, "mx_grouped_gemm")
-                             : grouped_launch<kMxE2M1>(a, stream, "mx_grouped_gemm");
+  return x_format == kMxE4M3 ? grouped_launch<kMxE4M3>(a, ep_size, stream, "mx_grouped_gemm")
+                             : grouped_launch<kMxE2M1>(a, ep_size, stream, "mx_grouped_gemm");
 }

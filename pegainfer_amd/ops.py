@@ -383,7 +383,7 @@ class KimiMarlinWna16Workspace:
         self.c_tmp = torch.zeros(max(1, c_tmp), dtype=torch.float32, device=device)
 
 
-def _ep_size(routing: KimiMarlinRouting, weight: MarlinInt4Weight, ep_size) -> int:
+def _ep_size(routing: KimiMarlinRouting, weight, ep_size) -> int:
     """GPUs that the routes' experts are spread over: the launch rules expect one route in
     ep_size to be local.  Kimi's share (48 experts, top-8) is one GPU's of eight; any other
     routing is taken to be all local unless the caller says otherwise."""
@@ -913,11 +913,11 @@ def mx_gemm(w: MxTensor, x: MxTensor, y: torch.Tensor) -> None:
 
 def mx_grouped_gemm(routing: KimiMarlinRouting, x: MxTensor, w: MxTensor, topk_weight,
                     output: torch.Tensor, *, top_k: int, mul_topk_weights: bool,
-                    size_m: int) -> None:
+                    size_m: int, ep_size: int = None) -> None:
     """output[sorted_id] = bf16(X[sorted_id / top_k] . W[expert]^T), times topk_weight[sorted_id]
     before the rounding with mul_topk_weights: wna16_gemm on microscaled operands.  w holds the
     experts' weights one after another, [local_experts * N, K] MXFP4.  Rows not routed here are
-    left as they are."""
+    left as they are.  `ep_size`: see _ep_size."""
     _mx_operands(w, x)
     experts = routing.local_experts
     if w.rows % experts != 0:
@@ -935,7 +935,7 @@ def mx_grouped_gemm(routing: KimiMarlinRouting, x: MxTensor, w: MxTensor, topk_w
         routing.num_tokens_post_padded, topk_weight if mul_topk_weights else None)
     _lib.call("pega_mx_grouped_gemm", xc, xs, x.format.value, po, wc, ws, ids, eids, ntp, tw,
               routing.max_padded_tokens, routing.block_size, top_k, bool(mul_topk_weights), size_m,
-              size_n, w.cols, experts, stream)
+              size_n, w.cols, experts, _ep_size(routing, routing, ep_size), stream)
 
 
 # --------------------------------------------------------------------------

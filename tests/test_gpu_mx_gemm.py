@@ -18,23 +18,27 @@ FORMATS = {"fp8": 0, "fp4": 1}
 
 
 def _operand(g, rows, cols, name, spread=3):
-    """Codes and scales of normal rows with uneven blocks, on the GPU, and their values."""
+    """Random codes with uneven blocks' scales, on the GPU, and their values."""
     from pegainfer_amd import ops
-    v = g.standard_normal((rows, cols)) * np.repeat(2.0 ** g.integers(-spread, spread + 1, (rows, cols // 32)), 32, 1)
-    codes, scales = mx_ref.quantize(v, name)
+    if name == "fp8":
+        v = torch.from_numpy(g.standard_normal((rows, cols)).astype(np.float32) * 60)
+        codes = v.to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    else:
+        codes = g.integers(0, 256, (rows, cols // 2)).astype(np.uint8)
+    scales = g.integers(120 - spread, 121 + spread, (rows, cols // 32)).astype(np.uint8)
     return (ops.MxTensor(rows, cols, ops.MxFormat(FORMATS[name]), dev(codes), dev(scales)),
             mx_ref.values(codes, scales, name))
 
 
 def _bounds(x, w, name):
     """want [N, M] and the tolerance."""
-    t = lambda a: torch.from_numpy(np.ascontiguousarray(a))  # noqa: E731
-    want = (t(x) @ t(w).T).numpy()
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    want = (t(x) @ t(w).T).cpu().numpy()
     ax, aw = np.abs(x), np.abs(w)
     peak = lambda a: a.reshape(len(a), -1, 128).max(-1)  # noqa: E731
     steps = x.shape[1] // 128
-    lost = (2.0 ** -11 if name == "fp8" else 2.0 ** -20) * (t(peak(ax)) @ t(peak(aw)).T).numpy()
-    sums = steps * 2.0 ** -23 * (t(ax) @ t(aw).T).numpy()
+    lost = (2.0 ** -11 if name == "fp8" else 2.0 ** -20) * (t(peak(ax)) @ t(peak(aw)).T).cpu().numpy()
+    sums = steps * 2.0 ** -23 * (t(ax) @ t(aw).T).cpu().numpy()
     return want, np.abs(want) * 2.0 ** -8 + lost + sums
 
 
@@ -48,7 +52,9 @@ def _check(got, want, tol, what=""):
     (1, 16, 128), (2, 48, 256), (3, 256, 384), (1, 9728, 2560), (15, 272, 512), (16, 64, 640),
     (17, 80, 1152), (31, 512, 2048), (33, 1408, 128), (64, 4096, 1024), (48, 16, 7168),
     (65, 16, 128), (100, 272, 256), (129, 640, 384), (300, 400, 2560), (128, 256, 640),
-    (257, 2816, 2048), (500, 32, 512), (1000, 1040, 128)])
+    (257, 2816, 2048), (500, 32, 512), (1000, 1040, 128),
+    # the tile shapes, ragged: 64 x 64, 128 x 64, 128 x 128, 256 x 128, 256 x 256
+    (200, 4080, 1152), (300, 4112, 640), (999, 4048, 512), (1001, 7088, 2048), (3990, 4080, 1408)])
 def test_dense(n, m, k, name):
     from pegainfer_amd import ops
     g = np.random.default_rng(n * 31 + m + k)
@@ -117,7 +123,9 @@ def _route(tokens, topk, experts, local, start, bs, seed, lean=False):
     (1, 1, 4, 4, 0, 8, 16, 128), (1, 8, 384, 48, 48, 8, 256, 1024), (5, 2, 8, 4, 4, 8, 48, 384),
     (64, 8, 96, 48, 48, 16, 512, 640), (64, 6, 64, 64, 0, 16, 80, 256), (33, 3, 16, 8, 8, 32, 272, 512),
     (90, 4, 12, 6, 0, 48, 128, 384), (200, 6, 16, 16, 0, 64, 400, 2048), (300, 2, 6, 3, 3, 64, 16, 128),
-    (40, 2, 40, 3, 7, 64, 256, 256)])
+    (40, 2, 40, 3, 7, 64, 256, 256),
+    # blocks of 8 and 32 rows in tiles, K split and not
+    (100, 4, 32, 32, 0, 8, 1040, 640), (400, 8, 32, 32, 0, 32, 1360, 512), (150, 8, 48, 48, 0, 16, 4096, 4096)])
 def test_grouped(tokens, topk, experts, local, start, bs, m, k, name):
     """W13's use (top_k rows a token) and W2's (one row a route, the routing weight applied)."""
     from pegainfer_amd import ops

@@ -166,14 +166,14 @@ def test_mx_gemm_takes_no_rows():
 
 
 GROUPED = [A, A << 1, 0, A << 2, A << 3, A << 4, A << 5, A << 6, A << 7, A << 8, 64, 16, 2, True,
-           4, 32, 256, 3, None]
+           4, 32, 256, 3, 1, None]
 
 
 @pytest.mark.parametrize("at,value,code", [
     (0, None, 1), (1, None, 1), (3, None, 1), (4, None, 1), (5, None, 1), (6, None, 1),
     (7, None, 1), (8, None, 1), (9, None, 1), (2, 2, 1), (10, -1, 1), (11, 24, 1), (11, 0, 1),
     (11, 128, 1), (12, 0, 1), (12, 1 << 30, 1), (14, -1, 1), (15, 40, 801), (16, 192, 801),
-    (16, 0, 1), (17, 0, 1), (3, (A << 2) + 2, 801), (14, 1 << 24, 801)])
+    (16, 0, 1), (17, 0, 1), (18, 0, 1), (3, (A << 2) + 2, 801), (14, 1 << 24, 801)])
 def test_mx_grouped_gemm_refuses(at, value, code):
     args = list(GROUPED)
     args[at] = value
