@@ -321,7 +321,7 @@ enum { PEGA_SHARED_NONE = 0, PEGA_SHARED_BF16 = 1, PEGA_SHARED_INT4 = 2 };
 enum { PEGA_FEW_MAX_SPLITS = 8 };
 
 /* Arguments of pega_moe_few_tokens.  INT4 weights are device packages (the layout of
- * pega_marlin_int4_*; W13 gate columns first).  Plain pointers and sizes; 208 bytes on LP64. */
+ * pega_marlin_int4_*; W13 gate columns first).  Plain pointers and sizes; 224 bytes on LP64. */
 typedef struct pega_moe_few {
     const uint16_t* x;           /* bf16 [tokens][hidden_dim], the normed rows */
     const float* logits;         /* router logits [tokens][n_experts] */
@@ -338,8 +338,10 @@ typedef struct pega_moe_few {
     uint16_t* out;               /* bf16 [tokens][hidden_dim]; may be residual's or x's buffer */
     float* topk_weight;          /* out: [tokens][topk] */
     int32_t* topk_idx;           /* out: [tokens][topk] */
-    uint16_t* act;               /* workspace: bf16 [min(tokens topk, local_experts)][tokens][inter] */
-    uint16_t* act_shared;        /* workspace: bf16 [tokens][shared_inter] */
+    uint16_t* act;               /* workspace: fp16 [min(tokens topk, local_experts)][tokens][inter] */
+    float* act_factors;          /* workspace: [min(tokens topk, local_experts)][inter / 64][16] */
+    uint16_t* act_shared;        /* workspace: fp16 or bf16 [tokens][shared_inter] */
+    float* act_shared_factors;   /* workspace, with an INT4 shared expert: [shared_inter / 64][16] */
     int32_t* slots;              /* workspace: 1 + min(tokens topk, local_experts) */
     float* partials;             /* workspace: PEGA_FEW_MAX_SPLITS * tokens * hidden_dim */
     uint32_t* counters;          /* workspace: hidden_dim / 64, zero before the first call; every
@@ -357,9 +359,11 @@ typedef struct pega_moe_few {
  *   topk_idx, topk_weight = the select entry's, bit for bit;
  *   out[t] = bf16(residual[t] + routed_scale * sum over t's local routes of weight *
  *            (silu(x G_e^T) * (x U_e^T)) D_e^T + the shared expert's rows).
- * INT4 weights count as (nibble - 8) * scale unrounded; the SwiGLU rows, times weight and
- * routed_scale, are rounded to bf16 once, out once, and all sums are fp32, in an order that the
- * sizes and the routing decide.  Experts without a route are not read.  Calls that share a
+ * INT4 weights count as (nibble - 8) * scale unrounded; x goes into the INT4 products exactly down to
+ * 2^-25 of its row's largest magnitude (to 2^-40 of it below); the SwiGLU rows, times weight and
+ * routed_scale, are rounded once to fp16 with a scale for each 64 (bf16 in front of a bf16 down
+ * projection), out once, and all sums are fp32, in an order that the sizes and the routing decide.  A
+ * row of x with an infinity or a NaN gives a row of NaN; other rows are as without it.  Experts without a route are not read.  Calls that share a
  * workspace must not overlap (two captured graphs that may run at once need one each); nothing is
  * kept in it from one call to the next but the zeroed counters.  At most 16 tokens, topk 32, 512
  * local experts, 1024 experts, sizes multiples of 64, 16-byte aligned buffers (801 otherwise). */

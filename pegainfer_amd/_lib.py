@@ -36,7 +36,7 @@ class MoeFew(ctypes.Structure):
     _fields_ = [(n, _P) for n in (
         "x", "logits", "bias", "w13", "w13_scales", "w2", "w2_scales", "shared_w13",
         "shared_w13_scales", "shared_w2", "shared_w2_scales", "residual", "out", "topk_weight",
-        "topk_idx", "act", "act_shared", "slots", "partials", "counters")] + [
+        "topk_idx", "act", "act_factors", "act_shared", "act_shared_factors", "slots", "partials", "counters")] + [
         ("route_scale", _F), ("routed_scale", _F)] + [(n, _I) for n in (
             "softmax", "shared_kind", "tokens", "hidden_dim", "inter", "shared_inter", "n_experts",
             "local_experts", "global_start", "topk")]

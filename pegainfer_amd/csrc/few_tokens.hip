@@ -9,28 +9,35 @@
 // a shared expert in bf16, in INT4, or none.  At these sizes the layer is a stream of weights cut
 // into eight short launches by the general path; here
 //
-//   launch 1   a workgroup per gate/up tile pair of the shared expert, then of each expert slot.
-//              A routed workgroup runs the select itself (every one of them: 3 to 4 us that the
-//              shared expert's workgroups, which need no routing, cover), takes the slot-th distinct
-//              local expert in id order, or ends.  The routing weight and routed_scale are
-//              multiplied into the SwiGLU rows, which are written for all tokens: zeros where the
-//              token has no route to the expert.
+//   launch 1   workgroups for the shared expert's gate/up tile pairs, and others for the routed
+//              experts.  A routed one runs the select itself (each of them does: 4 to 5 us, which the
+//              shared expert's workgroups, that need no routing, cover), and then takes gate/up tile
+//              pairs of the distinct local experts, in id order, in turn with the others.  The routing
+//              weight and routed_scale are multiplied into the SwiGLU rows, which are written for
+//              all tokens: zeros where the token has no route to the expert.
 //   launch 2   so the second products are one sum over the concatenated rows of all slots and the
 //              shared expert.  That list of 32-k groups, priced by its bytes, is cut into equal
 //              shares for the waves of `splits` workgroups per 64 output columns.  With several
 //              workgroups, each leaves fp32 sums and counts itself in, and the last one adds them
 //              in their order.
 //
-// An MFMA's 16 rows are the tokens themselves, so rows are never gathered.  INT4 weights: nibble v
-// of a word becomes the bf16 16 + v by a shift and one v_and_or (mantissa bits 3..6), a constant
-// -24 operand takes 24 * sum(x) off in the same accumulators' start value, and the group's fp32 sum
-// times its scale is added to the column's: about 1 VALU instruction a weight and no rounding of
-// q * s (the general kernels round it to bf16; the results differ by that).  Where 16 * x or 8 * x
-// passes fp32's range, and with infinite activations, such a sum is infinite or NaN: a wave that
-// ends with one forms its sums again from (v - 8) / 256, and takes those that were not finite.
+// INT4 products without a dequantisation: a nibble masked out of its word is the fp16 v 2^-24 (or
+// v 2^-20, four bits further up), so a mask a pair makes v_mfma_f32_16x16x32_f16 operands of whole
+// words, 5 instructions for 8 weights.  The activations go in as fp16 scaled by a power of two (a
+// row's largest to 2^14 .. 2^15; exact down to 2^-25 of it, and to 2^-40 of it below), the second half
+// of a fragment's k divided by 16; a constant operand of -8 steps starts the sums, and a 32-k
+// group's fp32 sum times its scale is added to the column's.  Weights count as (nibble - 8) * scale
+// unrounded (the general kernels round that product to bf16; the results differ by it).
 //
-// Roundings: the SwiGLU rows (with their weights) once to bf16, which the matrix instructions
-// take; out once.  Everything between is fp32.
+// An MFMA's 16 rows are the tokens themselves, never gathered.  With R = 4 (8) token rows, 4 (2)
+// groups share an instruction's rows: group g's instruction has the tokens in rows R g .. and zeros
+// elsewhere, the sums of all of them land in one accumulator, and the scale is a lane's own group's.
+// Then a scale is applied to 4 sums a lane instead of 16, and scales and activations are loaded
+// once per 4 (2) groups.
+//
+// Roundings: the SwiGLU rows, with their weights, once to fp16 with a scale for each 64 (bf16 in front of
+// a bf16 down projection); out once.  Everything between is fp32.  A row with an infinite or NaN
+// activation gives NaN.
 #include <type_traits>
 
 #include "common.h"
@@ -41,21 +48,30 @@ namespace pega {
 namespace {
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_t;
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8_t;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4_t;
 
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kMaxTokens = 16, kMaxTopk = 32, kMaxLocal = 512;
 constexpr int kSlotDwords = 320;  // one 32-k group of a 64-column tile, as wna16.hip's slots
 constexpr int kStream = 2;        // non-temporal: bytes read once
+constexpr uint32_t kOutOfRange = 0x80000000u;  // voffset that fails every range check
 
 struct FewArgs {
   pega_moe_few p;
   int sh_units, tiles, splits, shared_cost;
+  int routed_first, routed;  // routed workgroups before the shared expert's, and in all
 };
 
+// The base and the size in SGPRs: a resource that the compiler takes for a lane's own costs a loop
+// around every load.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0),
-                                           static_cast<int>(bytes), 0x00020000);
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(a)));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32)));
+  return __builtin_amdgcn_make_buffer_rsrc(
+      reinterpret_cast<void*>((static_cast<uint64_t>(hi) << 32) | lo), static_cast<short>(0),
+      __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), 0x00020000);
 }
 __device__ __forceinline__ u32x4_t load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
   return __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(voff), static_cast<int>(soff), 0);
@@ -63,157 +79,193 @@ __device__ __forceinline__ u32x4_t load16(__amdgpu_buffer_rsrc_t r, uint32_t vof
 __device__ __forceinline__ u32x4_t load16_once(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
   return __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(voff), static_cast<int>(soff), kStream);
 }
-__device__ __forceinline__ bf16x8_t as_bf16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+__device__ __forceinline__ f16x8_t as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   u32x4_t v = {a, b, c, d};
-  return __builtin_bit_cast(bf16x8_t, v);
+  return __builtin_bit_cast(f16x8_t, v);
 }
 __device__ __forceinline__ floatx4_t mfma16(bf16x8_t a, bf16x8_t b, floatx4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-
-// Two bf16 of a word's nibbles at bits `kBit` and kBit + 16: 16 + v, or (v - 8) / 256 with kWide.
-template <int kBit, bool kWide>
-__device__ __forceinline__ uint32_t nibble_pair(uint32_t x) {
-  if constexpr (kWide)
-    return pack_bf16x2((static_cast<float>((x >> kBit) & 15u) - 8.0f) * 0x1p-8f,
-                       (static_cast<float>((x >> (kBit + 16)) & 15u) - 8.0f) * 0x1p-8f);
-  const uint32_t y = kBit < 3 ? x << (3 - kBit) : x >> (kBit - 3);
-  return (y & 0x00780078u) | 0x41804180u;
+__device__ __forceinline__ floatx4_t mfma16(f16x8_t a, f16x8_t b, floatx4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// INT4 weights of NT 64-column tiles, and the activations, over 32-k groups [g0, g1): every lane's
-// columns are 32 (lane % 16 / 8) + 8 j + lane % 8 of a tile, j = 0..3, its sums tokens
-// 4 (lane / 16) .. + 3.  A wave reads whole 512-byte tiles (one 16-byte load a lane: word row
-// lane % 32 of k-tile lane / 32) and transposes them through its LDS slots, a group ahead of its
-// use, as wna16.hip's decode kernel does; the activations' 16 bytes (k 16 kt + 8 hf ..) swap their
-// middle halves between the lanes of the two k halves to follow the words' k order.
-template <int NT>
-struct Int4View {
-  __amdgpu_buffer_rsrc_t w, s, a;
-  uint32_t w_voff[NT], s_voff[NT], a_voff;
-  uint32_t w_step, s_step;
-};
-
-template <int NT>
-__device__ __forceinline__ Int4View<NT> int4_view(const uint8_t* q, const uint16_t* scales, int N,
-                                                  int K, const int (&tile)[NT], const uint16_t* act,
-                                                  int tokens) {
-  const int lane = threadIdx.x & 63;
-  const int n16 = lane & 15, kb = lane >> 4;
-  const uint32_t n_tiles = static_cast<uint32_t>(N) >> 6;
-  Int4View<NT> v;
-  v.w = make_rsrc(q, static_cast<uint32_t>(N) * static_cast<uint32_t>(K) / 2u);
-  v.s = make_rsrc(scales, static_cast<uint32_t>(K >> 5) * static_cast<uint32_t>(N) * 2u);
-  v.a = make_rsrc(act, static_cast<uint32_t>(tokens) * static_cast<uint32_t>(K) * 2u);
-  v.w_step = n_tiles * 1024u;
-  v.s_step = static_cast<uint32_t>(N) * 2u;
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    v.w_voff[i] = static_cast<uint32_t>(lane >> 5) * n_tiles * 512u +
-                  static_cast<uint32_t>(tile[i]) * 512u + 16u * (lane & 31);
-    v.s_voff[i] = static_cast<uint32_t>(tile[i]) * 128u + 16u * (n16 & 7) + 8u * (n16 >> 3);
-  }
-  // rows past the last token are past the range: zeros
-  v.a_voff = static_cast<uint32_t>(n16) * static_cast<uint32_t>(K) * 2u + 16u * kb;
+// A value that the compiler takes for a new one.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
   return v;
 }
 
-template <int NT, int D, bool kWide>
-__device__ __forceinline__ void int4_groups(floatx4_t (&acc)[NT][4], const Int4View<NT>& v, int g0,
-                                            int g1, uint32_t* slots /* [2][NT][kSlotDwords] */) {
-  static_assert(D % 2 == 0, "the two transpose slots alternate with the ring position");
+// 2^e as a float, e in -126 .. 127.
+__device__ __forceinline__ float pow2(int e) {
+  return __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23);
+}
+// The exponent of a magnitude's float bits (of an infinity or a NaN 128, of the smallest -127).
+__device__ __forceinline__ int exponent(uint32_t bits) { return static_cast<int>(bits >> 23) - 127; }
+
+// Where the bytes of a 64-column tile of an INT4 operand, and the activations that meet it, are.  Lane
+// columns of the tile are 32 (lane % 16 / 8) + 8 j + lane % 8, j = 0..3.  kScaled: the activations are
+// fp16 with a factor for each 64 columns and token (launch 2); otherwise bf16 rows, which the lane
+// turns into fp16 by its row's factor (launch 1).
+struct Int4View {
+  __amdgpu_buffer_rsrc_t w, s, a, f;
+  uint32_t w_voff, s_voff, a_voff, f_voff;
+  uint32_t w_step, s_step;
+};
+
+// R: token rows of an instruction that a group takes (4, 8 or 16).
+template <int R>
+__device__ __forceinline__ Int4View int4_view(const uint8_t* q, const uint16_t* scales, int N, int K,
+                                              int tile, const void* act, const float* factors,
+                                              int tokens) {
+  const int lane = fresh(threadIdx.x & 63);
+  const int n16 = lane & 15, kb = lane >> 4;
+  const uint32_t n_tiles = static_cast<uint32_t>(N) >> 6;
+  Int4View v;
+  v.w = make_rsrc(q, static_cast<uint32_t>(N) * static_cast<uint32_t>(K) / 2u);
+  v.s = make_rsrc(scales, static_cast<uint32_t>(K >> 5) * static_cast<uint32_t>(N) * 2u);
+  v.a = make_rsrc(act, static_cast<uint32_t>(tokens) * static_cast<uint32_t>(K) * 2u);
+  v.f = make_rsrc(factors, static_cast<uint32_t>(K >> 6) * 64u);
+  v.w_step = n_tiles * 1024u;
+  v.s_step = static_cast<uint32_t>(N) * 2u;
+  v.w_voff = static_cast<uint32_t>(lane >> 5) * n_tiles * 512u + static_cast<uint32_t>(tile) * 512u +
+             16u * (lane & 31);
+  v.s_voff = static_cast<uint32_t>(tile) * 128u + 16u * (n16 & 7) + 8u * (n16 >> 3);
+  // rows past the last token read zeros: past the range where R tokens end it, by the test otherwise
+  v.a_voff = n16 % R < tokens
+                 ? static_cast<uint32_t>(n16 % R) * static_cast<uint32_t>(K) * 2u + 16u * kb
+                 : kOutOfRange;
+  v.f_voff = static_cast<uint32_t>((4 * kb) % R) * 4u;
+  return v;
+}
+
+// 32-k groups [g0, g1) of a tile into acc: element e of lane (n16, q) sums, over the groups of its
+// place (4 q) / R in each set of 16 / R, token (4 q) % R + e.  A wave reads whole 512-byte tiles (one
+// 16-byte load a lane: word row lane % 32 of k-tile lane / 32) and transposes them through its LDS slots,
+// one ahead of their use, as wna16.hip's decode kernel does; the activations' 16 bytes (k 16 kt +
+// 8 hf ..) swap their middle halves between the lanes of the two k halves to follow the words' k order.
+// row_factor: of the lane's activation row, without kScaled.
+// D: groups in flight, a multiple of 16 / R.
+template <int R, int D, bool kScaled>
+__device__ __forceinline__ void int4_groups(floatx4_t (&acc)[4], const Int4View& v, int g0, int g1,
+                                            float row_factor, uint32_t* slots /* [2][kSlotDwords] */) {
+  constexpr int G = 16 / R;  // groups of a set
+  static_assert(D % G == 0 && D % 2 == 0, "whole sets, and two transpose slots in turn");
   if (g0 >= g1) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = fresh(threadIdx.x & 63);
   const int c = lane & 31, h = lane >> 5;
   const int n16 = lane & 15, kb = lane >> 4;
   const int cc = n16 & 7, a2 = n16 >> 3, kt = kb >> 1, hf = kb & 1;
+  const int row_group = n16 / R, sum_group = (4 * kb) / R;
   uint32_t* wr = slots + h * 160 + c;
   const uint32_t* rd = slots + kt * 160 + 64 * a2 + 4 * cc + 2 * hf;
-  struct Regs {
-    u32x4_t w[NT];
-    uint32_t s[NT][2];
-    u32x4_t a;
+  struct Set {
+    uint32_t s[2];
+    u32x4_t a, f;
   };
-  const auto load = [&](Regs& r, int g) {
+  const auto load_words = [&](u32x4_t& w, int g) {
+    w = load16_once(v.w, v.w_voff, static_cast<uint32_t>(min(g, g1 - 1)) * v.w_step);
+  };
+  // a set's scales and factors are those of the lane's own group; groups past the end bring the last
+  // one's, and activations of zero
+  const auto load_set = [&](Set& r, int g) {
+    const uint32_t mine = static_cast<uint32_t>(min(g + sum_group, g1 - 1));
+    const auto s = __builtin_amdgcn_raw_buffer_load_b64(
+        v.s, static_cast<int>(v.s_voff + mine * v.s_step), 0, 0);
+    r.s[0] = s[0];
+    r.s[1] = s[1];
+    const int row = g + row_group;
+    r.a = load16(v.a, row < g1 ? v.a_voff + static_cast<uint32_t>(row) * 64u : kOutOfRange, 0);
+    if (kScaled) r.f = load16(v.f, v.f_voff + (mine >> 1) * 64u, 0);
+  };
+  const auto write = [&](const u32x4_t& w, int par) {
+    uint32_t* p = wr + par * kSlotDwords;
+    p[0] = w[0];
+    p[32] = w[1];
+    p[64] = w[2];
+    p[96] = w[3];
+  };
+  // -8 steps of 2^-24 for the first half of a fragment's k, of 2^-20 for the second
+  const f16x8_t bias = as_f16x8(0x80088008u, 0x80088008u, 0x80808080u, 0x80808080u);
+  // bf16 rows become fp16 (exact but for the row's smallest values, which are cut off), k 8 .. 15 of
+  // each 16, which meet the v 2^-20 and come from the lanes of the second k half, divided by 16 as
+  // launch 1 leaves its fp16 rows
+  const float k = hf ? row_factor * 0.0625f : row_factor;
+  const auto activations = [&](u32x4_t a) {
+    if constexpr (!kScaled) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      r.w[i] = load16_once(v.w, v.w_voff[i], static_cast<uint32_t>(g) * v.w_step);
-      const auto s = __builtin_amdgcn_raw_buffer_load_b64(
-          v.s, static_cast<int>(v.s_voff[i]), static_cast<int>(static_cast<uint32_t>(g) * v.s_step), kStream);
-      r.s[i][0] = s[0];
-      r.s[i][1] = s[1];
+      for (int i = 0; i < 4; ++i)
+        a[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf_lo(a[i]) * k, bf_hi(a[i]) * k));
     }
-    r.a = load16(v.a, v.a_voff, static_cast<uint32_t>(g) * 64u);
+    const auto x0 = __builtin_amdgcn_permlane16_swap(a[0], a[2], false, false);
+    const auto x1 = __builtin_amdgcn_permlane16_swap(a[1], a[3], false, false);
+    return u32x4_t{x0[0], x1[0], x0[1], x1[1]};
   };
-  const auto write = [&](const Regs& r, int par) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      uint32_t* p = wr + (par * NT + i) * kSlotDwords;
-      p[0] = r.w[i][0];
-      p[32] = r.w[i][1];
-      p[64] = r.w[i][2];
-      p[96] = r.w[i][3];
-    }
-  };
-  // -24 in every element: the 16 + v that a nibble stands for less its own v - 8
-  const bf16x8_t bias = as_bf16x8(0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u);
-  const auto compute = [&](const Regs& r, int par) {
-    const auto x0 = __builtin_amdgcn_permlane16_swap(r.a[0], r.a[2], false, false);
-    const auto x1 = __builtin_amdgcn_permlane16_swap(r.a[1], r.a[3], false, false);
-    const bf16x8_t A = as_bf16x8(x0[0], x1[0], x0[1], x1[1]);
-    floatx4_t start = {};
-    if (!kWide) start = mfma16(A, bias, start);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const uint32_t* p = rd + (par * NT + i) * kSlotDwords;
-      const uint32_t wa0 = p[0], wa1 = p[1], wb0 = p[32], wb1 = p[33];
-      const auto frag0 = [&](uint32_t w0, uint32_t w1) {
-        return as_bf16x8(nibble_pair<0, kWide>(w0), nibble_pair<0, kWide>(w1),
-                         nibble_pair<4, kWide>(w0), nibble_pair<4, kWide>(w1));
-      };
-      const auto frag1 = [&](uint32_t w0, uint32_t w1) {
-        return as_bf16x8(nibble_pair<8, kWide>(w0), nibble_pair<8, kWide>(w1),
-                         nibble_pair<12, kWide>(w0), nibble_pair<12, kWide>(w1));
-      };
-      const floatx4_t t0 = mfma16(A, frag0(wa0, wa1), start), t1 = mfma16(A, frag1(wa0, wa1), start);
-      const floatx4_t t2 = mfma16(A, frag0(wb0, wb1), start), t3 = mfma16(A, frag1(wb0, wb1), start);
-      const float s0 = bf_lo(r.s[i][0]), s1 = bf_hi(r.s[i][0]), s2 = bf_lo(r.s[i][1]), s3 = bf_hi(r.s[i][1]);
-      const auto add = [](float t, float s, float a) {
-        return kWide ? __builtin_fmaf(t * s, 256.0f, a) : __builtin_fmaf(t, s, a);
-      };
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[i][0][e] = add(t0[e], s0, acc[i][0][e]);
-        acc[i][1][e] = add(t1[e], s1, acc[i][1][e]);
-        acc[i][2][e] = add(t2[e], s2, acc[i][2][e]);
-        acc[i][3][e] = add(t3[e], s3, acc[i][3][e]);
-      }
-    }
-  };
-  Regs slot[D];
+  u32x4_t words[D];
+  Set set, next;
+  load_set(set, g0);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int q = 0; q < D; ++q) {
-    load(slot[q], min(g0 + q, g1 - 1));
+    load_words(words[q], g0 + q);
     __builtin_amdgcn_sched_barrier(0);
   }
-  int g = g0;
-  write(slot[0], 0);
-  for (; g + D <= g1; g += D) {
+  write(words[0], 0);
+  for (int g = g0; g < g1; g += D) {
 #pragma unroll
-    for (int q = 0; q < D; ++q) {
-      write(slot[(q + 1) % D], (q + 1) & 1);
-      compute(slot[q], q & 1);
-      load(slot[q], min(g + q + D, g1 - 1));
+    for (int q = 0; q < D; q += G) {
+      if (q != 0 && g + q >= g1) break;
+      const u32x4_t x = activations(set.a);
+      floatx4_t start = {};
+      start = mfma16(__builtin_bit_cast(f16x8_t, x), bias, start);
+      floatx4_t t[4] = {start, start, start, start};
+      load_set(next, g + q + G);
       __builtin_amdgcn_sched_barrier(0);
-    }
-  }
 #pragma unroll
-  for (int q = 0; q < D - 1; ++q) {
-    if (g + q < g1) {
-      if (q + 1 < D - 1 && g + q + 1 < g1) write(slot[q + 1], (q + 1) & 1);
-      compute(slot[q], q & 1);
+      for (int u = 0; u < G; ++u) {
+        const int at = q + u;
+        write(words[(at + 1) % D], (at + 1) & 1);
+        f16x8_t A = __builtin_bit_cast(f16x8_t, x);
+        if (G > 1) {
+          const uint32_t keep = row_group == u ? ~0u : 0u;
+          A = as_f16x8(x[0] & keep, x[1] & keep, x[2] & keep, x[3] & keep);
+        }
+        const uint32_t* p = rd + (at & 1) * kSlotDwords;
+        const uint32_t wa0 = p[0], wa1 = p[1], wb0 = p[32], wb1 = p[33];
+        const auto frag = [](uint32_t w0, uint32_t w1) {
+          return as_f16x8(w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u);
+        };
+        t[0] = mfma16(A, frag(wa0, wa1), t[0]);
+        t[1] = mfma16(A, frag(wa0 >> 8, wa1 >> 8), t[1]);
+        t[2] = mfma16(A, frag(wb0, wb1), t[2]);
+        t[3] = mfma16(A, frag(wb0 >> 8, wb1 >> 8), t[3]);
+        load_words(words[at], g + at + D);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const float s[4] = {bf_lo(set.s[0]), bf_hi(set.s[0]), bf_lo(set.s[1]), bf_hi(set.s[1])};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t f = set.f[e];  // (a bit cast of the element itself takes element 0)
+          const float sum = kScaled ? t[j][e] * __builtin_bit_cast(float, f) : t[j][e];
+          acc[j][e] = __builtin_fmaf(sum, s[j], acc[j][e]);
+        }
+      set = next;
     }
   }
+}
+
+// The sums of a set's groups, together: afterwards lanes 0 .. 4 R - 1 have the token rows' totals.
+template <int R>
+__device__ __forceinline__ void add_places(floatx4_t (&acc)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (R == 4) acc[j][e] += __shfl_xor(acc[j][e], 16);
+      if (R <= 8) acc[j][e] += __shfl_xor(acc[j][e], 32);
+    }
 }
 
 // bf16 weights: MR sets of 16 rows (their byte offsets per lane in w_voff, for row lane / 4 of the
@@ -265,29 +317,6 @@ __device__ __forceinline__ void bf16_steps(floatx4_t* acc, __amdgpu_buffer_rsrc_
     if (s + q < s1) compute(slot[q]);
 }
 
-template <typename... F>
-__device__ __forceinline__ bool wave_any_nan(F... sums) {
-  float t = 0.0f;
-  ((t = __builtin_fmaf(sums, 0.0f, t)), ...);
-  return __ballot(t != t) != 0;
-}
-__device__ __forceinline__ bool any_nan(const floatx4_t (&a)[4]) {
-  bool r = false;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) r |= wave_any_nan(a[j][0], a[j][1], a[j][2], a[j][3]);
-  return r;
-}
-
-// The elements of a that are infinite or NaN, from b (a row's sums depend on that row alone, so
-// the other rows keep theirs).
-__device__ __forceinline__ void take_not_finite(floatx4_t (&a)[4], const floatx4_t (&b)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (!(__builtin_fabsf(a[j][e]) < __builtin_inff())) a[j][e] = b[j][e];
-}
-
 __device__ __forceinline__ float silu_mul(float g, float u) {
   return g / (1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f)) * u;
 }
@@ -298,25 +327,43 @@ __device__ __forceinline__ int sum_lane(int t, int col) {
 }
 
 // ---------------------------------------------------------------- launch 1
-// TR: token rows in fours (the lanes that hold them: 16 TR).
-template <int NS, bool kDsv2, int TR>
+// The largest magnitude (its float bits) of row t of x, by one wave.
+__device__ __forceinline__ uint32_t row_amax(const uint16_t* x, int t, int H) {
+  const int lane = threadIdx.x & 63;
+  const uint16_t* row = x + static_cast<long long>(t) * H;
+  uint32_t m = 0;
+  for (int v = lane; v < H / 8; v += 64) {
+    const uint4 q = *reinterpret_cast<const uint4*>(row + 8 * v);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, max((w[i] << 16) & 0x7fff0000u, w[i] & 0x7fff0000u));
+  }
+  return wave_reduce_u32(m, MaxU32{});
+}
+
+template <int NS, bool kDsv2, int R>
 __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
   const pega_moe_few& p = f.p;
   __shared__ union {
-    uint32_t tr[kWaves][2 * 2 * kSlotDwords];
-    floatx4_t red[kWaves][8][16 * TR];
+    uint32_t tr[kWaves][2 * kSlotDwords];
+    floatx4_t red[kWaves][4][4 * R];
   } lds;
   __shared__ int s_idx[kMaxTokens * kMaxTopk];
   __shared__ float s_w[kMaxTokens * kMaxTopk];
   __shared__ uint32_t s_mask[kMaxLocal];
-  __shared__ float s_tok[kMaxTokens];  // a token's factor for this slot's rows
-  __shared__ bool s_in[kMaxTokens];    // whether it has a route to the slot's expert
+  __shared__ uint16_t s_list[kMaxLocal];
+  __shared__ float s_tok[kMaxTokens];   // a token's factor for this slot's rows
+  __shared__ bool s_in[kMaxTokens];     // whether it has a route to the slot's expert
+  __shared__ uint32_t s_amax[kMaxTokens];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int T = p.tokens, H = p.hidden_dim;
-  int unit = blockIdx.x;
+  // routed workgroups that start with the launch come first: their router logits are then asked
+  // for before the shared expert's weights fill the memory's queues (10 against 5 us for the select)
+  int unit = static_cast<int>(blockIdx.x) - f.routed_first;
+  const bool shared = unit >= 0 && unit < f.sh_units;
 
-  if (p.shared_kind == PEGA_SHARED_BF16 && unit < f.sh_units) {
+  if (shared && p.shared_kind == PEGA_SHARED_BF16) {
     // 8 gate rows and their 8 up rows for all tokens, K shared by the waves
     const int inter = p.shared_inter, j0 = unit * 8;
     const int steps = H >> 5;
@@ -330,7 +377,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     floatx4_t acc[1] = {};
     bf16_steps<1, 8>(acc, wr, w_voff, ar, static_cast<uint32_t>(lane & 15) * row_bytes + 16u * (lane >> 4),
                      (steps * wave) / kWaves, (steps * (wave + 1)) / kWaves);
-    if (lane < 16 * TR) lds.red[wave][0][lane] = acc[0];
+    if (lane < 4 * R) lds.red[wave][0][lane] = acc[0];
     __syncthreads();
     if (tid < T * 8) {
       const int t = tid >> 3, c = tid & 7;
@@ -345,20 +392,15 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     return;
   }
 
-  const uint8_t* q = static_cast<const uint8_t*>(p.shared_w13);
-  const uint16_t* sc = p.shared_w13_scales;
-  uint16_t* act = p.act_shared;
-  int inter = p.shared_inter, tile = unit;
-  if (unit < f.sh_units) {  // the shared expert in INT4: every token, weight 1
-    if (tid < kMaxTokens) {
-      s_tok[tid] = 1.0f;
-      s_in[tid] = true;
-    }
-  } else {
-    unit -= f.sh_units;
-    const int slot = unit / f.tiles;
-    tile = unit - slot * f.tiles;
-    inter = p.inter;
+  for (int t = kWaves - 1 - wave; t < T; t += kWaves) {  // the select starts from wave 0
+    const uint32_t m = row_amax(p.x, t, H);
+    if (lane == 0) s_amax[t] = m;
+  }
+  int live = 1, first = unit, step = 1 << 30;  // this workgroup's tile pairs
+  const int inter = shared ? p.shared_inter : p.inter;
+  const int tiles = inter >> 6;
+  if (!shared) {
+    const int mine = unit < 0 ? static_cast<int>(blockIdx.x) : unit + f.routed_first - f.sh_units;
     for (int i = tid; i < p.local_experts; i += kThreads) s_mask[i] = 0;
     for (int t = wave; t < T; t += kWaves) {
       int id;
@@ -373,82 +415,103 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
       if (e >= 0 && e < p.local_experts) atomicOr(&s_mask[e], 1u << (r / p.topk));
     }
     __syncthreads();
-    // the distinct local experts in id order; this workgroup's is number `slot`
-    int expert = -1, seen = 0;
+    // the distinct local experts in id order: the slots
+    live = 0;
     for (int base = 0; base < p.local_experts; base += 64) {
       const bool has = base + lane < p.local_experts && s_mask[base + lane] != 0;
-      uint64_t m = __ballot(has);
-      const int n = __popcll(m);
-      if (unit == 0 && wave == 0 && has)
-        p.slots[1 + seen + __popcll(m & ((1ull << lane) - 1))] = base + lane;
-      if (expert < 0 && slot - seen < n) {
-        for (int i = slot - seen; i > 0; --i) m &= m - 1;
-        expert = base + __builtin_ctzll(m);
-      }
-      seen += n;
+      const uint64_t m = __ballot(has);
+      if (wave == 0 && has)
+        s_list[live + __popcll(m & ((1ull << lane) - 1))] = static_cast<uint16_t>(base + lane);
+      live += __popcll(m);
     }
-    if (unit == 0) {
-      if (tid == 0) p.slots[0] = seen;
+    if (mine == 0) {
+      __syncthreads();
+      if (tid == 0) p.slots[0] = live;
+      for (int i = tid; i < live; i += kThreads) p.slots[1 + i] = s_list[i];
       for (int r = tid; r < routes; r += kThreads) {
         p.topk_idx[r] = s_idx[r];
         p.topk_weight[r] = s_w[r];
       }
     }
-    if (expert < 0) return;
-    expert = __builtin_amdgcn_readfirstlane(expert);
-    if (tid < kMaxTokens) {
-      float w = 0.0f;
-      if (tid < T)
-        for (int k = 0; k < p.topk; ++k)
-          if (s_idx[tid * p.topk + k] - p.global_start == expert) w += s_w[tid * p.topk + k];
-      s_tok[tid] = w * p.routed_scale;
-      s_in[tid] = ((s_mask[expert] >> tid) & 1u) != 0;
-    }
-    const long long elems = 2LL * inter * H;
-    q = p.w13 + expert * (elems / 2);
-    sc = p.w13_scales + expert * (elems / 32);
-    act = p.act + static_cast<long long>(slot) * T * inter;
-  }
-  const int groups = H >> 5;
-  const int pair[2] = {tile, tile + (inter >> 6)};
-  const Int4View<2> v = int4_view<2>(q, sc, 2 * inter, H, pair, p.x, T);
-  const int g0 = (groups * wave) / kWaves, g1 = (groups * (wave + 1)) / kWaves;
-  floatx4_t acc[2][4] = {};
-  int4_groups<2, 4, false>(acc, v, g0, g1, lds.tr[wave]);
-  if (__builtin_expect(any_nan(acc[0]) || any_nan(acc[1]), 0)) {
-    floatx4_t again[2][4] = {};
-    int4_groups<2, 2, true>(again, v, g0, g1, lds.tr[wave]);
-    take_not_finite(acc[0], again[0]);
-    take_not_finite(acc[1], again[1]);
-  }
-  __syncthreads();  // the transpose slots become the sums' place
-  if (lane < 16 * TR) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) lds.red[wave][4 * i + j][lane] = acc[i][j];
+    first = mine;
+    step = f.routed;
   }
   __syncthreads();
-  for (int o = tid; o < T * 64; o += kThreads) {
-    const int t = o >> 6, col = o & 63, j = (col >> 3) & 3, l = sum_lane(t, col);
-    float g = 0.0f, u = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      g += lds.red[w][j][l][t & 3];
-      u += lds.red[w][4 + j][l][t & 3];
+  const int my_token = (lane & 15) % R;
+  const float row_factor = my_token < T ? pow2(min(14 - exponent(s_amax[my_token]), 127)) : 0.0f;
+  // waves 0 to 3 share K of the gate tile, 4 to 7 of the up tile
+  constexpr int kShares = kWaves / 2;
+  const int groups = H >> 5, half = wave / kShares, share = wave % kShares;
+  const int g0 = (groups * share) / kShares, g1 = (groups * (share + 1)) / kShares;
+  for (int at = first; at < live * tiles; at += step) {
+    const int slot = at / tiles, tile = at - slot * tiles;
+    const uint8_t* q = static_cast<const uint8_t*>(p.shared_w13);
+    const uint16_t* sc = p.shared_w13_scales;
+    uint16_t* act = p.act_shared;
+    float* factors = p.act_shared_factors;
+    if (shared) {
+      if (tid < kMaxTokens) {
+        s_tok[tid] = 1.0f;
+        s_in[tid] = true;
+      }
+    } else {
+      const int expert = s_list[slot];
+      if (tid < T) {
+        float w = 0.0f;
+        for (int k = 0; k < p.topk; ++k)
+          if (s_idx[tid * p.topk + k] - p.global_start == expert) w += s_w[tid * p.topk + k];
+        s_tok[tid] = w * p.routed_scale;
+        s_in[tid] = ((s_mask[expert] >> tid) & 1u) != 0;
+      }
+      const long long elems = 2LL * inter * H;
+      q = p.w13 + expert * (elems / 2);
+      sc = p.w13_scales + expert * (elems / 32);
+      act = p.act + static_cast<long long>(slot) * T * inter;
+      factors = p.act_factors + static_cast<long long>(slot) * tiles * kMaxTokens;
     }
-    act[static_cast<long long>(t) * inter + tile * 64 + col] =
-        s_in[t] ? f2bf(silu_mul(g, u) * s_tok[t]) : static_cast<uint16_t>(0);
+    const Int4View v = int4_view<R>(q, sc, 2 * inter, H, tile + half * tiles, p.x, nullptr, T);
+    floatx4_t acc[4] = {};
+    int4_groups<R, 8, false>(acc, v, g0, g1, row_factor, lds.tr[wave]);
+    add_places<R>(acc);
+    __syncthreads();  // the transpose slots become the sums' place
+    // the lane read anew: what is computed from it would otherwise sit in registers for the whole loop
+    const int lane = fresh(tid & 63);
+    if (lane < 4 * R) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) lds.red[wave][j][lane] = acc[j];
+    }
+    __syncthreads();
+    // a wave finishes a token's 64 columns: SwiGLU times the token's factor, in fp16 with the
+    // largest at 2^14 .. 2^15; the factor that undoes it takes the nibbles' 2^24 along
+    for (int t = wave; t < T; t += kWaves) {
+      const int j = (lane >> 3) & 3, l = sum_lane(t, lane);
+      float g = 0.0f, u = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kShares; ++w) {
+        g += lds.red[w][j][l][t & 3];
+        u += lds.red[kShares + w][j][l][t & 3];
+      }
+      // x came in times 2^(14 - exponent), at most 2^127, and v as v 2^-24
+      const int e = max(10 + exponent(s_amax[t]), -103);
+      const float a = s_in[t] ? silu_mul(__builtin_ldexpf(g, e), __builtin_ldexpf(u, e)) * s_tok[t] : 0.0f;
+      const uint32_t top = wave_reduce_u32(__builtin_bit_cast(uint32_t, a) & 0x7fffffffu, MaxU32{});
+      const int ae = top == 0 ? 0 : exponent(top);
+      const float down = (lane & 8) ? 0.0625f : 1.0f;  // what meets the nibbles at 2^-20
+      const _Float16 h = static_cast<_Float16>(a * pow2(min(14 - ae, 127)) * down);
+      act[static_cast<long long>(t) * inter + tile * 64 + lane] = __builtin_bit_cast(uint16_t, h);
+      if (lane == 0) factors[tile * kMaxTokens + t] = pow2(max(min(10 + ae, 127), -103));
+    }
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------- launch 2
-template <int TR>
+template <int R>
 __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
   const pega_moe_few& p = f.p;
   __shared__ union {
     uint32_t tr[kWaves][2 * kSlotDwords];
-    floatx4_t red[kWaves][4][16 * TR];
+    floatx4_t red[kWaves][4][4 * R];
   } lds;
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -467,50 +530,41 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
   const int sh0 = (max(lo - routed_end, 0) + cost - 1) / cost;
   const int sh1 = (max(hi - routed_end, 0) + cost - 1) / cost;
 
-  floatx4_t acc[1][4] = {};
-  const int tiles1[1] = {tile};
-  const auto run = [&](floatx4_t (&acc)[1][4], auto wide) {
-    constexpr bool kWide = decltype(wide)::value;
-    constexpr int D = kWide ? 2 : 4;
-    for (int at = lo; at < min(hi, routed_end);) {
-      const int s = at / per, g0 = at - s * per, g1 = min(per, g0 + min(hi, routed_end) - at);
-      const int expert = __builtin_amdgcn_readfirstlane(p.slots[1 + s]);
-      const long long elems = static_cast<long long>(H) * I;
-      const Int4View<1> v =
-          int4_view<1>(p.w2 + expert * (elems / 2), p.w2_scales + expert * (elems / 32), H, I,
-                       tiles1, p.act + static_cast<long long>(s) * T * I, T);
-      int4_groups<1, D, kWide>(acc, v, g0, g1, lds.tr[wave]);
-      at += g1 - g0;
-    }
-    if (p.shared_kind == PEGA_SHARED_INT4) {
-      const Int4View<1> v = int4_view<1>(static_cast<const uint8_t*>(p.shared_w2), p.shared_w2_scales,
-                                         H, p.shared_inter, tiles1, p.act_shared, T);
-      int4_groups<1, D, kWide>(acc, v, sh0, sh1, lds.tr[wave]);
-    } else if (p.shared_kind == PEGA_SHARED_BF16) {
-      const uint32_t row_bytes = static_cast<uint32_t>(p.shared_inter) * 2u;
-      const __amdgpu_buffer_rsrc_t wr =
-          make_rsrc(static_cast<const uint16_t*>(p.shared_w2) + static_cast<long long>(tile) * 64 * p.shared_inter,
-                    64u * row_bytes);
-      const uint32_t n = static_cast<uint32_t>(lane >> 2);  // as the INT4 tiles' columns
-      uint32_t w_voff[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w_voff[j] = (32u * (n >> 3) + 8u * j + (n & 7u)) * row_bytes + 16u * (lane & 3);
-      const __amdgpu_buffer_rsrc_t ar = make_rsrc(p.act_shared, static_cast<uint32_t>(T) * row_bytes);
-      bf16_steps<4, 4>(acc[0], wr, w_voff, ar,
-                       static_cast<uint32_t>(lane & 15) * row_bytes + 16u * (lane >> 4), sh0, sh1);
-    }
-  };
-  run(acc, std::integral_constant<bool, false>{});
-  if (__builtin_expect(any_nan(acc[0]), 0)) {
-    floatx4_t again[1][4] = {};
-    run(again, std::integral_constant<bool, true>{});
-    take_not_finite(acc[0], again[0]);
+  floatx4_t acc[4] = {};
+  for (int at = lo; at < min(hi, routed_end);) {
+    const int s = at / per, g0 = at - s * per, g1 = min(per, g0 + min(hi, routed_end) - at);
+    const int expert = __builtin_amdgcn_readfirstlane(p.slots[1 + s]);
+    const long long elems = static_cast<long long>(H) * I;
+    const Int4View v = int4_view<R>(
+        p.w2 + expert * (elems / 2), p.w2_scales + expert * (elems / 32), H, I, tile,
+        p.act + static_cast<long long>(s) * T * I,
+        p.act_factors + static_cast<long long>(s) * (I >> 6) * kMaxTokens, T);
+    int4_groups<R, 4, true>(acc, v, g0, g1, 1.0f, lds.tr[wave]);
+    at += g1 - g0;
   }
-  __syncthreads();
-  if (lane < 16 * TR) {
+  if (p.shared_kind == PEGA_SHARED_INT4) {
+    const Int4View v = int4_view<R>(static_cast<const uint8_t*>(p.shared_w2), p.shared_w2_scales, H,
+                                    p.shared_inter, tile, p.act_shared, p.act_shared_factors, T);
+    int4_groups<R, 4, true>(acc, v, sh0, sh1, 1.0f, lds.tr[wave]);
+  } else if (p.shared_kind == PEGA_SHARED_BF16) {
+    const uint32_t row_bytes = static_cast<uint32_t>(p.shared_inter) * 2u;
+    const __amdgpu_buffer_rsrc_t wr =
+        make_rsrc(static_cast<const uint16_t*>(p.shared_w2) + static_cast<long long>(tile) * 64 * p.shared_inter,
+                  64u * row_bytes);
+    const uint32_t n = static_cast<uint32_t>(lane >> 2);  // as the INT4 tiles' columns
+    uint32_t w_voff[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) lds.red[wave][j][lane] = acc[0][j];
+    for (int j = 0; j < 4; ++j)
+      w_voff[j] = (32u * (n >> 3) + 8u * j + (n & 7u)) * row_bytes + 16u * (lane & 3);
+    const __amdgpu_buffer_rsrc_t ar = make_rsrc(p.act_shared, static_cast<uint32_t>(T) * row_bytes);
+    bf16_steps<4, 4>(acc, wr, w_voff, ar,
+                     static_cast<uint32_t>(lane & 15) * row_bytes + 16u * (lane >> 4), sh0, sh1);
+  }
+  add_places<R>(acc);
+  __syncthreads();
+  if (lane < 4 * R) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lds.red[wave][j][lane] = acc[j];
   }
   __syncthreads();
   const auto finish = [&](int t, int col, float sum) {
@@ -554,9 +608,11 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
 template <int NS, bool kDsv2>
 void launch_w13(const FewArgs& f, unsigned grid, hipStream_t stream) {
   if (f.p.tokens <= 4)
-    hipLaunchKernelGGL((few_w13_kernel<NS, kDsv2, 1>), dim3(grid), dim3(kThreads), 0, stream, f);
-  else
     hipLaunchKernelGGL((few_w13_kernel<NS, kDsv2, 4>), dim3(grid), dim3(kThreads), 0, stream, f);
+  else if (f.p.tokens <= 8)
+    hipLaunchKernelGGL((few_w13_kernel<NS, kDsv2, 8>), dim3(grid), dim3(kThreads), 0, stream, f);
+  else
+    hipLaunchKernelGGL((few_w13_kernel<NS, kDsv2, 16>), dim3(grid), dim3(kThreads), 0, stream, f);
 }
 
 template <bool kDsv2>
@@ -588,7 +644,7 @@ PEGA_API int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream) {
   if (!args) return fail(kInvalidValue, "moe_few_tokens: null arguments");
   const pega_moe_few& p = *args;
   if (!p.x || !p.logits || !p.w13 || !p.w13_scales || !p.w2 || !p.w2_scales || !p.out ||
-      !p.topk_weight || !p.topk_idx || !p.act || !p.slots || !p.partials || !p.counters ||
+      !p.topk_weight || !p.topk_idx || !p.act || !p.act_factors || !p.slots || !p.partials || !p.counters ||
       (!p.softmax && !p.bias))
     return fail(kInvalidValue, "moe_few_tokens: null pointer");
   if (p.shared_kind != PEGA_SHARED_NONE && p.shared_kind != PEGA_SHARED_BF16 &&
@@ -596,7 +652,8 @@ PEGA_API int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream) {
     return fail(kInvalidValue, "moe_few_tokens: shared_kind %d", p.shared_kind);
   const bool shared = p.shared_kind != PEGA_SHARED_NONE;
   if (shared && (!p.shared_w13 || !p.shared_w2 || !p.act_shared ||
-                 (p.shared_kind == PEGA_SHARED_INT4 && (!p.shared_w13_scales || !p.shared_w2_scales))))
+                 (p.shared_kind == PEGA_SHARED_INT4 &&
+                  (!p.shared_w13_scales || !p.shared_w2_scales || !p.act_shared_factors))))
     return fail(kInvalidValue, "moe_few_tokens: null pointer of the shared expert");
   if (p.tokens <= 0 || p.hidden_dim <= 0 || p.inter <= 0 || p.local_experts <= 0 ||
       p.n_experts <= 0 || p.topk <= 0 || p.topk > p.n_experts || p.global_start < 0 ||
@@ -616,22 +673,29 @@ PEGA_API int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream) {
     return fail(kNotSupported, "moe_few_tokens: a projection over 2 GiB (H=%d)", p.hidden_dim);
   const void* vecs[] = {p.x, p.w13, p.w13_scales, p.w2, p.w2_scales, p.act, shared ? p.shared_w13 : nullptr,
                         shared ? p.shared_w2 : nullptr, shared ? p.act_shared : nullptr,
+                        p.act_factors, p.shared_kind == PEGA_SHARED_INT4 ? p.act_shared_factors : nullptr,
                         p.shared_kind == PEGA_SHARED_INT4 ? p.shared_w13_scales : nullptr,
                         p.shared_kind == PEGA_SHARED_INT4 ? p.shared_w2_scales : nullptr};
   for (const void* v : vecs)
     if (!aligned16(v)) return fail(kNotSupported, "moe_few_tokens: buffers must be 16-byte aligned");
-  FewArgs f{p, 0, p.inter / 64, few_splits(p.hidden_dim), p.shared_kind == PEGA_SHARED_BF16 ? 3 : 1};
+  const int cu = current_cu_count();
+  if (cu <= 0) return fail(kInvalidValue, "moe_few_tokens: no device");
+  FewArgs f{p, 0, p.inter / 64, few_splits(p.hidden_dim), p.shared_kind == PEGA_SHARED_BF16 ? 3 : 1, 0, 0};
   if (p.shared_kind == PEGA_SHARED_BF16) f.sh_units = p.shared_inter / 8;
   if (p.shared_kind == PEGA_SHARED_INT4) f.sh_units = p.shared_inter / 64;
   const int routes = p.tokens * p.topk;
   const int slots = routes < p.local_experts ? routes : p.local_experts;
-  const unsigned grid = static_cast<unsigned>(f.sh_units + slots * f.tiles);
+  // a routed workgroup per CU at first, and another once the shared expert's are done
+  f.routed = slots * f.tiles < 2 * cu ? slots * f.tiles : 2 * cu;
+  f.routed_first = f.routed < cu ? f.routed : cu;
+  const unsigned grid = static_cast<unsigned>(f.sh_units + f.routed);
   if (p.softmax) launch_w13_slots<true>(f, grid, stream);
   else launch_w13_slots<false>(f, grid, stream);
   const int rc = launch_status("moe_few_tokens (W13)");
   if (rc != kSuccess) return rc;
   const dim3 grid2(static_cast<unsigned>(p.hidden_dim / 64), static_cast<unsigned>(f.splits));
-  if (p.tokens <= 4) hipLaunchKernelGGL((few_w2_kernel<1>), grid2, dim3(kThreads), 0, stream, f);
-  else hipLaunchKernelGGL((few_w2_kernel<4>), grid2, dim3(kThreads), 0, stream, f);
+  if (p.tokens <= 4) hipLaunchKernelGGL((few_w2_kernel<4>), grid2, dim3(kThreads), 0, stream, f);
+  else if (p.tokens <= 8) hipLaunchKernelGGL((few_w2_kernel<8>), grid2, dim3(kThreads), 0, stream, f);
+  else hipLaunchKernelGGL((few_w2_kernel<16>), grid2, dim3(kThreads), 0, stream, f);
   return launch_status("moe_few_tokens (W2)");
 }

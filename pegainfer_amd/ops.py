@@ -735,9 +735,15 @@ class FewTokensWorkspace:
         self.max_tokens, self.hidden, self.inter = max_tokens, hidden, inter
         self.topk, self.local_experts, self.shared_inter = topk, local_experts, shared_inter
         slots = min(max_tokens * topk, local_experts)
-        self.act = torch.empty(slots * max_tokens * inter, dtype=torch.bfloat16, device=device)
-        self.act_shared = torch.empty(max(1, max_tokens * shared_inter), dtype=torch.bfloat16,
+        # 16-bit rows between the launches (fp16, bf16 in front of a bf16 down projection) and the
+        # fp16 rows' factors, one for each 64 columns and token
+        self.act = torch.empty(slots * max_tokens * inter, dtype=torch.float16, device=device)
+        self.act_factors = torch.empty(slots * (inter // 64) * FEW_TOKENS_MAX, dtype=torch.float32,
+                                       device=device)
+        self.act_shared = torch.empty(max(1, max_tokens * shared_inter), dtype=torch.float16,
                                       device=device)
+        self.act_shared_factors = torch.empty(max(1, shared_inter // 64) * FEW_TOKENS_MAX,
+                                              dtype=torch.float32, device=device)
         self.slots = torch.zeros(1 + slots, dtype=torch.int32, device=device)
         self.partials = torch.empty(_FEW_MAX_SPLITS * max_tokens * hidden, dtype=torch.float32,
                                     device=device)
@@ -806,7 +812,8 @@ def moe_few_tokens(workspace: FewTokensWorkspace, x: torch.Tensor, logits: torch
     *ptrs, stream = _ptrs_here(
         x, logits, bias, w13.weight_packed_uint4b8, w13.weight_scale_permuted,
         w2.weight_packed_uint4b8, w2.weight_scale_permuted, sw13, ss13, sw2, ss2, residual, out,
-        topk_weight, topk_idx, ws.act, ws.act_shared, ws.slots, ws.partials, ws.counters)
+        topk_weight, topk_idx, ws.act, ws.act_factors, ws.act_shared, ws.act_shared_factors,
+        ws.slots, ws.partials, ws.counters)
     args = _lib.MoeFew(*ptrs, route_scale, routed_scale, bias is None, kind, T, H, inter,
                        shared_inter, n_experts, E, global_start, ws.topk)
     _lib.call("pega_moe_few_tokens", ctypes.byref(args), stream)

@@ -211,7 +211,7 @@ def test_mx_gemm_wrappers_refuse_before_the_device():
 def _few(**kw):
     from pegainfer_amd import _lib
     a = _lib.MoeFew()
-    for i, (name, _) in enumerate(_lib.MoeFew._fields_[:20]):
+    for i, (name, _) in enumerate(_lib.MoeFew._fields_[:22]):
         setattr(a, name, A << i)
     a.route_scale = a.routed_scale = 1.0
     a.softmax, a.shared_kind, a.tokens, a.hidden_dim, a.inter, a.shared_inter = 0, 1, 4, 128, 64, 64
@@ -228,7 +228,7 @@ def _few_call(**kw):
 
 @pytest.mark.parametrize("name", [
     "x", "logits", "bias", "w13", "w13_scales", "w2", "w2_scales", "shared_w13", "shared_w2", "out",
-    "topk_weight", "topk_idx", "act", "act_shared", "slots", "partials", "counters"])
+    "topk_weight", "topk_idx", "act", "act_factors", "act_shared", "slots", "partials", "counters"])
 def test_few_tokens_refuses_null(name):
     assert _few_call(**{name: None}) == 1
 
@@ -241,6 +241,7 @@ def test_few_tokens_refuses_null(name):
     (dict(local_experts=513, n_experts=1000), 801), (dict(n_experts=1025), 801),
     (dict(local_experts=0), 1), (dict(shared_kind=3), 1), (dict(shared_kind=-1), 1),
     (dict(shared_kind=2, shared_w13_scales=None), 1), (dict(shared_kind=2, shared_w2_scales=None), 1),
+    (dict(shared_kind=2, act_shared_factors=None), 1),
     (dict(route_scale=0.0), 1), (dict(route_scale=float("nan")), 1), (dict(x=A + 8), 801),
     (dict(w13=A + 4), 801), (dict(act=A + 2), 801), (dict(shared_w2=A + 2), 801),
     (dict(hidden_dim=1 << 20, inter=1024), 801)])
@@ -263,7 +264,7 @@ def test_few_tokens_struct_matches_the_header(tmp_path):
     exe = tmp_path / "s"
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
-    assert got[0] == ctypes.sizeof(_lib.MoeFew) == 208
+    assert got[0] == ctypes.sizeof(_lib.MoeFew) == 224
     assert got[1:] == [getattr(_lib.MoeFew, n).offset for n in fields]
 
 
