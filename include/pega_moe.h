@@ -318,7 +318,7 @@ int pega_dense_w13_swiglu(const uint16_t* W13, const uint16_t* X, uint16_t* act,
 /* ---------------- a whole MoE layer for a few tokens ---------------- */
 
 enum { PEGA_SHARED_NONE = 0, PEGA_SHARED_BF16 = 1, PEGA_SHARED_INT4 = 2 };
-enum { PEGA_FEW_MAX_SPLITS = 8 };
+enum { PEGA_FEW_MAX_SPLITS = 8, PEGA_FEW_COUNTERS = 512 };
 
 /* Arguments of pega_moe_few_tokens.  INT4 weights are device packages (the layout of
  * pega_marlin_int4_*; W13 gate columns first).  Plain pointers and sizes; 224 bytes on LP64. */
@@ -343,9 +343,10 @@ typedef struct pega_moe_few {
     uint16_t* act_shared;        /* workspace: fp16 or bf16 [tokens][shared_inter] */
     float* act_shared_factors;   /* workspace, with an INT4 shared expert: [shared_inter / 64][16] */
     int32_t* slots;              /* workspace: 1 + min(tokens topk, local_experts) */
-    float* partials;             /* workspace: PEGA_FEW_MAX_SPLITS * tokens * hidden_dim */
-    uint32_t* counters;          /* workspace: hidden_dim / 64, zero before the first call; every
-                                    call leaves them zero */
+    float* partials;             /* workspace: tokens times the larger of PEGA_FEW_MAX_SPLITS *
+                                    hidden_dim and 128 * PEGA_FEW_COUNTERS */
+    uint32_t* counters;          /* workspace: hidden_dim / 64 + PEGA_FEW_COUNTERS, zero before the
+                                    first call; every call leaves them zero */
     float route_scale;           /* of the sigmoid select (> 0); unused with softmax */
     float routed_scale;          /* factor of the routed sum */
     int softmax;                 /* 0: pega_kimi_router_select, 1: pega_dsv2_router_select */

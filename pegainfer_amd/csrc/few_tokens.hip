@@ -53,6 +53,7 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4_t;
 
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kMaxTokens = 16, kMaxTopk = 32, kMaxLocal = 512;
+constexpr int kMaxShares = 4;     // of K that launch 1 cuts a tile pair into
 constexpr int kSlotDwords = 320;  // one 32-k group of a 64-column tile, as wna16.hip's slots
 constexpr int kStream = 2;        // non-temporal: bytes read once
 constexpr uint32_t kOutOfRange = 0x80000000u;  // voffset that fails every range check
@@ -317,6 +318,27 @@ __device__ __forceinline__ void bf16_steps(floatx4_t* acc, __amdgpu_buffer_rsrc_
     if (s + q < s1) compute(slot[q]);
 }
 
+// Sums between workgroups of a launch: device-coherent stores and loads (the L2 is per XCD), of
+// which every store has completed before the workgroup counts itself in.  last_of: whether this
+// workgroup is the last of n to do so, for all its threads; the last puts the counter back to zero.
+__device__ __forceinline__ void store_coherent(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float load_coherent(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ bool last_of(uint32_t* counter, int n, int* s_last) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t prev = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *s_last = prev == static_cast<uint32_t>(n - 1);
+    if (*s_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *s_last != 0;
+}
+
 __device__ __forceinline__ float silu_mul(float g, float u) {
   return g / (1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f)) * u;
 }
@@ -332,11 +354,16 @@ __device__ __forceinline__ uint32_t row_amax(const uint16_t* x, int t, int H) {
   const int lane = threadIdx.x & 63;
   const uint16_t* row = x + static_cast<long long>(t) * H;
   uint32_t m = 0;
-  for (int v = lane; v < H / 8; v += 64) {
-    const uint4 q = *reinterpret_cast<const uint4*>(row + 8 * v);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  for (int v0 = lane; v0 < H / 8; v0 += 8 * 64) {  // eight loads on their way at a time
+    uint4 q[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = max(m, max((w[i] << 16) & 0x7fff0000u, w[i] & 0x7fff0000u));
+    for (int i = 0; i < 8; ++i) q[i] = *reinterpret_cast<const uint4*>(row + 8 * min(v0 + 64 * i, H / 8 - 1));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = max(m, max((w[k] << 16) & 0x7fff0000u, w[k] & 0x7fff0000u));
+    }
   }
   return wave_reduce_u32(m, MaxU32{});
 }
@@ -355,6 +382,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
   __shared__ float s_tok[kMaxTokens];   // a token's factor for this slot's rows
   __shared__ bool s_in[kMaxTokens];     // whether it has a route to the slot's expert
   __shared__ uint32_t s_amax[kMaxTokens];
+  __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int T = p.tokens, H = p.hidden_dim;
@@ -396,7 +424,8 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     const uint32_t m = row_amax(p.x, t, H);
     if (lane == 0) s_amax[t] = m;
   }
-  int live = 1, first = unit, step = 1 << 30;  // this workgroup's tile pairs
+  int live = 1, first = unit, step = 1 << 30;  // this workgroup's shares of tile pairs
+  int shares = 1;                              // of K that a tile pair is cut into
   const int inter = shared ? p.shared_inter : p.inter;
   const int tiles = inter >> 6;
   if (!shared) {
@@ -435,16 +464,21 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     }
     first = mine;
     step = f.routed;
+    // few tile pairs are cut along K, while a CU of its own is there for each share: a workgroup
+    // streams about 35 GB/s, whatever the others leave free
+    if (live > 0) shares = max(1, min(kMaxShares, f.routed_first / (live * tiles)));
   }
   __syncthreads();
   const int my_token = (lane & 15) % R;
   const float row_factor = my_token < T ? pow2(min(14 - exponent(s_amax[my_token]), 127)) : 0.0f;
-  // waves 0 to 3 share K of the gate tile, 4 to 7 of the up tile
-  constexpr int kShares = kWaves / 2;
-  const int groups = H >> 5, half = wave / kShares, share = wave % kShares;
-  const int g0 = (groups * share) / kShares, g1 = (groups * (share + 1)) / kShares;
-  for (int at = first; at < live * tiles; at += step) {
-    const int slot = at / tiles, tile = at - slot * tiles;
+  // waves 0 to 3 share K, or the workgroup's share of it, of the gate tile, 4 to 7 of the up tile
+  constexpr int kPart = kWaves / 2;
+  const int groups = H >> 5, half = wave / kPart, part = wave % kPart;
+  for (int at = first; at < live * tiles * shares; at += step) {
+    const int pair = at / shares, share = at - pair * shares;
+    const int slot = pair / tiles, tile = pair - slot * tiles;
+    const int k0 = (groups * share) / shares, k1 = (groups * (share + 1)) / shares;
+    const int g0 = k0 + ((k1 - k0) * part) / kPart, g1 = k0 + ((k1 - k0) * (part + 1)) / kPart;
     const uint8_t* q = static_cast<const uint8_t*>(p.shared_w13);
     const uint16_t* sc = p.shared_w13_scales;
     uint16_t* act = p.act_shared;
@@ -483,14 +517,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     __syncthreads();
     // a wave finishes a token's 64 columns: SwiGLU times the token's factor, in fp16 with the
     // largest at 2^14 .. 2^15; the factor that undoes it takes the nibbles' 2^24 along
-    for (int t = wave; t < T; t += kWaves) {
-      const int j = (lane >> 3) & 3, l = sum_lane(t, lane);
-      float g = 0.0f, u = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kShares; ++w) {
-        g += lds.red[w][j][l][t & 3];
-        u += lds.red[kShares + w][j][l][t & 3];
-      }
+    const auto finish = [&](int t, float g, float u) {
       // x came in times 2^(14 - exponent), at most 2^127, and v as v 2^-24
       const int e = max(10 + exponent(s_amax[t]), -103);
       const float a = s_in[t] ? silu_mul(__builtin_ldexpf(g, e), __builtin_ldexpf(u, e)) * s_tok[t] : 0.0f;
@@ -500,6 +527,40 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
       const _Float16 h = static_cast<_Float16>(a * pow2(min(14 - ae, 127)) * down);
       act[static_cast<long long>(t) * inter + tile * 64 + lane] = __builtin_bit_cast(uint16_t, h);
       if (lane == 0) factors[tile * kMaxTokens + t] = pow2(max(min(10 + ae, 127), -103));
+    };
+    const auto place = [&](int of, int t, int up) {
+      return p.partials + (((static_cast<long long>(pair) * shares + of) * T + t) * 2 + up) * 64 + lane;
+    };
+    for (int t = wave; t < T; t += kWaves) {
+      const int j = (lane >> 3) & 3, l = sum_lane(t, lane);
+      float g = 0.0f, u = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kPart; ++w) {
+        g += lds.red[w][j][l][t & 3];
+        u += lds.red[kPart + w][j][l][t & 3];
+      }
+      if (shares == 1) {
+        finish(t, g, u);
+      } else {
+        store_coherent(place(share, t, 0), g);
+        store_coherent(place(share, t, 1), u);
+      }
+    }
+    if (shares > 1 && last_of(&p.counters[H / 64 + pair], shares, &s_last)) {
+      for (int t = wave; t < T; t += kWaves) {
+        float g[kMaxShares], u[kMaxShares], gs = 0.0f, us = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kMaxShares; ++i) {
+          g[i] = load_coherent(place(min(i, shares - 1), t, 0));
+          u[i] = load_coherent(place(min(i, shares - 1), t, 1));
+        }
+#pragma unroll
+        for (int i = 0; i < kMaxShares; ++i) {
+          gs = i < shares ? gs + g[i] : gs;
+          us = i < shares ? us + u[i] : us;
+        }
+        finish(t, gs, us);
+      }
     }
     __syncthreads();
   }
@@ -518,7 +579,8 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int T = p.tokens, H = p.hidden_dim, I = p.inter;
   const int tile = blockIdx.x, split = blockIdx.y;
-  const int slots = __builtin_amdgcn_readfirstlane(p.slots[0]);
+  const int listed = p.slots[min(lane, p.tokens * p.topk < p.local_experts ? p.tokens * p.topk : p.local_experts)];
+  const int slots = __builtin_amdgcn_readfirstlane(listed);
 
   // this wave's share of the priced list: slots' groups at 1, then the shared expert's
   const int per = I >> 5, sh_groups = p.shared_kind != PEGA_SHARED_NONE ? p.shared_inter >> 5 : 0;
@@ -533,7 +595,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
   floatx4_t acc[4] = {};
   for (int at = lo; at < min(hi, routed_end);) {
     const int s = at / per, g0 = at - s * per, g1 = min(per, g0 + min(hi, routed_end) - at);
-    const int expert = __builtin_amdgcn_readfirstlane(p.slots[1 + s]);
+    const int expert = s < 63 ? __builtin_amdgcn_readlane(listed, 1 + s) : __builtin_amdgcn_readfirstlane(p.slots[1 + s]);
     const long long elems = static_cast<long long>(H) * I;
     const Int4View v = int4_view<R>(
         p.w2 + expert * (elems / 2), p.w2_scales + expert * (elems / 32), H, I, tile,
@@ -581,26 +643,16 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) sum += lds.red[w][j][l][t & 3];
     if (f.splits == 1) finish(t, col, sum);
-    else __hip_atomic_store(place(split, t, col), sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else store_coherent(place(split, t, col), sum);
   }
-  if (f.splits == 1) return;
-  // The sums are device-coherent stores that have completed before the arrival is counted; the
-  // last arrival of the tile reads them the same way and puts the counter back to zero.
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (tid == 0) {
-    const uint32_t prev = __hip_atomic_fetch_add(&p.counters[tile], 1u, __ATOMIC_RELAXED,
-                                                 __HIP_MEMORY_SCOPE_AGENT);
-    s_last = prev == static_cast<uint32_t>(f.splits - 1);
-    if (s_last) __hip_atomic_store(&p.counters[tile], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (!s_last) return;
+  if (f.splits == 1 || !last_of(&p.counters[tile], f.splits, &s_last)) return;
   for (int o = tid; o < T * 64; o += kThreads) {
     const int t = o >> 6, col = o & 63;
-    float sum = 0.0f;
-    for (int s = 0; s < f.splits; ++s)
-      sum += __hip_atomic_load(place(s, t, col), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    float part[PEGA_FEW_MAX_SPLITS], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PEGA_FEW_MAX_SPLITS; ++i) part[i] = load_coherent(place(min(i, f.splits - 1), t, col));
+#pragma unroll
+    for (int i = 0; i < PEGA_FEW_MAX_SPLITS; ++i) sum = i < f.splits ? sum + part[i] : sum;
     finish(t, col, sum);
   }
 }

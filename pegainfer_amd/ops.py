@@ -715,7 +715,7 @@ def _ptrs_here(*tensors):
 # --------------------------------------------------------------------------
 FEW_TOKENS_MAX = 16        # rows of one matrix instruction
 FEW_TOKENS_MAX_TOPK = 32
-_FEW_MAX_SPLITS = 8        # PEGA_FEW_MAX_SPLITS
+_FEW_MAX_SPLITS, _FEW_COUNTERS = 8, 512  # PEGA_FEW_MAX_SPLITS, PEGA_FEW_COUNTERS
 _SHARED_NONE, _SHARED_BF16, _SHARED_INT4 = 0, 1, 2
 
 
@@ -745,9 +745,9 @@ class FewTokensWorkspace:
         self.act_shared_factors = torch.empty(max(1, shared_inter // 64) * FEW_TOKENS_MAX,
                                               dtype=torch.float32, device=device)
         self.slots = torch.zeros(1 + slots, dtype=torch.int32, device=device)
-        self.partials = torch.empty(_FEW_MAX_SPLITS * max_tokens * hidden, dtype=torch.float32,
-                                    device=device)
-        self.counters = torch.zeros(hidden // 64, dtype=torch.int32, device=device)
+        self.partials = torch.empty(max_tokens * max(_FEW_MAX_SPLITS * hidden, 128 * _FEW_COUNTERS),
+                                    dtype=torch.float32, device=device)
+        self.counters = torch.zeros(hidden // 64 + _FEW_COUNTERS, dtype=torch.int32, device=device)
 
 
 def moe_few_tokens(workspace: FewTokensWorkspace, x: torch.Tensor, logits: torch.Tensor,

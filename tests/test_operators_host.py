@@ -271,7 +271,7 @@ def test_few_tokens_struct_matches_the_header(tmp_path):
 def test_few_tokens_wrappers_refuse_before_the_device():
     from pegainfer_amd import ops
     ws = ops.FewTokensWorkspace(4, 128, 64, topk=2, local_experts=4, shared_inter=64, device="cpu")
-    assert ws.act.numel() == 4 * 4 * 64 and ws.counters.numel() == 2 and ws.slots.numel() == 5
+    assert ws.act.numel() == 4 * 4 * 64 and ws.counters.numel() == 2 + 512 and ws.slots.numel() == 5
     for bad in (dict(max_tokens=17), dict(max_tokens=0), dict(hidden=96), dict(inter=100),
                 dict(topk=0), dict(topk=33), dict(shared_inter=32), dict(local_experts=0)):
         kw = {**dict(max_tokens=4, hidden=128, inter=64, topk=2, local_experts=4, shared_inter=64), **bad}
