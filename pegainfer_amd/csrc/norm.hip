@@ -12,7 +12,9 @@
 // (in 32 bits about one value in 10^6 goes to the neighbouring code, and which ones depends on
 // the order of the sum).  y reaches 32 bits rounded to odd (the last bit set if anything was cut
 // off), after which one more rounding, to bf16 or to a code, is the rounding of y itself.  The
-// norm is of s itself, not of bf16(s).  The 64-bit work hides behind the memory.
+// norm is of s itself, not of bf16(s).  The 64-bit work hides behind the memory:
+// 4096 rows of 7168 with every output take 57 us (265 MB, 4.6 TB/s; a plain copy reaches 4.8),
+// one row 5.0 us, of which the launch itself is 2.3.
 #include "common.h"
 #include "mx_format.h"
 #include "pega_moe.h"
@@ -21,40 +23,52 @@ namespace pega {
 namespace {
 
 // y in fp32, rounded to odd: the low 29 mantissa bits cut off, and the last one kept set if any
-// of them was.  The cut value converts exactly (values below fp32's normal range aside, which
-// every output rounds to 0).
+// of them was (adding 2^29 - 1 to them carries into it then).  What is left converts exactly
+// (values below fp32's normal range aside, which every output rounds to 0).
 __device__ __forceinline__ float to_odd(double y) {
   const uint64_t b = __builtin_bit_cast(uint64_t, y);
   const uint32_t lo = static_cast<uint32_t>(b);
-  const uint64_t cut = (b & 0xffffffff00000000ull) | (lo & 0xe0000000u);
-  const float f = static_cast<float>(__builtin_bit_cast(double, cut));
-  const uint32_t u = __builtin_bit_cast(uint32_t, f);
-  // an infinite or NaN f keeps its bits
-  const bool sticky = (lo & 0x1fffffffu) != 0 && (u & 0x7f800000u) != 0x7f800000u;
-  return __builtin_bit_cast(float, sticky ? u | 1u : u);
+  const uint32_t odd = (lo & 0x1fffffffu) + 0x1fffffffu;
+  const uint64_t cut = (b & 0xffffffff00000000ull) | ((lo | odd) & 0xe0000000u);
+  return static_cast<float>(__builtin_bit_cast(double, cut));
 }
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int mask) {
+template <int kCtrl>
+__device__ __forceinline__ double dpp_add(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __shfl_xor(static_cast<uint32_t>(b), mask);
-  const uint32_t hi = __shfl_xor(static_cast<uint32_t>(b >> 32), mask);
-  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+  const uint64_t o = static_cast<uint64_t>(mx_dpp<kCtrl>(static_cast<uint32_t>(b >> 32))) << 32 |
+                     mx_dpp<kCtrl>(static_cast<uint32_t>(b));
+  return v + __builtin_bit_cast(double, o);
 }
 
-// WPR waves take a row, CH vectors of 8 columns a lane; below four waves a row, a workgroup of
-// four waves takes 4 / WPR rows.  Every load of a row has returned before its first store (the
-// sum needs them all), so an output may be the buffer of an input.
-template <int WPR, int CH, bool kX32>
-__global__ __launch_bounds__(64 * (WPR < 4 ? 4 : WPR)) void add_rmsnorm_kernel(
+// The sum of 16 consecutive lanes, in each of them.
+__device__ __forceinline__ double sum16(double v) {
+  v = dpp_add<0xB1>(v);     // quad_perm [1,0,3,2]
+  v = dpp_add<0x4E>(v);     // quad_perm [2,3,0,1]
+  v = dpp_add<0x141>(v);    // row_half_mirror
+  return dpp_add<0x140>(v); // row_mirror
+}
+
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(b)), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(b >> 32)), lane);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// A row is taken by blockDim.x threads, a whole number of waves, CH vectors of 8 columns a lane;
+// a workgroup takes blockDim.y rows.  Every load of a row has returned before its first store
+// (the sum needs them all), so an output may be the buffer of an input.
+constexpr int kMaxWaves = 16;
+
+template <int CH, bool kX32>
+__global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) void add_rmsnorm_kernel(
     const void* x, const uint16_t* residual, const uint16_t* __restrict__ weight, double eps,
     uint16_t* residual_out, uint16_t* normed, uint8_t* codes, uint8_t* scales, int rows,
     int hidden) {
-  constexpr int kWaves = WPR < 4 ? 4 : WPR;
-  constexpr int kLanes = 64 * WPR;
-  __shared__ double s_sum[kWaves];
-  const int wave = threadIdx.x >> 6;
-  const int row = blockIdx.x * (kWaves / WPR) + wave / WPR;
-  const int lane = static_cast<int>(threadIdx.x) % kLanes;  // within the row
+  __shared__ double s_sum[kMaxWaves];
+  const int lanes = blockDim.x, lane = threadIdx.x;
+  const int row = blockIdx.x * blockDim.y + threadIdx.y;
   const int vecs = hidden >> 3;
   const bool in = row < rows;
   const long long base = static_cast<long long>(row) * hidden;
@@ -63,7 +77,7 @@ __global__ __launch_bounds__(64 * (WPR < 4 ? 4 : WPR)) void add_rmsnorm_kernel(
   const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int v = lane + c * kLanes;
+    const int v = lane + c * lanes;
     const bool ok = in && v < vecs;
     const long long at = base + 8LL * v;
     if constexpr (kX32) {
@@ -73,7 +87,9 @@ __global__ __launch_bounds__(64 * (WPR < 4 ? 4 : WPR)) void add_rmsnorm_kernel(
     } else {
       xr[c][0] = ok ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at) : zero;
     }
-    rr[c] = ok && residual ? *reinterpret_cast<const uint4*>(residual + at) : zero;
+    // no residual: -0, which leaves every x as it is
+    rr[c] = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);
+    if (ok && residual) rr[c] = *reinterpret_cast<const uint4*>(residual + at);
     wr[c] = v < vecs ? *reinterpret_cast<const uint4*>(weight + 8 * v) : zero;
   }
   double s[CH][8], sum = 0.0;
@@ -93,27 +109,24 @@ __global__ __launch_bounds__(64 * (WPR < 4 ? 4 : WPR)) void add_rmsnorm_kernel(
         xv = (i & 1) ? bf_hi(w) : bf_lo(w);
       }
       const float rv = (i & 1) ? bf_hi(rw[i >> 1]) : bf_lo(rw[i >> 1]);
-      s[c][i] = residual ? static_cast<double>(xv) + static_cast<double>(rv)
-                         : static_cast<double>(xv);
+      s[c][i] = static_cast<double>(xv) + static_cast<double>(rv);
       sum = __builtin_fma(s[c][i], s[c][i], sum);
     }
   }
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) sum += shfl_xor_f64(sum, m);
-  if constexpr (WPR > 1) {
-    if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
+  sum = sum16(sum);
+  sum = (lane_f64(sum, 0) + lane_f64(sum, 16)) + (lane_f64(sum, 32) + lane_f64(sum, 48));
+  if (lanes > 64) {
+    if ((lane & 63) == 0) s_sum[lane >> 6] = sum;
     __syncthreads();
-    sum = 0.0;
-    const int first = wave / WPR * WPR;
-#pragma unroll
-    for (int w = 0; w < WPR; ++w) sum += s_sum[first + w];
+    const int w = lane & 15;
+    sum = sum16(w < lanes >> 6 ? s_sum[w] : 0.0);
   }
   const double inv = 1.0 / __builtin_sqrt(sum / hidden + eps);
 
   const bool whole = (hidden & 127) == 0;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int v = lane + c * kLanes;
+    const int v = lane + c * lanes;
     const bool ok = in && v < vecs;
     const long long at = base + 8LL * v;
     const uint32_t ww[4] = {wr[c].x, wr[c].y, wr[c].z, wr[c].w};
@@ -141,17 +154,17 @@ __global__ __launch_bounds__(64 * (WPR < 4 ? 4 : WPR)) void add_rmsnorm_kernel(
   }
 }
 
-template <int WPR, int CH>
+template <int CH>
 void launch_norm(bool x32, const void* x, const uint16_t* residual, const uint16_t* weight,
                  double eps, uint16_t* residual_out, uint16_t* normed, uint8_t* codes,
                  uint8_t* scales, int rows, int hidden, hipStream_t stream) {
-  constexpr int kRows = WPR < 4 ? 4 / WPR : 1;
-  const dim3 grid(ceil_div(rows, kRows)), block(64 * (WPR < 4 ? 4 : WPR));
+  const int waves = ceil_div(hidden / 8, 64 * CH), per = waves == 1 ? 4 : 1;
+  const dim3 grid(ceil_div(rows, per)), block(64 * waves, per);
   if (x32)
-    hipLaunchKernelGGL((add_rmsnorm_kernel<WPR, CH, true>), grid, block, 0, stream, x, residual,
+    hipLaunchKernelGGL((add_rmsnorm_kernel<CH, true>), grid, block, 0, stream, x, residual,
                        weight, eps, residual_out, normed, codes, scales, rows, hidden);
   else
-    hipLaunchKernelGGL((add_rmsnorm_kernel<WPR, CH, false>), grid, block, 0, stream, x, residual,
+    hipLaunchKernelGGL((add_rmsnorm_kernel<CH, false>), grid, block, 0, stream, x, residual,
                        weight, eps, residual_out, normed, codes, scales, rows, hidden);
 }
 
@@ -196,16 +209,16 @@ PEGA_API int pega_add_rmsnorm(const void* x, bool x_is_f32, const uint16_t* resi
         return fail(kInvalidValue, "add_rmsnorm: two outputs overlap");
   }
   const int vecs = hidden_dim / 8;
-#define PEGA_NORM(WPR, CH) \
-  launch_norm<WPR, CH>(x_is_f32, x, residual, weight, eps, residual_out, normed, mxfp8_codes, \
-                       mxfp8_scales, rows, hidden_dim, stream)
-  if (vecs <= 64) PEGA_NORM(1, 1);
-  else if (vecs <= 128) PEGA_NORM(1, 2);
-  else if (vecs <= 256) PEGA_NORM(4, 1);
-  else if (vecs <= 512) PEGA_NORM(4, 2);
-  else if (vecs <= 1024) PEGA_NORM(4, 4);
-  else if (vecs <= 2048) PEGA_NORM(8, 4);
-  else PEGA_NORM(16, 4);
+#define PEGA_NORM(CH) \
+  launch_norm<CH>(x_is_f32, x, residual, weight, eps, residual_out, normed, mxfp8_codes, \
+                  mxfp8_scales, rows, hidden_dim, stream)
+  // Few vectors a lane finish a row soonest, but a CU must hold eight waves a SIMD for the memory:
+  // one vector up to four waves, two up to eight.  More than a few thousand waves keep the memory
+  // busy anyway and then gain from fewer of them: 7168 columns take 5.0 us (two vectors a lane)
+  // against 5.5 (four) at one row, 19 both at 1024, 61 against 57 at 4096.
+  if (vecs <= 4 * 64) PEGA_NORM(1);
+  else if (vecs <= 8 * 2 * 64 && (vecs <= 8 * 64 || rows <= 1024)) PEGA_NORM(2);
+  else PEGA_NORM(4);
 #undef PEGA_NORM
   return launch_status("add_rmsnorm");
 }
