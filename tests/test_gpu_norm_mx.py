@@ -252,3 +252,58 @@ def test_norm_then_quantized_swiglu_in_a_graph_and_on_a_side_stream():
         torch.cuda.current_stream().wait_stream(side)
         for g0, t in zip(got, (y, q.codes, q.scales, a.codes, a.scales)):
             assert torch.equal(g0, t)
+
+
+@pytest.mark.parametrize("rows,cols,x32", [(1025, 4128, False), (1100, 7168, True), (1024, 7168, False),
+                                           (4097, 256, False)])
+def test_norm_of_many_rows(rows, cols, x32):
+    """Either side of the rule that gives long batches more vectors a lane: the same results."""
+    g = np.random.default_rng(cols)
+    x = _rows(g, rows, cols, 0.5)
+    x = x if x32 else mx_ref.bf16_round(x)
+    res = mx_ref.bf16_round(_rows(g, rows, cols, 2.0))
+    w = mx_ref.bf16_round(1 + 0.1 * g.standard_normal(cols).astype(np.float32))
+    s, y, q = _run_norm(x, res, w, 1e-6)
+    at = np.unique(np.r_[0:8, rows // 2, rows - 9:rows])
+    want_s, want_y = _norm_ref((x if x32 else bf(x))[at], bf(res)[at], bf(w), 1e-6)
+    _check_bf16(s[at], want_s, "sums")
+    _check_bf16(y[at], want_y, "normed")
+    codes, scales = mx_ref.quantize(want_y, "fp8")
+    assert np.array_equal(q[0][at], codes) and np.array_equal(q[1][at], scales)
+    for lo in range(0, rows, 300):  # each row as in a short batch
+        part = _run_norm(x[lo:lo + 300], res[lo:lo + 300], w, 1e-6)
+        for a, b in ((part[0], s), (part[1], y), (part[2][0], q[0]), (part[2][1], q[1])):
+            assert np.array_equal(a, b[lo:lo + 300])
+
+
+@pytest.mark.parametrize("name,n", FORMATS)
+def test_offsets_past_32_bits(name, n):
+    """17 GB of rows, more vectors than a launch indexes: the last rows are those of a short call."""
+    from pegainfer_amd import ops
+    cols, block = 1 << 13, 1 << 10
+    rows = (1 << 20) + 5
+    torch.manual_seed(n)
+    some = torch.randn(block, cols, device="cuda").bfloat16()
+    few = ops.MxTensor.empty(block, cols, _mx(name, n))
+    ops.mx_quantize(some, few)
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[:rows - 5].view(-1, block, cols).copy_(some)
+    x[rows - 5:].copy_(some[7:12])
+    q = ops.MxTensor.empty(rows, cols, _mx(name, n))
+    ops.mx_quantize(x, q)
+    for got, want in ((q.codes, few.codes), (q.scales, few.scales)):
+        assert (got[:rows - 5].view(-1, block, got.shape[1]) == want).all()
+        assert torch.equal(got[rows - 5:], want[7:12])
+    back = torch.empty(block, cols, dtype=torch.bfloat16, device="cuda")
+    ops.mx_dequantize(few, back)
+    ops.mx_dequantize(q, x)
+    assert (x[:rows - 5].view(-1, block, cols).view(torch.int16) == back.view(torch.int16)).all()
+    assert torch.equal(x[rows - 5:], back[7:12])
+    del q
+    a = ops.MxTensor.empty(rows, cols // 2, _mx(name, n))
+    ops.mx_swiglu_quantize(x, a)
+    b = ops.MxTensor.empty(block, cols // 2, _mx(name, n))
+    ops.mx_swiglu_quantize(back, b)
+    assert (a.codes[:rows - 5].view(-1, block, b.codes.shape[1]) == b.codes).all()
+    assert torch.equal(a.codes[rows - 5:], b.codes[7:12])
+    assert torch.equal(a.scales[rows - 5:], b.scales[7:12])
