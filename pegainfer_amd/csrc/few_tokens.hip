@@ -14,7 +14,7 @@
 //              shared expert's workgroups, that need no routing, cover), and then takes gate/up tile
 //              pairs of the distinct local experts, in id order, in turn with the others.  The routing
 //              weight and routed_scale are multiplied into the SwiGLU rows, which are written for
-//              all tokens: zeros where the token has no route to the expert.
+//              the expert's tokens (of up to four tokens, for all: zeros where there is no route).
 //   launch 2   so the second products are one sum over the concatenated rows of all slots and the
 //              shared expert.  That list of 32-k groups, priced by its bytes, is cut into equal
 //              shares for the waves of `splits` workgroups per 64 output columns.  With several
@@ -29,8 +29,9 @@
 // group's fp32 sum times its scale is added to the column's.  Weights count as (nibble - 8) * scale
 // unrounded (the general kernels round that product to bf16; the results differ by it).
 //
-// An MFMA's 16 rows are the tokens themselves, never gathered.  With R = 4 (8) token rows, 4 (2)
-// groups share an instruction's rows: group g's instruction has the tokens in rows R g .. and zeros
+// An MFMA's 16 rows are the tokens, with more than four of them those that have a route to the
+// expert (16 tokens bring an expert two of them at most sizes).  With up to 4 (8) rows, 4 (2) groups
+// share an instruction's rows, R = 4 (8) to each: group g's instruction has the tokens in rows R g .. and zeros
 // elsewhere, the sums of all of them land in one accumulator, and the scale is a lane's own group's.
 // Then a scale is applied to 4 sums a lane instead of 16, and scales and activations are loaded
 // once per 4 (2) groups.
@@ -114,28 +115,27 @@ struct Int4View {
   uint32_t w_step, s_step;
 };
 
-// R: token rows of an instruction that a group takes (4, 8 or 16).
+// R: token rows of an instruction that a group takes (4, 8 or 16).  row: of the `rows` activation
+// rows, the one that the lane brings, for row (lane % 16) % R of an instruction; -1 none.
 template <int R>
 __device__ __forceinline__ Int4View int4_view(const uint8_t* q, const uint16_t* scales, int N, int K,
                                               int tile, const void* act, const float* factors,
-                                              int tokens) {
+                                              int row, int rows) {
   const int lane = fresh(threadIdx.x & 63);
   const int n16 = lane & 15, kb = lane >> 4;
   const uint32_t n_tiles = static_cast<uint32_t>(N) >> 6;
   Int4View v;
   v.w = make_rsrc(q, static_cast<uint32_t>(N) * static_cast<uint32_t>(K) / 2u);
   v.s = make_rsrc(scales, static_cast<uint32_t>(K >> 5) * static_cast<uint32_t>(N) * 2u);
-  v.a = make_rsrc(act, static_cast<uint32_t>(tokens) * static_cast<uint32_t>(K) * 2u);
+  v.a = make_rsrc(act, static_cast<uint32_t>(rows) * static_cast<uint32_t>(K) * 2u);
   v.f = make_rsrc(factors, static_cast<uint32_t>(K >> 6) * 64u);
   v.w_step = n_tiles * 1024u;
   v.s_step = static_cast<uint32_t>(N) * 2u;
   v.w_voff = static_cast<uint32_t>(lane >> 5) * n_tiles * 512u + static_cast<uint32_t>(tile) * 512u +
              16u * (lane & 31);
   v.s_voff = static_cast<uint32_t>(tile) * 128u + 16u * (n16 & 7) + 8u * (n16 >> 3);
-  // rows past the last token read zeros: past the range where R tokens end it, by the test otherwise
-  v.a_voff = n16 % R < tokens
-                 ? static_cast<uint32_t>(n16 % R) * static_cast<uint32_t>(K) * 2u + 16u * kb
-                 : kOutOfRange;
+  v.a_voff = row >= 0 ? static_cast<uint32_t>(row) * static_cast<uint32_t>(K) * 2u + 16u * kb
+                      : kOutOfRange;  // reads zeros
   v.f_voff = static_cast<uint32_t>((4 * kb) % R) * 4u;
   return v;
 }
@@ -257,6 +257,14 @@ __device__ __forceinline__ void int4_groups(floatx4_t (&acc)[4], const Int4View&
   }
 }
 
+// work(rows of an instruction that a group takes) for that many token rows.
+template <bool kGather, typename Work>
+__device__ __forceinline__ void by_rows(int rows, Work work) {
+  if (!kGather || rows <= 4) work(std::integral_constant<int, 4>{});
+  else if (rows <= 8) work(std::integral_constant<int, 8>{});
+  else work(std::integral_constant<int, 16>{});
+}
+
 // The sums of a set's groups, together: afterwards lanes 0 .. 4 R - 1 have the token rows' totals.
 template <int R>
 __device__ __forceinline__ void add_places(floatx4_t (&acc)[4]) {
@@ -370,6 +378,7 @@ __device__ __forceinline__ uint32_t row_amax(const uint16_t* x, int t, int H) {
 
 template <int NS, bool kDsv2, int R>
 __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
+  constexpr bool kGather = R > 4;
   const pega_moe_few& p = f.p;
   __shared__ union {
     uint32_t tr[kWaves][2 * kSlotDwords];
@@ -379,8 +388,9 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
   __shared__ float s_w[kMaxTokens * kMaxTopk];
   __shared__ uint32_t s_mask[kMaxLocal];
   __shared__ uint16_t s_list[kMaxLocal];
-  __shared__ float s_tok[kMaxTokens];   // a token's factor for this slot's rows
-  __shared__ bool s_in[kMaxTokens];     // whether it has a route to the slot's expert
+  __shared__ float s_tok[kMaxTokens];   // a row's factor
+  __shared__ bool s_in[kMaxTokens];     // whether its token has a route to the slot's expert
+  __shared__ uint8_t s_row[kMaxTokens]; // its token
   __shared__ uint32_t s_amax[kMaxTokens];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -456,7 +466,8 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     if (mine == 0) {
       __syncthreads();
       if (tid == 0) p.slots[0] = live;
-      for (int i = tid; i < live; i += kThreads) p.slots[1 + i] = s_list[i];
+      for (int i = tid; i < live; i += kThreads)
+        p.slots[1 + i] = static_cast<int>(s_mask[s_list[i]] << 16 | s_list[i]);
       for (int r = tid; r < routes; r += kThreads) {
         p.topk_idx[r] = s_idx[r];
         p.topk_weight[r] = s_w[r];
@@ -469,8 +480,6 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     if (live > 0) shares = max(1, min(kMaxShares, f.routed_first / (live * tiles)));
   }
   __syncthreads();
-  const int my_token = (lane & 15) % R;
-  const float row_factor = my_token < T ? pow2(min(14 - exponent(s_amax[my_token]), 127)) : 0.0f;
   // waves 0 to 3 share K, or the workgroup's share of it, of the gate tile, 4 to 7 of the up tile
   constexpr int kPart = kWaves / 2;
   const int groups = H >> 5, half = wave / kPart, part = wave % kPart;
@@ -483,19 +492,22 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     const uint16_t* sc = p.shared_w13_scales;
     uint16_t* act = p.act_shared;
     float* factors = p.act_shared_factors;
+    int rows = T, row_of_mine = -1, expert = 0;
     if (shared) {
-      if (tid < kMaxTokens) {
+      if (tid < T) {
         s_tok[tid] = 1.0f;
         s_in[tid] = true;
+        s_row[tid] = static_cast<uint8_t>(tid);
       }
     } else {
-      const int expert = s_list[slot];
-      if (tid < T) {
-        float w = 0.0f;
-        for (int k = 0; k < p.topk; ++k)
-          if (s_idx[tid * p.topk + k] - p.global_start == expert) w += s_w[tid * p.topk + k];
-        s_tok[tid] = w * p.routed_scale;
-        s_in[tid] = ((s_mask[expert] >> tid) & 1u) != 0;
+      expert = s_list[slot];
+      const uint32_t mask = s_mask[expert];
+      if constexpr (kGather) rows = __builtin_amdgcn_readfirstlane(__popc(mask));
+      const bool has = ((mask >> (tid & 31)) & 1u) != 0;
+      if (tid < T && (has || !kGather)) {
+        row_of_mine = kGather ? __popc(mask & ((1u << tid) - 1u)) : tid;
+        s_in[row_of_mine] = has;
+        s_row[row_of_mine] = static_cast<uint8_t>(tid);
       }
       const long long elems = 2LL * inter * H;
       q = p.w13 + expert * (elems / 2);
@@ -503,10 +515,22 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
       act = p.act + static_cast<long long>(slot) * T * inter;
       factors = p.act_factors + static_cast<long long>(slot) * tiles * kMaxTokens;
     }
-    const Int4View v = int4_view<R>(q, sc, 2 * inter, H, tile + half * tiles, p.x, nullptr, T);
+    if (kGather) __syncthreads();
+    if (row_of_mine >= 0) {
+      float w = 0.0f;
+      for (int k = 0; k < p.topk; ++k)
+        if (s_idx[tid * p.topk + k] - p.global_start == expert) w += s_w[tid * p.topk + k];
+      s_tok[row_of_mine] = w * p.routed_scale;
+    }
     floatx4_t acc[4] = {};
-    int4_groups<R, 8, false>(acc, v, g0, g1, row_factor, lds.tr[wave]);
-    add_places<R>(acc);
+    by_rows<kGather>(rows, [&](auto r) {
+      constexpr int RU = decltype(r)::value;
+      const int row = (tid & 15) % RU, token = row >= rows ? -1 : kGather ? s_row[row] : row;
+      const float row_factor = token >= 0 ? pow2(min(14 - exponent(s_amax[token]), 127)) : 0.0f;
+      const Int4View v = int4_view<RU>(q, sc, 2 * inter, H, tile + half * tiles, p.x, nullptr, token, T);
+      int4_groups<RU, 8, false>(acc, v, g0, g1, row_factor, lds.tr[wave]);
+      add_places<RU>(acc);
+    });
     __syncthreads();  // the transpose slots become the sums' place
     // the lane read anew: what is computed from it would otherwise sit in registers for the whole loop
     const int lane = fresh(tid & 63);
@@ -515,11 +539,11 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
       for (int j = 0; j < 4; ++j) lds.red[wave][j][lane] = acc[j];
     }
     __syncthreads();
-    // a wave finishes a token's 64 columns: SwiGLU times the token's factor, in fp16 with the
+    // a wave finishes a row's 64 columns: SwiGLU times the row's factor, in fp16 with the
     // largest at 2^14 .. 2^15; the factor that undoes it takes the nibbles' 2^24 along
     const auto finish = [&](int t, float g, float u) {
       // x came in times 2^(14 - exponent), at most 2^127, and v as v 2^-24
-      const int e = max(10 + exponent(s_amax[t]), -103);
+      const int e = max(10 + exponent(s_amax[s_row[t]]), -103);
       const float a = s_in[t] ? silu_mul(__builtin_ldexpf(g, e), __builtin_ldexpf(u, e)) * s_tok[t] : 0.0f;
       const uint32_t top = wave_reduce_u32(__builtin_bit_cast(uint32_t, a) & 0x7fffffffu, MaxU32{});
       const int ae = top == 0 ? 0 : exponent(top);
@@ -531,7 +555,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     const auto place = [&](int of, int t, int up) {
       return p.partials + (((static_cast<long long>(pair) * shares + of) * T + t) * 2 + up) * 64 + lane;
     };
-    for (int t = wave; t < T; t += kWaves) {
+    for (int t = wave; t < rows; t += kWaves) {
       const int j = (lane >> 3) & 3, l = sum_lane(t, lane);
       float g = 0.0f, u = 0.0f;
 #pragma unroll
@@ -547,7 +571,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
       }
     }
     if (shares > 1 && last_of(&p.counters[H / 64 + pair], shares, &s_last)) {
-      for (int t = wave; t < T; t += kWaves) {
+      for (int t = wave; t < rows; t += kWaves) {
         float g[kMaxShares], u[kMaxShares], gs = 0.0f, us = 0.0f;
 #pragma unroll
         for (int i = 0; i < kMaxShares; ++i) {
@@ -569,11 +593,10 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
 // ---------------------------------------------------------------- launch 2
 template <int R>
 __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
+  constexpr bool kGather = R > 4;
   const pega_moe_few& p = f.p;
-  __shared__ union {
-    uint32_t tr[kWaves][2 * kSlotDwords];
-    floatx4_t red[kWaves][4][4 * R];
-  } lds;
+  __shared__ uint32_t s_tr[kWaves][2 * kSlotDwords];
+  __shared__ float s_sum[kWaves][R][64];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -592,22 +615,51 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
   const int sh0 = (max(lo - routed_end, 0) + cost - 1) / cost;
   const int sh1 = (max(hi - routed_end, 0) + cost - 1) / cost;
 
+  // A gathered slot's rows are its own tokens: its sums go to theirs in LDS, where they wait for the
+  // wave's other slots.  Otherwise rows are tokens throughout, and the sums stay in acc.
   floatx4_t acc[4] = {};
+  for (int t = 0; t < R; ++t) s_sum[wave][t][lane] = 0.0f;
+  const auto leave = [&](auto r, uint32_t mask) {
+    constexpr int RU = decltype(r)::value;
+    add_places<RU>(acc);
+#pragma unroll
+    for (int i = 0; i < RU; ++i) {
+      const bool some = mask != 0;
+      const int t = __builtin_ctz(mask | 0x10000u) & 15;
+      mask &= mask - 1;
+      if (some && lane >> 4 == i >> 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_sum[wave][t][32 * ((lane >> 3) & 1) + 8 * j + (lane & 7)] += acc[j][i & 3];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = floatx4_t{};
+  };
+  const auto groups = [&](const uint8_t* q, const uint16_t* scales, int K, const void* act,
+                          const float* factors, uint32_t mask, int g0, int g1) {
+    const int rows = kGather ? __popc(mask) : T;
+    by_rows<kGather>(rows, [&](auto r) {
+      constexpr int RU = decltype(r)::value;
+      const int row = (lane & 15) % RU;
+      const Int4View v = int4_view<RU>(q, scales, H, K, tile, act, factors, row < rows ? row : -1, rows);
+      int4_groups<RU, 4, true>(acc, v, g0, g1, 1.0f, s_tr[wave]);
+      if (kGather) leave(r, mask);
+    });
+  };
+  const uint32_t everyone = (1u << T) - 1u;
   for (int at = lo; at < min(hi, routed_end);) {
     const int s = at / per, g0 = at - s * per, g1 = min(per, g0 + min(hi, routed_end) - at);
-    const int expert = s < 63 ? __builtin_amdgcn_readlane(listed, 1 + s) : __builtin_amdgcn_readfirstlane(p.slots[1 + s]);
-    const long long elems = static_cast<long long>(H) * I;
-    const Int4View v = int4_view<R>(
-        p.w2 + expert * (elems / 2), p.w2_scales + expert * (elems / 32), H, I, tile,
-        p.act + static_cast<long long>(s) * T * I,
-        p.act_factors + static_cast<long long>(s) * (I >> 6) * kMaxTokens, T);
-    int4_groups<R, 4, true>(acc, v, g0, g1, 1.0f, lds.tr[wave]);
+    const uint32_t slot = static_cast<uint32_t>(
+        s < 63 ? __builtin_amdgcn_readlane(listed, 1 + s) : __builtin_amdgcn_readfirstlane(p.slots[1 + s]));
+    const long long elems = static_cast<long long>(H) * I, expert = slot & 0xffffu;
+    groups(p.w2 + expert * (elems / 2), p.w2_scales + expert * (elems / 32), I,
+           p.act + static_cast<long long>(s) * T * I,
+           p.act_factors + static_cast<long long>(s) * (I >> 6) * kMaxTokens, slot >> 16, g0, g1);
     at += g1 - g0;
   }
-  if (p.shared_kind == PEGA_SHARED_INT4) {
-    const Int4View v = int4_view<R>(static_cast<const uint8_t*>(p.shared_w2), p.shared_w2_scales, H,
-                                    p.shared_inter, tile, p.act_shared, p.act_shared_factors, T);
-    int4_groups<R, 4, true>(acc, v, sh0, sh1, 1.0f, lds.tr[wave]);
+  if (p.shared_kind == PEGA_SHARED_INT4 && sh0 < sh1) {
+    groups(static_cast<const uint8_t*>(p.shared_w2), p.shared_w2_scales, p.shared_inter, p.act_shared,
+           p.act_shared_factors, everyone, sh0, sh1);
   } else if (p.shared_kind == PEGA_SHARED_BF16) {
     const uint32_t row_bytes = static_cast<uint32_t>(p.shared_inter) * 2u;
     const __amdgpu_buffer_rsrc_t wr =
@@ -621,13 +673,9 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
     const __amdgpu_buffer_rsrc_t ar = make_rsrc(p.act_shared, static_cast<uint32_t>(T) * row_bytes);
     bf16_steps<4, 4>(acc, wr, w_voff, ar,
                      static_cast<uint32_t>(lane & 15) * row_bytes + 16u * (lane >> 4), sh0, sh1);
+    if (kGather) leave(std::integral_constant<int, 16>{}, everyone);
   }
-  add_places<R>(acc);
-  __syncthreads();
-  if (lane < 4 * R) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) lds.red[wave][j][lane] = acc[j];
-  }
+  if (!kGather) leave(std::integral_constant<int, R>{}, everyone);
   __syncthreads();
   const auto finish = [&](int t, int col, float sum) {
     const long long o = static_cast<long long>(t) * H + tile * 64 + col;
@@ -638,10 +686,10 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
     return p.partials + (static_cast<long long>(s) * T + t) * H + tile * 64 + col;
   };
   for (int o = tid; o < T * 64; o += kThreads) {
-    const int t = o >> 6, col = o & 63, j = (col >> 3) & 3, l = sum_lane(t, col);
+    const int t = o >> 6, col = o & 63;
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += lds.red[w][j][l][t & 3];
+    for (int w = 0; w < kWaves; ++w) sum += s_sum[w][t][col];
     if (f.splits == 1) finish(t, col, sum);
     else store_coherent(place(split, t, col), sum);
   }
@@ -661,8 +709,6 @@ template <int NS, bool kDsv2>
 void launch_w13(const FewArgs& f, unsigned grid, hipStream_t stream) {
   if (f.p.tokens <= 4)
     hipLaunchKernelGGL((few_w13_kernel<NS, kDsv2, 4>), dim3(grid), dim3(kThreads), 0, stream, f);
-  else if (f.p.tokens <= 8)
-    hipLaunchKernelGGL((few_w13_kernel<NS, kDsv2, 8>), dim3(grid), dim3(kThreads), 0, stream, f);
   else
     hipLaunchKernelGGL((few_w13_kernel<NS, kDsv2, 16>), dim3(grid), dim3(kThreads), 0, stream, f);
 }
@@ -747,7 +793,6 @@ PEGA_API int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream) {
   if (rc != kSuccess) return rc;
   const dim3 grid2(static_cast<unsigned>(p.hidden_dim / 64), static_cast<unsigned>(f.splits));
   if (p.tokens <= 4) hipLaunchKernelGGL((few_w2_kernel<4>), grid2, dim3(kThreads), 0, stream, f);
-  else if (p.tokens <= 8) hipLaunchKernelGGL((few_w2_kernel<8>), grid2, dim3(kThreads), 0, stream, f);
   else hipLaunchKernelGGL((few_w2_kernel<16>), grid2, dim3(kThreads), 0, stream, f);
   return launch_status("moe_few_tokens (W2)");
 }
