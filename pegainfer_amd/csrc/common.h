@@ -172,15 +172,6 @@ __device__ __forceinline__ void dma_b32(u32x4_t rsrc, uint32_t lds, uint32_t vof
   asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
                :: "{m0}"(lds), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
 }
-// dma_b128 where `now` (the same for the whole wave, every lane of which is active), nothing
-// otherwise, without a branch.
-__device__ __forceinline__ void dma_b128_if(bool now, u32x4_t rsrc, uint32_t lds, uint32_t voff,
-                                            uint32_t soff) {
-  const int lanes = __builtin_amdgcn_readfirstlane(now ? -1 : 0);
-  asm volatile("s_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
-               "s_mov_b64 exec, -1"
-               :: "{m0}"(lds), "v"(voff), "s"(rsrc), "s"(soff), "s"(lanes) : "memory");
-}
 template <int N>
 __device__ __forceinline__ void vm_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");

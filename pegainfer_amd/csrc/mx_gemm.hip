@@ -249,21 +249,23 @@ struct MxTile {
   static constexpr int kXRow = kXFormat == kMxE4M3 ? 128 : 64;  // bytes of a row of X in a stage
   static constexpr int kXLoadRows = 1024 / kXRow;
   static constexpr int kWLoads = BM / 16, kXLoads = BN / kXLoadRows;
-  static constexpr int kLoads = kWLoads + kXLoads, kSLoads = BM / 64 + (BN + 63) / 64;
-  static constexpr int P = (kLoads + kWaves - 1) / kWaves;    // data loads per wave and stage
+  static constexpr int kSLoads = BM / 64 + (BN + 63) / 64;
+  static constexpr int PW = (kWLoads + kWaves - 1) / kWaves;  // loads per wave and stage
+  static constexpr int PX = (kXLoads + kWaves - 1) / kWaves, P = PW + PX;
   static constexpr int PS = (kSLoads + kWaves - 1) / kWaves;  // scale loads per wave and four
   static constexpr int kX = BM * 64, kStage = kX + BN * kXRow;
   static constexpr int kFour = kSLoads * 1024;                // four steps' scales
   static constexpr int kS = NS * kStage, kLds = kS + 2 * kFour;
   static_assert(BM % 64 == 0 && BN % kXLoadRows == 0 && TN % 2 == 0, "tile shape");
-  static_assert(NS >= 3 && kLds <= 160 * 1024, "tile shape");
+  static_assert(NS >= 3 && NS <= 6 && kLds <= 160 * 1024, "tile shape");
 };
 
 // Workgroups go to the eight XCDs in turn; each XCD's are made to cover a compact part of the grid
 // of tiles (runs of the order that goes down panels four feature tiles wide), so that its L2 brings
 // in as few operand rows as it can.
-__device__ __forceinline__ void xcd_tile(int& tx, int& ty) {
-  const int gx = gridDim.x, gy = gridDim.y;
+// gy: of the grid's rows of tiles, those that are there.
+__device__ __forceinline__ void xcd_tile(int& tx, int& ty, int gy) {
+  const int gx = gridDim.x;
   const int total = gx * gy, id = ty * gx + tx;
   const int xcd = id & 7, each = total >> 3, more = total & 7;
   const int at = xcd * each + min(xcd, more) + (id >> 3);
@@ -272,6 +274,9 @@ __device__ __forceinline__ void xcd_tile(int& tx, int& ty) {
   ty = in / wide;
   tx = 4 * panel + in - ty * wide;
 }
+
+template <int V>
+using Int = std::integral_constant<int, V>;
 
 template <typename S, bool kGrouped>
 __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
@@ -284,20 +289,42 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
   const int wm = wave % S::WM, wn = wave / S::WM;
   const int c = lane & 15, g = lane >> 4;
   int tx = blockIdx.x, ty = blockIdx.y;
-  if constexpr (!kGrouped) xcd_tile(tx, ty);
+  int live = gridDim.y;  // blocks with rows
+  if constexpr (kGrouped) {
+    live = min(p.ntp[0], p.sorted_len) / p.bs;
+    if (ty >= live) return;
+  }
+  // grouped tiles of few rows share little, and lose 2% by the mapping; wide ones gain (256 x 128, 4096
+  // x 7168 over 48 experts of 341 rows: 879 and 542 us)
+  if constexpr (!kGrouped || BN >= 128) xcd_tile(tx, ty, live);
   const int m0 = tx * BM;
   int n0 = ty * BN;
   const int K = p.K, steps = K >> 7;
   long long expert = 0;
   if constexpr (kGrouped) {
-    const int mb = ty;
+    // up to BN / bs blocks of one expert (an expert's blocks follow each other): this one, if the
+    // number of the expert's blocks before it is a multiple of that, and those after it
+    const int mb = ty, take = max(BN / p.bs, 1);
     const int limit = p.N * p.top_k;
     const int e = __builtin_amdgcn_readfirstlane(p.expert_ids[mb]);
-    if (min(p.ntp[0], p.sorted_len) < (mb + 1) * p.bs || e < 0 || e >= p.experts) return;
+    if (e < 0 || e >= p.experts) return;
+    int before = 0, blocks = 1;
+    if (take > 1) {
+      for (int at = mb; at > 0;) {
+        const uint64_t other = ~__ballot(lane < at && p.expert_ids[max(at - 1 - lane, 0)] == e);
+        const int same = other == 0 ? 64 : __builtin_ctzll(other);
+        before += same;
+        at -= 64;
+        if (same < 64) break;
+      }
+      if (before % take != 0) return;
+      const uint64_t other = ~__ballot(mb + lane < live && p.expert_ids[min(mb + lane, live - 1)] == e);
+      blocks = min(take, other == 0 ? 64 : __builtin_ctzll(other));
+    }
     expert = e;
     for (int i = tid; i < BN; i += S::kThreads) {
       int sid = limit;
-      if (i < p.bs && mb * p.bs + i < p.sorted_len) sid = p.sorted_ids[mb * p.bs + i];
+      if (i < blocks * p.bs && mb * p.bs + i < p.sorted_len) sid = p.sorted_ids[mb * p.bs + i];
       s_sid[i] = static_cast<unsigned>(sid) < static_cast<unsigned>(limit) ? sid : -1;
     }
     __syncthreads();
@@ -317,25 +344,21 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
     const int sid = s_sid[min(r, BN - 1)];
     return sid < 0 ? kOutOfRange : static_cast<uint32_t>(sid / p.top_k) * row_bytes;
   };
-  // This wave's loads of a stage.
-  u32x4_t rsrc[P];
-  uint32_t dst[P], voff[P], soff_step[P];
+  // This wave's loads of a stage (a repeat brings the same): PW of W, then PX of X.
+  u32x4_t w_rsrc = rsrc_words(p.wq + w_first * w_bytes, static_cast<uint32_t>(w_rows) * w_bytes);
+  u32x4_t x_rsrc = rsrc_words(p.xq + static_cast<long long>(n0) * x_bytes, static_cast<uint32_t>(x_rows) * x_bytes);
+  const uint32_t w_size = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w_rsrc[2])));
+  const uint32_t x_size = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x_rsrc[2])));
+  uint32_t dst[P], voff[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) {
-    const int i = min(wave * P + j, S::kLoads - 1);  // a repeat brings the same
-    const bool x = i >= S::kWLoads;
+    const bool x = j >= S::PW;
+    const int i = x ? min(wave * S::PX + j - S::PW, S::kXLoads - 1) : min(wave * S::PW + j, S::kWLoads - 1);
     const int rows_per = x ? S::kXLoadRows : 16, pieces = 64 / rows_per;
-    const int r = (x ? i - S::kWLoads : i) * rows_per + lane / pieces;
+    const int r = i * rows_per + lane / pieces;
     const int swz = pieces == 8 ? r & 7 : (r >> 1) & 3;
-    const uint32_t piece = static_cast<uint32_t>((lane % pieces) ^ swz);
-    const uint32_t row_bytes = x ? x_bytes : w_bytes;
-    const long long first = x ? n0 : w_first;
-    rsrc[j] = rsrc_words((x ? p.xq : p.wq) + first * row_bytes,
-                         static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
-                             static_cast<int>((x ? x_rows : w_rows) * row_bytes))));
-    dst[j] = lds0 + (x ? S::kX : 0) + 1024u * static_cast<uint32_t>(x ? i - S::kWLoads : i);
-    soff_step[j] = x ? S::kXRow : 64;
-    voff[j] = row_off(x, r, row_bytes) + 16u * piece;
+    dst[j] = lds0 + (x ? S::kX : 0) + 1024u * static_cast<uint32_t>(i);
+    voff[j] = row_off(x, r, x ? x_bytes : w_bytes) + 16u * static_cast<uint32_t>((lane % pieces) ^ swz);
   }
   u32x4_t s_rsrc[S::PS];
   uint32_t s_dst[S::PS], s_voff[S::PS];
@@ -351,24 +374,29 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
     const int r = 64 * (x ? i - BM / 64 : i) + lane;
     s_voff[j] = x && r >= BN ? kOutOfRange : row_off(x, r, s_bytes);
   }
-  // Past the last step every lane is out of range and brings zeros that nothing reads: a branch
-  // there would cut the step in two, and the compiler moves products across it.
-  const auto stage_in = [&](int step, int st) {
-    const uint32_t past = step < steps ? 0u : kOutOfRange;
+  // Stages come in turn; past the last one the operands have no bytes, and the loads bring zeros that
+  // nothing reads: a branch there would cut the step in two, and the compiler moves products across it.
+  uint32_t w_at = 0, x_at = 0;
+  int to_come = steps;
+  const auto stage_in = [&](uint32_t st) {
+    w_rsrc[2] = to_come > 0 ? w_size : 0u;
+    x_rsrc[2] = to_come > 0 ? x_size : 0u;
 #pragma unroll
     for (int j = 0; j < P; ++j)
-      dma_b128(rsrc[j], dst[j] + static_cast<uint32_t>(st), voff[j] | past,
-               past ? 0u : soff_step[j] * static_cast<uint32_t>(step));
+      dma_b128(j < S::PW ? w_rsrc : x_rsrc, dst[j] + st, voff[j], j < S::PW ? w_at : x_at);
+    w_at += 64;
+    x_at += S::kXRow;
+    --to_come;
   };
   // Scales come for four steps at a time, 16 bytes a row (a word a step would touch as many lines
   // four times as often: 4096 x 4096 x 7168 in MXFP4 84 us instead of 68 without scale loads); the
   // last four are steps - 4 .. steps - 1, wherever that starts.
   const auto four_first = [&](int four) { return min(4 * four, steps - 4); };
-  const auto scales_in = [&](int four, bool now) {
+  const auto scales_in = [&](int four) {
 #pragma unroll
     for (int j = 0; j < S::PS; ++j)
-      dma_b128_if(now, s_rsrc[j], s_dst[j] + static_cast<uint32_t>((four & 1) * S::kFour), s_voff[j],
-                  4u * static_cast<uint32_t>(max(four_first(four), 0)));
+      dma_b128(s_rsrc[j], s_dst[j] + static_cast<uint32_t>((four & 1) * S::kFour), s_voff[j],
+               4u * static_cast<uint32_t>(four_first(four)));
   };
   struct WFrags {
     u32x4_t w[TM];
@@ -384,10 +412,9 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
   const int x_at1 = 16 * ((4 + g) ^ (c & 7));
   const uint8_t* sw_rd = smem + S::kS + (wm * TM * 16 + c) * 16 + g;
   const uint8_t* sx_rd = smem + S::kS + (BM + wn * TN * 16 + c) * 16 + g;
-  // where a step's scale bytes are
-  const auto scale_at = [&](int s) {
-    const int four = s >> 2;
-    return (four & 1) * S::kFour + 4 * (s - four_first(four));
+  // where the scale bytes of a four's first step are
+  const auto scales_at = [&](int four) {
+    return (four & 1) * S::kFour + 4 * min(4 * four - four_first(four), 3);
   };
   const auto read_w = [&](WFrags& f, int t, int st, int sc) {
     f.w[t] = *reinterpret_cast<const u32x4_t*>(w_rd + st + 1024 * t);
@@ -401,12 +428,12 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
   };
   floatx4_t acc[TM][TN] = {};
 
-  scales_in(0, true);
+  scales_in(0);
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) stage_in(i, i * S::kStage);
+  for (int i = 0; i < NS - 1; ++i) stage_in(i * S::kStage);
   vm_wait<(NS - 2) * P>();
   lds_barrier();
-  int st = 0, st_in = (NS - 1) * S::kStage;
+  int st_now = 0, st_in_now = (NS - 1) * S::kStage;
   const auto next = [](int at) { return at + S::kStage == NS * S::kStage ? 0 : at + S::kStage; };
   // Step s multiplies the rows' fragments one after another, each read while the one before it is
   // multiplied.  Half way the next stage has landed (each wave waits for its own loads, the barrier
@@ -418,20 +445,26 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
 #pragma unroll
   for (int t = 0; t < TM; ++t) read_w(wa, t, 0, 0);
   read_x(x[0], 0, 0, 0);
-  const auto step = [&](const WFrags& w, WFrags& w_next, int s) {
-    // after the last step a stage that nothing uses
-    const int st_next = next(st), sc = scale_at(s), sc_next = scale_at(min(s + 1, steps - 1));
+  // Steps go four at a time, whose scales lie one after another from sc on (the next four's from
+  // sc_four on); with a ring of four stages every place in it is then a constant.
+  const auto step = [&](auto of_four, const WFrags& w, WFrags& w_next, int four, int sc, int sc_four) {
+    constexpr int Q = decltype(of_four)::value;
+    const int st = NS == 4 ? Q * S::kStage : st_now, st_next = NS == 4 ? (Q + 1) % 4 * S::kStage : next(st_now);
+    const int st_in = NS == 4 ? (Q + 3) % 4 * S::kStage : st_in_now;
+    const int sc_now = sc + 4 * Q, sc_next = Q == 3 ? sc_four : sc + 4 * Q + 4;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       if (j == kMid) {
-        vm_wait<(NS - 3) * P>();
+        // loads since the next stage's: NS - 3 stages, and scales where a four's first step is among
+        // theirs (all of them have landed two steps on, before anything reads them)
+        vm_wait<(NS - 3) * P + (Q >= 1 && Q <= 2 && Q <= NS - 3 ? S::PS : 0)>();
         lds_barrier();
-        // the four steps after this one's four, whose place every wave has read to the end
-        scales_in((s >> 2) + 1, (s & 3) == 0 && s + 4 < steps);
-        stage_in(s + NS - 1, st_in);
-        st_in = next(st_in);
+        // the four steps after these, in whose place every wave has read to the end; after the last
+        // the same again
+        if constexpr (Q == 0) scales_in(four + 1);
+        stage_in(static_cast<uint32_t>(st_in));
       }
-      if (j + 1 < TN) read_x(x[(j + 1) & 1], j + 1, st, sc);
+      if (j + 1 < TN) read_x(x[(j + 1) & 1], j + 1, st, sc_now);
       else read_x(x[0], 0, st_next, sc_next);
       if (j >= kMid) {
 #pragma unroll
@@ -444,14 +477,23 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
                                          x[j & 1].s, acc[t][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    st = st_next;
+    st_now = next(st_now);
+    st_in_now = next(st_in_now);
   };
-  int s = 0;
-  for (; s + 1 < steps; s += 2) {
-    step(wa, wb, s);
-    step(wb, wa, s + 1);
+  int four = 0, sc = 0;
+  for (; four < steps >> 2; ++four) {
+    const int sc_four = scales_at(four + 1);
+    step(Int<0>{}, wa, wb, four, sc, sc_four);
+    step(Int<1>{}, wb, wa, four, sc, sc_four);
+    step(Int<2>{}, wa, wb, four, sc, sc_four);
+    step(Int<3>{}, wb, wa, four, sc, sc_four);
+    sc = sc_four;
   }
-  if (s < steps) step(wa, wb, s);
+  const int left = steps & 3;
+  if (left > 0) step(Int<0>{}, wa, wb, four, sc, 0);
+  if (left > 1) step(Int<1>{}, wb, wa, four, sc, 0);
+  if (left > 2) step(Int<2>{}, wa, wb, four, sc, 0);
+  vm_wait<0>();  // nothing lands in LDS that is another workgroup's by then
 
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
@@ -465,9 +507,6 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
     }
   }
 }
-
-template <int V>
-using Int = std::integral_constant<int, V>;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -505,11 +544,12 @@ constexpr int kTileMinK = 512;
 
 // The tile shapes, smallest first, with what a step of 128 k costs a CU that has one tile, and each
 // of several, and what a tile costs besides its steps (its start, and its results, which the large
-// ones write while nothing else runs on their CU), in ns.  Measured with MXFP8 rows at K = 7168
-// and 2048 (64 x 64 to 256 x 256: 200 rows x 4096 x 7168 21 / 27 / 36 / 51 / 85 us, 4096 rows x 7168 x
-// 2048 117 / 85 / 89 / 75 / 67 us); MXFP4 rows are 5 to 30% faster everywhere and rank the shapes alike.
-// More stages where they fit: the loads' latency is what a step waits for (256 x 128 with three and
-// four stages, 4096 x 4096 x 7168: 121 and 101 us).
+// ones write while nothing else runs on their CU), in ns.  Measured with MXFP8 rows, 64 x 64 to
+// 256 x 256: 256 rows x 4096 x 7168 19 / 26 / 35 / 51 / 86 us, 1024 rows 57 / 46 / 40 / 54 / 91, 4096 rows 203 /
+// 168 / 154 / 113 / 98; over 106 sizes the chosen shape is within 5% of the best one (rms).  MXFP4
+// rows are 5 to 30% faster everywhere and rank the shapes alike.  Four stages make every place in
+// the ring a constant; 64 x 64 tiles, whose steps are shortest, gain more from a fifth (256 rows x 4096 x
+// 7168 22.2 and 18.8 us), and 256 x 256 of MXFP8 have room for three.
 template <int F> using Tile64 = MxTile<F, 2, 2, 2, 2, 5>;
 template <int F> using Tile128x64 = MxTile<F, 2, 2, 4, 2, 4>;
 template <int F> using Tile128 = MxTile<F, 2, 2, 4, 4, 4>;
@@ -518,11 +558,11 @@ template <int F> using Tile256 = MxTile<F, 4, 2, 4, 8, F == kMxE4M3 ? 3 : 4>;
 struct TileCost {
   int m, n, alone, each, besides;
 };
-constexpr TileCost kTileCosts[] = {{64, 64, 370, 260, 200},
-                                   {128, 64, 480, 385, 400},
-                                   {128, 128, 630, 600, 700},
-                                   {256, 128, 900, 870, 4000},
-                                   {256, 256, 1450, 1450, 8000}};
+constexpr TileCost kTileCosts[] = {{64, 64, 270, 215, 900},
+                                   {128, 64, 385, 335, 1900},
+                                   {128, 128, 570, 600, 3000},
+                                   {256, 128, 840, 950, 6000},
+                                   {256, 256, 1400, 1450, 9500}};
 
 int best_tile(int M, int N, int K, int cu) {
   int best = 0;
@@ -543,10 +583,11 @@ int dense_launch(const MxArgs& a, hipStream_t stream, const char* name) {
   if (cu <= 0) return fail(kInvalidValue, "%s: no device", name);
   if (ceil_div(a.N, 32) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
   const long long tiles64 = static_cast<long long>(ceil_div(a.M, 64)) * ceil_div(a.N, 64);
-  // The streaming kernel to 16 rows, and while 64 x 64 tiles would leave half of the CUs idle, since
-  // its waves share K (64 rows x 4096 x 7168, 64 tiles: 10.6 against 19.6 us; 128 rows, 128 tiles: 15.3
-  // and 21.6; 64 rows x 9728 x 2560, 152 tiles: 12.8 and 10.1).
-  if (a.N <= 16 || a.K < kTileMinK || tiles64 <= cu / 2) {
+  // The streaming kernel to 16 rows, and while 64 x 64 tiles would leave many CUs idle, since its
+  // waves share K: half of the CUs where K is long or a workgroup has all rows (64 rows x 4096 x 7168, 64
+  // tiles: 10.6 against 18.4 us; 128 rows, 128 tiles: 15.1 and 18.5; 32 rows x 7168 x 2048, 112 tiles: 5.7
+  // and 6.9), else three quarters (96 rows x 2816 x 2048, 88 tiles: 7.1 and 6.1).
+  if (a.N <= 16 || a.K < kTileMinK || tiles64 <= (a.K > 4096 || a.N <= 32 ? cu / 2 : cu / 4)) {
     // To 16 rows as many workgroups as there are (9728 x 2560, 16 rows: 608 of 16 features 7.6 us,
     // 304 of 32 8.4); beyond, more features a workgroup, which read X less often, as long as
     // three quarters of the CUs have one (64 rows x 4096 x 7168 with 1 / 2 / 4 sets of 16: 15.7 / 10.6 /
@@ -587,7 +628,17 @@ int grouped_launch(const MxArgs& a, int ep_size, hipStream_t stream, const char*
   const double reached = a.experts * (1.0 - __builtin_exp(local * __builtin_log1p(-1.0 / (a.experts + 1e-9))));
   const double live = reached > local / a.bs ? reached : local / a.bs;
   const double units = live * ceil_div(a.M, 128);
-  if (a.bs > 32) {
+  // Tiles as wide as the experts' rows: 256 x 128 (and then a mapping that keeps an expert's tiles
+  // on one XCD) from 64 rows an expert on, 128 x 64 from 32, or where a block is over 32.  MXFP8 in
+  // 128 x 64 / 256 x 128: 4096 x 7168 over 48 experts at 43, 85, 341 rows each 182 / 186, 265 / 207, 730 /
+  // 542 us; 2816 x 2048 over 64 at 47, 94, 375 rows 57 / 65, 86 / 89, 244 / 222 us.  In 128 x 32 / 128 x 64 with
+  // blocks of 32: 2816 x 2048 at 47 rows 73 / 61 us, 4096 x 7168 at 21 rows 162 / 167 us.
+  const double rows = local / a.experts;
+  if (a.K >= kTileMinK && rows >= 64.0) {
+    launch_tile<Tile256x128<kXFormat>, true>(a, blocks, stream);
+    return launch_status(name);
+  }
+  if (a.bs > 32 || (a.K >= kTileMinK && rows >= 32.0)) {
     if (a.K < kTileMinK) launch_stream<kXFormat, 4, 1, 4, true>(a, blocks, stream);
     else launch_tile<Tile128x64<kXFormat>, true>(a, blocks, stream);
     return launch_status(name);

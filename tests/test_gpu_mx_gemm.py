@@ -175,6 +175,28 @@ def test_grouped_skewed_and_without_local_routes():
         assert (bf(host(y)) == 9).all()
 
 
+@pytest.mark.parametrize("name", ["fp8", "fp4"])
+@pytest.mark.parametrize("tokens,bs,m,k,lean", [
+    (1500, 8, 272, 512, True), (1500, 16, 272, 1152, False), (700, 48, 528, 640, True), (300, 32, 144, 768, False),
+    (500, 64, 256, 512, False), (160, 8, 272, 640, False), (2300, 64, 16, 640, True)])
+def test_grouped_blocks_of_one_expert_together(tokens, bs, m, k, lean, name):
+    """Many blocks an expert, which workgroups take several of: all on two experts (of a run of over
+    64 blocks), or spread unevenly."""
+    from pegainfer_amd import ops
+    g = np.random.default_rng(tokens + bs)
+    idx, routing = _route(tokens, 2, 16, 4, 8, bs, tokens, lean=lean)
+    w, wv = _operand(g, 4 * m, k, "fp4")
+    x, xv = _operand(g, tokens, k, name)
+    y = torch.full((tokens * 2, m), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.mx_grouped_gemm(routing, x, w, None, y, top_k=2, mul_topk_weights=False, size_m=tokens)
+    got, flat = bf(host(y)).astype(np.float64), idx.reshape(-1) - 8
+    for e in range(4):
+        r = np.flatnonzero(flat == e)
+        if len(r):
+            _check(got[r], *_bounds(xv[r // 2], wv.reshape(4, m, k)[e], name), f"expert {e}")
+    assert (got[(flat < 0) | (flat > 3)] == 3).all()
+
+
 def test_repeat_and_graph_give_the_same_bits():
     from pegainfer_amd import layer, ops
     g = np.random.default_rng(2)
