@@ -776,6 +776,14 @@ PEGA_API int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream) {
                         p.shared_kind == PEGA_SHARED_INT4 ? p.shared_w2_scales : nullptr};
   for (const void* v : vecs)
     if (!aligned16(v)) return fail(kNotSupported, "moe_few_tokens: buffers must be 16-byte aligned");
+  // out may be residual, place for place, or any of what only launch 1 reads
+  const long long row_bytes = 2LL * p.hidden_dim * p.tokens, route_bytes = 4LL * p.tokens * p.topk;
+  const long long logit_bytes = 4LL * p.tokens * p.n_experts;
+  if ((p.residual != p.out && overlap(p.residual, row_bytes, p.out, row_bytes)) ||
+      overlap(p.topk_weight, route_bytes, p.logits, logit_bytes) ||
+      overlap(p.topk_idx, route_bytes, p.logits, logit_bytes) ||
+      overlap(p.topk_weight, route_bytes, p.topk_idx, route_bytes))
+    return fail(kInvalidValue, "moe_few_tokens: buffers overlap");
   const int cu = current_cu_count();
   if (cu <= 0) return fail(kInvalidValue, "moe_few_tokens: no device");
   FewArgs f{p, 0, p.inter / 64, few_splits(p.hidden_dim), p.shared_kind == PEGA_SHARED_BF16 ? 3 : 1, 0, 0};

@@ -590,15 +590,15 @@ int dense_launch(const MxArgs& a, hipStream_t stream, const char* name) {
   if (a.N <= 16 || a.K < kTileMinK || tiles64 <= (a.K > 4096 || a.N <= 32 ? cu / 2 : cu / 4)) {
     // To 16 rows as many workgroups as there are (9728 x 2560, 16 rows: 608 of 16 features 7.6 us,
     // 304 of 32 8.4); beyond, more features a workgroup, which read X less often, as long as
-    // three quarters of the CUs have one (64 rows x 4096 x 7168 with 1 / 2 / 4 sets of 16: 15.7 / 10.6 /
-    // 14.5 us).
+    // three quarters of the CUs have one (64 rows x 4096 x 7168 with 1 / 2 / 4 sets of 16: 14.2 / 10.6 /
+    // 14.3 us; 32 rows x 7168 x 2048 7.9 / 5.7 / 7.9).
     const int blocks = ceil_div(a.N, 32);
     const auto enough = [&](int mr) {
       return a.M % (16 * mr) == 0 && 4LL * (a.M / (16 * mr)) * blocks >= 3LL * cu;
     };
     if (a.N <= 16) launch_stream<kXFormat, 4, 1, 1, false>(a, 1, stream);
-    else if (a.N > 32 && enough(4)) launch_stream<kXFormat, 4, 4, 2, false>(a, blocks, stream);
-    else if (a.N > 32 && enough(2)) launch_stream<kXFormat, 4, 2, 2, false>(a, blocks, stream);
+    else if (enough(4)) launch_stream<kXFormat, 4, 4, 2, false>(a, blocks, stream);
+    else if (enough(2)) launch_stream<kXFormat, 4, 2, 2, false>(a, blocks, stream);
     else launch_stream<kXFormat, 4, 1, 2, false>(a, blocks, stream);
     return launch_status(name);
   }

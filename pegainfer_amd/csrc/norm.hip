@@ -159,13 +159,17 @@ void launch_norm(bool x32, const void* x, const uint16_t* residual, const uint16
                  double eps, uint16_t* residual_out, uint16_t* normed, uint8_t* codes,
                  uint8_t* scales, int rows, int hidden, hipStream_t stream) {
   const int waves = ceil_div(hidden / 8, 64 * CH), per = waves == 1 ? 4 : 1;
-  const dim3 grid(ceil_div(rows, per)), block(64 * waves, per);
-  if (x32)
-    hipLaunchKernelGGL((add_rmsnorm_kernel<CH, true>), grid, block, 0, stream, x, residual,
-                       weight, eps, residual_out, normed, codes, scales, rows, hidden);
-  else
-    hipLaunchKernelGGL((add_rmsnorm_kernel<CH, false>), grid, block, 0, stream, x, residual,
-                       weight, eps, residual_out, normed, codes, scales, rows, hidden);
+  const auto kernel = x32 ? add_rmsnorm_kernel<CH, true> : add_rmsnorm_kernel<CH, false>;
+  const int most = (1 << 25) / waves;  // rows a launch: below 2^32 threads, a multiple of four where per is
+  for (int r = 0; r < rows; r += most) {
+    const int n = rows - r < most ? rows - r : most;
+    const long long at = static_cast<long long>(r) * hidden;
+    hipLaunchKernelGGL(kernel, dim3(ceil_div(n, per)), dim3(64 * waves, per), 0, stream,
+                       static_cast<const uint8_t*>(x) + (x32 ? 4 : 2) * at, residual ? residual + at : nullptr,
+                       weight, eps, residual_out ? residual_out + at : nullptr, normed ? normed + at : nullptr,
+                       codes ? codes + at : nullptr, scales ? scales + at / kMxBlock : nullptr, n, hidden);
+    if (rows - r <= most) break;
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

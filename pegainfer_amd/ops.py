@@ -762,7 +762,8 @@ def moe_few_tokens(workspace: FewTokensWorkspace, x: torch.Tensor, logits: torch
 
     x: the normed rows, bf16 [T, hidden]; logits: f32 [T, n_experts]; w13, w2: the local experts'
     INT4 packages; shared: None, a pair of bf16 matrices (gate-then-up [2 Is, hidden], down
-    [hidden, Is]) or a pair of one-expert INT4 packages.  out may be x or residual itself."""
+    [hidden, Is]) or a pair of one-expert INT4 packages.  out may be x or residual itself, and
+    is otherwise apart from residual."""
     ws = workspace
     if x.dim() != 2:
         raise ValueError("x must be bf16 [tokens, hidden]")

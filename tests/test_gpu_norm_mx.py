@@ -307,3 +307,18 @@ def test_offsets_past_32_bits(name, n):
     assert (a.codes[:rows - 5].view(-1, block, b.codes.shape[1]) == b.codes).all()
     assert torch.equal(a.codes[rows - 5:], b.codes[7:12])
     assert torch.equal(a.scales[rows - 5:], b.scales[7:12])
+
+
+def test_norm_of_more_rows_than_a_launch_takes():
+    from pegainfer_amd import ops
+    rows, cols, block = (1 << 26) + 5, 8, 1 << 12
+    torch.manual_seed(0)
+    some, w = torch.randn(block, cols, device="cuda").bfloat16(), torch.randn(cols, device="cuda").bfloat16()
+    want, y = torch.empty_like(some), torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    ops.add_rmsnorm(some, some, w, 1e-6, normed=want)
+    x = torch.empty_like(y)
+    x[:rows - 5].view(-1, block, cols).copy_(some)
+    x[rows - 5:].copy_(some[7:12])
+    ops.add_rmsnorm(x, x, w, 1e-6, normed=y)
+    assert (y[:rows - 5].view(-1, block, cols).view(torch.int16) == want.view(torch.int16)).all()
+    assert torch.equal(y[rows - 5:], want[7:12])

@@ -249,6 +249,14 @@ def test_few_tokens_refuses(kw, code):
     assert _few_call(**kw) == code
 
 
+@pytest.mark.parametrize("kw", [
+    dict(out=A << 40, residual=(A << 40) + 256), dict(out=(A << 40) + 256, residual=A << 40),
+    dict(logits=A << 40, topk_weight=(A << 40) + 64), dict(logits=A << 40, topk_idx=(A << 40) + 64),
+    dict(topk_weight=A << 40, topk_idx=(A << 40) + 16)])
+def test_few_tokens_refuses_overlaps(kw):
+    assert _few_call(**kw) == 1
+
+
 def test_few_tokens_struct_matches_the_header(tmp_path):
     import ctypes
     import os
