@@ -583,11 +583,13 @@ int dense_launch(const MxArgs& a, hipStream_t stream, const char* name) {
   if (cu <= 0) return fail(kInvalidValue, "%s: no device", name);
   if (ceil_div(a.N, 32) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
   const long long tiles64 = static_cast<long long>(ceil_div(a.M, 64)) * ceil_div(a.N, 64);
-  // The streaming kernel to 16 rows, and while 64 x 64 tiles would leave many CUs idle, since its
-  // waves share K: half of the CUs where K is long or a workgroup has all rows (64 rows x 4096 x 7168, 64
+  // The streaming kernel while 64 x 64 tiles would leave many CUs idle, since its waves share K: a
+  // quarter of the CUs to 16 rows (16 rows x 9728 x 2560, 152 tiles: 7.5 against 8.9 us, x 14336 x 4096,
+  // 224 tiles: 17.0 and 10.8), half where K is long or a workgroup has all rows (64 rows x 4096 x 7168, 64
   // tiles: 10.6 against 18.4 us; 128 rows, 128 tiles: 15.1 and 18.5; 32 rows x 7168 x 2048, 112 tiles: 5.7
   // and 6.9), else three quarters (96 rows x 2816 x 2048, 88 tiles: 7.1 and 6.1).
-  if (a.N <= 16 || a.K < kTileMinK || tiles64 <= (a.K > 4096 || a.N <= 32 ? cu / 2 : cu / 4)) {
+  const int most = a.N <= 16 ? 3 * cu / 4 : a.K > 4096 || a.N <= 32 ? cu / 2 : cu / 4;
+  if (a.K < kTileMinK || tiles64 <= most) {
     // To 16 rows as many workgroups as there are (9728 x 2560, 16 rows: 608 of 16 features 7.6 us,
     // 304 of 32 8.4); beyond, more features a workgroup, which read X less often, as long as
     // three quarters of the CUs have one (64 rows x 4096 x 7168 with 1 / 2 / 4 sets of 16: 14.2 / 10.6 /
@@ -643,11 +645,14 @@ int grouped_launch(const MxArgs& a, int ep_size, hipStream_t stream, const char*
     else launch_tile<Tile128x64<kXFormat>, true>(a, blocks, stream);
     return launch_status(name);
   }
-  // Short blocks: tiles of 128 x 32 where they fill the CUs, and for long K several times over;
-  // else the streaming kernel, whose waves share K.  Streaming / tiled, MXFP8: 4096 x 7168 over 48 of
-  // 384 experts at 2, 8, 64, 160 tokens 7.8 / 16.8, 29.5 / 41.1, 113 / 115, 155 / 145 us; 7168 x 2048
-  // at 64 tokens 87 / 57; 2816 x 2048 over 64 experts at 3 tokens 17 / 12.5 us.
-  const bool tiled = a.K >= kTileMinK && units >= (a.K >= 4096 ? 5.0 * cu : 1.0 * cu);
+  // Short blocks: tiles of 128 x 32, or, where too few of them have rows, the streaming kernel, whose
+  // waves share K.  Rows of 2 KB of weights or multiples of it meet in few memory channels when
+  // streamed; other long ones stream as well until there are several tiles a CU.  Streaming / tiled, MXFP8,
+  // in us: 4096 features of k 4096 in 8, 16, 63 experts 21 / 14, 40 / 27, 176 / 105; of k 5120 in 2, 4, 16
+  // 9 / 11, 15 / 13, 50 / 38; of k 7168 in 2, 10, 25, 62 10 / 14, 34 / 42, 78 / 87, 195 / 184; 2816 of k
+  // 2048 in 6, 18 8.2 / 6.5, 17.5 / 12.1.
+  const double enough = a.K <= 2560 ? 0.25 * cu : a.K < 6144 || a.K % 4096 == 0 ? 0.5 * cu : 5.0 * cu;
+  const bool tiled = a.K >= kTileMinK && units >= enough;
   if (tiled) launch_tile<MxTile<kXFormat, 4, 1, 2, 2, 6>, true>(a, blocks, stream);
   else if (a.bs > 16) launch_stream<kXFormat, 4, 1, 2, true>(a, blocks, stream);
   else if (kXFormat == kMxE4M3 && a.M % 32 == 0) launch_stream<kXFormat, 4, 2, 1, true>(a, blocks, stream);
