@@ -511,7 +511,8 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 int mx_gemm_checks(const char* name, const MxArgs& a, int x_format) {
-  if (!a.wq || !a.ws || !a.xq || !a.xs || !a.y) return fail(kInvalidValue, "%s: null pointer", name);
+  // no rows: nothing to do, and empty tensors have no address
+  if (a.N != 0 && (!a.wq || !a.ws || !a.xq || !a.xs || !a.y)) return fail(kInvalidValue, "%s: null pointer", name);
   if (a.M <= 0 || a.N < 0 || a.K <= 0)
     return fail(kInvalidValue, "%s: bad shape M=%d N=%d K=%d", name, a.M, a.N, a.K);
   if (x_format != kMxE4M3 && x_format != kMxE2M1)

@@ -184,8 +184,10 @@ PEGA_API int pega_add_rmsnorm(const void* x, bool x_is_f32, const uint16_t* resi
                               const uint16_t* weight, double eps, uint16_t* residual_out,
                               uint16_t* normed, uint8_t* mxfp8_codes, uint8_t* mxfp8_scales,
                               int rows, int hidden_dim, hipStream_t stream) {
-  if (!x || !weight || rows < 0 || hidden_dim <= 0 || !(eps >= 0.0))
+  if (rows < 0 || hidden_dim <= 0 || !(eps >= 0.0))
     return fail(kInvalidValue, "add_rmsnorm: bad arguments (rows=%d hidden=%d)", rows, hidden_dim);
+  if (rows == 0) return kSuccess;  // empty tensors have no address
+  if (!x || !weight) return fail(kInvalidValue, "add_rmsnorm: null pointer");
   if (!residual_out && !normed && !mxfp8_codes)
     return fail(kInvalidValue, "add_rmsnorm: no output");
   if (!mxfp8_codes != !mxfp8_scales)
@@ -196,7 +198,6 @@ PEGA_API int pega_add_rmsnorm(const void* x, bool x_is_f32, const uint16_t* resi
   if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(residual_out) ||
       !aligned16(normed) || !aligned16(mxfp8_codes) || (reinterpret_cast<uintptr_t>(mxfp8_scales) & 3u))
     return fail(kNotSupported, "add_rmsnorm: buffers must be 16-byte aligned (scales 4)");
-  if (rows == 0) return kSuccess;
   // An output may be the bf16 buffer of x or of residual, row for row; any other overlap would
   // let one row's stores meet another row's loads.
   const long long n = static_cast<long long>(rows) * hidden_dim;

@@ -180,3 +180,17 @@ def test_few_token_block(tokens):
     _check_bf16(host(y2), want_y, "normed after")
     _same(q, want_y)
     _replays(step, (x, res), (s, y, out, y2, q.codes, q.scales), g)
+
+
+def test_no_rows():
+    from pegainfer_amd import ops
+    e = lambda c: torch.zeros(0, c, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    w, _ = _mx_weight(np.random.default_rng(0), 128, 128)
+    for f in ops.MxFormat:
+        q = ops.MxTensor.empty(0, 128, f)
+        ops.mx_quantize(e(128), q)
+        ops.mx_swiglu_quantize(e(256), q)
+        ops.mx_dequantize(q, e(128))
+        ops.mx_gemm(w, q, e(128))
+    ops.add_rmsnorm(e(128), e(128), torch.ones(128, dtype=torch.bfloat16, device="cuda"), 1e-6, normed=e(128))
+    torch.cuda.synchronize()

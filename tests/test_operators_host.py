@@ -305,3 +305,16 @@ def test_few_tokens_wrappers_refuse_before_the_device():
                 dict(shared=(pack(1, 128, 64), pack(1, 64, 128)))):
         with pytest.raises(ValueError):
             ops.moe_few_tokens(ws, **{**good, **bad})
+
+
+def test_no_rows_is_nothing_to_do():
+    """Empty tensors have no address: nothing is asked of it, sizes are still checked."""
+    for fmt in (0, 1):
+        assert _call("pega_mx_quantize", None, None, None, fmt, 0, 64, None) == 0
+        assert _call("pega_mx_swiglu_quantize", None, None, None, fmt, 0, 64, None) == 0
+        assert _call("pega_mx_dequantize", None, None, None, fmt, 0, 64, None) == 0
+        assert _call("pega_mx_gemm", A, A << 1, None, None, fmt, None, 32, 0, 256, None) == 0
+        assert _call("pega_mx_quantize", None, None, None, fmt, 0, 40, None) == 801
+        assert _call("pega_mx_gemm", A, A << 1, None, None, fmt, None, 32, 0, 200, None) == 801
+    assert _call("pega_add_rmsnorm", None, False, None, A, 1e-6, None, None, None, None, 0, 64, None) == 0
+    assert _call("pega_add_rmsnorm", None, False, None, A, -1.0, None, None, None, None, 0, 64, None) == 1
