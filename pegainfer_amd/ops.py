@@ -50,8 +50,11 @@ def _ptr(t: torch.Tensor | None) -> int:
     return t.data_ptr()
 
 
+_BF16 = torch.bfloat16
+
+
 def _is_bf16(t: torch.Tensor) -> bool:
-    return t.dtype in (torch.bfloat16, torch.uint16, torch.int16)
+    return t.dtype is _BF16 or t.dtype in (torch.uint16, torch.int16)
 
 
 # --------------------------------------------------------------------------
@@ -695,14 +698,16 @@ def _ptrs_here(*tensors):
     """Device pointers of tensors (0 for None), which must be contiguous and on the current device,
     whose current stream the launch goes to; then that stream.  Messages are only formed on
     failure: at decode sizes a wrapper's host time is of the order of its kernel's."""
-    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    here = -2  # until a tensor is found on a GPU
     out = []
     for t in tensors:
         if t is None:
             out.append(0)
             continue
         if t.get_device() != here:
-            raise ValueError(f"tensor must live on the current GPU, got {t.device}")
+            if here != -2 or t.get_device() < 0 or t.get_device() != torch._C._cuda_getDevice():
+                raise ValueError(f"tensor must live on the current GPU, got {t.device}")
+            here = t.get_device()
         if not t.is_contiguous():
             raise ValueError("tensor must be contiguous")
         out.append(t.data_ptr())
@@ -876,7 +881,7 @@ class MxTensor:
 
 
 def _mx_rows(name: str, t: torch.Tensor, rows: int, cols: int) -> None:
-    if t.shape != (rows, cols) or not _is_bf16(t):
+    if t.shape != (rows, cols) or not (t.dtype is _BF16 or _is_bf16(t)):
         raise ValueError(f"{name} must be bf16 [{rows}, {cols}], got {t.dtype} {tuple(t.shape)}")
 
 
