@@ -528,6 +528,16 @@ int mx_gemm_checks(const char* name, const MxArgs& a, int x_format) {
   return kSuccess;
 }
 
+// The last check, once the sizes are known to be sound.
+int mx_gemm_apart(const char* name, const MxArgs& a, int x_format) {
+  const long long w = static_cast<long long>(a.M) * a.K * a.experts, x = static_cast<long long>(a.N) * a.K;
+  const long long y = 2LL * a.M * a.N * a.top_k;
+  if (overlap(a.y, y, a.wq, w / 2) || overlap(a.y, y, a.ws, w / kMxBlock) ||
+      overlap(a.y, y, a.xq, mx_code_bytes(x_format, x)) || overlap(a.y, y, a.xs, x / kMxBlock))
+    return fail(kInvalidValue, "%s: the output overlaps an operand", name);
+  return kSuccess;
+}
+
 template <int kXFormat, int WV, int MR, int RB, bool kGrouped>
 void launch_stream(const MxArgs& a, int row_blocks, hipStream_t stream) {
   hipLaunchKernelGGL((mx_stream_kernel<kXFormat, WV, MR, RB, kGrouped>),
@@ -674,6 +684,8 @@ PEGA_API int pega_mx_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const
   const int rc = mx_gemm_checks("mx_gemm", a, x_format);
   if (rc != kSuccess) return rc;
   if (N == 0) return kSuccess;
+  const int apart = mx_gemm_apart("mx_gemm", a, x_format);
+  if (apart != kSuccess) return apart;
   return x_format == kMxE4M3 ? dense_launch<kMxE4M3>(a, stream, "mx_gemm")
                              : dense_launch<kMxE2M1>(a, stream, "mx_gemm");
 }
@@ -703,6 +715,8 @@ PEGA_API int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scale
   if (static_cast<long long>(size_m) * size_k >= static_cast<long long>(kOutOfRange))
     return fail(kNotSupported, "mx_grouped_gemm: activations over 2 GiB (%d x %d)", size_m, size_k);
   if (size_m == 0 || sorted_token_ids_len == 0) return kSuccess;
+  const int apart = mx_gemm_apart("mx_grouped_gemm", a, x_format);
+  if (apart != kSuccess) return apart;
   return x_format == kMxE4M3 ? grouped_launch<kMxE4M3>(a, ep_size, stream, "mx_grouped_gemm")
                              : grouped_launch<kMxE2M1>(a, ep_size, stream, "mx_grouped_gemm");
 }

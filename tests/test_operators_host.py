@@ -187,6 +187,20 @@ def test_mx_grouped_gemm_with_nothing_to_do():
         assert _call("pega_mx_grouped_gemm", *args) == 0
 
 
+@pytest.mark.parametrize("operand,size", [(0, 32 * 128), (1, 32 * 8), (2, 4 * 256), (3, 4 * 8)])
+def test_mx_products_refuse_an_output_on_an_operand(operand, size):
+    for y in (0, 16, size - 16):
+        args = list(GEMM)
+        args[operand] = A << 20
+        args[5] = (A << 20) + y
+        assert _call("pega_mx_gemm", *args) == 1
+    place = {0: 4, 1: 5, 2: 0, 3: 1}[operand]
+    args = list(GROUPED)
+    args[place] = A << 20
+    args[3] = (A << 20) + (size if operand < 2 else 0)  # the weights are three experts'
+    assert _call("pega_mx_grouped_gemm", *args) == 1
+
+
 def test_mx_gemm_wrappers_refuse_before_the_device():
     from pegainfer_amd import ops
     q = lambda r, c, f=ops.MxFormat.Fp4E2M1: ops.MxTensor.empty(r, c, f, device="cpu")  # noqa: E731
