@@ -39,6 +39,11 @@
 // Roundings: the SwiGLU rows, with their weights, once to fp16 with a scale for each 64 (bf16 in front of
 // a bf16 down projection); out once.  Everything between is fp32.  A row with an infinite or NaN
 // activation gives NaN.
+//
+// The weights' bytes bound it, below them the select in front of the routed stream (4 us, 9 from nine
+// tokens on), 2 us between the launches and 3 for the last workgroups' join.  48 of 384 experts of 7168 x
+// 2048 with a bf16 shared expert at 1 / 2 / 4 / 8 / 16 tokens 27 / 33 / 50 / 66 / 90 us (112 to 429 MB, 3.7 to 4.8
+// TB/s); 64 experts of 2048 x 1408 with an INT4 one at 1 / 3 / 5 / 8 / 16 23 / 33 / 42 / 51 / 72 us (39 to 257 MB).
 #include <type_traits>
 
 #include "common.h"

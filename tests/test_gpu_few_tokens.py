@@ -259,3 +259,58 @@ def test_dsv2_layer_graph_replays():
         moe.forward(xd, ld, out)
         assert np.array_equal(host(out), got)
         _check(got, *c.want(x, host(moe.topk_idx), host(moe.topk_w), None, 1.0))
+
+
+@pytest.mark.parametrize("tokens", [2, 7])
+def test_packages_past_32_bits(tokens):
+    """Experts whose weights lie past 4 GB: the bits of a package of the last few alone, as many as the
+    tokens have routes (the launch, and so the order of the sums, is by the smaller of the two)."""
+    from pegainfer_amd import ops
+    e, h, i = 300, 7168, 2048
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+
+    def package(out_dim, in_dim):
+        q = torch.empty(e, out_dim * in_dim // 2, dtype=torch.uint8, device="cuda").random_(0, 256, generator=gen)
+        s = torch.empty(e, out_dim * in_dim // 32, device="cuda").uniform_(0.001, 0.02, generator=gen).bfloat16()
+        return q, s
+    w13, w2 = package(2 * i, h), package(h, i)
+    pick = lambda p, lo, o, k: ops.MarlinInt4Weight(e - lo, k, o, p[0][lo:].contiguous(), p[1][lo:].contiguous())  # noqa: E731
+    x = torch.randn(tokens, h, device="cuda", generator=gen).bfloat16()
+    logits = torch.randn(tokens, e, device="cuda", generator=gen)
+    logits[:, e - 2:] += 100.0  # every token to the last two
+    outs = []
+    for lo in (0, e - 2 * tokens):
+        ws = ops.FewTokensWorkspace(tokens, h, i, topk=2, local_experts=e - lo)
+        out = torch.zeros(tokens, h, dtype=torch.bfloat16, device="cuda")
+        w, idx = torch.zeros(tokens, 2, device="cuda"), torch.zeros(tokens, 2, dtype=torch.int32, device="cuda")
+        ops.moe_few_tokens(ws, x, logits, pick(w13, lo, 2 * i, h), pick(w2, lo, h, i), w, idx, out, global_start=lo)
+        assert (idx >= e - 2).all()
+        outs.append(out)
+    assert outs[0].abs().max() > 0 and torch.equal(*outs)
+
+
+def test_two_streams_with_a_workspace_each():
+    """Calls at the same time do not meet: the bits of each call alone."""
+    from pegainfer_amd import ops
+    c = Case(1024, 448, 16, 64, 6, 16, "int4", 3, 64)
+    jobs = []
+    for t in (3, 11):
+        x, logits, bias, res = c.inputs(t)
+        jobs.append(dict(t=t, x=dev(x, bf16=True), l=dev(logits), b=dev(bias), r=dev(res, bf16=True), ws=c.workspace(t),
+                         w=torch.zeros(t, 6, device="cuda"), i=torch.zeros(t, 6, dtype=torch.int32, device="cuda"),
+                         out=[torch.zeros(t, c.h, dtype=torch.bfloat16, device="cuda") for _ in range(31)],
+                         stream=torch.cuda.Stream()))
+
+    def call(j, n):
+        ops.moe_few_tokens(j["ws"], j["x"], j["l"], c.w13, c.w2, j["w"], j["i"], j["out"][n], bias=j["b"],
+                           global_start=c.start, residual=j["r"], shared=c.shared)
+    for j in jobs:
+        call(j, 30)
+    torch.cuda.synchronize()
+    for n in range(30):
+        for j in jobs:
+            with torch.cuda.stream(j["stream"]):
+                call(j, n)
+    torch.cuda.synchronize()
+    for j in jobs:
+        assert all(torch.equal(o, j["out"][30]) for o in j["out"])

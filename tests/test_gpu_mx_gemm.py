@@ -212,3 +212,58 @@ def test_repeat_and_graph_give_the_same_bits():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, first)
+
+
+def _exact(rows, cols, seed):
+    """Random MXFP4 rows of one scale: every sum of their products is exact in fp32."""
+    from pegainfer_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device="cuda")
+    codes.random_(0, 256, generator=gen)
+    return ops.MxTensor(rows, cols, ops.MxFormat.Fp4E2M1, codes,
+                        torch.full((rows, cols // 32), 127, dtype=torch.uint8, device="cuda"))
+
+
+def _part(q, lo, hi):
+    from pegainfer_amd import ops
+    return ops.MxTensor(hi - lo, q.cols, q.format, q.codes[lo:hi].clone(), q.scales[lo:hi].clone())
+
+
+def _product(w, x):
+    from pegainfer_amd import ops
+    y = torch.empty(x.rows, w.rows, dtype=torch.bfloat16, device="cuda")
+    ops.mx_gemm(w, x, y)
+    return y
+
+
+@pytest.mark.parametrize("rows", [5, 40, 200])
+def test_weights_past_32_bits(rows):
+    m, k = (1 << 20) + 16, 8192
+    w, x = _exact(m, k, 1), _exact(rows, k, 2)
+    y = _product(w, x)
+    for lo, hi in ((0, 64), (m // 2, m // 2 + 64), (m - 64, m)):
+        assert torch.equal(y[:, lo:hi], _product(_part(w, lo, hi), x))
+
+
+def test_results_past_32_bits():
+    n, m, k = 70001, 65536, 512
+    w, x = _exact(m, k, 3), _exact(n, k, 4)
+    y = _product(w, x)
+    for lo, hi in ((0, 9), (n // 2, n // 2 + 40), (n - 130, n)):
+        assert torch.equal(y[lo:hi], _product(w, _part(x, lo, hi)))
+
+
+@pytest.mark.parametrize("tokens,bs", [(4, 8), (300, 16), (300, 64)])
+def test_grouped_weights_past_32_bits(tokens, bs):
+    from pegainfer_amd import ops
+    e, m, k = 66, 16384, 8192
+    w, x = _exact(e * m, k, 5), _exact(tokens, k, 6)
+    idx = torch.randint(0, 2, (tokens, 1), dtype=torch.int32, device="cuda") * (e - 1)
+    ws = ops.KimiMarlinRouteWorkspace(tokens, bs, topk=1, local_experts=e)
+    routing = ops.moe_align_block_size(ws, idx, tokens, tokens, 0)
+    y = torch.empty(tokens, m, dtype=torch.bfloat16, device="cuda")
+    ops.mx_grouped_gemm(routing, x, w, None, y, top_k=1, mul_topk_weights=False, size_m=tokens)
+    for expert in (0, e - 1):
+        want = _product(_part(w, expert * m, (expert + 1) * m), x)
+        at = (idx[:, 0] == expert).nonzero()[:, 0]
+        assert torch.equal(y[at], want[at])

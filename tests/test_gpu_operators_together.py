@@ -194,3 +194,32 @@ def test_no_rows():
         ops.mx_gemm(w, q, e(128))
     ops.add_rmsnorm(e(128), e(128), torch.ones(128, dtype=torch.bfloat16, device="cuda"), 1e-6, normed=e(128))
     torch.cuda.synchronize()
+
+
+def test_strided_parts_are_refused_and_offset_parts_are_not():
+    """Column slices are not rows one after another; row slices are, wherever they begin."""
+    from pegainfer_amd import ops
+    g = np.random.default_rng(7)
+    w, _ = _mx_weight(g, 64, 128)
+    big = _bf16_rows(g, 12, 256)
+    q, y = ops.MxTensor.empty(4, 128, ops.MxFormat.Fp8E4M3), torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    ones = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    for bad in (lambda: ops.mx_quantize(big[:4, :128], q), lambda: ops.mx_gemm(w, q, big[:4, :64]),
+                lambda: ops.add_rmsnorm(big[:4, 128:], None, ones, 1e-6, quantized=q),
+                lambda: ops.add_rmsnorm(big[:8].reshape(16, 128)[:4], big[4:8, :128], ones, 1e-6, quantized=q)):
+        with pytest.raises(ValueError):
+            bad()
+    rows = big.reshape(24, 128)
+    for lo in (0, 1, 5, 20):
+        ops.add_rmsnorm(rows[lo:lo + 4], rows[20 - lo:24 - lo], ones, 1e-6, quantized=q)
+        _same(q, _norm_ref(_f64(rows[lo:lo + 4]), _f64(rows[20 - lo:24 - lo]), np.ones(128), 1e-6)[1])
+        ops.mx_quantize(rows[lo:lo + 4], q)
+        _same(q, _f64(rows[lo:lo + 4]))
+        part = ops.MxTensor.empty(9, 128, ops.MxFormat.Fp8E4M3)
+        ops.mx_quantize(rows[:9], part)
+        at = lo % 5
+        some = ops.MxTensor(4, 128, part.format, part.codes[at:at + 4], part.scales[at:at + 4])
+        ops.mx_gemm(w, some, y)
+        first = host(y)
+        ops.mx_gemm(w, ops.MxTensor(4, 128, part.format, some.codes.clone(), some.scales.clone()), y)
+        assert np.array_equal(host(y), first)
