@@ -223,6 +223,37 @@ def test_swiglu_quantize_is_the_two_calls(rows, inter, name, n):
     assert np.array_equal(host(b.codes), codes) and np.array_equal(host(b.scales), scales)
 
 
+@pytest.mark.parametrize("u", [1.0, -0.3, 2.0 ** 100, 2.0 ** -100, np.inf, np.nan, 0.0])
+def test_swiglu_quantize_every_gate(u):
+    """All 65536 bf16 gates, a block each (the others of its block zero), against the two calls."""
+    from pegainfer_amd import ops
+    bits = np.zeros((1 << 11, 32, 32), np.uint16)
+    bits[..., 5] = np.arange(1 << 16, dtype=np.uint16).reshape(1 << 11, 32)
+    gate = bits.reshape(1 << 11, 1024)
+    up = np.broadcast_to(mx_ref.bf16_round(np.float64(u)), gate.shape).astype(np.uint16)
+    w13 = dev(np.concatenate([gate, up], 1), bf16=True)
+    act = torch.zeros(1 << 11, 1024, dtype=torch.bfloat16, device="cuda")
+    ops.kimi_marlin_w13_swiglu(w13, act, 1 << 11, 1024)
+    for name, n in FORMATS:
+        a, b = (ops.MxTensor.empty(1 << 11, 1024, _mx(name, n)) for _ in range(2))
+        ops.mx_quantize(act, a)
+        ops.mx_swiglu_quantize(w13, b)
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
+def test_swiglu_quantize_random_pairs():
+    """Four million pairs of gates and values: fp8 codes of the two calls."""
+    from pegainfer_amd import ops
+    torch.manual_seed(1)
+    w13 = (torch.randn(2048, 4096, device="cuda") * 4).bfloat16()
+    act = torch.zeros(2048, 2048, dtype=torch.bfloat16, device="cuda")
+    ops.kimi_marlin_w13_swiglu(w13, act, 2048, 2048)
+    a, b = (ops.MxTensor.empty(2048, 2048, ops.MxFormat.Fp8E4M3) for _ in range(2))
+    ops.mx_quantize(act, a)
+    ops.mx_swiglu_quantize(w13, b)
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
 def test_norm_then_quantized_swiglu_in_a_graph_and_on_a_side_stream():
     """The operators in the order a block uses them, captured once and replayed on new inputs."""
     from pegainfer_amd import layer, ops
