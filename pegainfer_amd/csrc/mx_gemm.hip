@@ -85,9 +85,8 @@ struct MxStep {
   u32x4_t x[RB][kXFormat == kMxE4M3 ? 2 : 1];
 };
 
-template <int kXFormat, int WV, int MR, int RB, bool kGrouped>
+template <int kXFormat, int WV, int MR, int RB, int D, bool kGrouped>
 __global__ __launch_bounds__(64 * WV) void mx_stream_kernel(MxArgs p) {
-  constexpr int D = RB == 1 ? 8 : 4;
   constexpr int kQuads = D / 4;
   constexpr int kHalves = kXFormat == kMxE4M3 ? 2 : 1;
   constexpr int kXStep = 64 * kHalves;  // bytes of a row of X per step
@@ -538,9 +537,10 @@ int mx_gemm_apart(const char* name, const MxArgs& a, int x_format) {
   return kSuccess;
 }
 
-template <int kXFormat, int WV, int MR, int RB, bool kGrouped>
+template <int kXFormat, int MR, int RB, bool kGrouped, int D = 4>
 void launch_stream(const MxArgs& a, int row_blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((mx_stream_kernel<kXFormat, WV, MR, RB, kGrouped>),
+  constexpr int WV = 4;  // eight waves take 2 to 10% longer
+  hipLaunchKernelGGL((mx_stream_kernel<kXFormat, WV, MR, RB, D, kGrouped>),
                      dim3(a.M / (16 * MR), row_blocks), dim3(64 * WV), 0, stream, a);
 }
 
@@ -595,24 +595,31 @@ int dense_launch(const MxArgs& a, hipStream_t stream, const char* name) {
   if (ceil_div(a.N, 32) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
   const long long tiles64 = static_cast<long long>(ceil_div(a.M, 64)) * ceil_div(a.N, 64);
   // The streaming kernel while 64 x 64 tiles would leave many CUs idle, since its waves share K: a
-  // quarter of the CUs to 16 rows (16 rows x 9728 x 2560, 152 tiles: 7.5 against 8.9 us, x 14336 x 4096,
-  // 224 tiles: 17.0 and 10.8), half where K is long or a workgroup has all rows (64 rows x 4096 x 7168, 64
+  // quarter of the CUs to 8 rows (one row x 9728 x 2560, 152 tiles: 6.5 against 7.0 us, x 14336 x 4096, 224
+  // tiles: 11.9 and 10.3), half where K is long or a workgroup has all rows (64 rows x 4096 x 7168, 64
   // tiles: 10.6 against 18.4 us; 128 rows, 128 tiles: 15.1 and 18.5; 32 rows x 7168 x 2048, 112 tiles: 5.7
-  // and 6.9), else three quarters (96 rows x 2816 x 2048, 88 tiles: 7.1 and 6.1).
-  const int most = a.N <= 16 ? 3 * cu / 4 : a.K > 4096 || a.N <= 32 ? cu / 2 : cu / 4;
+  // and 6.9; 16 rows x 9728 x 2560 8.9 and 7.3), else three quarters (96 rows x 2816 x 2048, 88 tiles: 7.1
+  // and 6.1).
+  const int most = a.N <= 8 ? 3 * cu / 4 : a.K > 4096 || a.N <= 32 ? cu / 2 : cu / 4;
   if (a.K < kTileMinK || tiles64 <= most) {
-    // To 16 rows as many workgroups as there are (9728 x 2560, 16 rows: 608 of 16 features 7.6 us,
-    // 304 of 32 8.4); beyond, more features a workgroup, which read X less often, as long as
-    // three quarters of the CUs have one (64 rows x 4096 x 7168 with 1 / 2 / 4 sets of 16: 14.2 / 10.6 /
-    // 14.3 us; 32 rows x 7168 x 2048 7.9 / 5.7 / 7.9).
+    // To 16 rows as many workgroups as there are (9728 x 2560, 16 rows: 608 of 16 features 7.8 us,
+    // 304 of 32 8.1), but 32 features each where that is one for most CUs (8192 x 4096, 256: 8.7 and 6.7 us);
+    // beyond, more features a workgroup, which read X less often, as long as three quarters of the CUs
+    // have one (64 rows x 4096 x 7168 with 1 / 2 / 4 sets of 16: 14.2 / 10.6 / 14.3 us; 32 rows x 7168 x
+    // 2048 7.9 / 5.7 / 7.9).  Four steps in flight; eight only for few MXFP8 rows of long K (one row x
+    // 2560 x 9728 7.1 and 6.6 us; eight cost x 8192 x 4096 6.4 and 7.3, 64 rows x 4096 x 7168 10.4 and 11.6).
     const int blocks = ceil_div(a.N, 32);
     const auto enough = [&](int mr) {
       return a.M % (16 * mr) == 0 && 4LL * (a.M / (16 * mr)) * blocks >= 3LL * cu;
     };
-    if (a.N <= 16) launch_stream<kXFormat, 4, 1, 1, false>(a, 1, stream);
-    else if (enough(4)) launch_stream<kXFormat, 4, 4, 2, false>(a, blocks, stream);
-    else if (enough(2)) launch_stream<kXFormat, 4, 2, 2, false>(a, blocks, stream);
-    else launch_stream<kXFormat, 4, 1, 2, false>(a, blocks, stream);
+    const int wide = a.M / 32;  // workgroups of 32 features
+    if (a.N <= 16 && a.M % 32 == 0 && wide <= cu && 4 * wide >= 3 * cu)
+      launch_stream<kXFormat, 2, 1, false>(a, 1, stream);
+    else if (a.N <= 8 && kXFormat == kMxE4M3 && a.K > 4096) launch_stream<kXFormat, 1, 1, false, 8>(a, 1, stream);
+    else if (a.N <= 16) launch_stream<kXFormat, 1, 1, false>(a, 1, stream);
+    else if (enough(4)) launch_stream<kXFormat, 4, 2, false>(a, blocks, stream);
+    else if (enough(2)) launch_stream<kXFormat, 2, 2, false>(a, blocks, stream);
+    else launch_stream<kXFormat, 1, 2, false>(a, blocks, stream);
     return launch_status(name);
   }
   const auto go = [&](auto shape) {
@@ -652,7 +659,7 @@ int grouped_launch(const MxArgs& a, int ep_size, hipStream_t stream, const char*
     return launch_status(name);
   }
   if (a.bs > 32 || (a.K >= kTileMinK && rows >= 32.0)) {
-    if (a.K < kTileMinK) launch_stream<kXFormat, 4, 1, 4, true>(a, blocks, stream);
+    if (a.K < kTileMinK) launch_stream<kXFormat, 1, 4, true>(a, blocks, stream);
     else launch_tile<Tile128x64<kXFormat>, true>(a, blocks, stream);
     return launch_status(name);
   }
@@ -665,9 +672,14 @@ int grouped_launch(const MxArgs& a, int ep_size, hipStream_t stream, const char*
   const double enough = a.K <= 2560 ? 0.25 * cu : a.K < 6144 || a.K % 4096 == 0 ? 0.5 * cu : 5.0 * cu;
   const bool tiled = a.K >= kTileMinK && units >= enough;
   if (tiled) launch_tile<MxTile<kXFormat, 4, 1, 2, 2, 6>, true>(a, blocks, stream);
-  else if (a.bs > 16) launch_stream<kXFormat, 4, 1, 2, true>(a, blocks, stream);
-  else if (kXFormat == kMxE4M3 && a.M % 32 == 0) launch_stream<kXFormat, 4, 2, 1, true>(a, blocks, stream);
-  else launch_stream<kXFormat, 4, 1, 1, true>(a, blocks, stream);
+  else if (a.bs > 16) launch_stream<kXFormat, 1, 2, true>(a, blocks, stream);
+  // Eight steps in flight where the workgroups follow each other, four where each CU has few (4096 x
+  // 7168 over 48 experts, MXFP8, at 4, 8, 32, 64 tokens: 12 / 13.5, 16.7 / 18.5, 77 / 69, 131 / 116 us).
+  else if (kXFormat == kMxE4M3 && a.M % 32 == 0) {
+    if (units <= cu) launch_stream<kXFormat, 2, 1, true>(a, blocks, stream);
+    else launch_stream<kXFormat, 2, 1, true, 8>(a, blocks, stream);
+  } else if (units <= cu) launch_stream<kXFormat, 1, 1, true>(a, blocks, stream);
+  else launch_stream<kXFormat, 1, 1, true, 8>(a, blocks, stream);
   return launch_status(name);
 }
 
