@@ -42,8 +42,8 @@
 //
 // The weights' bytes bound it, below them the select in front of the routed stream (4 us, 9 from nine
 // tokens on), 2 us between the launches and 3 for the last workgroups' join.  48 of 384 experts of 7168 x
-// 2048 with a bf16 shared expert at 1 / 2 / 4 / 8 / 16 tokens 27 / 33 / 50 / 66 / 90 us (112 to 429 MB, 3.7 to 4.8
-// TB/s); 64 experts of 2048 x 1408 with an INT4 one at 1 / 3 / 5 / 8 / 16 23 / 33 / 42 / 51 / 72 us (39 to 257 MB).
+// 2048 with a bf16 shared expert at 1 / 2 / 4 / 8 / 16 tokens 28 / 32 / 50 / 64 / 88 us (112 to 429 MB, 3.7 to 4.9
+// TB/s); 64 experts of 2048 x 1408 with an INT4 one at 1 / 3 / 5 / 8 / 16 23 / 32 / 42 / 49 / 68 us (39 to 257 MB).
 #include <type_traits>
 
 #include "common.h"
@@ -151,11 +151,12 @@ __device__ __forceinline__ Int4View int4_view(const uint8_t* q, const uint16_t* 
 // one ahead of their use, as wna16.hip's decode kernel does; the activations' 16 bytes (k 16 kt +
 // 8 hf ..) swap their middle halves between the lanes of the two k halves to follow the words' k order.
 // row_factor: of the lane's activation row, without kScaled.
-// D: groups in flight, a multiple of 16 / R.
-template <int R, int D, bool kScaled>
+// D groups are in flight: eight in launch 1 took 1 to 5% longer (16 tokens 90.2 and 72.1 against 87.9 and
+// 68.5 us).
+template <int R, bool kScaled>
 __device__ __forceinline__ void int4_groups(floatx4_t (&acc)[4], const Int4View& v, int g0, int g1,
                                             float row_factor, uint32_t* slots /* [2][kSlotDwords] */) {
-  constexpr int G = 16 / R;  // groups of a set
+  constexpr int D = 4, G = 16 / R;  // groups of a set
   static_assert(D % G == 0 && D % 2 == 0, "whole sets, and two transpose slots in turn");
   if (g0 >= g1) return;
   const int lane = fresh(threadIdx.x & 63);
@@ -533,7 +534,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
       const int row = (tid & 15) % RU, token = row >= rows ? -1 : kGather ? s_row[row] : row;
       const float row_factor = token >= 0 ? pow2(min(14 - exponent(s_amax[token]), 127)) : 0.0f;
       const Int4View v = int4_view<RU>(q, sc, 2 * inter, H, tile + half * tiles, p.x, nullptr, token, T);
-      int4_groups<RU, 8, false>(acc, v, g0, g1, row_factor, lds.tr[wave]);
+      int4_groups<RU, false>(acc, v, g0, g1, row_factor, lds.tr[wave]);
       add_places<RU>(acc);
     });
     __syncthreads();  // the transpose slots become the sums' place
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
       constexpr int RU = decltype(r)::value;
       const int row = (lane & 15) % RU;
       const Int4View v = int4_view<RU>(q, scales, H, K, tile, act, factors, row < rows ? row : -1, rows);
-      int4_groups<RU, 4, true>(acc, v, g0, g1, 1.0f, s_tr[wave]);
+      int4_groups<RU, true>(acc, v, g0, g1, 1.0f, s_tr[wave]);
       if (kGather) leave(r, mask);
     });
   };
