@@ -112,8 +112,11 @@ __device__ __forceinline__ int exponent(uint32_t bits) { return static_cast<int>
 
 // Where the bytes of a 64-column tile of an INT4 operand, and the activations that meet it, are.  Lane
 // columns of the tile are 32 (lane % 16 / 8) + 8 j + lane % 8, j = 0..3.  kScaled: the activations are
-// fp16 with a factor for each 64 columns and token (launch 2); otherwise bf16 rows, which the lane
-// turns into fp16 by its row's factor (launch 1).
+// fp16 with a factor for each 64 columns and token (launch 2), which undoes their scaling and half of
+// the nibbles' 2^-24, so that the sums are kUndo times too small: the whole of it passes fp32's range
+// for rows of 2^118 and more, and so would a group's products before their scale.  Otherwise they are
+// bf16 rows, which the lane turns into fp16 by its row's factor (launch 1).
+constexpr float kUndo = 4096.0f;
 struct Int4View {
   __amdgpu_buffer_rsrc_t w, s, a, f;
   uint32_t w_voff, s_voff, a_voff, f_voff;
@@ -546,7 +549,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     }
     __syncthreads();
     // a wave finishes a row's 64 columns: SwiGLU times the row's factor, in fp16 with the
-    // largest at 2^14 .. 2^15; the factor that undoes it takes the nibbles' 2^24 along
+    // largest at 2^14 .. 2^15; the factor that undoes it takes 2^12 of the nibbles' 2^24 along
     const auto finish = [&](int t, float g, float u) {
       // x came in times 2^(14 - exponent), at most 2^127, and v as v 2^-24
       const int e = max(10 + exponent(s_amax[s_row[t]]), -103);
@@ -556,7 +559,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
       const float down = (lane & 8) ? 0.0625f : 1.0f;  // what meets the nibbles at 2^-20
       const _Float16 h = static_cast<_Float16>(a * pow2(min(14 - ae, 127)) * down);
       act[static_cast<long long>(t) * inter + tile * 64 + lane] = __builtin_bit_cast(uint16_t, h);
-      if (lane == 0) factors[tile * kMaxTokens + t] = pow2(max(min(10 + ae, 127), -103));
+      if (lane == 0) factors[tile * kMaxTokens + t] = pow2(max(ae - 2, -115));
     };
     const auto place = [&](int of, int t, int up) {
       return p.partials + (((static_cast<long long>(pair) * shares + of) * T + t) * 2 + up) * 64 + lane;
@@ -641,6 +644,12 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j] = floatx4_t{};
   };
+  const auto undo = [&] {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] *= kUndo;
+  };
   const auto groups = [&](const uint8_t* q, const uint16_t* scales, int K, const void* act,
                           const float* factors, uint32_t mask, int g0, int g1) {
     const int rows = kGather ? __popc(mask) : T;
@@ -649,7 +658,10 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
       const int row = (lane & 15) % RU;
       const Int4View v = int4_view<RU>(q, scales, H, K, tile, act, factors, row < rows ? row : -1, rows);
       int4_groups<RU, true>(acc, v, g0, g1, 1.0f, s_tr[wave]);
-      if (kGather) leave(r, mask);
+      if (kGather) {
+        undo();
+        leave(r, mask);
+      }
     });
   };
   const uint32_t everyone = (1u << T) - 1u;
@@ -666,7 +678,9 @@ __global__ __launch_bounds__(kThreads, 4) void few_w2_kernel(FewArgs f) {
   if (p.shared_kind == PEGA_SHARED_INT4 && sh0 < sh1) {
     groups(static_cast<const uint8_t*>(p.shared_w2), p.shared_w2_scales, p.shared_inter, p.act_shared,
            p.act_shared_factors, everyone, sh0, sh1);
-  } else if (p.shared_kind == PEGA_SHARED_BF16) {
+  }
+  if (!kGather) undo();
+  if (p.shared_kind == PEGA_SHARED_BF16) {
     const uint32_t row_bytes = static_cast<uint32_t>(p.shared_inter) * 2u;
     const __amdgpu_buffer_rsrc_t wr =
         make_rsrc(static_cast<const uint16_t*>(p.shared_w2) + static_cast<long long>(tile) * 64 * p.shared_inter,

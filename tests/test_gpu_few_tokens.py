@@ -314,3 +314,23 @@ def test_two_streams_with_a_workspace_each():
     torch.cuda.synchronize()
     for j in jobs:
         assert all(torch.equal(o, j["out"][30]) for o in j["out"])
+
+
+@pytest.mark.parametrize("kind", ["none", "int4", "bf16"])
+@pytest.mark.parametrize("t", [3, 7, 16])
+def test_rows_whose_swiglu_is_near_the_largest_floats(t, kind):
+    """SwiGLU rows of 2^118 to 2^126, whose factor from fp16 to the nibbles' products is no float, and
+    down projections of them that bf16 holds, beside ordinary rows."""
+    c = Case(512, 128, 5, 5, 2, 0, kind, 11)
+    ws = c.workspace(16)
+    x, logits, bias, _ = c.inputs(t, residual=False)
+    v = bf(x).astype(np.float64)
+    v[0] *= 2.0 ** 59
+    v[t // 2] *= 2.0 ** 61
+    v[t - 1] *= 2.0 ** 63
+    x = _bits(v)
+    out, w, idx = c.run(ws, x, logits, bias, None, True, 1.0)
+    want, tol = c.want(x, idx, w, None, 1.0)
+    act = _silu(bf(x)[0].astype(np.float64) @ c.G.transpose(0, 2, 1)) * (bf(x)[0] @ c.U.transpose(0, 2, 1))
+    assert np.abs(act).max() > 2.0 ** 117 and np.abs(want).max() < 2.0 ** 127
+    _check(out, want, tol)
