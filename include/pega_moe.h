@@ -379,8 +379,9 @@ int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream);
  *   MXFP8 (below).
  * x is bf16, or fp32 with x_is_f32.  Each output may be NULL, not all of them; codes and scales go
  * together.  An output may be the buffer of x or of residual (its first byte the input's); no two
- * outputs may overlap.  The sums and products are in 64 bits, and every output is the formula's
- * value rounded once.  A row's result does not depend on the other rows.  hidden_dim % 8 == 0
+ * outputs may overlap.  The sums and products are in 64 bits, and every output is their value
+ * rounded once (y past fp32's range is an infinity); y is the norm of s itself, not of bf16(s).  A
+ * row's result does not depend on the other rows.  hidden_dim % 8 == 0
  * (32 with MXFP8), at most 32768; 16-byte aligned buffers, scales 4-byte (801 otherwise). */
 int pega_add_rmsnorm(const void* x, bool x_is_f32, const uint16_t* residual,
                      const uint16_t* weight, double eps, uint16_t* residual_out,

@@ -7,12 +7,13 @@
 // One pass: a row's values stay in registers between the sum of squares and the outputs, so a
 // row is read once and each output written once; the bytes bound it.
 //
-// The sums and the products are in 64 bits: the values' squares are exact there, and a value's
-// E4M3 code and its block's scale follow the formula however near y lies to a rounding border
-// (in 32 bits about one value in 10^6 goes to the neighbouring code, and which ones depends on
-// the order of the sum).  y reaches 32 bits rounded to odd (the last bit set if anything was cut
-// off), after which one more rounding, to bf16 or to a code, is the rounding of y itself.  The
-// norm is of s itself, not of bf16(s).  The 64-bit work hides behind the memory:
+// The sums and the products are in 64 bits: a value's E4M3 code and its block's scale follow the
+// formula however near y lies to a rounding border (in 32 bits about one value in 10^6 goes to the
+// neighbouring code, and which ones depends on the order of the sum).  y reaches 32 bits rounded to
+// odd (the last bit set if anything was cut off), after which one more rounding, to bf16 or to a
+// code, is the rounding of y itself, among fp32's smallest numbers too.  Past fp32's range y is an
+// infinity.  The norm is of s itself, not of bf16(s), so normed is not quite the norm of
+// residual_out.  The 64-bit work hides behind the memory:
 // 4096 rows of 7168 with every output take 57 us (265 MB, 4.6 TB/s; a plain copy reaches 4.8),
 // one row 5.0 us, of which the launch itself is 2.3.
 #include "common.h"
@@ -23,8 +24,8 @@ namespace pega {
 namespace {
 
 // y in fp32, rounded to odd: the low 29 mantissa bits cut off, and the last one kept set if any
-// of them was (adding 2^29 - 1 to them carries into it then).  What is left converts exactly
-// (values below fp32's normal range aside, which every output rounds to 0).
+// of them was (adding 2^29 - 1 to them carries into it then).  What is left converts exactly in
+// fp32's normal range.
 __device__ __forceinline__ float to_odd(double y) {
   const uint64_t b = __builtin_bit_cast(uint64_t, y);
   const uint32_t lo = static_cast<uint32_t>(b);
@@ -32,6 +33,17 @@ __device__ __forceinline__ float to_odd(double y) {
   const uint64_t cut = (b & 0xffffffff00000000ull) | ((lo | odd) & 0xe0000000u);
   return static_cast<float>(__builtin_bit_cast(double, cut));
 }
+
+// The same below that range (2^-126), where fp32 holds the multiples of 2^-149: bf16's smallest
+// numbers (from 2^-133 on) and MXFP8's of the lowest scale (2^-136) would be rounded twice otherwise.
+__device__ __forceinline__ float to_odd_small(double y) {
+  const double steps = __builtin_fabs(y) * 0x1p149;  // exact, below 2^23
+  const uint32_t whole = static_cast<uint32_t>(steps);
+  const uint32_t odd = whole | (static_cast<double>(whole) != steps ? 1u : 0u);
+  return __builtin_copysignf(__builtin_bit_cast(float, odd), static_cast<float>(y));
+}
+// (what rounds to 0 there is 0 in every output)
+__device__ __forceinline__ bool is_subnormal(float v) { return __builtin_amdgcn_classf(v, 0x90); }
 
 template <int kCtrl>
 __device__ __forceinline__ double dpp_add(double v) {
@@ -138,9 +150,16 @@ __global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) voi
     }
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float w = (i & 1) ? bf_hi(ww[i >> 1]) : bf_lo(ww[i >> 1]);
-      y[i] = to_odd(s[c][i] * inv * static_cast<double>(w));
+    for (int i = 0; i < 8; i += 2) {
+      const double p0 = s[c][i] * inv * static_cast<double>(bf_lo(ww[i >> 1]));
+      const double p1 = s[c][i + 1] * inv * static_cast<double>(bf_hi(ww[i >> 1]));
+      y[i] = to_odd(p0);
+      y[i + 1] = to_odd(p1);
+      // hardly ever, in any lane: a jump
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(is_subnormal(y[i]) | is_subnormal(y[i + 1])) != 0, 0)) {
+        y[i] = is_subnormal(y[i]) ? to_odd_small(p0) : y[i];
+        y[i + 1] = is_subnormal(y[i + 1]) ? to_odd_small(p1) : y[i + 1];
+      }
     }
     if (normed && ok)
       *reinterpret_cast<uint4*>(normed + at) =

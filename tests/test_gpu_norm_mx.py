@@ -353,3 +353,43 @@ def test_norm_of_more_rows_than_a_launch_takes():
     ops.add_rmsnorm(x, x, w, 1e-6, normed=y)
     assert (y[:rows - 5].view(-1, block, cols).view(torch.int16) == want.view(torch.int16)).all()
     assert torch.equal(y[rows - 5:], want[7:12])
+
+
+def test_norm_rounds_once_below_fp32s_normal_range():
+    """Results a little off the middle between two of bf16's smallest numbers (2^-133 apart) and
+    between two MXFP8 values of the lowest scale (2^-136 apart), nearer to it than fp32's smallest
+    step: rounded to fp32 first, they would lie on it."""
+    cols = 1024
+    x, w = np.zeros((3, cols)), np.full(cols, 2.0 ** -132)
+    # half of a row at the middle and a bit: above 0.5, below 1.5 steps of bf16, above 0.5 of MXFP8
+    # (ties go to the even one, the other side); the rest brings the mean of the squares to 1
+    for row, (base, off) in enumerate(((0.25, 2.0 ** -18), (0.75, -2.0 ** -19), (2.0 ** -5, 2.0 ** -15))):
+        a = base * (1 + off)
+        x[row, ::2] = a
+        x[row, 1::2] = np.sqrt(2 - a * a)
+        x[row, ::4] *= -1
+    x, w = x.astype(np.float32), mx_ref.bf16_round(w)
+    s, y = _norm_ref(x, None, bf(w), 0.0)
+    small = np.abs(y[:, ::2])
+    middle = np.array([[2.0 ** -134], [1.5 * 2.0 ** -133], [2.0 ** -137]])
+    assert (small != middle).all() and (np.abs(small - middle) < 2.0 ** -151).all()
+    _, gy, (gc, gsc) = _run_norm(x, None, w, 0.0)
+    assert np.array_equal(gy, mx_ref.bf16_round(y))
+    codes, scales = mx_ref.quantize(y, "fp8")
+    assert np.array_equal(gsc, scales) and np.array_equal(gc, codes)
+
+
+@pytest.mark.parametrize("x32", [False, True])
+def test_norm_of_tiny_weights(x32):
+    """Weights and so results throughout bf16's and MXFP8's smallest numbers."""
+    rows, cols = 61, 4096
+    g = np.random.default_rng(8)
+    xb = mx_ref.bf16_round(_rows(g, rows, cols))
+    x = _rows(g, rows, cols) if x32 else xb
+    res = mx_ref.bf16_round(_rows(g, rows, cols))
+    w = mx_ref.bf16_round(2.0 ** g.uniform(-140, -120, cols) * g.choice([-1, 1], cols))
+    _, y = _norm_ref(x if x32 else bf(x), bf(res), bf(w), 1e-6)
+    _, gy, (gc, gsc) = _run_norm(x, res, w, 1e-6)
+    assert np.array_equal(gy, mx_ref.bf16_round(y))
+    codes, scales = mx_ref.quantize(y, "fp8")
+    assert np.array_equal(gsc, scales) and np.array_equal(gc, codes)
