@@ -267,3 +267,59 @@ def test_grouped_weights_past_32_bits(tokens, bs):
         want = _product(_part(w, expert * m, (expert + 1) * m), x)
         at = (idx[:, 0] == expert).nonzero()[:, 0]
         assert torch.equal(y[at], want[at])
+
+
+def _small(rows, cols, name, seed):
+    """Rows of few bits with two scales: with MXFP4 weights of the same kind no sum of their products
+    loses any (a product is a multiple of 1/2 up to 48), so the results are bf16 of the exact ones.
+    Also the values, in float64 on the GPU."""
+    from pegainfer_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    pick = lambda hi, shape: torch.randint(0, hi, shape, device="cuda", generator=gen)  # noqa: E731
+    if name == "fp8":
+        table = torch.tensor([0.0, 1.0, -1.0, 2.0, -2.0], device="cuda")
+        v = table[pick(5, (rows, cols))]
+        codes = v.to(torch.float8_e4m3fn).view(torch.uint8)
+    else:
+        table = torch.tensor(np.concatenate([mx_ref.E2M1, -mx_ref.E2M1]), device="cuda", dtype=torch.float32)
+        nibbles = pick(16, (rows, cols))
+        v, codes = table[nibbles], (nibbles[:, 0::2] | nibbles[:, 1::2] << 4).to(torch.uint8)
+    scales = 127 + pick(2, (rows, cols // 32))
+    v = v.double() * torch.exp2((scales - 127).double()).repeat_interleave(32, 1)
+    return ops.MxTensor(rows, cols, ops.MxFormat(FORMATS[name]), codes, scales.to(torch.uint8)), v
+
+
+# The streaming kernel's forms by their rules (256 CUs): 32 features a workgroup where that is one for
+# most CUs; eight steps in flight for up to 8 MXFP8 rows of k over 4096; 64 features where that is still
+# three quarters of the CUs.  Steps that do and do not divide by the waves and by the steps in flight.
+@pytest.mark.parametrize("name", ["fp8", "fp4"])
+@pytest.mark.parametrize("n,m,k", [
+    (1, 8192, 640), (5, 6144, 1408), (16, 8160, 1152), (16, 6176, 4096),
+    (5, 272, 4224), (8, 256, 9728), (1, 9728, 4480), (2, 528, 7168), (7, 80, 4352),
+    (32, 12288, 256), (17, 12352, 384), (64, 6144, 4224), (100, 3200, 4352), (33, 8192, 4992)])
+def test_streaming_forms(n, m, k, name):
+    from pegainfer_amd import ops
+    (x, xv), (w, wv) = _small(n, k, name, n + m), _small(m, k, "fp4", k)
+    y = torch.full((n + 1, m), 5.0, dtype=torch.bfloat16, device="cuda")
+    ops.mx_gemm(w, x, y[:n])
+    assert torch.equal(y[:n], (xv @ wv.T).float().bfloat16()) and (y[n] == 5).all()
+
+
+# Grouped: four steps in flight to one workgroup a CU, eight with more, by 16 or 32 features (short k,
+# and k over 6144 below five tiles a CU); two sets of rows for blocks of 32.
+@pytest.mark.parametrize("name", ["fp8", "fp4"])
+@pytest.mark.parametrize("tokens,topk,experts,bs,m,k", [
+    (40, 4, 40, 8, 928, 6272), (40, 4, 40, 16, 912, 6528), (60, 3, 60, 8, 1056, 384), (60, 3, 60, 16, 1040, 384),
+    (30, 2, 24, 8, 1536, 7040), (6, 2, 12, 8, 544, 7168), (6, 2, 12, 8, 528, 4480), (90, 4, 40, 32, 912, 6272),
+    (90, 4, 40, 32, 912, 384), (90, 4, 40, 48, 912, 384)])
+def test_grouped_streaming_forms(tokens, topk, experts, bs, m, k, name):
+    from pegainfer_amd import ops
+    idx, routing = _route(tokens, topk, experts, experts, 0, bs, tokens)
+    (x, xv), (w, wv) = _small(tokens, k, name, tokens), _small(experts * m, k, "fp4", k)
+    y = torch.full((tokens * topk, m), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.mx_grouped_gemm(routing, x, w, None, y, top_k=topk, mul_topk_weights=False, size_m=tokens)
+    flat = torch.from_numpy(idx.reshape(-1)).cuda()
+    for e in range(experts):
+        r = (flat == e).nonzero()[:, 0]
+        want = (xv[r // topk] @ wv[e * m:(e + 1) * m].T).float().bfloat16()
+        assert torch.equal(y[r], want), e
