@@ -283,7 +283,8 @@ class KimiMoeDecodeLayer:
 
     few_tokens: batches of up to that many tokens (at most ops.FEW_TOKENS_MAX) take the
     two-launch form instead, ops.moe_few_tokens, which rounds less in between (the INT4
-    weights' products, the routed rows and the joins stay fp32), so its bits differ."""
+    weights' products, the routed rows and the joins stay fp32), so its bits differ.  Sizes
+    that it does not take (ops.FewTokensWorkspace) are refused here."""
 
     def __init__(self, routed: RoutedExperts, shared: KimiSharedExpert, *, n_experts: int = 384,
                  device="cuda", few_tokens: int = 0):

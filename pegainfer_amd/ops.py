@@ -720,23 +720,28 @@ def _ptrs_here(*tensors):
 # --------------------------------------------------------------------------
 FEW_TOKENS_MAX = 16        # rows of one matrix instruction
 FEW_TOKENS_MAX_TOPK = 32
+FEW_TOKENS_MAX_LOCAL = 512
 _FEW_MAX_SPLITS, _FEW_COUNTERS = 8, 512  # PEGA_FEW_MAX_SPLITS, PEGA_FEW_COUNTERS
 _SHARED_NONE, _SHARED_BF16, _SHARED_INT4 = 0, 1, 2
 
 
 class FewTokensWorkspace:
-    """Buffers between moe_few_tokens' two launches, sized once for `max_tokens`.  Calls that
-    share one must not overlap: graphs that may replay at the same time need one each."""
+    """Buffers between moe_few_tokens' two launches, sized once for `max_tokens`, for the sizes
+    that it takes.  Calls that share one must not overlap: graphs that may replay at the same
+    time need one each."""
 
     def __init__(self, max_tokens: int, hidden: int, inter: int, *, topk: int, local_experts: int,
                  shared_inter: int = 0, device="cuda"):
         _ensure(0 < max_tokens <= FEW_TOKENS_MAX,
                 f"few-token batches have 1 to {FEW_TOKENS_MAX} tokens, got {max_tokens}")
-        _ensure(0 < topk <= FEW_TOKENS_MAX_TOPK and local_experts > 0,
-                f"few-token layers take top-1 to top-{FEW_TOKENS_MAX_TOPK}, got {topk}")
+        _ensure(0 < topk <= FEW_TOKENS_MAX_TOPK and 0 < local_experts <= FEW_TOKENS_MAX_LOCAL,
+                f"few-token layers take top-1 to top-{FEW_TOKENS_MAX_TOPK} and up to "
+                f"{FEW_TOKENS_MAX_LOCAL} local experts, got top-{topk} of {local_experts}")
         _ensure(hidden > 0 and inter > 0 and hidden % 64 == 0 and inter % 64 == 0
                 and shared_inter >= 0 and shared_inter % 64 == 0,
                 "hidden and intermediate sizes must be multiples of 64")
+        _ensure((2 * max(inter, shared_inter) + 16) * hidden * 2 < 1 << 31,
+                f"few-token layers take projections under 2 GiB, got {inter}, {shared_inter} x {hidden}")
         self.max_tokens, self.hidden, self.inter = max_tokens, hidden, inter
         self.topk, self.local_experts, self.shared_inter = topk, local_experts, shared_inter
         slots = min(max_tokens * topk, local_experts)

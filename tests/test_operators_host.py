@@ -332,3 +332,40 @@ def test_no_rows_is_nothing_to_do():
         assert _call("pega_mx_gemm", A, A << 1, None, None, fmt, None, 32, 0, 200, None) == 801
     assert _call("pega_add_rmsnorm", None, False, None, A, 1e-6, None, None, None, None, 0, 64, None) == 0
     assert _call("pega_add_rmsnorm", None, False, None, A, -1.0, None, None, None, None, 0, 64, None) == 1
+
+
+@pytest.mark.parametrize("bad", [dict(local_experts=513), dict(hidden=1 << 20, inter=1024),
+                                 dict(hidden=1 << 20, inter=64, shared_inter=1024)])
+def test_few_tokens_workspace_refuses_what_its_calls_would(bad):
+    """The entry's limits, and the same sizes refused there."""
+    from pegainfer_amd import ops
+    kw = {**dict(hidden=128, inter=64, topk=2, local_experts=4, shared_inter=64), **bad}
+    with pytest.raises(ValueError):
+        ops.FewTokensWorkspace(1, kw.pop("hidden"), kw.pop("inter"), device="meta", **kw)
+    entry = {**{"hidden" if k == "hidden_dim" else k: v for k, v in bad.items()}, "n_experts": 1000}
+    entry["hidden_dim"] = entry.pop("hidden", 128)
+    assert _few_call(**entry) == 801
+
+
+def test_few_tokens_workspace_takes_the_limits():
+    from pegainfer_amd import ops
+    ops.FewTokensWorkspace(1, 128, 64, topk=2, local_experts=512, device="meta")
+    ops.FewTokensWorkspace(1, 1 << 20, 448, topk=2, local_experts=4, device="meta")
+
+
+def test_decode_layers_refuse_few_tokens_of_other_sizes_when_built():
+    from pegainfer_amd import layer, ops
+
+    def pack(e, k, n):
+        u8, bf = dict(dtype=torch.uint8, device="meta"), dict(dtype=torch.bfloat16, device="meta")
+        return ops.MarlinInt4Weight(e, k, n, torch.empty(e * k * n // 2, **u8), torch.empty(e * n * (k // 32), **bf))
+    routed = layer.RoutedExperts(pack(513, 128, 128), pack(513, 64, 128), max_tokens=8, topk=2, block_size=8,
+                                 device="meta")
+    bf = dict(dtype=torch.bfloat16, device="meta")
+    kimi = layer.KimiSharedExpert(torch.empty(128, 128, **bf), torch.empty(128, 64, **bf), max_tokens=8, device="meta")
+    dsv2 = layer.ExpertFFN(pack(1, 128, 128), pack(1, 64, 128), max_rows=8, device="meta")
+    for make in (lambda n: layer.KimiMoeDecodeLayer(routed, kimi, device="meta", few_tokens=n),
+                 lambda n: layer.Dsv2MoeLayer(routed, dsv2, device="meta", few_tokens=n)):
+        make(0)
+        with pytest.raises(ValueError, match="local experts"):
+            make(4)
