@@ -770,10 +770,10 @@ def moe_few_tokens(workspace: FewTokensWorkspace, x: torch.Tensor, logits: torch
         topk_idx, topk_weight = kimi_router_select (with `bias`) or dsv2_router_select (without)
         out = bf16(residual + routed_scale * sum of the local routes' weighted experts + shared)
 
-    x: the normed rows, bf16 [T, hidden]; logits: f32 [T, n_experts]; w13, w2: the local experts'
-    INT4 packages; shared: None, a pair of bf16 matrices (gate-then-up [2 Is, hidden], down
-    [hidden, Is]) or a pair of one-expert INT4 packages.  out may be x or residual itself, and
-    is otherwise apart from residual."""
+    x: the normed rows, bf16 [T, hidden]; logits: f32, T rows or more of n_experts, as the router
+    selects take them; w13, w2: the local experts' INT4 packages; shared: None, a pair of bf16
+    matrices (gate-then-up [2 Is, hidden], down [hidden, Is]) or a pair of one-expert INT4
+    packages.  out may be x or residual itself, and is otherwise apart from residual."""
     ws = workspace
     if x.dim() != 2:
         raise ValueError("x must be bf16 [tokens, hidden]")
@@ -790,9 +790,9 @@ def moe_few_tokens(workspace: FewTokensWorkspace, x: torch.Tensor, logits: torch
     _mx_rows("out", out, T, H)
     if residual is not None:
         _mx_rows("residual", residual, T, H)
-    if logits.dim() != 2 or logits.shape[0] != T or logits.dtype != torch.float32:
-        raise ValueError("logits must be f32 [tokens, n_experts]")
-    n_experts = logits.shape[1]
+    n_experts = logits.shape[-1]
+    if logits.dtype != torch.float32 or logits.numel() < T * n_experts:
+        raise ValueError(f"logits must be f32 covering {T} rows of {n_experts} experts")
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() < n_experts):
         raise ValueError(f"bias must be f32 covering {n_experts} experts")
     if not 0 <= global_start <= n_experts - E:

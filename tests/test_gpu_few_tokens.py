@@ -334,3 +334,34 @@ def test_rows_whose_swiglu_is_near_the_largest_floats(t, kind):
     act = _silu(bf(x)[0].astype(np.float64) @ c.G.transpose(0, 2, 1)) * (bf(x)[0] @ c.U.transpose(0, 2, 1))
     assert np.abs(act).max() > 2.0 ** 117 and np.abs(want).max() < 2.0 ** 127
     _check(out, want, tol)
+
+
+@pytest.mark.parametrize("kind", ["kimi", "dsv2"])
+def test_layers_take_the_inputs_of_their_general_form(kind):
+    """Logits of a larger batch's buffer: the layer with and without few_tokens, and the bits of
+    logits of the batch's own rows."""
+    from pegainfer_amd import layer
+    c = Case(512, 128, 8, 16, 4, 4, "bf16" if kind == "kimi" else "int4", 21, 128)
+    routed = layer.RoutedExperts(c.w13, c.w2, max_tokens=8, topk=4, block_size=8, global_start=4)
+    if kind == "kimi":
+        shared = layer.KimiSharedExpert(*c.shared, max_tokens=8)
+        make = lambda n: layer.KimiMoeDecodeLayer(routed, shared, n_experts=16, few_tokens=n)  # noqa: E731
+    else:
+        shared = layer.ExpertFFN(*c.shared, max_rows=8)
+        make = lambda n: layer.Dsv2MoeLayer(routed, shared, few_tokens=n)  # noqa: E731
+    x, lg, bi, res = c.inputs(8)
+    xd, ld, bd, rd = dev(x, bf16=True), dev(lg), dev(bi), dev(res, bf16=True)
+    for n in (0, 8):
+        lay, outs = make(n), []
+        for logits in (ld, ld[:5]):
+            out = torch.zeros(5, 512, dtype=torch.bfloat16, device="cuda")
+            if kind == "kimi":
+                lay.forward(rd[:5], xd[:5], logits, bd, out)
+            else:
+                lay.forward(xd[:5], logits, out)
+            outs.append(out)
+        assert torch.equal(*outs)
+        idx, w = host(lay.topk_idx[:5]), host(lay.topk_w[:5])
+        if n:
+            _check(host(outs[0]), *c.want(x[:5], idx, w, res[:5] if kind == "kimi" else None,
+                                          2.827 if kind == "kimi" else 1.0))

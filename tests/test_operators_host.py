@@ -369,3 +369,19 @@ def test_decode_layers_refuse_few_tokens_of_other_sizes_when_built():
         make(0)
         with pytest.raises(ValueError, match="local experts"):
             make(4)
+
+
+@pytest.mark.parametrize("shape", [(3, 16), (8, 16), (1, 4, 16)])
+def test_few_tokens_takes_logits_as_the_selects_do(shape):
+    """Whatever covers the tokens' rows (a buffer of a larger batch): refused for its place alone."""
+    from pegainfer_amd import ops
+    u8, bf = dict(dtype=torch.uint8), dict(dtype=torch.bfloat16)
+    pack = lambda e, k, n: ops.MarlinInt4Weight(  # noqa: E731
+        e, k, n, torch.zeros(e * k * n // 2, **u8), torch.zeros(e * n * (k // 32), **bf))
+    ws = ops.FewTokensWorkspace(4, 128, 64, topk=2, local_experts=4, device="cpu")
+    with pytest.raises(ValueError, match="current GPU"):
+        ops.moe_few_tokens(ws, torch.zeros(3, 128, **bf), torch.zeros(*shape), pack(4, 128, 128), pack(4, 64, 128),
+                           torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 128, **bf))
+    with pytest.raises(ValueError, match="logits"):
+        ops.moe_few_tokens(ws, torch.zeros(3, 128, **bf), torch.zeros(2, 16), pack(4, 128, 128), pack(4, 64, 128),
+                           torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 128, **bf))
