@@ -414,8 +414,9 @@ int pega_mx_dequantize(const uint8_t* codes, const uint8_t* scales, uint16_t* ou
 
 /* Y[n][m] = bf16(sum_k X[n][k] * W[m][k]): W [M][K] MXFP4, X [N][K] in x_format, Y [N][M] bf16,
  * fp32 accumulation on the scaled matrix instructions (E4M3 products are aligned to the largest of
- * 128 inside an instruction: about 2^-12 of it).  M % 16 == 0, K % 128 == 0, codes and Y 16-byte
- * aligned, scales 4-byte, N at most 2^21 - 32 (801 otherwise), Y apart from the operands (1).
+ * 128 inside an instruction: about 2^-12 of it).  M % 16 == 0, M below 2^28, K % 128 == 0, K below
+ * 2^23, codes and Y 16-byte aligned, scales 4-byte, N at most 2^21 - 32 (801 otherwise), Y apart from
+ * the operands (1).
  * Never allocates.  A call's bits depend on its sizes and formats alone; a block of scale 255
  * makes its row's results NaN. */
 int pega_mx_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,

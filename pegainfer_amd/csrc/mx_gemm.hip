@@ -509,6 +509,8 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(MxArgs p) {
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+constexpr int kMaxGridY = 65535;
+
 int mx_gemm_checks(const char* name, const MxArgs& a, int x_format) {
   // no rows: nothing to do, and empty tensors have no address
   if (a.N != 0 && (!a.wq || !a.ws || !a.xq || !a.xs || !a.y)) return fail(kInvalidValue, "%s: null pointer", name);
@@ -521,6 +523,8 @@ int mx_gemm_checks(const char* name, const MxArgs& a, int x_format) {
   if (!aligned(a.wq, 16) || !aligned(a.xq, 16) || !aligned(a.y, 16) || !aligned(a.ws, 4) ||
       !aligned(a.xs, 4))
     return fail(kNotSupported, "%s: codes and output must be 16-byte aligned, scales 4-byte", name);
+  // a launch has fewer than 2^32 threads a dimension, the streaming kernel 256 for 16 features
+  if (a.M >= (1 << 28)) return fail(kNotSupported, "%s: M=%d is not below 2^28", name, a.M);
   // a workgroup addresses up to 256 rows of either operand through one 32-bit range
   if (256LL * a.K >= static_cast<long long>(kOutOfRange))
     return fail(kNotSupported, "%s: K=%d is over 2^23", name, a.K);
@@ -592,7 +596,6 @@ template <int kXFormat>
 int dense_launch(const MxArgs& a, hipStream_t stream, const char* name) {
   const int cu = current_cu_count();
   if (cu <= 0) return fail(kInvalidValue, "%s: no device", name);
-  if (ceil_div(a.N, 32) > 65535) return fail(kNotSupported, "%s: too many rows (N=%d)", name, a.N);
   const long long tiles64 = static_cast<long long>(ceil_div(a.M, 64)) * ceil_div(a.N, 64);
   // The streaming kernel while 64 x 64 tiles would leave many CUs idle, since its waves share K: a
   // quarter of the CUs to 8 rows (one row x 9728 x 2560, 152 tiles: 6.5 against 7.0 us, x 14336 x 4096, 224
@@ -641,7 +644,6 @@ int grouped_launch(const MxArgs& a, int ep_size, hipStream_t stream, const char*
   const int cu = current_cu_count();
   if (cu <= 0) return fail(kInvalidValue, "%s: no device", name);
   const int blocks = ceil_div(a.sorted_len, a.bs);
-  if (blocks > 65535) return fail(kNotSupported, "%s: too many blocks (%d)", name, blocks);
   // Workgroups of 128 features that will have rows: the blocks that the local routes (one in ep_size)
   // fill, at least one for each expert that routes spread evenly would reach.
   const double local = static_cast<double>(a.N) * a.top_k / ep_size;
@@ -695,6 +697,7 @@ PEGA_API int pega_mx_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const
   MxArgs a{w_codes, w_scales, x_codes, x_scales, Y, M, N, K, nullptr, nullptr, nullptr, nullptr, 0, 0, 1, 0, 1};
   const int rc = mx_gemm_checks("mx_gemm", a, x_format);
   if (rc != kSuccess) return rc;
+  if (N > 32 * kMaxGridY) return fail(kNotSupported, "mx_gemm: too many rows (N=%d)", N);
   if (N == 0) return kSuccess;
   const int apart = mx_gemm_apart("mx_gemm", a, x_format);
   if (apart != kSuccess) return apart;
@@ -723,6 +726,9 @@ PEGA_API int pega_mx_grouped_gemm(const uint8_t* x_codes, const uint8_t* x_scale
       static_cast<long long>(size_m) * top_k >= (1LL << 31))
     return fail(kInvalidValue, "mx_grouped_gemm: bad shape top_k=%d experts=%d sorted=%d", top_k,
                 local_experts, sorted_token_ids_len);
+  if (sorted_token_ids_len > static_cast<long long>(kMaxGridY) * moe_block_size)
+    return fail(kNotSupported, "mx_grouped_gemm: too many blocks (%d ids in blocks of %d)",
+                sorted_token_ids_len, moe_block_size);
   // the gathered rows are addressed through one 32-bit range
   if (static_cast<long long>(size_m) * size_k >= static_cast<long long>(kOutOfRange))
     return fail(kNotSupported, "mx_grouped_gemm: activations over 2 GiB (%d x %d)", size_m, size_k);

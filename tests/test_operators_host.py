@@ -385,3 +385,22 @@ def test_few_tokens_takes_logits_as_the_selects_do(shape):
     with pytest.raises(ValueError, match="logits"):
         ops.moe_few_tokens(ws, torch.zeros(3, 128, **bf), torch.zeros(2, 16), pack(4, 128, 128), pack(4, 64, 128),
                            torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 128, **bf))
+
+
+@pytest.mark.parametrize("at,value", [(6, 1 << 28), (6, (1 << 31) - 16), (7, (1 << 21) - 31), (7, (1 << 31) - 1)])
+def test_mx_gemm_refuses_more_than_a_launch_holds(at, value):
+    args = list(GEMM)
+    args[at], args[8] = value, 128
+    for operand in range(4):
+        args[operand] = (A << 40) + (operand << 60)
+    assert _call("pega_mx_gemm", *args) == 801
+
+
+@pytest.mark.parametrize("ids,bs", [((1 << 31) - 1, 8), (65535 * 8 + 1, 8), (65535 * 64 + 1, 64)])
+def test_mx_grouped_gemm_refuses_more_blocks_than_a_launch_holds(ids, bs):
+    args = list(GROUPED)
+    args[10], args[11] = ids, bs
+    assert _call("pega_mx_grouped_gemm", *args) == 801
+    args = list(GROUPED)
+    args[15] = 1 << 28
+    assert _call("pega_mx_grouped_gemm", *args) == 801
