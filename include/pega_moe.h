@@ -366,7 +366,9 @@ typedef struct pega_moe_few {
  * projection), out once, and all sums are fp32, in an order that the sizes and the routing decide.  A
  * row of x with an infinity or a NaN gives a row of NaN; other rows are as without it.  Experts without a route are not read.  Calls that share a
  * workspace must not overlap (two captured graphs that may run at once need one each); nothing is
- * kept in it from one call to the next but the zeroed counters.  At most 16 tokens, topk 32, 512
+ * kept in it from one call to the next but the zeroed counters.  topk_weight and topk_idx are apart
+ * from every input and from out, and out from what the second launch reads (residual, unless it is
+ * out itself, and the down projections).  At most 16 tokens, topk 32, 512
  * local experts, 1024 experts, sizes multiples of 64, 2 hidden_dim (2 inter + 16) bytes under 2 GiB
  * for the larger of inter and shared_inter, 16-byte aligned buffers (801 otherwise). */
 int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream);

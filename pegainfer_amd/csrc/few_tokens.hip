@@ -796,14 +796,32 @@ PEGA_API int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream) {
                         p.shared_kind == PEGA_SHARED_INT4 ? p.shared_w2_scales : nullptr};
   for (const void* v : vecs)
     if (!aligned16(v)) return fail(kNotSupported, "moe_few_tokens: buffers must be 16-byte aligned");
-  // out may be residual, place for place, or any of what only launch 1 reads
-  const long long row_bytes = 2LL * p.hidden_dim * p.tokens, route_bytes = 4LL * p.tokens * p.topk;
-  const long long logit_bytes = 4LL * p.tokens * p.n_experts;
-  if ((p.residual != p.out && overlap(p.residual, row_bytes, p.out, row_bytes)) ||
-      overlap(p.topk_weight, route_bytes, p.logits, logit_bytes) ||
-      overlap(p.topk_idx, route_bytes, p.logits, logit_bytes) ||
-      overlap(p.topk_weight, route_bytes, p.topk_idx, route_bytes))
-    return fail(kInvalidValue, "moe_few_tokens: buffers overlap");
+  // The ids and weights are written while launch 1's other workgroups read, and out by launch 2's, place
+  // for place over residual at most, or over what only launch 1 reads.
+  struct Span {
+    const void* p;
+    long long bytes;
+  };
+  const long long rows = 2LL * p.hidden_dim * p.tokens, routes_b = 4LL * p.tokens * p.topk;
+  const long long w2 = static_cast<long long>(p.local_experts) * p.hidden_dim * p.inter;  // values
+  const long long s2 = shared ? static_cast<long long>(p.hidden_dim) * p.shared_inter : 0;
+  const bool s4 = p.shared_kind == PEGA_SHARED_INT4;
+  const Span outs[] = {{p.topk_weight, routes_b}, {p.topk_idx, routes_b}, {p.out, rows}};
+  const Span second[] = {{p.residual != p.out ? p.residual : nullptr, rows}, {p.w2, w2 / 2}, {p.w2_scales, w2 / 16},
+                         {shared ? p.shared_w2 : nullptr, s4 ? s2 / 2 : 2 * s2},
+                         {s4 ? p.shared_w2_scales : nullptr, s2 / 16}};
+  const Span first[] = {{p.x, rows}, {p.logits, 4LL * p.tokens * p.n_experts},
+                        {p.softmax ? nullptr : p.bias, 4LL * p.n_experts}, {p.w13, w2}, {p.w13_scales, w2 / 8},
+                        {shared ? p.shared_w13 : nullptr, s4 ? s2 : 4 * s2},
+                        {s4 ? p.shared_w13_scales : nullptr, s2 / 8}, {p.residual, rows}};
+  for (int o = 0; o < 3; ++o) {
+    bool meets = false;
+    for (const Span& in : second) meets |= overlap(outs[o].p, outs[o].bytes, in.p, in.bytes);
+    if (o < 2)
+      for (const Span& in : first) meets |= overlap(outs[o].p, outs[o].bytes, in.p, in.bytes);
+    for (int i = 0; i < o; ++i) meets |= overlap(outs[o].p, outs[o].bytes, outs[i].p, outs[i].bytes);
+    if (meets) return fail(kInvalidValue, "moe_few_tokens: buffers overlap");
+  }
   const int cu = current_cu_count();
   if (cu <= 0) return fail(kInvalidValue, "moe_few_tokens: no device");
   FewArgs f{p, 0, p.inter / 64, few_splits(p.hidden_dim), p.shared_kind == PEGA_SHARED_BF16 ? 3 : 1, 0, 0};

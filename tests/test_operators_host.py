@@ -404,3 +404,24 @@ def test_mx_grouped_gemm_refuses_more_blocks_than_a_launch_holds(ids, bs):
     args = list(GROUPED)
     args[15] = 1 << 28
     assert _call("pega_mx_grouped_gemm", *args) == 801
+
+
+@pytest.mark.parametrize("output", ["topk_weight", "topk_idx", "out"])
+@pytest.mark.parametrize("kind", [1, 2])
+@pytest.mark.parametrize("operand,size", [
+    ("x", 1024), ("bias", 64), ("w13", 32768), ("w13_scales", 4096), ("w2", 16384), ("w2_scales", 2048),
+    ("shared_w13", (32768, 8192)), ("shared_w13_scales", (0, 1024)), ("shared_w2", (16384, 4096)),
+    ("shared_w2_scales", (0, 512)), ("residual", 1024)])
+def test_few_tokens_refuses_outputs_on_operands(output, kind, operand, size):
+    """128 columns, 64 between, 4 tokens of top 2, 4 local experts: the operand's first and last bytes."""
+    size = size if isinstance(size, int) else size[kind - 1]
+    if not size or output == "out" and operand not in ("w2", "w2_scales", "shared_w2", "shared_w2_scales"):
+        return  # not an operand of this kind; out may be on what only the first launch reads
+    for place in (A << 40, (A << 40) + size - 16):
+        assert _few_call(**{"shared_kind": kind, operand: A << 40, output: place}) == 1
+        assert "overlap" in _last_error()
+
+
+def _last_error():
+    from pegainfer_amd import _lib
+    return _lib.last_error()
