@@ -363,14 +363,16 @@ typedef struct pega_moe_few {
  * INT4 weights count as (nibble - 8) * scale unrounded; x goes into the INT4 products exactly down to
  * 2^-25 of its row's largest magnitude (to 2^-40 of it below); the SwiGLU rows, times weight and
  * routed_scale, are rounded once to fp16 with a scale for each 64 (bf16 in front of a bf16 down
- * projection), out once, and all sums are fp32, in an order that the sizes and the routing decide.  A
- * row of x with an infinity or a NaN gives a row of NaN; other rows are as without it.  Experts without a route are not read.  Calls that share a
- * workspace must not overlap (two captured graphs that may run at once need one each); nothing is
- * kept in it from one call to the next but the zeroed counters.  topk_weight and topk_idx are apart
- * from every input and from out, and out from what the second launch reads (residual, unless it is
- * out itself, and the down projections).  At most 16 tokens, topk 32, 512
- * local experts, 1024 experts, sizes multiples of 64, 2 hidden_dim (2 inter + 16) bytes under 2 GiB
- * for the larger of inter and shared_inter, 16-byte aligned buffers (801 otherwise). */
+ * projection, whose products take bf16 rows), out once, and all sums are fp32, in an order that the
+ * sizes and the routing decide.  A row of x with an infinity or a NaN gives NaN wherever an INT4 expert
+ * takes it; what takes no part (an expert that is not local, no shared expert) leaves its residual as it
+ * is, a bf16 shared expert gives what fp32 gives, and other rows are as without it.  Experts without a
+ * route are not read.  Calls that share a workspace must not overlap (two captured graphs that may run
+ * at once need one each); nothing is kept in it from one call to the next but the zeroed counters.
+ * topk_weight and topk_idx are apart from every input and from out, and out from what the second launch
+ * reads (residual, unless it is out itself, and the down projections).  At most 16 tokens, topk 32, 512
+ * local experts, 1024 experts, sizes multiples of 64, 2 hidden_dim (2 inter + 16) bytes under 2 GiB for
+ * the larger of inter and shared_inter, 16-byte aligned buffers (801 otherwise). */
 int pega_moe_few_tokens(const pega_moe_few* args, hipStream_t stream);
 
 /* ---------------- residual add + norm ---------------- */

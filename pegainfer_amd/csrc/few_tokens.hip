@@ -36,9 +36,11 @@
 // Then a scale is applied to 4 sums a lane instead of 16, and scales and activations are loaded
 // once per 4 (2) groups.
 //
-// Roundings: the SwiGLU rows, with their weights, once to fp16 with a scale for each 64 (bf16 in front of
-// a bf16 down projection); out once.  Everything between is fp32.  A row with an infinite or NaN
-// activation gives NaN.
+// Roundings: the SwiGLU rows, with their weights, once to fp16 with a scale for each 64, the type that the
+// nibbles' products take (2^-11 of each at most); to bf16 in front of a bf16 down projection, since an
+// instruction's operands are of one type (2^-8 of each at most: one token of a Kimi share is 0.0021 off the
+// formula, of which rounding out alone makes 0.0017); out once.  Everything between is fp32.  A row with an
+// infinite or NaN activation gives NaN where an INT4 expert takes it.
 //
 // The weights' bytes bound it, below them the select in front of the routed stream (4 us, 9 from nine
 // tokens on), 2 us between the launches and 3 for the last workgroups' join.  48 of 384 experts of 7168 x

@@ -365,3 +365,28 @@ def test_layers_take_the_inputs_of_their_general_form(kind):
         if n:
             _check(host(outs[0]), *c.want(x[:5], idx, w, res[:5] if kind == "kimi" else None,
                                           2.827 if kind == "kimi" else 1.0))
+
+
+@pytest.mark.parametrize("t", [3, 9])
+def test_not_finite_rows_that_no_local_expert_takes(t):
+    """Only the other tokens have local routes: without a shared expert the residual stays as it is,
+    with one the row is NaN; the other rows keep their bits."""
+    for kind in ("none", "int4", "bf16"):
+        c = Case(256, 64, 4, 16, 2, 8, kind, 8)
+        ws = c.workspace(t)
+        x, logits, bias, res = c.inputs(t)
+        logits[:, 8:12] = 20.0
+        logits[1, 8:12] = -20.0
+        clean, _, _ = c.run(ws, x, logits, bias, res, False, 1.0)
+        keep = np.arange(t) != 1
+        for v in (0x7FC0, 0x7F80, 0xFF80):
+            bad = x.copy()
+            bad[1, 100] = v
+            out, _, idx = c.run(ws, bad, logits, bias, res, False, 1.0)
+            local = (idx >= 8) & (idx < 12)
+            assert not local[1].any() and local[keep].any(1).all()
+            assert np.array_equal(out[keep], clean[keep])
+            if kind == "none":
+                assert np.array_equal(out[1], res[1])
+            else:
+                assert np.isnan(bf(out)[1]).all()
