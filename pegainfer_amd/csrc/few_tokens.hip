@@ -486,8 +486,10 @@ __global__ __launch_bounds__(kThreads, 4) void few_w13_kernel(FewArgs f) {
     }
     first = mine;
     step = f.routed;
-    // few tile pairs are cut along K, while a CU of its own is there for each share: a workgroup
-    // streams about 35 GB/s, whatever the others leave free
+    // Few tile pairs are cut along K, while a CU of its own is there for each share: a workgroup
+    // streams about 35 GB/s, whatever the others leave free.  The launch has a workgroup for every tile
+    // pair that the routes could need, so this is where some go to other GPUs or several to one expert;
+    // with all of them here and apart there is one for each pair and no cut.
     if (live > 0) shares = max(1, min(kMaxShares, f.routed_first / (live * tiles)));
   }
   __syncthreads();

@@ -390,3 +390,17 @@ def test_not_finite_rows_that_no_local_expert_takes(t):
                 assert np.array_equal(out[1], res[1])
             else:
                 assert np.isnan(bf(out)[1]).all()
+
+
+@pytest.mark.parametrize("t,topk,live", [(8, 2, 2), (3, 3, 3), (16, 6, 6)])
+def test_every_expert_here_and_the_tokens_on_the_same(t, topk, live):
+    """No route to another GPU, and fewer experts than there could be: the first launch's K is cut."""
+    c = Case(1024, 128, 16, 16, topk, 0, "int4", t, 64)
+    ws = c.workspace(t)
+    x, logits, bias, res = c.inputs(t)
+    logits[:] = logits[0]
+    for softmax in (True, False):
+        out, w, idx = c.run(ws, x, logits, bias, res, softmax, 1.25)
+        assert len(np.unique(idx)) == live
+        _check(out, *c.want(x, idx, w, res, 1.25))
+    assert (host(ws.counters) == 0).all()
