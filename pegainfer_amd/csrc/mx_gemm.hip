@@ -651,12 +651,15 @@ int grouped_launch(const MxArgs& a, int ep_size, hipStream_t stream, const char*
   const double live = reached > local / a.bs ? reached : local / a.bs;
   const double units = live * ceil_div(a.M, 128);
   // Tiles as wide as the experts' rows: 256 x 128 (and then a mapping that keeps an expert's tiles
-  // on one XCD) from 64 rows an expert on, 128 x 64 from 32, or where a block is over 32.  MXFP8 in
-  // 128 x 64 / 256 x 128: 4096 x 7168 over 48 experts at 43, 85, 341 rows each 182 / 186, 265 / 207, 730 /
-  // 542 us; 2816 x 2048 over 64 at 47, 94, 375 rows 57 / 65, 86 / 89, 244 / 222 us.  In 128 x 32 / 128 x 64 with
-  // blocks of 32: 2816 x 2048 at 47 rows 73 / 61 us, 4096 x 7168 at 21 rows 162 / 167 us.
+  // on one XCD) from 72 rows an expert on, 128 x 64 from 32, or where a block is over 32.  MXFP8 in
+  // 128 x 64 / 256 x 128, in us, at 48, 64, 80, 192 rows an expert on average: 4096 x 7168 over 48 experts
+  // 197 / 219, 224 / 233, 262 / 203, 437 / 360; 7168 x 2048 over 48 104 / 122, 119 / 130, 142 / 135, 232 / 226;
+  // 2816 x 2048 over 64 57 / 66, 69 / 81, 86 / 87, 148 / 140; 2048 x 1408 over 64 33 / 37, 43 / 51, 52 / 42, 86 /
+  // 82 (16 experts of 4096 x 4096, few tiles a CU, go either way: 54 / 42 at 64, 54 / 71 at 80).  MXFP4 rows
+  // rank alike.  In 128 x 32 / 128 x 64 with blocks of 32: 2816 x 2048 at 24 and 48 rows 50 / 53, 71 / 67,
+  // 4096 x 7168 177 / 169, 229 / 179.
   const double rows = local / a.experts;
-  if (a.K >= kTileMinK && rows >= 64.0) {
+  if (a.K >= kTileMinK && rows >= 72.0) {
     launch_tile<Tile256x128<kXFormat>, true>(a, blocks, stream);
     return launch_status(name);
   }
@@ -668,9 +671,13 @@ int grouped_launch(const MxArgs& a, int ep_size, hipStream_t stream, const char*
   // Short blocks: tiles of 128 x 32, or, where too few of them have rows, the streaming kernel, whose
   // waves share K.  Rows of 2 KB of weights or multiples of it meet in few memory channels when
   // streamed; other long ones stream as well until there are several tiles a CU.  Streaming / tiled, MXFP8,
-  // in us: 4096 features of k 4096 in 8, 16, 63 experts 21 / 14, 40 / 27, 176 / 105; of k 5120 in 2, 4, 16
-  // 9 / 11, 15 / 13, 50 / 38; of k 7168 in 2, 10, 25, 62 10 / 14, 34 / 42, 78 / 87, 195 / 184; 2816 of k
-  // 2048 in 6, 18 8.2 / 6.5, 17.5 / 12.1.
+  // in us, 2816 features with 6, 20, 35, 61 experts reached (127, 443, 747, 1340 units): k 2560 8.3 / 7.4,
+  // 17 / 15, 31 / 26, 66 / 53; k 4096 11.6 / 10.6, 33 / 27, 60 / 50, 101 / 77; k 5120 12.9 / 12.6, 34 / 34, 64 / 56,
+  // 115 / 104; k 6144 15.3 / 14.2, 43 / 41, 71 / 64, 127 / 120; k 7168 15.9 / 15.1, 49 / 47, 73 / 71, 134 / 133; k 8192
+  // 18.1 / 16.8, 56 / 56, 98 / 102, 172 / 160.  With 10 or 12 experts (a tile and a bit a CU) k 6144 to 8192
+  // stream 20 to 35% faster, with 2 (63 units) any k does, 4.3 / 6.7 to 12 / 16.  MXFP4 rows, streamed with
+  // eight steps in flight, gain 5 to 20% on the tiles from k 6144 on below 1340 units, and at k 8192 lose
+  // it by the rule (747 units 91 / 105).
   const double enough = a.K <= 2560 ? 0.25 * cu : a.K < 6144 || a.K % 4096 == 0 ? 0.5 * cu : 5.0 * cu;
   const bool tiled = a.K >= kTileMinK && units >= enough;
   if (tiled) launch_tile<MxTile<kXFormat, 4, 1, 2, 2, 6>, true>(a, blocks, stream);

@@ -323,3 +323,20 @@ def test_grouped_streaming_forms(tokens, topk, experts, bs, m, k, name):
         r = (flat == e).nonzero()[:, 0]
         want = (xv[r // topk] @ wv[e * m:(e + 1) * m].T).float().bfloat16()
         assert torch.equal(y[r], want), e
+
+
+@pytest.mark.parametrize("name", ["fp8", "fp4"])
+@pytest.mark.parametrize("tokens,bs", [(280, 64), (300, 64), (270, 32), (320, 48)])
+def test_grouped_either_side_of_the_widest_tile(tokens, bs, name):
+    """About 70, 75, 68 and 80 rows an expert: 128 x 64 tiles below 72, 256 x 128 above, several blocks an
+    expert."""
+    from pegainfer_amd import ops
+    topk, experts, m, k = 2, 8, 528, 1152
+    idx, routing = _route(tokens, topk, experts, experts, 0, bs, tokens)
+    (x, xv), (w, wv) = _small(tokens, k, name, tokens), _small(experts * m, k, "fp4", k)
+    y = torch.full((tokens * topk, m), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.mx_grouped_gemm(routing, x, w, None, y, top_k=topk, mul_topk_weights=False, size_m=tokens)
+    flat = torch.from_numpy(idx.reshape(-1)).cuda()
+    for e in range(experts):
+        r = (flat == e).nonzero()[:, 0]
+        assert torch.equal(y[r], (xv[r // topk] @ wv[e * m:(e + 1) * m].T).float().bfloat16()), e
