@@ -1,9 +1,12 @@
 // Rows into a microscaled format and back (mx_format.h): the load-time quantisation of MXFP4
 // weights, the activations' quantisation in front of an MX product, SwiGLU with the quantisation
 // in its epilogue, and the values that codes and scales stand for.  Each is one pass over its
-// bytes, which bound it; eight columns a lane, 16-byte loads.  9728 x 2560: to MXFP4 13.8 us and
-// back 14.8 (63 MB each way, 4.6 and 4.3 TB/s; a plain copy reaches 4.8), SwiGLU of as many
-// outputs to MXFP8 34.7 (126 MB, 3.6 TB/s, 4.4 at four times the rows).
+// bytes; eight columns a lane, 16-byte loads.  9728 x 2560, three sets in turn: to MXFP4 and back 10.7 us
+// each (63 MB, 5.9 TB/s, partly out of the last-level cache), to MXFP8 and back 12.5; 16384 x 7168 to
+// MXFP4 52 us (5.7 TB/s; a copy of 1 GiB reaches 5.1), to MXFP8 61 us.  The bytes bound these.  SwiGLU of
+// 9728 x 2560 takes 32 us to MXFP8 (126 MB, 3.9 TB/s) and 31 to MXFP4 (113 MB), of four times the rows 116
+// and 113 (4.3 and 4.0 TB/s): the vector instructions bound it, 386 for a wave's 512 values (the hardware
+// exponential, a division and the checks that make it the exact bf16 SwiGLU), four cycles each.
 #include "common.h"
 #include "mx_format.h"
 #include "pega_moe.h"

@@ -559,11 +559,13 @@ constexpr int kTileMinK = 512;
 
 // The tile shapes, smallest first, with what a step of 128 k costs a CU that has one tile, and each
 // of several, and what a tile costs besides its steps (its start, and its results, which the large
-// ones write while nothing else runs on their CU), in ns.  Measured with MXFP8 rows, 64 x 64 to
-// 256 x 256: 256 rows x 4096 x 7168 19 / 26 / 35 / 51 / 86 us, 1024 rows 57 / 46 / 40 / 54 / 91, 4096 rows 203 /
-// 168 / 154 / 113 / 98; over 106 sizes the chosen shape is within 5% of the best one (rms).  MXFP4
-// rows are 5 to 30% faster everywhere and rank the shapes alike.  Four stages make every place in
-// the ring a constant; 64 x 64 tiles, whose steps are shortest, gain more from a fifth (256 rows x 4096 x
+// ones write while nothing else runs on their CU), in ns.  Measured with MXFP8 rows and operands that come
+// from HBM, 64 x 64 to 256 x 256: 256 rows x 4096 x 7168 20 / 27 / 37 / 53 / 90 us, 1024 rows 57 / 47 / 40 / 53 /
+// 89, 4096 rows 200 / 166 / 151 / 111 / 96 (15, 34 and 86 us by the chosen shapes where the last-level cache
+// has the operands); MXFP4 rows 17 / 25 / 29 / 43 / 59, 46 / 39 / 32 / 44 / 59, 157 / 134 / 99 / 91 / 69.  Over 53 sizes
+// each, drawn from 65 to 4096 rows, 512 to 10240 features and k 1024 to 9216, the chosen shape is within
+// 0.6% (MXFP8) and 2.9% (MXFP4) of the best one, rms, and 4% and 15% at most.  Four stages make every place
+// in the ring a constant; 64 x 64 tiles, whose steps are shortest, gain more from a fifth (256 rows x 4096 x
 // 7168 22.2 and 18.8 us), and 256 x 256 of MXFP8 have room for three.
 template <int F> using Tile64 = MxTile<F, 2, 2, 2, 2, 5>;
 template <int F> using Tile128x64 = MxTile<F, 2, 2, 4, 2, 4>;

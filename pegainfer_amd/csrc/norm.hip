@@ -13,9 +13,9 @@
 // odd (the last bit set if anything was cut off), after which one more rounding, to bf16 or to a
 // code, is the rounding of y itself, among fp32's smallest numbers too.  Past fp32's range y is an
 // infinity.  The norm is of s itself, not of bf16(s), so normed is not quite the norm of
-// residual_out.  The 64-bit work hides behind the memory:
-// 4096 rows of 7168 with every output take 57 us (265 MB, 4.6 TB/s; a plain copy reaches 4.8),
-// one row 5.0 us, of which the launch itself is 2.3.
+// residual_out.  The 64-bit work hides behind the memory: 4096 rows of 7168 with every output take
+// 56 us (265 MB, 4.7 TB/s; a copy of 1 GiB reaches 5.1), one row 4.9 us, of which the launch itself is
+// 2.3.
 #include "common.h"
 #include "mx_format.h"
 #include "pega_moe.h"

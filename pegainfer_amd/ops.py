@@ -971,7 +971,10 @@ def add_rmsnorm(x: torch.Tensor, residual, weight: torch.Tensor, eps: float, *,
 
     x is bf16, or float32 (a routed sum); residual, weight and the outputs are bf16.  Outputs
     left None are not formed (at least one is needed); an output may be x or residual itself,
-    and no two may share memory.  Every output is the formula's value rounded once."""
+    and no two may share memory.  Every output is the formula's value rounded once: y is of s
+    itself, so normed differs, by up to a rounding of s, from the norm of residual_out that a
+    model with a rounded residual defines.  For that one add first (a call with residual_out
+    alone) and norm its result."""
     if x.dim() != 2 or not (x.dtype == torch.float32 or _is_bf16(x)):
         raise ValueError("x must be bf16 or float32 [rows, hidden]")
     rows, hidden = x.shape
