@@ -393,6 +393,72 @@ int pega_add_rmsnorm(const void* x, bool x_is_f32, const uint16_t* residual,
                      uint16_t* normed, uint8_t* mxfp8_codes, uint8_t* mxfp8_scales, int rows,
                      int hidden_dim, hipStream_t stream);
 
+/* No reference counterpart: what stands between two blocks that are normed on both sides, for rows
+ * [rows][hidden_dim]:
+ *   y = x * post_weight / sqrt(mean(x^2) + eps)         (x itself where post_weight is NULL)
+ *   s = residual_scale * residual + gate * y            (gate * y where residual is NULL)
+ *   z = s * pre_weight / sqrt(mean(s^2) + eps)
+ *   residual_out = bf16(s); normed = bf16(z); mxfp8_codes / mxfp8_scales = z in MXFP8 (below).
+ * gate_kind 0: no gate; 1: bf16 [hidden_dim], one for each column; 2: bf16 [rows], one for each row;
+ * 3: bf16 [rows][hidden_dim].  With unit_offset the weights are stored less one: 1 + post_weight and
+ * 1 + pre_weight are meant.  pre_weight may be NULL where residual_out alone is asked for.  What
+ * pega_add_rmsnorm says of x, of the outputs, of their places, of rounding and of sizes holds here; no
+ * output may overlap the gate or a weight. */
+int pega_sandwich_rmsnorm(const void* x, bool x_is_f32, const uint16_t* residual,
+                          double residual_scale, const uint16_t* post_weight, const uint16_t* gate,
+                          int gate_kind, const uint16_t* pre_weight, bool unit_offset, double eps,
+                          uint16_t* residual_out, uint16_t* normed, uint8_t* mxfp8_codes,
+                          uint8_t* mxfp8_scales, int rows, int hidden_dim, hipStream_t stream);
+
+/* ---------------- dense products with 4-bit weights ----------------
+ * Weights [out_dim][in_dim] of 4-bit codes q with a bf16 scale s, and where `zeros` is given a zero
+ * point z, for each group of 32, 64 or 128 columns: (q - z) * s, z = 8 without zero points. */
+
+/* No reference counterpart: a checkpoint's weight into the device layout of pega_w4_gemm.
+ * packed [out_dim][in_dim / 2] bytes, the even column in the low nibble; scales bf16
+ * [out_dim][in_dim / group_size]; zeros bytes of the same shape, 0 to 127, or NULL.  codes takes
+ * ceil(out_dim / 16) * ceil(in_dim / 128) * 1024 bytes, meta the same number of units of
+ * 16 * 128 / group_size * (zeros ? 4 : 2) bytes.  in_dim is whole groups, at most 2^20.  packed is
+ * 4-byte aligned, codes and meta 16-byte (801 otherwise). */
+int pega_w4_pack(const uint8_t* packed, const uint16_t* scales, const uint8_t* zeros,
+                 uint8_t* codes, uint8_t* meta, int out_dim, int in_dim, int group_size,
+                 hipStream_t stream);
+
+/* No reference counterpart: Y[n][m] = sum_k X[n][k] * (q[m][k] - z[m][k / g]) * s[m][k / g], X [N][K]
+ * bf16, Y [N][M] bf16 or, with y_is_f32, fp32; any M, N and whole groups of K.  No weight is
+ * rounded: products with the codes' integers are exact, group sums and their products with the scales
+ * fp32.  A row of X with an infinity or a NaN gives NaN.  A row's result does not depend on the other
+ * rows' values.  No workspace.  16-byte aligned buffers (801 otherwise); Y overlaps no input. */
+int pega_w4_gemm(const uint8_t* codes, const uint8_t* meta, bool has_zeros, int group_size,
+                 const uint16_t* X, void* Y, bool y_is_f32, int M, int N, int K,
+                 hipStream_t stream);
+
+/* ---------------- next tokens ---------------- */
+
+/* No reference counterpart: a token for each row of logits (fp32, or bf16 with logits_bf16), rows
+ * row_stride elements apart:
+ *   w[v] = e^((l[v] - max l) / temperature); zero where that is below e^-28 or below min_p
+ *   of these the first top_k by logit (ties to the lower index) keep their weight;
+ *   of these, in that order, the ones with less than top_p of their sum before them;
+ *   token = the first v in index order with w[0] + .. + w[v] > uniform * (sum of w), and
+ *   logprob = ln(w[token] / sum of w).
+ * temperature, top_k, top_p, min_p: one value a row, or NULL (1, all, 1, 0).  temperature <= 0 takes
+ * the largest logit; top_k <= 0 and top_p >= 1 leave all; the first token of the order always stays.
+ * uniform is in [0, 1) (1 and more take the last kept token).  NaN logits count as -inf and are never
+ * drawn; +inf ones share all weight; a row without any other logit than -inf gives token -1 and
+ * logprob -inf.  Weights are rounded to 2^-44 once and summed exactly, so a row's result depends
+ * on its own inputs alone.  vocab at most 2^19 (801 above).  workspace: 16-byte aligned, at least
+ * pega_sample_workspace_bytes(rows, vocab) bytes, for one call at a time; it keeps nothing from one
+ * call to the next.  logprobs may be NULL.  No output overlaps another or an input. */
+int pega_sample_tokens(const void* logits, bool logits_bf16, long long row_stride, int rows,
+                       int vocab, const float* uniform, const float* temperature,
+                       const int32_t* top_k, const float* top_p, const float* min_p,
+                       int32_t* tokens, float* logprobs, void* workspace,
+                       long long workspace_bytes, hipStream_t stream);
+
+/* The workspace that pega_sample_tokens needs for up to `rows` rows of up to `vocab` logits. */
+long long pega_sample_workspace_bytes(int rows, int vocab);
+
 /* ---------------- microscaled formats (MXFP8, MXFP4) ----------------
  * 32 consecutive values of a row share a scale 2^s, stored as the byte s + 127 (255: NaN).
  * format 0: E4M3 codes [rows][cols] bytes; format 1: E2M1 codes [rows][cols / 2] bytes, the even

@@ -83,6 +83,11 @@ SIGNATURES = {
     "gemm_graphsafe_cuda": [_P, _P, _P, _I, _I, _I, _P],
     "pega_dense_w13_swiglu": [_P, _P, _P, _I, _I, _I, _P],
     "pega_add_rmsnorm": [_P, _B, _P, _P, _D, _P, _P, _P, _P, _I, _I, _P],
+    "pega_sandwich_rmsnorm": [_P, _B, _P, _D, _P, _P, _I, _P, _B, _D] + [_P] * 4 + [_I, _I, _P],
+    "pega_w4_pack": [_P] * 5 + [_I] * 3 + [_P],
+    "pega_w4_gemm": [_P, _P, _B, _I, _P, _P, _B] + [_I] * 3 + [_P],
+    "pega_sample_tokens": [_P, _B, _LL, _I, _I] + [_P] * 8 + [_LL, _P],
+    "pega_sample_workspace_bytes": [_I, _I],
     "pega_mx_quantize": [_P, _P, _P, _I, _I, _I, _P],
     "pega_mx_swiglu_quantize": [_P, _P, _P, _I, _I, _I, _P],
     "pega_mx_dequantize": [_P, _P, _P, _I, _I, _I, _P],
@@ -90,7 +95,8 @@ SIGNATURES = {
     "pega_mx_gemm": [_P] * 4 + [_I, _P] + [_I] * 3 + [_P],
     "pega_mx_grouped_gemm": [_P, _P, _I] + [_P] * 7 + [_I] * 3 + [_B] + [_I] * 5 + [_P],
 }
-_RESTYPE = {"pegainfer_kernels_last_error": ctypes.c_char_p}
+_RESTYPE = {"pegainfer_kernels_last_error": ctypes.c_char_p,
+            "pega_sample_workspace_bytes": _LL}
 
 _lib = None
 

@@ -73,6 +73,35 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
 // (the sum needs them all), so an output may be the buffer of an input.
 constexpr int kMaxWaves = 16;
 
+// y in fp32 for one more rounding (to_odd, to_odd_small where one of the wave's pairs needs it).
+__device__ __forceinline__ void to_odd2(double p0, double p1, float* y) {
+  y[0] = to_odd(p0);
+  y[1] = to_odd(p1);
+  // hardly ever, in any lane: a jump
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(is_subnormal(y[0]) || is_subnormal(y[1])) != 0, 0)) {
+    y[0] = is_subnormal(y[0]) ? to_odd_small(p0) : y[0];
+    y[1] = is_subnormal(y[1]) ? to_odd_small(p1) : y[1];
+  }
+}
+
+// The sum over a row's lanes, in each of them.  s_sum: a place a wave, used by this sum alone.
+__device__ __forceinline__ double row_sum(double sum, double* s_sum, int lanes, int lane) {
+  sum = sum16(sum);
+  sum = (lane_f64(sum, 0) + lane_f64(sum, 16)) + (lane_f64(sum, 32) + lane_f64(sum, 48));
+  if (lanes > 64) {
+    if ((lane & 63) == 0) s_sum[lane >> 6] = sum;
+    __syncthreads();
+    const int w = lane & 15;
+    sum = sum16(w < lanes >> 6 ? s_sum[w] : 0.0);
+  }
+  return sum;
+}
+
+__device__ __forceinline__ float bf_at(uint4 q, int i) {
+  const uint32_t w = (i >> 1) == 0 ? q.x : (i >> 1) == 1 ? q.y : (i >> 1) == 2 ? q.z : q.w;
+  return (i & 1) ? bf_hi(w) : bf_lo(w);
+}
+
 template <int CH, bool kX32>
 __global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) void add_rmsnorm_kernel(
     const void* x, const uint16_t* residual, const uint16_t* __restrict__ weight, double eps,
@@ -125,15 +154,7 @@ __global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) voi
       sum = __builtin_fma(s[c][i], s[c][i], sum);
     }
   }
-  sum = sum16(sum);
-  sum = (lane_f64(sum, 0) + lane_f64(sum, 16)) + (lane_f64(sum, 32) + lane_f64(sum, 48));
-  if (lanes > 64) {
-    if ((lane & 63) == 0) s_sum[lane >> 6] = sum;
-    __syncthreads();
-    const int w = lane & 15;
-    sum = sum16(w < lanes >> 6 ? s_sum[w] : 0.0);
-  }
-  const double inv = 1.0 / __builtin_sqrt(sum / hidden + eps);
+  const double inv = 1.0 / __builtin_sqrt(row_sum(sum, s_sum, lanes, lane) / hidden + eps);
 
   const bool whole = (hidden & 127) == 0;
 #pragma unroll
@@ -150,17 +171,9 @@ __global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) voi
     }
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const double p0 = s[c][i] * inv * static_cast<double>(bf_lo(ww[i >> 1]));
-      const double p1 = s[c][i + 1] * inv * static_cast<double>(bf_hi(ww[i >> 1]));
-      y[i] = to_odd(p0);
-      y[i + 1] = to_odd(p1);
-      // hardly ever, in any lane: a jump
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(is_subnormal(y[i]) | is_subnormal(y[i + 1])) != 0, 0)) {
-        y[i] = is_subnormal(y[i]) ? to_odd_small(p0) : y[i];
-        y[i + 1] = is_subnormal(y[i + 1]) ? to_odd_small(p1) : y[i + 1];
-      }
-    }
+    for (int i = 0; i < 8; i += 2)
+      to_odd2(s[c][i] * inv * static_cast<double>(bf_lo(ww[i >> 1])),
+              s[c][i + 1] * inv * static_cast<double>(bf_hi(ww[i >> 1])), y + i);
     if (normed && ok)
       *reinterpret_cast<uint4*>(normed + at) =
           make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
@@ -170,6 +183,155 @@ __global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) voi
       const uint32_t scale = mx_encode8<kMxE4M3>(y, w);
       mx_store8<kMxE4M3>(codes + base, scales + (base >> 5), v, ok, whole, w, scale);
     }
+  }
+}
+
+// The same between two blocks that are normed on both sides:
+//
+//   y = x * post_weight / sqrt(mean(x^2) + eps)      (x itself without a post_weight)
+//   s = residual_scale * residual + gate * y         residual_out = bf16(s)
+//   z = s * pre_weight / sqrt(mean(s^2) + eps)       normed = bf16(z), codes, scales = MXFP8(z)
+//
+// with a gate for each column, each row, each value, or none, and weights that are stored less one
+// (`one` = 1) or as they are (0).  One pass as above with two sums; all loads of a row are in flight
+// before the first sum.
+struct SandwichArgs {
+  const void* x;
+  const uint16_t *residual, *post, *pre, *gate;
+  long long gate_row;  // elements from a row's gate to the next row's
+  bool gate_cols;      // a gate for each column of a row, not one for the row
+  double eps, scale, one;
+  uint16_t *residual_out, *normed;
+  uint8_t *codes, *scales;
+  int rows, hidden;
+};
+
+template <int CH, bool kX32>
+__global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) void sandwich_rmsnorm_kernel(
+    SandwichArgs p) {
+  __shared__ double s_sum[2][kMaxWaves];
+  const int lanes = blockDim.x, lane = threadIdx.x;
+  const int row = blockIdx.x * blockDim.y + threadIdx.y;
+  const int vecs = p.hidden >> 3;
+  const bool in = row < p.rows;
+  const long long base = static_cast<long long>(row) * p.hidden;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint4 ones = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);
+  const uint4 none = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);  // -0: adds nothing
+
+  uint4 xr[CH][kX32 ? 2 : 1], rr[CH], pw[CH], gr[CH], nw[CH];
+  uint4 gate_one = ones;
+  if (p.gate && !p.gate_cols && in) {
+    const uint32_t g = p.gate[row * p.gate_row] * 0x10001u;
+    gate_one = make_uint4(g, g, g, g);
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int v = lane + c * lanes;
+    const bool ok = in && v < vecs;
+    const long long at = base + 8LL * v;
+    if constexpr (kX32) {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + at);
+      xr[c][0] = ok ? q[0] : zero;
+      xr[c][1] = ok ? q[1] : zero;
+    } else {
+      xr[c][0] = ok ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + at) : zero;
+    }
+    rr[c] = none;
+    if (ok && p.residual) rr[c] = *reinterpret_cast<const uint4*>(p.residual + at);
+    gr[c] = gate_one;
+    if (ok && p.gate_cols) gr[c] = *reinterpret_cast<const uint4*>(p.gate + row * p.gate_row + 8 * v);
+    pw[c] = ones;
+    if (v < vecs && p.post) pw[c] = *reinterpret_cast<const uint4*>(p.post + 8 * v);
+    nw[c] = zero;
+    if (v < vecs && p.pre) nw[c] = *reinterpret_cast<const uint4*>(p.pre + 8 * v);
+  }
+  const auto x_at = [&](int c, int i) {
+    if constexpr (kX32) {
+      const uint4 q = xr[c][i >> 2];
+      return __builtin_bit_cast(float, (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w);
+    } else {
+      return bf_at(xr[c][0], i);
+    }
+  };
+  double inv = 1.0;
+  const double post_one = p.post ? p.one : 0.0;
+  if (p.post) {
+    double sum = 0.0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double v = static_cast<double>(x_at(c, i));
+        sum = __builtin_fma(v, v, sum);
+      }
+    inv = 1.0 / __builtin_sqrt(row_sum(sum, s_sum[0], lanes, lane) / p.hidden + p.eps);
+  }
+  double s[CH][8], sum = 0.0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      double y = static_cast<double>(x_at(c, i));
+      if (p.post) y = y * inv * (post_one + static_cast<double>(bf_at(pw[c], i)));
+      const double r = p.scale * static_cast<double>(bf_at(rr[c], i));
+      s[c][i] = p.gate ? __builtin_fma(static_cast<double>(bf_at(gr[c], i)), y, r) : y + r;
+      if (lane + c * lanes >= vecs) s[c][i] = 0.0;  // a row's gate may be an infinity
+      sum = __builtin_fma(s[c][i], s[c][i], sum);
+    }
+  if (p.residual_out) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int v = lane + c * lanes;
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) to_odd2(s[c][i], s[c][i + 1], y + i);
+      if (in && v < vecs)
+        *reinterpret_cast<uint4*>(p.residual_out + base + 8LL * v) =
+            make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                       pack_bf16x2(y[6], y[7]));
+    }
+  }
+  if (!p.pre) return;
+  inv = 1.0 / __builtin_sqrt(row_sum(sum, s_sum[1], lanes, lane) / p.hidden + p.eps);
+  const bool whole = (p.hidden & 127) == 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int v = lane + c * lanes;
+    const bool ok = in && v < vecs;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+      to_odd2(s[c][i] * inv * (p.one + static_cast<double>(bf_at(nw[c], i))),
+              s[c][i + 1] * inv * (p.one + static_cast<double>(bf_at(nw[c], i + 1))), y + i);
+    if (p.normed && ok)
+      *reinterpret_cast<uint4*>(p.normed + base + 8LL * v) =
+          make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                     pack_bf16x2(y[6], y[7]));
+    if (p.codes) {
+      uint32_t w[2];
+      const uint32_t scale = mx_encode8<kMxE4M3>(y, w);
+      mx_store8<kMxE4M3>(p.codes + base, p.scales + (base >> 5), v, ok, whole, w, scale);
+    }
+  }
+}
+
+template <int CH>
+void launch_sandwich(SandwichArgs p, bool x32, hipStream_t stream) {
+  const int waves = ceil_div(p.hidden / 8, 64 * CH), per = waves == 1 ? 4 : 1;
+  const auto kernel = x32 ? sandwich_rmsnorm_kernel<CH, true> : sandwich_rmsnorm_kernel<CH, false>;
+  const int most = (1 << 25) / waves;  // rows a launch, as launch_norm's
+  for (int rows = p.rows;; rows -= most) {
+    p.rows = rows < most ? rows : most;
+    hipLaunchKernelGGL(kernel, dim3(ceil_div(p.rows, per)), dim3(64 * waves, per), 0, stream, p);
+    if (rows <= most) return;
+    const long long at = static_cast<long long>(most) * p.hidden;
+    p.x = static_cast<const uint8_t*>(p.x) + (x32 ? 4 : 2) * at;
+    if (p.residual) p.residual += at;
+    if (p.gate) p.gate += most * p.gate_row;
+    if (p.residual_out) p.residual_out += at;
+    if (p.normed) p.normed += at;
+    if (p.codes) p.codes += at, p.scales += at / kMxBlock;
   }
 }
 
@@ -245,4 +407,57 @@ PEGA_API int pega_add_rmsnorm(const void* x, bool x_is_f32, const uint16_t* resi
   else PEGA_NORM(4);
 #undef PEGA_NORM
   return launch_status("add_rmsnorm");
+}
+
+// No reference counterpart: what stands between two blocks normed on both sides.
+PEGA_API int pega_sandwich_rmsnorm(const void* x, bool x_is_f32, const uint16_t* residual,
+                                   double residual_scale, const uint16_t* post_weight,
+                                   const uint16_t* gate, int gate_kind, const uint16_t* pre_weight,
+                                   bool unit_offset, double eps, uint16_t* residual_out,
+                                   uint16_t* normed, uint8_t* mxfp8_codes, uint8_t* mxfp8_scales,
+                                   int rows, int hidden_dim, hipStream_t stream) {
+  if (rows < 0 || hidden_dim <= 0 || !(eps >= 0.0) || gate_kind < 0 || gate_kind > 3)
+    return fail(kInvalidValue, "sandwich_rmsnorm: bad arguments (rows=%d hidden=%d gate_kind=%d)", rows,
+                hidden_dim, gate_kind);
+  if (rows == 0) return kSuccess;  // empty tensors have no address
+  const bool want_norm = normed || mxfp8_codes;
+  if (!x || (gate_kind != 0 && !gate) || (want_norm && !pre_weight))
+    return fail(kInvalidValue, "sandwich_rmsnorm: null pointer");
+  if (!residual_out && !want_norm) return fail(kInvalidValue, "sandwich_rmsnorm: no output");
+  if (!mxfp8_codes != !mxfp8_scales)
+    return fail(kInvalidValue, "sandwich_rmsnorm: MXFP8 codes and scales go together");
+  if (hidden_dim % 8 != 0 || hidden_dim > 32768 || (mxfp8_codes && hidden_dim % kMxBlock != 0))
+    return fail(kNotSupported, "sandwich_rmsnorm: hidden_dim %d (a multiple of 8, of 32 for MXFP8, at "
+                "most 32768)", hidden_dim);
+  if (!aligned16(x) || !aligned16(residual) || !aligned16(post_weight) || !aligned16(pre_weight) ||
+      (gate_kind == 2 ? reinterpret_cast<uintptr_t>(gate) & 1u : gate_kind != 0 && !aligned16(gate)) ||
+      !aligned16(residual_out) || !aligned16(normed) || !aligned16(mxfp8_codes) ||
+      (reinterpret_cast<uintptr_t>(mxfp8_scales) & 3u))
+    return fail(kNotSupported, "sandwich_rmsnorm: buffers must be 16-byte aligned (scales 4, a gate per "
+                "row 2)");
+  // As in add_rmsnorm: an output may be the bf16 buffer of x or of residual, and overlaps nothing else.
+  const long long n = static_cast<long long>(rows) * hidden_dim;
+  const long long gates = gate_kind == 0 ? 0 : gate_kind == 1 ? hidden_dim : gate_kind == 2 ? rows : n;
+  struct Span { const void* p; long long bytes; };
+  const Span outs[4] = {{residual_out, 2 * n}, {normed, 2 * n}, {mxfp8_codes, n}, {mxfp8_scales, n / kMxBlock}};
+  const Span ins[5] = {{x, (x_is_f32 ? 4 : 2) * n}, {residual, 2 * n}, {post_weight, 2LL * hidden_dim},
+                       {pre_weight, 2LL * hidden_dim}, {gate, 2 * gates}};
+  for (int o = 0; o < 4; ++o) {
+    for (int i = 0; i < 5; ++i)
+      if (overlap(outs[o].p, outs[o].bytes, ins[i].p, ins[i].bytes) &&
+          !(o < 2 && i < 2 && outs[o].p == ins[i].p && ins[i].bytes == 2 * n))
+        return fail(kInvalidValue, "sandwich_rmsnorm: an output overlaps an input");
+    for (int i = 0; i < o; ++i)
+      if (overlap(outs[o].p, outs[o].bytes, outs[i].p, outs[i].bytes))
+        return fail(kInvalidValue, "sandwich_rmsnorm: two outputs overlap");
+  }
+  SandwichArgs p{x, residual, post_weight, want_norm ? pre_weight : nullptr, gate_kind ? gate : nullptr,
+                 gate_kind == 2 ? 1 : gate_kind == 3 ? hidden_dim : 0, gate_kind == 1 || gate_kind == 3,
+                 eps, residual ? residual_scale : 1.0, unit_offset ? 1.0 : 0.0, residual_out, normed,
+                 mxfp8_codes, mxfp8_scales, rows, hidden_dim};
+  const int vecs = hidden_dim / 8;
+  if (vecs <= 4 * 64) launch_sandwich<1>(p, x_is_f32, stream);
+  else if (vecs <= 8 * 2 * 64 && (vecs <= 8 * 64 || rows <= 1024)) launch_sandwich<2>(p, x_is_f32, stream);
+  else launch_sandwich<4>(p, x_is_f32, stream);
+  return launch_status("sandwich_rmsnorm");
 }

@@ -1003,6 +1003,199 @@ def add_rmsnorm(x: torch.Tensor, residual, weight: torch.Tensor, eps: float, *,
               hidden, stream)
 
 
+def sandwich_rmsnorm(x: torch.Tensor, residual, pre_weight, eps: float, *,
+                     post_weight: torch.Tensor = None, gate: torch.Tensor = None,
+                     residual_scale: float = 1.0, unit_offset: bool = False,
+                     residual_out: torch.Tensor = None, normed: torch.Tensor = None,
+                     quantized: MxTensor = None) -> None:
+    """What stands between two blocks that are normed on both sides, in one launch, for rows
+    [rows, hidden]:
+
+        y = x * post_weight / sqrt(mean(x^2) + eps)       (x itself without a post_weight)
+        s = residual_scale * residual + gate * y          (gate * y where residual is None)
+        z = s * pre_weight / sqrt(mean(s^2) + eps)
+        residual_out = bf16(s), normed = bf16(z), quantized = z in MXFP8
+
+    x is bf16 or float32, everything else bf16.  gate: None, [hidden] (one a column), [rows, 1] (one
+    a row) or [rows, hidden].  unit_offset: weights are stored less one.  pre_weight may be None
+    where residual_out alone is asked for.  Outputs, their places and their rounding as
+    add_rmsnorm's: each is the formula's value rounded once, an output may be x or residual itself."""
+    if x.dim() != 2 or not (x.dtype == torch.float32 or _is_bf16(x)):
+        raise ValueError("x must be bf16 or float32 [rows, hidden]")
+    rows, hidden = x.shape
+    for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
+        if w is not None and (not _is_bf16(w) or w.numel() != hidden):
+            raise ValueError(f"{name} must be bf16 [{hidden}]")
+    kind = 0
+    if gate is not None:
+        if not _is_bf16(gate):
+            raise ValueError("gate must be bf16")
+        shape = tuple(gate.shape)
+        if shape == (hidden,):
+            kind = 1
+        elif shape == (rows, 1):
+            kind = 2
+        elif shape == (rows, hidden):
+            kind = 3
+        else:
+            raise ValueError(f"gate must be [{hidden}], [{rows}, 1] or [{rows}, {hidden}], got {list(shape)}")
+    if residual is not None:
+        _mx_rows("residual", residual, rows, hidden)
+    if residual_out is not None:
+        _mx_rows("residual_out", residual_out, rows, hidden)
+    if normed is not None:
+        _mx_rows("normed", normed, rows, hidden)
+    codes = scales = None
+    if quantized is not None:
+        if quantized.format is not MxFormat.Fp8E4M3:
+            raise ValueError("sandwich_rmsnorm quantizes into MXFP8")
+        if (quantized.rows, quantized.cols) != (rows, hidden):
+            raise ValueError(f"quantized must be [{rows}, {hidden}]")
+        codes, scales = quantized.codes, quantized.scales
+    elif residual_out is None and normed is None:
+        raise ValueError("sandwich_rmsnorm needs an output")
+    if pre_weight is None and (normed is not None or quantized is not None):
+        raise ValueError("normed rows need a pre_weight")
+    if residual_out is not None and residual_out is normed:
+        raise ValueError("residual_out and normed must be different buffers")
+    px, pr, pp, pg, pw, ps, pn, pc, psc, stream = _ptrs_here(
+        x, residual, post_weight, gate, pre_weight, residual_out, normed, codes, scales)
+    _lib.call("pega_sandwich_rmsnorm", px, x.dtype == torch.float32, pr, residual_scale, pp, pg, kind,
+              pw, bool(unit_offset), eps, ps, pn, pc, psc, rows, hidden, stream)
+
+
+# --------------------------------------------------------------------------
+# Dense products with 4-bit weights (no reference counterpart)
+# --------------------------------------------------------------------------
+W4_GROUPS = (32, 64, 128)
+_W4_TILE, _W4_STEP = 16, 128  # features and columns of a unit of the device layout
+
+
+@dataclasses.dataclass
+class W4Weight:
+    """A weight of 4-bit codes in w4_gemm's device layout (w4_pack): out_dim features of in_dim
+    columns, a scale (with_zeros: and a zero point) for each `group` columns."""
+    out_dim: int
+    in_dim: int
+    group: int
+    with_zeros: bool
+    codes: torch.Tensor
+    meta: torch.Tensor
+
+    def __post_init__(self):
+        self.validate()
+
+    @staticmethod
+    def sizes(out_dim: int, in_dim: int, group: int, with_zeros: bool):
+        """Bytes of codes and of meta."""
+        units = -(-out_dim // _W4_TILE) * -(-in_dim // _W4_STEP)
+        return units * 1024, units * _W4_TILE * (_W4_STEP // group) * (4 if with_zeros else 2)
+
+    def validate(self) -> None:
+        _ensure(self.group in W4_GROUPS, f"groups have 32, 64 or 128 columns, got {self.group}")
+        _ensure(self.out_dim > 0 and self.in_dim > 0 and self.in_dim % self.group == 0,
+                f"4-bit weights have whole groups of {self.group} columns, got {self.out_dim} x {self.in_dim}")
+        _ensure(self.codes.dtype == torch.uint8 and self.meta.dtype == torch.uint8
+                and (self.codes.numel(), self.meta.numel())
+                == self.sizes(self.out_dim, self.in_dim, self.group, self.with_zeros),
+                "4-bit weight buffers do not match their sizes")
+
+
+def w4_pack(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor = None, *,
+            group: int) -> W4Weight:
+    """A checkpoint's 4-bit weight in the device layout, once at load time: packed uint8
+    [out, in / 2] (the even column in the low nibble), scales bf16 [out, in / group], zeros uint8
+    of the scales' shape (0 to 127), or None for codes offset by 8."""
+    _ensure(packed.dim() == 2 and packed.dtype == torch.uint8, "packed must be uint8 [out, in / 2]")
+    _ensure(group in W4_GROUPS, f"groups have 32, 64 or 128 columns, got {group}")
+    out_dim, in_dim = packed.shape[0], 2 * packed.shape[1]
+    _ensure(out_dim > 0 and in_dim > 0 and in_dim % group == 0,
+            f"4-bit weights have whole groups of {group} columns, got {out_dim} x {in_dim}")
+    shape = (out_dim, in_dim // group)
+    _ensure(_is_bf16(scales) and tuple(scales.shape) == shape, f"scales must be bf16 {list(shape)}")
+    _ensure(zeros is None or (zeros.dtype == torch.uint8 and tuple(zeros.shape) == shape),
+            f"zeros must be uint8 {list(shape)}")
+    codes, meta = (torch.empty(n, dtype=torch.uint8, device=packed.device)
+                   for n in W4Weight.sizes(out_dim, in_dim, group, zeros is not None))
+    pp, ps, pz, pc, pm, stream = _ptrs_here(packed, scales, zeros, codes, meta)
+    _lib.call("pega_w4_pack", pp, ps, pz, pc, pm, out_dim, in_dim, group, stream)
+    return W4Weight(out_dim, in_dim, group, zeros is not None, codes, meta)
+
+
+def w4_gemm(w: W4Weight, x: torch.Tensor, y: torch.Tensor) -> None:
+    """Y[n][m] = sum_k X[n][k] * (q[m][k] - z[m][k / group]) * s[m][k / group]: x bf16 [N, in], y bf16
+    or float32 [N, out].  No weight is rounded; sums are fp32 (gemm_graphsafe on 4-bit weights)."""
+    if x.dim() != 2 or x.shape[1] != w.in_dim or not _is_bf16(x):
+        raise ValueError(f"x must be bf16 [rows, {w.in_dim}], got {x.dtype} {tuple(x.shape)}")
+    f32 = y.dtype == torch.float32
+    if tuple(y.shape) != (x.shape[0], w.out_dim) or not (f32 or _is_bf16(y)):
+        raise ValueError(f"y must be bf16 or float32 [{x.shape[0]}, {w.out_dim}], got {y.dtype} {tuple(y.shape)}")
+    pc, pm, px, py, stream = _ptrs_here(w.codes, w.meta, x, y)
+    _lib.call("pega_w4_gemm", pc, pm, w.with_zeros, w.group, px, py, f32, w.out_dim, x.shape[0],
+              w.in_dim, stream)
+
+
+# --------------------------------------------------------------------------
+# Next tokens (no reference counterpart)
+# --------------------------------------------------------------------------
+SAMPLE_MAX_VOCAB = 1 << 19
+
+
+class SampleWorkspace:
+    """What sample_tokens' launches hand to each other, for up to max_rows rows of up to max_vocab
+    logits.  Calls that share one must not overlap: graphs that may replay at the same time need one
+    each."""
+
+    def __init__(self, max_rows: int, max_vocab: int, *, device="cuda"):
+        _ensure(max_rows > 0, f"sampling needs rows, got {max_rows}")
+        _ensure(0 < max_vocab <= SAMPLE_MAX_VOCAB,
+                f"sampling takes 1 to {SAMPLE_MAX_VOCAB} tokens, got {max_vocab}")
+        self.max_rows, self.max_vocab = max_rows, max_vocab
+        self.buffer = torch.empty(_lib.lib().pega_sample_workspace_bytes(max_rows, max_vocab),
+                                  dtype=torch.uint8, device=device)
+
+
+def sample_tokens(workspace: SampleWorkspace, logits: torch.Tensor, uniform: torch.Tensor,
+                  tokens: torch.Tensor, *, temperature: torch.Tensor = None,
+                  top_k: torch.Tensor = None, top_p: torch.Tensor = None,
+                  min_p: torch.Tensor = None, logprobs: torch.Tensor = None) -> None:
+    """tokens[r] drawn from row r of logits (float32 or bf16 [rows, vocab]; rows may lie further apart
+    than vocab):
+
+        w = e^((l - max l) / temperature), zero below e^-28 and below min_p
+        the first top_k by logit (ties: lower index), then of these the ones with less than top_p of
+        their sum before them, keep their weight
+        token = the first in index order whose cumulative weight passes uniform * (sum of weights)
+        logprob = ln(weight / sum of weights)
+
+    uniform, temperature, top_p, min_p float32, top_k int32, one value a row; None leaves a step out
+    (as do top_k 0, top_p 1, min_p 0), temperature 0 takes the largest logit.  tokens int32,
+    logprobs float32 or None.  NaN logits count as -inf; a row of nothing else gives token -1."""
+    if logits.dim() != 2 or not (logits.dtype == torch.float32 or logits.dtype is _BF16):
+        raise ValueError("logits must be float32 or bf16 [rows, vocab]")
+    rows, vocab = logits.shape
+    if rows > workspace.max_rows or vocab > workspace.max_vocab:
+        raise ValueError(f"{rows} x {vocab} logits exceed the workspace's "
+                         f"{workspace.max_rows} x {workspace.max_vocab}")
+    if vocab == 0 or (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        raise ValueError("logits must have rows of adjacent values that do not overlap")
+    for name, t, dtype in (("uniform", uniform, torch.float32), ("tokens", tokens, torch.int32),
+                           ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
+                           ("logprobs", logprobs, torch.float32)):
+        if t is None and name not in ("uniform", "tokens"):
+            continue
+        if t.dtype != dtype or tuple(t.shape) != (rows,):
+            raise ValueError(f"{name} must be {dtype} [{rows}], got {t.dtype} {tuple(t.shape)}")
+    pu, pt, ptemp, pk, pp, pm, pl, pw, stream = _ptrs_here(
+        uniform, tokens, temperature, top_k, top_p, min_p, logprobs, workspace.buffer)
+    if logits.device != tokens.device:
+        raise ValueError(f"tensor must live on the current GPU, got {logits.device}")
+    _lib.call("pega_sample_tokens", logits.data_ptr(), logits.dtype is _BF16,
+              max(logits.stride(0), vocab), rows, vocab, pu, ptemp, pk, pp, pm, pt, pl, pw,
+              workspace.buffer.numel(), stream)
+
+
 # --------------------------------------------------------------------------
 # Routing select
 # --------------------------------------------------------------------------
