@@ -15,8 +15,10 @@
 // integers: exact in any order, so that a row's token depends on nothing but its inputs, and every
 // comparison is of exact sums (the weights' rounding moves a border by 10^-11 at most).
 //
-// No sort.  A histogram of the weights' logarithms (counts and masses in LDS) finds the bin in which a cut falls,
-// and histograms of the keys inside the bin narrow it to one key; equal keys are cut by index.
+// No sort.  A histogram of the weights' logarithms (counts and masses in LDS) finds the bin in which
+// each cut falls; its elements are listed, and compared with each other or, where they are many,
+// narrowed down by histograms of their keys; equal keys are cut by index.  Three passes over the
+// row: its maximum, the histogram, and the list with the masses of what is kept whole.
 #include "common.h"
 #include "pega_moe.h"
 
@@ -25,8 +27,12 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 1024;
-constexpr int kList = 4096;            // elements of a bin kept in LDS
-constexpr int kParts = 128;            // of a row, whose masses the draw goes over first
+constexpr int kList = 4096;            // elements of the cuts' bins kept in LDS
+constexpr int kParts = 128;            // of a row, whose masses the draw goes over first; more with splits
+constexpr int kMaxSplit = 16;          // workgroups of a row
+constexpr int kMaxParts = kWaves * kMaxSplit;
+constexpr int kPairs = 256;            // candidates that are compared with each other
+constexpr int kWorkgroups = 512;       // two a CU
 constexpr int kMaxVocab = 1 << 19;     // sums of weights stay below 2^63
 constexpr double kRange = 28.0;        // smaller weights than e^-28 are zero
 constexpr double kLog2e = 1.4426950408889634;
@@ -134,15 +140,26 @@ struct Scale {
   __device__ __forceinline__ int bin(double d) const {
     return min(kBins - 1, static_cast<int>(-d * per * kBinsPerOctave));
   }
+  // below every d of a bin
+  __device__ __forceinline__ double edge(int b) const { return -(b + 1) / (per * kBinsPerOctave) * (1 + 0x1p-30); }
+  // a float below every logit that lies d or less below the maximum
+  __device__ __forceinline__ float bound(double d) const {
+    if (infinite) return __builtin_inff();
+    const float f = static_cast<float>(max + d);
+    return f - __builtin_fabsf(f) * 0x1p-22f - 0x1p-126f;
+  }
 };
 
 struct Shared {
-  u64 mass[kBins];
+  u64 mass[kBins];  // the row's histogram
   uint32_t count[kBins];
-  uint32_t key[kList];
+  u64 fine_mass[kBins];  // a narrower one inside a bin of it
+  uint32_t fine_count[kBins];
+  u64 part[kMaxParts];  // masses of the row's parts
+  uint32_t key[kList];  // elements of the bins in which the cuts fall
   int32_t index[kList];
   u64 wave_mass[kWaves];
-  uint32_t wave_count[kWaves], wave_b[kWaves];
+  uint32_t wave_count[kWaves];
   u64 found_mass;
   uint32_t found_count;
   int found, last, listed;
@@ -163,24 +180,16 @@ __device__ __forceinline__ void block_scan(Shared& s, uint32_t& count, u64& mass
   for (int w = 0; w < wave; ++w) count += s.wave_count[w], mass += s.wave_mass[w];
 }
 
-// The least and largest over the workgroup.
-__device__ __forceinline__ void block_range(Shared& s, uint32_t& lo, uint32_t& hi, int tid) {
+// The largest over the workgroup, in each thread.
+__device__ __forceinline__ u64 block_max(Shared& s, u64 v, int tid) {
 #pragma unroll
-  for (int by = 32; by > 0; by >>= 1) {
-    lo = min(lo, static_cast<uint32_t>(__shfl_xor(lo, by)));
-    hi = max(hi, static_cast<uint32_t>(__shfl_xor(hi, by)));
-  }
+  for (int by = 32; by > 0; by >>= 1) v = max(v, static_cast<u64>(__shfl_xor(v, by)));
   __syncthreads();
-  if ((tid & 63) == 0) s.wave_count[tid >> 6] = lo, s.wave_b[tid >> 6] = hi;
+  if ((tid & 63) == 0) s.wave_mass[tid >> 6] = v;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) lo = min(lo, s.wave_count[w]), hi = max(hi, s.wave_b[w]);
-}
-
-__device__ __forceinline__ void clear_bins(Shared& s, int tid) {
-  __syncthreads();
-  s.count[tid] = 0, s.mass[tid] = 0;
-  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) v = max(v, s.wave_mass[w]);
+  return v;
 }
 
 // A cut of the order: the first `count` elements, or those with less than `mass` before them,
@@ -190,18 +199,18 @@ struct Target {
   u64 mass;
 };
 
-// The bin in which the cut falls, given what lies before bin 0; on return what lies before that bin.
-// The last bin that is not empty if the cut lies past all of them.
-__device__ __forceinline__ int find_bin(Shared& s, const Target& t, uint32_t& before, u64& mass_before, int tid) {
-  const uint32_t own = s.count[tid];
-  const u64 own_mass = s.mass[tid];
+// The bin of a histogram in which the cut falls, given what lies before bin 0; on return what lies before
+// that bin.  -1 if the bins do not reach it.
+__device__ __forceinline__ int find_bin(Shared& s, const uint32_t* count, const u64* mass, const Target& t,
+                                        uint32_t& before, u64& mass_before, int tid) {
+  const uint32_t own = count[tid];
+  const u64 own_mass = mass[tid];
   uint32_t c = own;
   u64 m = own_mass;
   block_scan(s, c, m, tid);
   c += before, m += mass_before;
   if (tid == 0) s.found = -1;
   __syncthreads();
-  // the first bin with which either limit is reached: the bins before it do not reach them
   const bool reached = own && (c >= t.count || m >= t.mass);
   const bool earlier = c - own >= t.count || m - own_mass >= t.mass;
   if (reached && !earlier) s.found = tid, s.found_count = c - own, s.found_mass = m - own_mass;
@@ -216,126 +225,65 @@ struct Cut {
   uint32_t key;
   int32_t index;
   u64 mass;  // of what is kept
-  __device__ __forceinline__ bool keeps(float l, int i) const {
-    const uint32_t k = key_of(l);
+  __device__ __forceinline__ bool keeps(uint32_t k, int i) const {
     return k > key || (k == key && i <= index);
   }
 };
 
-// Where the cut falls in the histogram's bin `bin`, of which before and mass_before lie ahead.
-template <typename T>
-__device__ Cut resolve(Shared& s, const Row<T>& row, const Scale& scale, const Target& t, int bin,
-                       uint32_t before, u64 mass_before, const Cut& inside, int tid) {
-  if (tid == 0) s.listed = 0;
-  __syncthreads();
-  row.each(0, row.n, tid, kThreads, [&](int i, float l) {
-    const double d = scale.below(l);
-    if (!scale.live(d) || scale.bin(d) != bin || !inside.keeps(l, i)) return;
-    const int at = atomicAdd(&s.listed, 1);
-    if (at < kList) s.key[at] = key_of(l), s.index[at] = i;
-  });
-  __syncthreads();
-  const int listed = s.listed;
-  const bool whole = listed <= kList;
-  // f(key, index) of the bin's elements, from the list or from the row
-  const auto each = [&](auto f) {
-    if (whole) {
-      for (int i = tid; i < listed; i += kThreads) f(s.key[i], s.index[i]);
-    } else {
-      row.each(0, row.n, tid, kThreads, [&](int i, float l) {
-        const double d = scale.below(l);
-        if (scale.live(d) && scale.bin(d) == bin && inside.keeps(l, i)) f(key_of(l), i);
-      });
-    }
-  };
-  const auto value_of = [](uint32_t k) {
-    return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
-  };
-  uint32_t lo = 0xffffffffu, hi = 0;
-  each([&](uint32_t k, int) { lo = min(lo, k), hi = max(hi, k); });
-  block_range(s, lo, hi, tid);
-  uint32_t ties = 0;
-  while (true) {  // the range falls to a 1024th each time
-    int shift = 0;
-    while (((hi - lo) >> shift) >= kBins) ++shift;
-    clear_bins(s, tid);
-    each([&](uint32_t k, int) {
-      if (k < lo || k > hi) return;
-      const uint32_t b = (hi - k) >> shift;
-      atomicAdd(&s.count[b], 1u);
-      atomicAdd(&s.mass[b], scale.weight(scale.below(value_of(k))));
-    });
-    __syncthreads();
-    const int b = find_bin(s, t, before, mass_before, tid);
-    ties = s.count[b];
-    hi = hi - (static_cast<uint32_t>(b) << shift);
-    if (shift == 0) break;
-    const uint32_t span = (1u << shift) - 1u;
-    lo = hi - lo > span ? hi - span : lo;
-    if (lo == hi) break;
-  }
-  Cut cut;
-  cut.key = hi;
-  const u64 w = scale.weight(scale.below(value_of(hi)));
-  const u64 by_mass = (t.mass - mass_before + w - 1) / w;
-  const uint32_t keep = static_cast<uint32_t>(min(static_cast<u64>(min(t.count - before, ties)), max(by_mass, u64{1})));
-  cut.mass = mass_before + keep * w;
-  cut.index = row.n;
-  if (keep < ties) {  // the keep-th smallest index among them
-    uint32_t first = 0, last = static_cast<uint32_t>(row.n - 1), passed = 0;
-    while (true) {
-      int shift = 0;
-      while (((last - first) >> shift) >= kBins) ++shift;
-      clear_bins(s, tid);
-      each([&](uint32_t k, int i) {
-        const uint32_t at = static_cast<uint32_t>(i);
-        if (k == hi && at >= first && at <= last) atomicAdd(&s.count[(at - first) >> shift], 1u);
-      });
-      __syncthreads();
-      u64 none = 0;
-      const int b = find_bin(s, Target{keep, kNoMass}, passed, none, tid);
-      first += static_cast<uint32_t>(b) << shift;
-      if (shift == 0) break;
-      last = min(last, first + (1u << shift) - 1u);
-    }
-    cut.index = static_cast<int>(first);
-  }
-  __syncthreads();
-  return cut;
+// What a row asks for, and what its largest logit makes of that.
+struct Request {
+  Scale scale;
+  double temp;
+  float top_p, u;
+  int k;        // 0: all
+  bool none;    // no logit above -inf
+  bool first;   // the first of the order alone
+};
+
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
-  __shared__ Shared s;
-  const int tid = threadIdx.x, row_id = blockIdx.x;
-  const Row<T> row{static_cast<const T*>(p.logits) + row_id * p.stride, p.vocab};
-  uint32_t least = 0xffffffffu, most = 0;
-  row.each(0, row.n, tid, kThreads, [&](int, float l) { most = max(most, key_of(l)); });
-  block_range(s, least, most, tid);
-  const float top = __builtin_bit_cast(float, most & 0x80000000u ? most & 0x7fffffffu : ~most);
-  if (top == -__builtin_inff()) {
-    if (tid == 0) {
-      p.tokens[row_id] = -1;
-      if (p.logprobs) p.logprobs[row_id] = -__builtin_inff();
-    }
-    return;
-  }
-  float temp = p.temperature ? p.temperature[row_id] : 1.0f;
-  const bool greedy = !(temp > 0.0f);
-  temp = greedy ? 1.0f : fminf(temp, 3.40282347e38f);
-  const float min_p = p.min_p ? p.min_p[row_id] : 0.0f;
-  const float top_p = p.top_p ? p.top_p[row_id] : 1.0f;
-  const int k = greedy ? 1 : p.top_k ? p.top_k[row_id] : 0;
-  Scale scale;
-  scale.max = top;
-  scale.infinite = top == __builtin_inff();
-  scale.per = kLog2e / temp;
-  scale.least = -kRange * temp;
-  if (min_p > 0.0f) scale.least = fmax(scale.least, temp * ::log(static_cast<double>(fminf(min_p, 1.0f))));
+// A logit and its index in one number: the larger, the further ahead in the order.
+__device__ __forceinline__ u64 place(float l, int i) {
+  return static_cast<u64>(key_of(l)) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
+}
 
-  // the histogram, and each part's mass for the draw
-  clear_bins(s, tid);
-  row.each(0, row.n, tid, kThreads, [&](int, float l) {
+__device__ __forceinline__ Request request(const SampleArgs& p, int row, u64 best) {
+  Request q;
+  const float top = value_of(static_cast<uint32_t>(best >> 32));
+  const float temp = p.temperature ? p.temperature[row] : 1.0f;
+  const float min_p = p.min_p ? p.min_p[row] : 0.0f;
+  const bool greedy = !(temp > 0.0f);
+  q.k = greedy ? 1 : p.top_k ? max(p.top_k[row], 0) : 0;
+  q.first = q.k == 1;
+  q.none = top == -__builtin_inff();
+  q.top_p = p.top_p ? p.top_p[row] : 1.0f;
+  q.u = p.u[row];
+  q.temp = greedy ? 1.0 : static_cast<double>(fminf(temp, 3.40282347e38f));
+  q.scale.max = top;
+  q.scale.infinite = top == __builtin_inff();
+  q.scale.per = kLog2e / q.temp;
+  q.scale.least = -kRange * q.temp;
+  if (min_p > 0.0f)
+    q.scale.least = fmax(q.scale.least, q.temp * ::log(static_cast<double>(fminf(min_p, 1.0f))));
+  return q;
+}
+
+__device__ __forceinline__ void write(const SampleArgs& p, int row, int token, float logprob) {
+  p.tokens[row] = token;
+  if (p.logprobs) p.logprobs[row] = logprob;
+}
+
+// The histogram of elements [from, to).
+template <typename T>
+__device__ __forceinline__ void histogram(Shared& s, const Row<T>& row, const Scale& scale, int from,
+                                          int to, int tid) {
+  s.count[tid] = 0, s.mass[tid] = 0;
+  __syncthreads();
+  const float low = scale.bound(scale.least);
+  row.each(from, to, tid, kThreads, [&](int, float l) {
+    if (l < low) return;
     const double d = scale.below(l);
     if (!scale.live(d)) return;
     const int b = scale.bin(d);
@@ -343,95 +291,442 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     atomicAdd(&s.mass[b], scale.weight(d));
   });
   __syncthreads();
-  const uint32_t own = s.count[tid];
-  const u64 own_mass = s.mass[tid];
-  uint32_t live = own;
-  u64 total = own_mass;
-  block_scan(s, live, total, tid);
-  if (tid == kThreads - 1) s.found_count = live, s.found_mass = total;
+}
+
+// Which bins the cuts fall in.
+struct Plan {
+  uint32_t live;    // elements with weight
+  u64 total;        // and their mass
+  bool by_k, by_p;  // cuts that leave something out
+  int sure;         // bins before it are kept whole
+  int k_bin, p_first, p_last;  // of the cuts, -1 without one; the p cut's within a range
+  uint32_t candidates;         // elements of those bins
+  __device__ __forceinline__ bool has(int b) const { return b == k_bin || (b >= p_first && b <= p_last); }
+};
+
+__device__ __forceinline__ u64 p_mass(float p, u64 total) {
+  const double want = static_cast<double>(fmaxf(p, 0.0f)) * static_cast<double>(total);
+  return min(max(static_cast<u64>(__builtin_ceil(want)), u64{1}), total);
+}
+
+__device__ __forceinline__ Plan make_plan(Shared& s, const Request& q, int tid) {
+  Plan plan{0, 0, false, false, kBins, -1, -1, -2, 0};
+  uint32_t c = s.count[tid];
+  u64 m = s.mass[tid];
+  block_scan(s, c, m, tid);
+  if (tid == kThreads - 1) s.found_count = c, s.found_mass = m;
   __syncthreads();
-  live = s.found_count, total = s.found_mass;
-  Cut cut{0, row.n, total};
-  if (k > 0 && static_cast<uint32_t>(k) < live) {
-    const Target t{static_cast<uint32_t>(k), kNoMass};
+  plan.live = s.found_count, plan.total = s.found_mass;
+  plan.by_k = q.k > 0 && static_cast<uint32_t>(q.k) < plan.live;
+  plan.by_p = q.top_p < 1.0f;
+  u64 least = plan.total, most = plan.total;  // what the k cut leaves
+  if (plan.by_k) {
+    uint32_t before = 0;
+    least = 0;
+    plan.k_bin = find_bin(s, s.count, s.mass, Target{static_cast<uint32_t>(q.k), kNoMass}, before, least, tid);
+    most = least + s.mass[plan.k_bin];
+    plan.sure = plan.k_bin;
+    plan.candidates = s.count[plan.k_bin];
+  }
+  if (plan.by_p) {
     uint32_t before = 0;
     u64 mass_before = 0;
-    const int b = find_bin(s, t, before, mass_before, tid);
-    cut = resolve(s, row, scale, t, b, before, mass_before, cut, tid);
-    total = cut.mass;
-    s.count[tid] = own, s.mass[tid] = own_mass;
-    __syncthreads();
+    plan.p_first = find_bin(s, s.count, s.mass, Target{kNoCount, p_mass(q.top_p, max(least, u64{1}))}, before,
+                            mass_before, tid);
+    const uint32_t ahead = before;
+    before = 0, mass_before = 0;
+    plan.p_last = find_bin(s, s.count, s.mass, Target{kNoCount, p_mass(q.top_p, most)}, before, mass_before, tid);
+    plan.sure = plan.p_first;
+    plan.candidates = before + s.count[plan.p_last] - ahead +
+                      (plan.k_bin > plan.p_last ? s.count[plan.k_bin] : 0u);
   }
-  if (top_p < 1.0f) {
-    const double want = static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(total);
-    const u64 mass = max(static_cast<u64>(__builtin_ceil(want)), u64{1});
-    const Target t{kNoCount, min(mass, total)};
-    uint32_t before = 0;
-    u64 mass_before = 0;
-    const int b = find_bin(s, t, before, mass_before, tid);
-    cut = resolve(s, row, scale, t, b, before, mass_before, cut, tid);
-    total = cut.mass;
-  }
-  // The draw: masses of kParts parts of the row, then of the elements of the part that it falls in.
-  const float given = p.u[row_id];
-  const double want = given > 0.0f ? static_cast<double>(given) * static_cast<double>(total) : 0.0;
-  const auto kept = [&](int i, float l) -> u64 {
-    if (!cut.keeps(l, i)) return 0;
-    const double d = scale.below(l);
-    return scale.live(d) ? scale.weight(d) : 0;
-  };
-  const int part = ceil_div(row.n, kParts), lane = tid & 63, wave = tid >> 6;
-  clear_bins(s, tid);
-  for (int i = wave; i < kParts; i += kWaves) {
+  return plan;
+}
+
+// Elements [from, to): those of the cuts' bins into the list, and the masses of what lies before them by
+// parts of the row.
+template <typename T>
+__device__ __forceinline__ void pick(Shared& s, const Row<T>& row, const Scale& scale, const Plan& plan,
+                                     int part, int first_part, int end_part, int tid) {
+  const int lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  const bool gather = plan.candidates <= kList;
+  const int lowest = plan.sure == kBins ? kBins - 1 : max(plan.k_bin, plan.p_last);
+  const float low = fmaxf(scale.bound(scale.least), scale.bound(scale.edge(lowest)));
+  for (int i = first_part + wave; i < end_part; i += kWaves) {
     u64 m = 0;
     const int from = min(i * part, row.n), to = min(from + part, row.n);
-    row.each(from, to, lane, 64, [&](int at, float l) { m += kept(at, l); });
+    row.each(from, to, lane, 64, [&](int at, float l) {
+      if (l < low) return;
+      const double d = scale.below(l);
+      if (!scale.live(d)) return;
+      const int b = scale.bin(d);
+      if (b < plan.sure) {
+        m += scale.weight(d);
+      } else if (gather && plan.has(b)) {
+        const int to_list = atomicAdd(&s.listed, 1);
+        if (to_list < kList) s.key[to_list] = key_of(l), s.index[to_list] = at;
+      }
+    });
 #pragma unroll
     for (int by = 32; by > 0; by >>= 1) m += __shfl_xor(m, by);
-    if (lane == 0) s.mass[i] = m;
+    if (lane == 0) s.part[i] = m;
   }
   __syncthreads();
+}
+
+// Where a cut falls in bin `bin`, of which before and mass_before lie ahead.  each(f) calls f(key, index)
+// for the candidates, `listed` of them from the list (more than it holds: from the row).
+template <typename E>
+__device__ Cut resolve(Shared& s, const E& each, int listed, const Scale& scale, const Target& t, int bin,
+                       uint32_t before, u64 mass_before, const Cut& inside, int tid) {
+  const auto mine = [&](uint32_t k, int i) {
+    return scale.bin(scale.below(value_of(k))) == bin && inside.keeps(k, i);
+  };
+  Cut cut;
+  if (listed <= kPairs) {  // each element against all others
+    const uint32_t k = s.key[min(tid, listed - 1)];
+    const int i = s.index[min(tid, listed - 1)];
+    const bool ours = tid < listed && mine(k, i);
+    const u64 w = ours ? scale.weight(scale.below(value_of(k))) : 0;
+    __syncthreads();
+    if (tid < listed) s.fine_mass[tid] = w;
+    __syncthreads();
+    if (ours) {
+      for (int j = 0; j < listed; ++j) {
+        const uint32_t kj = s.key[j];
+        const u64 wj = s.fine_mass[j];
+        if (wj && (kj > k || (kj == k && s.index[j] < i))) ++before, mass_before += wj;
+      }
+      const bool kept = before < t.count && mass_before < t.mass;
+      if (kept && (before + 1 >= t.count || mass_before + w >= t.mass))
+        s.found = tid, s.found_mass = mass_before + w;
+    }
+    __syncthreads();
+    cut.key = s.key[s.found], cut.index = s.index[s.found], cut.mass = s.found_mass;
+    __syncthreads();
+    return cut;
+  }
+  u64 up = 0, down = 0;
+  each([&](uint32_t k, int i) {
+    if (mine(k, i)) up = max(up, static_cast<u64>(k)), down = max(down, static_cast<u64>(~k));
+  });
+  uint32_t hi = static_cast<uint32_t>(block_max(s, up, tid));
+  uint32_t lo = ~static_cast<uint32_t>(block_max(s, down, tid));
+  uint32_t ties = 0;
+  while (true) {  // the range falls to a 1024th each time
+    int shift = 0;
+    while (((hi - lo) >> shift) >= kBins) ++shift;
+    __syncthreads();
+    s.fine_count[tid] = 0, s.fine_mass[tid] = 0;
+    __syncthreads();
+    each([&](uint32_t k, int i) {
+      if (k < lo || k > hi || !mine(k, i)) return;
+      const uint32_t b = (hi - k) >> shift;
+      atomicAdd(&s.fine_count[b], 1u);
+      atomicAdd(&s.fine_mass[b], scale.weight(scale.below(value_of(k))));
+    });
+    __syncthreads();
+    const int b = find_bin(s, s.fine_count, s.fine_mass, t, before, mass_before, tid);
+    ties = s.fine_count[b];
+    hi = hi - (static_cast<uint32_t>(b) << shift);
+    if (shift == 0) break;
+    const uint32_t span = (1u << shift) - 1u;
+    lo = hi - lo > span ? hi - span : lo;
+  }
+  cut.key = hi;
+  const u64 w = scale.weight(scale.below(value_of(hi)));
+  const u64 by_mass = (t.mass - mass_before + w - 1) / w;
+  const uint32_t keep = static_cast<uint32_t>(min(static_cast<u64>(min(t.count - before, ties)), max(by_mass, u64{1})));
+  cut.mass = mass_before + keep * w;
+  cut.index = 0x7fffffff;
+  if (keep < ties) {  // the keep-th smallest index among them
+    uint32_t first = 0, last = kMaxVocab - 1, passed = 0;
+    while (true) {
+      int shift = 0;
+      while (((last - first) >> shift) >= kBins) ++shift;
+      __syncthreads();
+      s.fine_count[tid] = 0, s.fine_mass[tid] = 0;
+      __syncthreads();
+      each([&](uint32_t k, int i) {
+        const uint32_t at = static_cast<uint32_t>(i);
+        if (k == hi && at >= first && at <= last && inside.keeps(k, i)) atomicAdd(&s.fine_count[(at - first) >> shift], 1u);
+      });
+      __syncthreads();
+      u64 none = 0;
+      const int b = find_bin(s, s.fine_count, s.fine_mass, Target{keep, kNoMass}, passed, none, tid);
+      first += static_cast<uint32_t>(b) << shift;
+      if (shift == 0) break;
+      last = first + (1u << shift) - 1u;
+    }
+    cut.index = static_cast<int>(first);
+  }
+  __syncthreads();
+  return cut;
+}
+
+// The cuts and the draw, once the histogram, the list and the parts' masses are there.
+template <typename T>
+__device__ void finish(Shared& s, const SampleArgs& p, int row_id, const Row<T>& row, const Request& q,
+                       const Plan& plan, int part, int parts, int tid) {
+  const Scale& scale = q.scale;
+  const int listed = static_cast<int>(plan.candidates);
+  const auto each = [&](auto f) {
+    if (listed <= kList) {
+      for (int i = tid; i < listed; i += kThreads) f(s.key[i], s.index[i]);
+    } else {
+      row.each(0, row.n, tid, kThreads, [&](int i, float l) {
+        const double d = scale.below(l);
+        if (scale.live(d) && plan.has(scale.bin(d))) f(key_of(l), i);
+      });
+    }
+  };
+  Cut cut{0, 0x7fffffff, plan.total};
+  if (plan.by_k) {
+    const Target t{static_cast<uint32_t>(q.k), kNoMass};
+    uint32_t before = 0;
+    u64 mass_before = 0;
+    const int b = find_bin(s, s.count, s.mass, t, before, mass_before, tid);
+    cut = resolve(s, each, listed, scale, t, b, before, mass_before, cut, tid);
+  }
+  if (plan.by_p) {
+    const Target t{kNoCount, p_mass(q.top_p, cut.mass)};
+    uint32_t before = 0;
+    u64 mass_before = 0;
+    const int b = find_bin(s, s.count, s.mass, t, before, mass_before, tid);
+    cut = resolve(s, each, listed, scale, t, b, before, mass_before, cut, tid);
+  }
+  if (plan.sure < kBins) {
+    each([&](uint32_t k, int i) {
+      if (!cut.keeps(k, i)) return;
+      const double d = scale.below(value_of(k));
+      if (scale.bin(d) >= plan.sure) atomicAdd(&s.part[i / part], scale.weight(d));
+    });
+  }
+  __syncthreads();
+  // the first part with which the sum passes u times the whole, or the last one with any mass
   uint32_t none = 0;
-  const u64 part_mass = s.mass[tid];
+  const u64 part_mass = tid < parts ? s.part[tid] : 0;
   u64 sum = part_mass;
   block_scan(s, none, sum, tid);
-  if (tid == 0) s.found = -1, s.last = -1;
+  if (tid == kThreads - 1) s.found_mass = sum;
+  if (tid == 0) s.found = -1;
   __syncthreads();
-  // the first part with more than `want`, or the last one with any mass (u = 1 and its like)
-  if (part_mass && static_cast<double>(sum) > want && !(static_cast<double>(sum - part_mass) > want))
-    s.found = tid, s.found_mass = sum - part_mass;
+  const u64 total = s.found_mass;
+  const double want = q.u > 0.0f ? static_cast<double>(q.u) * static_cast<double>(total) : 0.0;
+  const auto passes = [&](u64 v) { return static_cast<double>(v) > want; };
+  if (part_mass && passes(sum) && !passes(sum - part_mass)) s.found = tid;
   if (part_mass && sum == total) s.last = tid;
   __syncthreads();
   const bool past = s.found < 0;
-  const int begin = (past ? s.last : s.found) * part, end = min(begin + part, row.n);
-  const u64 ahead = past ? 0 : s.found_mass;
-  const int each = ceil_div(part, kThreads), from = begin + tid * each;
+  const int chosen = past ? s.last : s.found;
+  if (tid == chosen) s.found_mass = sum - part_mass;
+  // its elements in index order, `span` to a thread
+  const int begin = chosen * part, end = min(begin + part, row.n);
+  const int span = ceil_div(part, kThreads), from = begin + tid * span, to = min(from + span, end);
+  const auto kept = [&](int i) -> u64 {
+    const float l = row.at(i);
+    const double d = scale.below(l);
+    return cut.keeps(key_of(l), i) && scale.live(d) ? scale.weight(d) : 0;
+  };
   u64 mine = 0;
-  for (int i = from; i < min(from + each, end); ++i) mine += kept(i, row.at(i));
+  for (int i = from; i < to; ++i) mine += kept(i);
   u64 until = mine;
   block_scan(s, none, until, tid);
-  if (tid == kThreads - 1) s.found_mass = until;
-  __syncthreads();
-  const u64 all = s.found_mass;
-  // of the threads with mass the one in which the sum passes `want`, or the last
-  u64 at = ahead + until - mine;
-  const bool here = past ? mine && until == all
-                         : mine && static_cast<double>(at + mine) > want && !(static_cast<double>(at) > want);
-  if (here) {
+  until += s.found_mass;
+  const u64 chosen_end = s.part[chosen] + s.found_mass;
+  if (mine && (past ? until == chosen_end : passes(until) && !passes(until - mine))) {
+    u64 at = until - mine;
     int token = -1;
-    for (int i = from; i < min(from + each, end); ++i) {
-      const u64 w = kept(i, row.at(i));
+    for (int i = from; i < to; ++i) {
+      const u64 w = kept(i);
       if (!w) continue;
       at += w;
       token = i;
-      if (!past && static_cast<double>(at) > want) break;
+      if (!past && passes(at)) break;
     }
-    p.tokens[row_id] = token;
-    if (p.logprobs) {
-      const double d = scale.below(row.at(token));
-      p.logprobs[row_id] = static_cast<float>(d / temp - ::log(static_cast<double>(total) * 0x1p-44));
+    write(p, row_id, token,
+          static_cast<float>(scale.below(row.at(token)) / q.temp - ::log(static_cast<double>(total) * 0x1p-44)));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ Row<T> row_of(const SampleArgs& p, int row) {
+  return Row<T>{static_cast<const T*>(p.logits) + row * p.stride, p.vocab};
+}
+
+template <typename T>
+__device__ __forceinline__ u64 best_of(Shared& s, const Row<T>& row, int from, int to, int tid) {
+  u64 best = 0;
+  row.each(from, to, tid, kThreads, [&](int i, float l) { best = max(best, place(l, i)); });
+  return block_max(s, best, tid);
+}
+
+__device__ __forceinline__ bool settled(const SampleArgs& p, const Request& q, int row, u64 best, bool writes) {
+  if (!q.none && !q.first) return false;
+  if (writes) write(p, row, q.none ? -1 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(best)), q.none ? -__builtin_inff() : 0.0f);
+  return true;
+}
+
+// A workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs p) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, row_id = blockIdx.x;
+  const Row<T> row = row_of<T>(p, row_id);
+  const u64 best = best_of(s, row, 0, row.n, tid);
+  const Request q = request(p, row_id, best);
+  if (settled(p, q, row_id, best, tid == 0)) return;
+  Plan plan{0, 0, false, false, kBins, -1, -1, -2, 0};
+  if (q.k > 0 || q.top_p < 1.0f) {
+    histogram(s, row, q.scale, 0, row.n, tid);
+    plan = make_plan(s, q, tid);
+  }
+  const int part = ceil_div(row.n, kParts);
+  pick(s, row, q.scale, plan, part, 0, kParts, tid);
+  finish(s, p, row_id, row, q, plan, part, kParts, tid);
+}
+
+// Few rows: several workgroups a row, and three launches.  What they hand on, for each row:
+struct Hand {
+  u64 best[kMaxSplit];        // launch 1: the first of the order in each split
+  uint32_t listed, done;      // launch 3: elements in the list, workgroups that have ended
+  u64 part[kMaxParts];
+  uint32_t key[kList];
+  int32_t index[kList];
+};
+struct Histogram {  // launch 2, of each split
+  u64 mass[kBins];
+  uint32_t count[kBins];
+};
+
+// Between workgroups of a launch: device-coherent (the L2 is per XCD).
+template <typename V>
+__device__ __forceinline__ void store_coherent(V* p, V v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename V>
+__device__ __forceinline__ V load_coherent(const V* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+struct SplitArgs {
+  SampleArgs p;
+  Hand* hand;
+  Histogram* hist;
+  int splits, part, parts;  // parts: of the row, a multiple of splits
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_best_kernel(SplitArgs a) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
+  const Row<T> row = row_of<T>(a.p, row_id);
+  const int per = a.parts / a.splits * a.part;
+  const int from = min(split * per, row.n), to = min(from + per, row.n);
+  const u64 best = best_of(s, row, from, to, tid);
+  Hand& h = a.hand[row_id];
+  if (tid == 0) {
+    h.best[split] = best;
+    if (split == 0) h.listed = 0, h.done = 0;
+  }
+}
+
+__device__ __forceinline__ u64 best_of(const Hand& h, int splits) {
+  u64 best = 0;
+  for (int i = 0; i < splits; ++i) best = max(best, h.best[i]);
+  return best;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_histogram_kernel(SplitArgs a) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
+  const Row<T> row = row_of<T>(a.p, row_id);
+  const u64 best = best_of(a.hand[row_id], a.splits);
+  const Request q = request(a.p, row_id, best);
+  if (settled(a.p, q, row_id, best, split == 0 && tid == 0) || !(q.k > 0 || q.top_p < 1.0f)) return;
+  const int per = a.parts / a.splits * a.part;
+  const int from = min(split * per, row.n), to = min(from + per, row.n);
+  histogram(s, row, q.scale, from, to, tid);
+  Histogram& h = a.hist[static_cast<long long>(row_id) * a.splits + split];
+  h.count[tid] = s.count[tid], h.mass[tid] = s.mass[tid];
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SplitArgs a) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
+  const Row<T> row = row_of<T>(a.p, row_id);
+  Hand& hand = a.hand[row_id];
+  const u64 best = best_of(hand, a.splits);
+  const Request q = request(a.p, row_id, best);
+  if (settled(a.p, q, row_id, best, false)) return;  // launch 2 has written it
+  Plan plan{0, 0, false, false, kBins, -1, -1, -2, 0};
+  if (q.k > 0 || q.top_p < 1.0f) {
+    const Histogram* h = a.hist + static_cast<long long>(row_id) * a.splits;
+    uint32_t c = 0;
+    u64 m = 0;
+    for (int i = 0; i < a.splits; ++i) c += h[i].count[tid], m += h[i].mass[tid];
+    s.count[tid] = c, s.mass[tid] = m;
+    __syncthreads();
+    plan = make_plan(s, q, tid);
+  }
+  const int per = a.parts / a.splits, first = split * per;
+  pick(s, row, q.scale, plan, a.part, first, first + per, tid);
+  if (tid < per) store_coherent(&hand.part[first + tid], s.part[first + tid]);
+  const int listed = min(s.listed, kList);
+  if (listed > 0) {
+    if (tid == 0)
+      s.last = static_cast<int>(__hip_atomic_fetch_add(&hand.listed, static_cast<uint32_t>(listed),
+                                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    __syncthreads();
+    for (int i = tid; i < listed && s.last + i < kList; i += kThreads) {
+      store_coherent(&hand.key[s.last + i], s.key[i]);
+      store_coherent(&hand.index[s.last + i], s.index[i]);
     }
   }
+  // every store has completed before the workgroup counts itself in; the row's last one goes on
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0)
+    s.found = __hip_atomic_fetch_add(&hand.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u ==
+              static_cast<uint32_t>(a.splits);
+  __syncthreads();
+  if (!s.found) return;
+  if (tid < a.parts) s.part[tid] = load_coherent(&hand.part[tid]);
+  if (plan.candidates <= kList)
+    for (int i = tid; i < static_cast<int>(plan.candidates); i += kThreads) {
+      s.key[i] = load_coherent(&hand.key[i]);
+      s.index[i] = load_coherent(&hand.index[i]);
+    }
+  __syncthreads();
+  finish(s, a.p, row_id, row, q, plan, a.part, a.parts, tid);
+}
+
+// Workgroups a row: rows that fill the card by themselves take one.
+int splits_of(int rows, int vocab) {
+  int n = 1;
+  while (n < kMaxSplit && 2 * n * rows <= kWorkgroups && vocab / (2 * n) >= kThreads) n *= 2;
+  return n;
+}
+
+template <typename T>
+void launch(const SampleArgs& p, void* workspace, hipStream_t stream) {
+  const int splits = splits_of(p.rows, p.vocab);
+  if (splits == 1) {
+    hipLaunchKernelGGL(sample_row_kernel<T>, dim3(p.rows), dim3(kThreads), 0, stream, p);
+    return;
+  }
+  const int parts = kParts > kWaves * splits ? kParts : kWaves * splits;
+  SplitArgs a{p, static_cast<Hand*>(workspace),
+              reinterpret_cast<Histogram*>(static_cast<Hand*>(workspace) + p.rows), splits,
+              ceil_div(p.vocab, parts), parts};
+  const dim3 grid(splits, p.rows), block(kThreads);
+  hipLaunchKernelGGL(sample_best_kernel<T>, grid, block, 0, stream, a);
+  hipLaunchKernelGGL(sample_histogram_kernel<T>, grid, block, 0, stream, a);
+  hipLaunchKernelGGL(sample_draw_kernel<T>, grid, block, 0, stream, a);
 }
 
 }  // namespace
@@ -440,7 +735,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
 using namespace pega;
 
 PEGA_API long long pega_sample_workspace_bytes(int rows, int vocab) {
-  return rows <= 0 || vocab <= 0 ? 0 : 16LL * rows;
+  if (rows <= 0 || vocab <= 0) return 0;
+  // of the batches up to `rows` that are split, the most rows and the most splits
+  const long long most = rows < kWorkgroups / 2 ? rows : kWorkgroups / 2;
+  const long long hists = most * kMaxSplit < kWorkgroups ? most * kMaxSplit : kWorkgroups;
+  return most * static_cast<long long>(sizeof(Hand)) + hists * static_cast<long long>(sizeof(Histogram));
 }
 
 // No reference counterpart here: the reference samples outside the expert path.
@@ -474,7 +773,7 @@ PEGA_API int pega_sample_tokens(const void* logits, bool logits_bf16, long long 
         return fail(kInvalidValue, "sample_tokens: two outputs overlap");
   }
   const SampleArgs p{logits, row_stride, rows, vocab, uniform, temperature, top_p, min_p, top_k, tokens, logprobs};
-  if (logits_bf16) hipLaunchKernelGGL(sample_kernel<uint16_t>, dim3(rows), dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL(sample_kernel<float>, dim3(rows), dim3(kThreads), 0, stream, p);
+  if (logits_bf16) launch<uint16_t>(p, workspace, stream);
+  else launch<float>(p, workspace, stream);
   return launch_status("sample_tokens");
 }
