@@ -28,9 +28,9 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 1024;
 constexpr int kList = 4096;            // elements of the cuts' bins kept in LDS
-constexpr int kParts = 128;            // of a row, whose masses the draw goes over first; more with splits
 constexpr int kMaxSplit = 16;          // workgroups of a row
-constexpr int kMaxParts = kWaves * kMaxSplit;
+constexpr int kMaxParts = 256;         // of a row, whose masses the draw goes over first (a multiple of kMaxSplit)
+constexpr int kFlight = 4;              // vectors of a thread in flight
 constexpr int kPairs = 256;            // candidates that are compared with each other
 constexpr int kWorkgroups = 512;       // two a CU
 constexpr int kMaxVocab = 1 << 19;     // sums of weights stay below 2^63
@@ -60,14 +60,22 @@ __device__ __forceinline__ uint32_t key_of(float l) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <typename T>
-struct Row {
-  const T* p;
-  int n;
-  static constexpr int kVec = 16 / sizeof(T);
+// A logit and its index in one number: the larger, the further ahead in the order.
+__device__ __forceinline__ u64 place(float l, int i) {
+  return static_cast<u64>(key_of(l)) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
+}
 
+// A row as vectors of 16 bytes, wherever it starts (the loads need no alignment); the last one reaches back to
+// end with the row.  kTiny: rows shorter than a vector.
+template <typename T, bool kTiny = false>
+struct Row {
+  static constexpr int kVec = kTiny ? 4 : 16 / static_cast<int>(sizeof(T));
+  const T* p;
+  int n, vecs;  // elements, vectors
+
+  __device__ __forceinline__ Row(const T* row, int size) : p(row), n(size), vecs(ceil_div(size, kVec)) {}
   static __device__ __forceinline__ float value(uint4 q, int e) {
-    if constexpr (sizeof(T) == 4)
+    if constexpr (sizeof(T) == 4 || kTiny)
       return clean(__builtin_bit_cast(float, e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w));
     const uint32_t w = (e >> 1) == 0 ? q.x : (e >> 1) == 1 ? q.y : (e >> 1) == 2 ? q.z : q.w;
     return clean(e & 1 ? bf_hi(w) : bf_lo(w));
@@ -76,33 +84,75 @@ struct Row {
     if constexpr (sizeof(T) == 4) return clean(p[i]);
     else return clean(bf2f(p[i]));
   }
-  // f(i, l[i]) for i in [from, to), over `threads` threads: 16-byte loads, four in flight, of what is
-  // aligned, element by element before and after
+  __device__ __forceinline__ int start(int v) const { return kTiny ? v * kVec : min(v * kVec, n - kVec); }
+  __device__ __forceinline__ uint4 load(int v) const {  // past the last: the last
+    const int from = start(min(v, vecs - 1));
+    uint4 q;
+    if constexpr (kTiny) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = __builtin_bit_cast(uint32_t, at(min(from + e, n - 1)));
+      q = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      __builtin_memcpy(&q, p + from, 16);
+    }
+    return q;
+  }
+  // The largest place of the vectors in [from, to), over `threads` threads.
+  __device__ __forceinline__ u64 best(int from, int to, int tid, int threads) const {
+    u64 best = 0;
+    for (int v = from + tid; v < to; v += kFlight * threads) {
+      uint4 q[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) q[j] = load(v + j * threads);
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const int i = start(min(v + j * threads, vecs - 1));
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)  // (a tiny row's last one several times over: the first of them counts)
+          best = max(best, place(value(q[j], e), min(i + e, n - 1)));
+      }
+    }
+    return best;
+  }
+  // f(i, l[i]) for the vectors' elements with l >= low, over `threads` threads with kFlight loads in flight
+  // each.  Few copies of f: the passes are short enough for a CU's instruction fetches to show.
   template <typename F>
-  __device__ __forceinline__ void each(int from, int to, int tid, int threads, F f) const {
-    const T* q = p + from;
-    const int lead = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(q) & 15u)) & 15u) / static_cast<int>(sizeof(T));
-    const int head = min(to - from, lead), vecs = (to - from - head) / kVec;
-    if (tid < head) f(from + tid, at(from + tid));
-    const uint4* v = reinterpret_cast<const uint4*>(q + head);
-    const int first = from + head;
-    int i = tid;
-    for (; i + 3 * threads < vecs; i += 4 * threads) {
-      uint4 r[4];
+  __device__ __forceinline__ void each(int from, int to, int tid, int threads, float low, F f) const {
+    uint4 q[kFlight];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = v[i + j * threads];
+    for (int j = 0; j < kFlight; ++j) q[j] = load(from + tid + j * threads);
+#pragma unroll 1
+    for (int v = from + tid; v < to; v += threads) {
+      uint4 now = q[0];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j + 1 < kFlight; ++j) q[j] = q[j + 1];
+      q[kFlight - 1] = load(v + kFlight * threads);
+      float most = value(now, 0);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) f(first + (i + j * threads) * kVec + e, value(r[j], e));
+      for (int e = 1; e < kVec; ++e) most = fmaxf(most, value(now, e));
+      if (most < low) continue;
+      int i = start(v);
+#pragma unroll 1
+      for (int w = 0; w < kVec; w += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float l = value(now, e);
+          if (l >= low && i + e >= v * kVec && (!kTiny || i + e < n)) f(i + e, l);
+        }
+        i += 4;
+        now = make_uint4(now.z, now.w, now.x, now.y);
+      }
     }
-    for (; i < vecs; i += threads) {
-      const uint4 r = v[i];
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) f(first + i * kVec + e, value(r, e));
+  }
+  // The same, element by element: where speed does not count.
+  template <typename F>
+  __device__ __forceinline__ void each_plain(int tid, int threads, float low, F f) const {
+#pragma unroll 1
+    for (int i = tid; i < n; i += threads) {
+      const float l = at(i);
+      if (l >= low) f(i, l);
     }
-    const int rest = first + vecs * kVec + tid;
-    if (rest < to) f(rest, at(rest));
   }
 };
 
@@ -165,31 +215,73 @@ struct Shared {
   int found, last, listed;
 };
 
+// Lane moves without an "old" operand; lanes that nothing reaches, or outside the rows of the mask, get 0.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRows, 0xF, false));
+}
+template <int kCtrl, int kRows = 0xF>
+__device__ __forceinline__ u64 dpp64(u64 v) {
+  return static_cast<u64>(dpp<kCtrl, kRows>(static_cast<uint32_t>(v >> 32))) << 32 | dpp<kCtrl, kRows>(static_cast<uint32_t>(v));
+}
+// Inclusive sums over 16 lanes, over the wave's 64.
+__device__ __forceinline__ u64 scan16(u64 v) {
+  v += dpp64<0x111>(v);  // row_shr:1, 2, 4, 8
+  v += dpp64<0x112>(v);
+  v += dpp64<0x114>(v);
+  return v + dpp64<0x118>(v);
+}
+__device__ __forceinline__ uint32_t scan16(uint32_t v) {
+  v += dpp<0x111, 0xF>(v);
+  v += dpp<0x112, 0xF>(v);
+  v += dpp<0x114, 0xF>(v);
+  return v + dpp<0x118, 0xF>(v);
+}
+__device__ __forceinline__ u64 scan64(u64 v) {
+  v = scan16(v);
+  v += dpp64<0x142, 0xA>(v);         // row_bcast:15 into rows 1 and 3
+  return v + dpp64<0x143, 0xC>(v);   // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ uint32_t scan64(uint32_t v) {
+  v = scan16(v);
+  v += dpp<0x142, 0xA>(v);
+  return v + dpp<0x143, 0xC>(v);
+}
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), lane));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), lane));
+  return static_cast<u64>(hi) << 32 | lo;
+}
+
 // Inclusive sums over the workgroup's threads, in their order.
 __device__ __forceinline__ void block_scan(Shared& s, uint32_t& count, u64& mass, int tid) {
-  const int lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-  for (int by = 1; by < 64; by <<= 1) {
-    const uint32_t c = __shfl_up(count, by);
-    const u64 m = __shfl_up(mass, by);
-    if (lane >= by) count += c, mass += m;
-  }
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  count = scan64(count), mass = scan64(mass);
   __syncthreads();  // the places of an earlier scan have been read
   if (lane == 63) s.wave_count[wave] = count, s.wave_mass[wave] = mass;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) count += s.wave_count[w], mass += s.wave_mass[w];
+  const uint32_t c = scan16(s.wave_count[lane & 15]);
+  const u64 m = scan16(s.wave_mass[lane & 15]);
+  if (wave > 0) {
+    count += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(c), wave - 1));
+    mass += lane64(m, wave - 1);
+  }
 }
 
 // The largest over the workgroup, in each thread.
 __device__ __forceinline__ u64 block_max(Shared& s, u64 v, int tid) {
-#pragma unroll
-  for (int by = 32; by > 0; by >>= 1) v = max(v, static_cast<u64>(__shfl_xor(v, by)));
+  const auto max16 = [](u64 x) {
+    x = max(x, dpp64<0xB1>(x));     // quad_perm [1,0,3,2]
+    x = max(x, dpp64<0x4E>(x));     // quad_perm [2,3,0,1]
+    x = max(x, dpp64<0x141>(x));    // row_half_mirror
+    return max(x, dpp64<0x140>(x)); // row_mirror
+  };
+  v = max16(v);
+  v = max(max(lane64(v, 0), lane64(v, 16)), max(lane64(v, 32), lane64(v, 48)));
   __syncthreads();
   if ((tid & 63) == 0) s.wave_mass[tid >> 6] = v;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) v = max(v, s.wave_mass[w]);
-  return v;
+  return lane64(max16(s.wave_mass[tid & 15]), 0);
 }
 
 // A cut of the order: the first `count` elements, or those with less than `mass` before them,
@@ -199,21 +291,29 @@ struct Target {
   u64 mass;
 };
 
-// The bin of a histogram in which the cut falls, given what lies before bin 0; on return what lies before
-// that bin.  -1 if the bins do not reach it.
-__device__ __forceinline__ int find_bin(Shared& s, const uint32_t* count, const u64* mass, const Target& t,
-                                        uint32_t& before, u64& mass_before, int tid) {
-  const uint32_t own = count[tid];
-  const u64 own_mass = mass[tid];
-  uint32_t c = own;
-  u64 m = own_mass;
-  block_scan(s, c, m, tid);
-  c += before, m += mass_before;
+// A histogram's bin of this thread, and the sums up to and with it.
+struct Bin {
+  uint32_t own, count;
+  u64 own_mass, mass;
+};
+__device__ __forceinline__ Bin scan_bins(Shared& s, const uint32_t* count, const u64* mass, int tid) {
+  Bin b{count[tid], count[tid], mass[tid], mass[tid]};
+  block_scan(s, b.count, b.mass, tid);
+  return b;
+}
+
+// The bin in which the cut falls, given what lies before bin 0; on return what lies before that bin.  -1 if
+// the bins do not reach it.
+__device__ __forceinline__ int find_bin(Shared& s, const Bin& bin, const Target& t, uint32_t& before,
+                                        u64& mass_before, int tid) {
+  const uint32_t c = bin.count + before;
+  const u64 m = bin.mass + mass_before;
+  __syncthreads();  // what an earlier call found has been read
   if (tid == 0) s.found = -1;
   __syncthreads();
-  const bool reached = own && (c >= t.count || m >= t.mass);
-  const bool earlier = c - own >= t.count || m - own_mass >= t.mass;
-  if (reached && !earlier) s.found = tid, s.found_count = c - own, s.found_mass = m - own_mass;
+  const bool reached = bin.own && (c >= t.count || m >= t.mass);
+  const bool earlier = c - bin.own >= t.count || m - bin.own_mass >= t.mass;
+  if (reached && !earlier) s.found = tid, s.found_count = c - bin.own, s.found_mass = m - bin.own_mass;
   __syncthreads();
   const int found = s.found;
   if (found >= 0) before = s.found_count, mass_before = s.found_mass;
@@ -238,15 +338,12 @@ struct Request {
   int k;        // 0: all
   bool none;    // no logit above -inf
   bool first;   // the first of the order alone
+  bool few;     // k fits the list: all that the k cut leaves is listed, and has weights only then
+  __device__ __forceinline__ bool cuts() const { return k > 0 || top_p < 1.0f; }
 };
 
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
-
-// A logit and its index in one number: the larger, the further ahead in the order.
-__device__ __forceinline__ u64 place(float l, int i) {
-  return static_cast<u64>(key_of(l)) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
 }
 
 __device__ __forceinline__ Request request(const SampleArgs& p, int row, u64 best) {
@@ -257,6 +354,7 @@ __device__ __forceinline__ Request request(const SampleArgs& p, int row, u64 bes
   const bool greedy = !(temp > 0.0f);
   q.k = greedy ? 1 : p.top_k ? max(p.top_k[row], 0) : 0;
   q.first = q.k == 1;
+  q.few = q.k > 0 && q.k <= kList / 2;
   q.none = top == -__builtin_inff();
   q.top_p = p.top_p ? p.top_p[row] : 1.0f;
   q.u = p.u[row];
@@ -275,21 +373,23 @@ __device__ __forceinline__ void write(const SampleArgs& p, int row, int token, f
   if (p.logprobs) p.logprobs[row] = logprob;
 }
 
-// The histogram of elements [from, to).
-template <typename T>
-__device__ __forceinline__ void histogram(Shared& s, const Row<T>& row, const Scale& scale, int from,
-                                          int to, int tid) {
+// One element's share of the histogram.
+__device__ __forceinline__ void count_in(Shared& s, const Scale& scale, bool masses, float l) {
+  const double d = scale.below(l);
+  if (!scale.live(d)) return;
+  const int b = scale.bin(d);
+  atomicAdd(&s.count[b], 1u);
+  if (masses) atomicAdd(&s.mass[b], scale.weight(d));
+}
+
+// The histogram of vectors [from, to): counts, and masses unless few will have weight.
+template <typename R>
+__device__ __forceinline__ void histogram(Shared& s, const R& row, const Scale& scale, bool masses,
+                                          int from, int to, int tid) {
   s.count[tid] = 0, s.mass[tid] = 0;
   __syncthreads();
-  const float low = scale.bound(scale.least);
-  row.each(from, to, tid, kThreads, [&](int, float l) {
-    if (l < low) return;
-    const double d = scale.below(l);
-    if (!scale.live(d)) return;
-    const int b = scale.bin(d);
-    atomicAdd(&s.count[b], 1u);
-    atomicAdd(&s.mass[b], scale.weight(d));
-  });
+  row.each(from, to, tid, kThreads, scale.bound(scale.least),
+           [&](int, float l) { count_in(s, scale, masses, l); });
   __syncthreads();
 }
 
@@ -304,61 +404,68 @@ struct Plan {
   __device__ __forceinline__ bool has(int b) const { return b == k_bin || (b >= p_first && b <= p_last); }
 };
 
+__device__ __forceinline__ Plan no_plan() { return Plan{0, 0, false, false, kBins, -1, -1, -2, 0}; }
+
 __device__ __forceinline__ u64 p_mass(float p, u64 total) {
   const double want = static_cast<double>(fmaxf(p, 0.0f)) * static_cast<double>(total);
   return min(max(static_cast<u64>(__builtin_ceil(want)), u64{1}), total);
 }
 
-__device__ __forceinline__ Plan make_plan(Shared& s, const Request& q, int tid) {
-  Plan plan{0, 0, false, false, kBins, -1, -1, -2, 0};
-  uint32_t c = s.count[tid];
-  u64 m = s.mass[tid];
-  block_scan(s, c, m, tid);
-  if (tid == kThreads - 1) s.found_count = c, s.found_mass = m;
+// few: as in Request (the row's masses are not known then).
+__device__ __forceinline__ Plan make_plan(Shared& s, const Request& q, bool few, const Bin& bin, int tid) {
+  Plan plan = no_plan();
+  __syncthreads();
+  if (tid == kThreads - 1) s.found_count = bin.count, s.found_mass = bin.mass;
   __syncthreads();
   plan.live = s.found_count, plan.total = s.found_mass;
   plan.by_k = q.k > 0 && static_cast<uint32_t>(q.k) < plan.live;
   plan.by_p = q.top_p < 1.0f;
   u64 least = plan.total, most = plan.total;  // what the k cut leaves
+  uint32_t before = 0;
   if (plan.by_k) {
-    uint32_t before = 0;
     least = 0;
-    plan.k_bin = find_bin(s, s.count, s.mass, Target{static_cast<uint32_t>(q.k), kNoMass}, before, least, tid);
+    plan.k_bin = find_bin(s, bin, Target{static_cast<uint32_t>(q.k), kNoMass}, before, least, tid);
     most = least + s.mass[plan.k_bin];
     plan.sure = plan.k_bin;
     plan.candidates = s.count[plan.k_bin];
   }
-  if (plan.by_p) {
-    uint32_t before = 0;
+  if (few) {
+    plan.p_first = 0, plan.p_last = plan.by_k ? plan.k_bin : kBins - 1;
+    plan.sure = 0;
+    plan.candidates = plan.by_k ? before + s.count[plan.k_bin] : plan.live;
+  } else if (plan.by_p) {
+    before = 0;
     u64 mass_before = 0;
-    plan.p_first = find_bin(s, s.count, s.mass, Target{kNoCount, p_mass(q.top_p, max(least, u64{1}))}, before,
-                            mass_before, tid);
-    const uint32_t ahead = before;
-    before = 0, mass_before = 0;
-    plan.p_last = find_bin(s, s.count, s.mass, Target{kNoCount, p_mass(q.top_p, most)}, before, mass_before, tid);
+    plan.p_last = find_bin(s, bin, Target{kNoCount, p_mass(q.top_p, most)}, before, mass_before, tid);
+    const uint32_t until = before + s.count[plan.p_last];
+    if (plan.by_k) {
+      before = 0, mass_before = 0;
+      plan.p_first = find_bin(s, bin, Target{kNoCount, p_mass(q.top_p, max(least, u64{1}))}, before, mass_before, tid);
+    } else {
+      plan.p_first = plan.p_last;
+    }
     plan.sure = plan.p_first;
-    plan.candidates = before + s.count[plan.p_last] - ahead +
-                      (plan.k_bin > plan.p_last ? s.count[plan.k_bin] : 0u);
+    plan.candidates = until - before + (plan.k_bin > plan.p_last ? s.count[plan.k_bin] : 0u);
   }
   return plan;
 }
 
-// Elements [from, to): those of the cuts' bins into the list, and the masses of what lies before them by
-// parts of the row.
-template <typename T>
-__device__ __forceinline__ void pick(Shared& s, const Row<T>& row, const Scale& scale, const Plan& plan,
-                                     int part, int first_part, int end_part, int tid) {
+// Of the parts first .. end - 1, `part` vectors each, the elements of the cuts' bins into the list, and the
+// masses of what lies before those bins.
+template <typename R>
+__device__ __forceinline__ void pick(Shared& s, const R& row, const Scale& scale, const Plan& plan,
+                                     int part, int first, int end, int tid) {
   const int lane = tid & 63, wave = tid >> 6;
+  __syncthreads();
   if (tid == 0) s.listed = 0;
   __syncthreads();
   const bool gather = plan.candidates <= kList;
   const int lowest = plan.sure == kBins ? kBins - 1 : max(plan.k_bin, plan.p_last);
   const float low = fmaxf(scale.bound(scale.least), scale.bound(scale.edge(lowest)));
-  for (int i = first_part + wave; i < end_part; i += kWaves) {
+  for (int i = first + wave; i < end; i += kWaves) {
     u64 m = 0;
-    const int from = min(i * part, row.n), to = min(from + part, row.n);
-    row.each(from, to, lane, 64, [&](int at, float l) {
-      if (l < low) return;
+    const int from = i * part, to = min(from + part, row.vecs);
+    row.each(from, to, lane, 64, low, [&](int at, float l) {
       const double d = scale.below(l);
       if (!scale.live(d)) return;
       const int b = scale.bin(d);
@@ -369,9 +476,8 @@ __device__ __forceinline__ void pick(Shared& s, const Row<T>& row, const Scale& 
         if (to_list < kList) s.key[to_list] = key_of(l), s.index[to_list] = at;
       }
     });
-#pragma unroll
-    for (int by = 32; by > 0; by >>= 1) m += __shfl_xor(m, by);
-    if (lane == 0) s.part[i] = m;
+    m = scan64(m);
+    if (lane == 63) s.part[i] = m;
   }
   __syncthreads();
 }
@@ -385,24 +491,33 @@ __device__ Cut resolve(Shared& s, const E& each, int listed, const Scale& scale,
     return scale.bin(scale.below(value_of(k))) == bin && inside.keeps(k, i);
   };
   Cut cut;
-  if (listed <= kPairs) {  // each element against all others
-    const uint32_t k = s.key[min(tid, listed - 1)];
-    const int i = s.index[min(tid, listed - 1)];
-    const bool ours = tid < listed && mine(k, i);
+  if (listed <= kPairs) {
+    // each element against all others, four threads to one: a fourth of them each
+    const int own = tid >> 2, quarter = tid & 3;
+    const uint32_t k = s.key[min(own, listed - 1)];
+    const int i = s.index[min(own, listed - 1)];
+    const bool ours = own < listed && mine(k, i);
     const u64 w = ours ? scale.weight(scale.below(value_of(k))) : 0;
     __syncthreads();
-    if (tid < listed) s.fine_mass[tid] = w;
+    if (quarter == 0) s.fine_mass[own] = w;  // 0: not in this bin, or past the last
     __syncthreads();
-    if (ours) {
-      for (int j = 0; j < listed; ++j) {
-        const uint32_t kj = s.key[j];
-        const u64 wj = s.fine_mass[j];
-        if (wj && (kj > k || (kj == k && s.index[j] < i))) ++before, mass_before += wj;
-      }
-      const bool kept = before < t.count && mass_before < t.mass;
-      if (kept && (before + 1 >= t.count || mass_before + w >= t.mass))
-        s.found = tid, s.found_mass = mass_before + w;
+    uint32_t c = 0;
+    u64 m = 0;
+    const int n4 = (listed + 3) >> 2;
+#pragma unroll 4
+    for (int j = 0; j < n4; ++j) {
+      const int at = 4 * j + quarter;  // below kPairs, where the list has places
+      const uint32_t kj = s.key[at];
+      const u64 wj = s.fine_mass[at];
+      const bool ahead = wj && (kj > k || (kj == k && s.index[at] < i));
+      c += ahead ? 1u : 0u, m += ahead ? wj : 0;
     }
+    c += dpp<0xB1, 0xF>(c), m += dpp64<0xB1>(m);
+    c += dpp<0x4E, 0xF>(c), m += dpp64<0x4E>(m);
+    before += c, mass_before += m;
+    if (ours && quarter == 0 && before < t.count && mass_before < t.mass &&
+        (before + 1 >= t.count || mass_before + w >= t.mass))
+      s.found = own, s.found_mass = mass_before + w;
     __syncthreads();
     cut.key = s.key[s.found], cut.index = s.index[s.found], cut.mass = s.found_mass;
     __syncthreads();
@@ -428,7 +543,7 @@ __device__ Cut resolve(Shared& s, const E& each, int listed, const Scale& scale,
       atomicAdd(&s.fine_mass[b], scale.weight(scale.below(value_of(k))));
     });
     __syncthreads();
-    const int b = find_bin(s, s.fine_count, s.fine_mass, t, before, mass_before, tid);
+    const int b = find_bin(s, scan_bins(s, s.fine_count, s.fine_mass, tid), t, before, mass_before, tid);
     ties = s.fine_count[b];
     hi = hi - (static_cast<uint32_t>(b) << shift);
     if (shift == 0) break;
@@ -455,7 +570,7 @@ __device__ Cut resolve(Shared& s, const E& each, int listed, const Scale& scale,
       });
       __syncthreads();
       u64 none = 0;
-      const int b = find_bin(s, s.fine_count, s.fine_mass, Target{keep, kNoMass}, passed, none, tid);
+      const int b = find_bin(s, scan_bins(s, s.fine_count, s.fine_mass, tid), Target{keep, kNoMass}, passed, none, tid);
       first += static_cast<uint32_t>(b) << shift;
       if (shift == 0) break;
       last = first + (1u << shift) - 1u;
@@ -466,42 +581,87 @@ __device__ Cut resolve(Shared& s, const E& each, int listed, const Scale& scale,
   return cut;
 }
 
+// A row whose candidates are too many for the list, by one workgroup from its histogram on.
+template <typename R>
+__device__ __forceinline__ void again(Shared& s, const R& row, const Request& q, Plan& plan, Bin& bin, int part,
+                                   int parts, int tid) {
+  const float low = q.scale.bound(q.scale.least);
+  s.count[tid] = 0, s.mass[tid] = 0;
+  if (tid < parts) s.part[tid] = 0;
+  __syncthreads();
+  row.each_plain(tid, kThreads, low, [&](int, float l) { count_in(s, q.scale, true, l); });
+  __syncthreads();
+  bin = scan_bins(s, s.count, s.mass, tid);
+  plan = make_plan(s, q, false, bin, tid);
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  row.each_plain(tid, kThreads, low, [&](int i, float l) {
+    const double d = q.scale.below(l);
+    if (!q.scale.live(d)) return;
+    const int b = q.scale.bin(d);
+    if (b < plan.sure) {
+      atomicAdd(&s.part[i / (part * R::kVec)], q.scale.weight(d));
+    } else if (plan.has(b)) {
+      const int at = atomicAdd(&s.listed, 1);
+      if (at < kList) s.key[at] = key_of(l), s.index[at] = i;
+    }
+  });
+  __syncthreads();
+}
+
 // The cuts and the draw, once the histogram, the list and the parts' masses are there.
-template <typename T>
-__device__ void finish(Shared& s, const SampleArgs& p, int row_id, const Row<T>& row, const Request& q,
-                       const Plan& plan, int part, int parts, int tid) {
+template <typename R>
+__device__ __forceinline__ void finish(Shared& s, const SampleArgs& p, int row_id, const R& row, const Request& q,
+                                       Plan plan, Bin bin, int part, int parts, int tid) {
   const Scale& scale = q.scale;
+  const bool few = q.few && plan.candidates <= kList;
+  if (q.few && !few) again(s, row, q, plan, bin, part, parts, tid);
   const int listed = static_cast<int>(plan.candidates);
   const auto each = [&](auto f) {
-    if (listed <= kList) {
-      for (int i = tid; i < listed; i += kThreads) f(s.key[i], s.index[i]);
-    } else {
-      row.each(0, row.n, tid, kThreads, [&](int i, float l) {
+    // one loop for both, so that f is there once
+    const bool list = listed <= kList;
+#pragma unroll 1
+    for (int i = tid; i < (list ? listed : row.n); i += kThreads) {
+      uint32_t k;
+      int at = i;
+      if (list) {
+        k = s.key[i], at = s.index[i];
+      } else {
+        const float l = row.at(i);
         const double d = scale.below(l);
-        if (scale.live(d) && plan.has(scale.bin(d))) f(key_of(l), i);
-      });
+        if (!scale.live(d) || !plan.has(scale.bin(d))) continue;
+        k = key_of(l);
+      }
+      f(k, at);
     }
   };
   Cut cut{0, 0x7fffffff, plan.total};
-  if (plan.by_k) {
-    const Target t{static_cast<uint32_t>(q.k), kNoMass};
+#pragma unroll 1
+  for (int which = plan.by_k ? 0 : 1; which < (plan.by_p ? 2 : 1); ++which) {  // the k cut, the p cut
+    if (which == 1 && few) {  // the masses of what is left
+      __syncthreads();
+      s.count[tid] = 0, s.mass[tid] = 0;
+      __syncthreads();
+      each([&](uint32_t k, int i) {
+        if (cut.keeps(k, i)) count_in(s, scale, true, value_of(k));
+      });
+      __syncthreads();
+      bin = scan_bins(s, s.count, s.mass, tid);
+      if (tid == kThreads - 1) s.found_mass = bin.mass;
+      __syncthreads();
+      cut.mass = s.found_mass;
+    }
+    const Target t = which == 0 ? Target{static_cast<uint32_t>(q.k), kNoMass} : Target{kNoCount, p_mass(q.top_p, cut.mass)};
     uint32_t before = 0;
     u64 mass_before = 0;
-    const int b = find_bin(s, s.count, s.mass, t, before, mass_before, tid);
-    cut = resolve(s, each, listed, scale, t, b, before, mass_before, cut, tid);
-  }
-  if (plan.by_p) {
-    const Target t{kNoCount, p_mass(q.top_p, cut.mass)};
-    uint32_t before = 0;
-    u64 mass_before = 0;
-    const int b = find_bin(s, s.count, s.mass, t, before, mass_before, tid);
+    const int b = find_bin(s, bin, t, before, mass_before, tid);
     cut = resolve(s, each, listed, scale, t, b, before, mass_before, cut, tid);
   }
   if (plan.sure < kBins) {
     each([&](uint32_t k, int i) {
       if (!cut.keeps(k, i)) return;
       const double d = scale.below(value_of(k));
-      if (scale.bin(d) >= plan.sure) atomicAdd(&s.part[i / part], scale.weight(d));
+      if (scale.bin(d) >= plan.sure) atomicAdd(&s.part[i / (part * R::kVec)], scale.weight(d));
     });
   }
   __syncthreads();
@@ -523,8 +683,8 @@ __device__ void finish(Shared& s, const SampleArgs& p, int row_id, const Row<T>&
   const int chosen = past ? s.last : s.found;
   if (tid == chosen) s.found_mass = sum - part_mass;
   // its elements in index order, `span` to a thread
-  const int begin = chosen * part, end = min(begin + part, row.n);
-  const int span = ceil_div(part, kThreads), from = begin + tid * span, to = min(from + span, end);
+  const int size = part * R::kVec, begin = chosen * size, end = min(begin + size, row.n);
+  const int span = ceil_div(size, kThreads), from = begin + tid * span, to = min(from + span, end);
   const auto kept = [&](int i) -> u64 {
     const float l = row.at(i);
     const double d = scale.below(l);
@@ -551,16 +711,14 @@ __device__ void finish(Shared& s, const SampleArgs& p, int row_id, const Row<T>&
   }
 }
 
-template <typename T>
-__device__ __forceinline__ Row<T> row_of(const SampleArgs& p, int row) {
-  return Row<T>{static_cast<const T*>(p.logits) + row * p.stride, p.vocab};
+template <typename T, bool kTiny = false>
+__device__ __forceinline__ Row<T, kTiny> row_of(const SampleArgs& p, int row) {
+  return Row<T, kTiny>(static_cast<const T*>(p.logits) + row * p.stride, p.vocab);
 }
 
-template <typename T>
-__device__ __forceinline__ u64 best_of(Shared& s, const Row<T>& row, int from, int to, int tid) {
-  u64 best = 0;
-  row.each(from, to, tid, kThreads, [&](int i, float l) { best = max(best, place(l, i)); });
-  return block_max(s, best, tid);
+template <typename R>
+__device__ __forceinline__ u64 best_of(Shared& s, const R& row, int from, int to, int tid) {
+  return block_max(s, row.best(from, to, tid, kThreads), tid);
 }
 
 __device__ __forceinline__ bool settled(const SampleArgs& p, const Request& q, int row, u64 best, bool writes) {
@@ -570,22 +728,23 @@ __device__ __forceinline__ bool settled(const SampleArgs& p, const Request& q, i
 }
 
 // A workgroup a row.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs p) {
+template <typename T, bool kTiny>
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs p, int part, int parts) {
   __shared__ Shared s;
   const int tid = threadIdx.x, row_id = blockIdx.x;
-  const Row<T> row = row_of<T>(p, row_id);
-  const u64 best = best_of(s, row, 0, row.n, tid);
+  const auto row = row_of<T, kTiny>(p, row_id);
+  const u64 best = best_of(s, row, 0, row.vecs, tid);
   const Request q = request(p, row_id, best);
   if (settled(p, q, row_id, best, tid == 0)) return;
-  Plan plan{0, 0, false, false, kBins, -1, -1, -2, 0};
-  if (q.k > 0 || q.top_p < 1.0f) {
-    histogram(s, row, q.scale, 0, row.n, tid);
-    plan = make_plan(s, q, tid);
+  Plan plan = no_plan();
+  Bin bin{};
+  if (q.cuts()) {
+    histogram(s, row, q.scale, !q.few, 0, row.vecs, tid);
+    bin = scan_bins(s, s.count, s.mass, tid);
+    plan = make_plan(s, q, q.few, bin, tid);
   }
-  const int part = ceil_div(row.n, kParts);
-  pick(s, row, q.scale, plan, part, 0, kParts, tid);
-  finish(s, p, row_id, row, q, plan, part, kParts, tid);
+  pick(s, row, q.scale, plan, part, 0, parts, tid);
+  finish(s, p, row_id, row, q, plan, bin, part, parts, tid);
 }
 
 // Few rows: several workgroups a row, and three launches.  What they hand on, for each row:
@@ -624,7 +783,7 @@ __global__ __launch_bounds__(kThreads) void sample_best_kernel(SplitArgs a) {
   const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
   const Row<T> row = row_of<T>(a.p, row_id);
   const int per = a.parts / a.splits * a.part;
-  const int from = min(split * per, row.n), to = min(from + per, row.n);
+  const int from = split * per, to = min(from + per, row.vecs);
   const u64 best = best_of(s, row, from, to, tid);
   Hand& h = a.hand[row_id];
   if (tid == 0) {
@@ -635,7 +794,8 @@ __global__ __launch_bounds__(kThreads) void sample_best_kernel(SplitArgs a) {
 
 __device__ __forceinline__ u64 best_of(const Hand& h, int splits) {
   u64 best = 0;
-  for (int i = 0; i < splits; ++i) best = max(best, h.best[i]);
+#pragma unroll
+  for (int i = 0; i < kMaxSplit; ++i) best = max(best, h.best[min(i, splits - 1)]);
   return best;
 }
 
@@ -646,12 +806,13 @@ __global__ __launch_bounds__(kThreads) void sample_histogram_kernel(SplitArgs a)
   const Row<T> row = row_of<T>(a.p, row_id);
   const u64 best = best_of(a.hand[row_id], a.splits);
   const Request q = request(a.p, row_id, best);
-  if (settled(a.p, q, row_id, best, split == 0 && tid == 0) || !(q.k > 0 || q.top_p < 1.0f)) return;
+  if (settled(a.p, q, row_id, best, split == 0 && tid == 0) || !q.cuts()) return;
   const int per = a.parts / a.splits * a.part;
-  const int from = min(split * per, row.n), to = min(from + per, row.n);
-  histogram(s, row, q.scale, from, to, tid);
+  const int from = split * per, to = min(from + per, row.vecs);
+  histogram(s, row, q.scale, !q.few, from, to, tid);
   Histogram& h = a.hist[static_cast<long long>(row_id) * a.splits + split];
-  h.count[tid] = s.count[tid], h.mass[tid] = s.mass[tid];
+  h.count[tid] = s.count[tid];
+  if (!q.few) h.mass[tid] = s.mass[tid];
 }
 
 template <typename T>
@@ -663,15 +824,22 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SplitArgs a) {
   const u64 best = best_of(hand, a.splits);
   const Request q = request(a.p, row_id, best);
   if (settled(a.p, q, row_id, best, false)) return;  // launch 2 has written it
-  Plan plan{0, 0, false, false, kBins, -1, -1, -2, 0};
-  if (q.k > 0 || q.top_p < 1.0f) {
+  Plan plan = no_plan();
+  Bin bin{};
+  if (q.cuts()) {
     const Histogram* h = a.hist + static_cast<long long>(row_id) * a.splits;
-    uint32_t c = 0;
-    u64 m = 0;
-    for (int i = 0; i < a.splits; ++i) c += h[i].count[tid], m += h[i].mass[tid];
-    s.count[tid] = c, s.mass[tid] = m;
+    uint32_t c[kMaxSplit];
+    u64 m[kMaxSplit];
+#pragma unroll
+    for (int i = 0; i < kMaxSplit; ++i)  // all in flight
+      if (i < a.splits) c[i] = h[i].count[tid], m[i] = q.few ? 0 : h[i].mass[tid];
+      else c[i] = 0, m[i] = 0;
+#pragma unroll
+    for (int i = 1; i < kMaxSplit; ++i) c[0] += c[i], m[0] += m[i];
+    s.count[tid] = c[0], s.mass[tid] = m[0];
     __syncthreads();
-    plan = make_plan(s, q, tid);
+    bin = scan_bins(s, s.count, s.mass, tid);
+    plan = make_plan(s, q, q.few, bin, tid);
   }
   const int per = a.parts / a.splits, first = split * per;
   pick(s, row, q.scale, plan, a.part, first, first + per, tid);
@@ -702,7 +870,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SplitArgs a) {
       s.index[i] = load_coherent(&hand.index[i]);
     }
   __syncthreads();
-  finish(s, a.p, row_id, row, q, plan, a.part, a.parts, tid);
+  finish(s, a.p, row_id, row, q, plan, bin, a.part, a.parts, tid);
 }
 
 // Workgroups a row: rows that fill the card by themselves take one.
@@ -715,15 +883,19 @@ int splits_of(int rows, int vocab) {
 template <typename T>
 void launch(const SampleArgs& p, void* workspace, hipStream_t stream) {
   const int splits = splits_of(p.rows, p.vocab);
+  const dim3 grid(splits, p.rows), block(kThreads);
+  const bool tiny = p.vocab < Row<T>::kVec;
+  // parts of whole rounds of a wave's loads, a multiple of `splits` in number
+  const int vecs = ceil_div(p.vocab, tiny ? Row<T, true>::kVec : Row<T>::kVec), round = 64 * kFlight;
+  const int part = round * ceil_div(vecs, round * kMaxParts);
+  const int parts = splits * ceil_div(ceil_div(vecs, part), splits);
   if (splits == 1) {
-    hipLaunchKernelGGL(sample_row_kernel<T>, dim3(p.rows), dim3(kThreads), 0, stream, p);
+    const auto kernel = tiny ? sample_row_kernel<T, true> : sample_row_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3(p.rows), block, 0, stream, p, part, parts);
     return;
   }
-  const int parts = kParts > kWaves * splits ? kParts : kWaves * splits;
-  SplitArgs a{p, static_cast<Hand*>(workspace),
-              reinterpret_cast<Histogram*>(static_cast<Hand*>(workspace) + p.rows), splits,
-              ceil_div(p.vocab, parts), parts};
-  const dim3 grid(splits, p.rows), block(kThreads);
+  const SplitArgs a{p, static_cast<Hand*>(workspace),
+                    reinterpret_cast<Histogram*>(static_cast<Hand*>(workspace) + p.rows), splits, part, parts};
   hipLaunchKernelGGL(sample_best_kernel<T>, grid, block, 0, stream, a);
   hipLaunchKernelGGL(sample_histogram_kernel<T>, grid, block, 0, stream, a);
   hipLaunchKernelGGL(sample_draw_kernel<T>, grid, block, 0, stream, a);
