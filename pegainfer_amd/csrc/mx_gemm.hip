@@ -259,21 +259,6 @@ struct MxTile {
   static_assert(NS >= 3 && NS <= 6 && kLds <= 160 * 1024, "tile shape");
 };
 
-// Workgroups go to the eight XCDs in turn; each XCD's are made to cover a compact part of the grid
-// of tiles (runs of the order that goes down panels four feature tiles wide), so that its L2 brings
-// in as few operand rows as it can.
-// gy: of the grid's rows of tiles, those that are there.
-__device__ __forceinline__ void xcd_tile(int& tx, int& ty, int gy) {
-  const int gx = gridDim.x;
-  const int total = gx * gy, id = ty * gx + tx;
-  const int xcd = id & 7, each = total >> 3, more = total & 7;
-  const int at = xcd * each + min(xcd, more) + (id >> 3);
-  const int panel = at / (4 * gy), in = at - panel * 4 * gy;
-  const int wide = min(4, gx - 4 * panel);
-  ty = in / wide;
-  tx = 4 * panel + in - ty * wide;
-}
-
 template <int V>
 using Int = std::integral_constant<int, V>;
 

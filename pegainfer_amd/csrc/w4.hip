@@ -49,12 +49,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, ui
                                            static_cast<int>(bytes), 0x00020000);
 }
 
-// Eight codes as (16 + q) / 16.
-__device__ __forceinline__ bf16x8_t expand(uint32_t w) {
+// Eight codes as (16 + q) / 16.  The constants stand in registers that the compiler cannot see through: as
+// literals they would cost an instruction of their own each.
+struct Masks {
+  uint32_t code = 0x00780078u, one = 0x3F803F80u;
+  __device__ __forceinline__ Masks() { asm volatile("" : "+v"(code), "+v"(one)); }
+};
+__device__ __forceinline__ bf16x8_t expand(uint32_t w, const Masks& k) {
   u32x4_t v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v[i] = (__builtin_amdgcn_alignbit(w, w, 4 * i) & 0x00780078u) | 0x3F803F80u;
+  for (int i = 0; i < 4; ++i) v[i] = (__builtin_amdgcn_alignbit(w, w, 4 * i) & k.code) | k.one;
   return __builtin_bit_cast(bf16x8_t, v);
 }
 __device__ __forceinline__ bf16x8_t repeat(uint32_t pair) {
@@ -173,6 +177,7 @@ __global__ __launch_bounds__(64 * WV) void w4_stream_kernel(W4Args p) {
       }
   };
   floatx4_t acc[MR][RB] = {};
+  const Masks masks;
   const auto compute = [&](const Step& r) {
 #pragma unroll
     for (int m = 0; m < MR; ++m)
@@ -190,7 +195,7 @@ __global__ __launch_bounds__(64 * WV) void w4_stream_kernel(W4Args p) {
         floatx4_t d[RB] = {};
 #pragma unroll
         for (int j = g * (4 / kPer); j < (g + 1) * (4 / kPer); ++j) {
-          const bf16x8_t w = expand(r.w[m][j]);
+          const bf16x8_t w = expand(r.w[m][j], masks);
 #pragma unroll
           for (int b = 0; b < RB; ++b) d[b] = mfma(r.x[b][j], repeat(bias), d[b]);
 #pragma unroll
@@ -259,10 +264,322 @@ void launch_stream(const W4Args& p, hipStream_t stream) {
                      stream, p);
 }
 
+// ---------------------------------------------------------------- many rows
+// A workgroup of WM x WN waves owns 16 TM WM features x 16 TN WN rows, each wave 16 TM of the features and
+// 16 TN of the rows, for all of K; a stage of the ring in LDS holds a step of X, codes and scales,
+// brought in by loads straight to LDS, one barrier a step.  A row of X has its 16-byte pieces at slot
+// piece ^ (row % 8), which spreads eight lanes' fragment reads over all banks.
+// sum_k x over a group (times -24 / 16 without zero points) is one more chain a row block, with a
+// constant operand, which the waves share out a step ahead; its features' chains start from it.
+template <int G_, bool kZeros_, int WM_, int WN_, int TM_, int TN_, int NS_>
+struct W4Tile {
+  static constexpr int G = G_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, NS = NS_;
+  static constexpr bool kZeros = kZeros_;
+  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN;
+  static constexpr int kMeta = meta_bytes(G, kZeros), kMetaBytes = BM * kMeta;
+  static constexpr int kXLoads = BN / 4, kWLoads = BM / 16, kMLoads = (kMetaBytes + 255) / 256;
+  static constexpr int PX = (kXLoads + kWaves - 1) / kWaves;  // loads of a wave and stage
+  static constexpr int PW = (kWLoads + kWaves - 1) / kWaves, PM = (kMLoads + kWaves - 1) / kWaves;
+  static constexpr int P = PX + PW + PM;
+  static constexpr int kX = BN * 256, kW = BM * 64;
+  static constexpr int kStage = kX + kW + kMLoads * 256, kRing = NS * kStage;
+  static constexpr int kSum = kStep / G * BN * 4;  // a step's group sums of X
+  static constexpr int kLds = kRing + 2 * kSum;
+  static_assert(NS >= 3 && kLds <= 160 * 1024, "tile shape");
+};
+
+template <typename S>
+__global__ __launch_bounds__(S::kThreads) void w4_tile_kernel(W4Args p) {
+  constexpr int TM = S::TM, TN = S::TN, NS = S::NS, kMeta = S::kMeta, kPer = kStep / S::G;
+  __shared__ __align__(1024) uint8_t smem[S::kLds];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % S::WM, wn = wave / S::WM;
+  const int c = lane & 15, h = lane >> 4;
+  int tx = blockIdx.x, ty = blockIdx.y;
+  xcd_tile(tx, ty, gridDim.y);
+  const int K = p.K, steps = ceil_div(K, kStep);
+  const int t0 = tx * (S::BM / 16), n0 = ty * S::BN;
+  const int live = min(S::BM / 16, ceil_div(p.M, 16) - t0), rows = min(S::BN, p.N - n0);
+  const uint32_t w_tile = static_cast<uint32_t>(steps) * 1024u;
+  const uint32_t m_tile = static_cast<uint32_t>(steps) * (16u * kMeta);
+  const uint32_t x_row = static_cast<uint32_t>(K) * 2u;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) uint8_t*)smem));
+
+  u32x4_t x_rsrc = rsrc_words(p.x + static_cast<long long>(n0) * K, static_cast<uint32_t>(rows) * x_row);
+  u32x4_t w_rsrc = rsrc_words(p.codes + static_cast<long long>(t0) * w_tile, static_cast<uint32_t>(live) * w_tile);
+  u32x4_t m_rsrc = rsrc_words(p.meta + static_cast<long long>(t0) * m_tile, static_cast<uint32_t>(live) * m_tile);
+  const uint32_t x_size = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x_rsrc[2])));
+  const uint32_t w_size = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w_rsrc[2])));
+  const uint32_t m_size = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(m_rsrc[2])));
+  // This wave's loads of a stage (a repeat brings the same).  Rows past the last one and tiles past the
+  // last one are past their operands' ranges, and come as zeros.
+  uint32_t x_voff[S::PX], w_voff[S::PW], m_voff[S::PM], x_dst[S::PX], w_dst[S::PW], m_dst[S::PM];
+  int x_col[S::PX];
+#pragma unroll
+  for (int j = 0; j < S::PX; ++j) {
+    const int i = min(wave * S::PX + j, S::kXLoads - 1);
+    const int r = 4 * i + (lane >> 4), piece = (lane & 15) ^ (r & 7);
+    x_dst[j] = lds0 + 1024u * static_cast<uint32_t>(i);
+    x_col[j] = 8 * piece;
+    x_voff[j] = static_cast<uint32_t>(r) * x_row + 16u * static_cast<uint32_t>(piece);
+  }
+#pragma unroll
+  for (int j = 0; j < S::PW; ++j) {
+    const int i = min(wave * S::PW + j, S::kWLoads - 1);
+    w_dst[j] = lds0 + S::kX + 1024u * static_cast<uint32_t>(i);
+    w_voff[j] = static_cast<uint32_t>(i) * w_tile + 16u * lane;
+  }
+#pragma unroll
+  for (int j = 0; j < S::PM; ++j) {
+    const int i = min(wave * S::PM + j, S::kMLoads - 1), b = i * 256 + lane * 4;
+    m_dst[j] = lds0 + S::kX + S::kW + 256u * static_cast<uint32_t>(i);
+    m_voff[j] = b < S::kMetaBytes ? static_cast<uint32_t>(b / (16 * kMeta)) * m_tile +
+                                        static_cast<uint32_t>(b % (16 * kMeta))
+                                  : kOutOfRange;
+  }
+  // Stages come in turn; past the last one the operands have no bytes, and zeros come that nothing uses.
+  const auto stage_in = [&](int s, uint32_t at) {
+    x_rsrc[2] = s < steps ? x_size : 0u;
+    w_rsrc[2] = s < steps ? w_size : 0u;
+    m_rsrc[2] = s < steps ? m_size : 0u;
+    const int cols = K - s * kStep;  // columns past the last one are another row's
+#pragma unroll
+    for (int j = 0; j < S::PX; ++j)
+      dma_b128(x_rsrc, x_dst[j] + at, x_col[j] < cols ? x_voff[j] : kOutOfRange, static_cast<uint32_t>(s) * 256u);
+#pragma unroll
+    for (int j = 0; j < S::PW; ++j)
+      dma_b128(w_rsrc, w_dst[j] + at, w_voff[j], static_cast<uint32_t>(s) * 1024u);
+#pragma unroll
+    for (int j = 0; j < S::PM; ++j)
+      dma_b32(m_rsrc, m_dst[j] + at, m_voff[j], static_cast<uint32_t>(s) * (16u * kMeta));
+  };
+
+  floatx4_t acc[TM][TN] = {};
+  const Masks masks;
+  struct Rows {
+    u32x4_t v[4];
+  };
+  const auto x_rows = [&](uint32_t at, int b) {  // row block b of the workgroup's
+    Rows x;
+    const uint8_t* xl = smem + at + (16 * b + c) * 256;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.v[j] = *reinterpret_cast<const u32x4_t*>(xl + 16 * ((4 * j + h) ^ (c & 7)));
+    return x;
+  };
+  // a step's group sums of X, row blocks in turn by wave: block `wave` + i kWaves
+  constexpr int kSumBlocks = (S::BN / 16 + S::kWaves - 1) / S::kWaves;
+  const auto sum_rows = [&](uint32_t at, int i) { return x_rows(at, min(wave + i * S::kWaves, S::BN / 16 - 1)); };
+  const auto sum_up = [&](const Rows& x, uint32_t sums, int i) {
+    const bf16x8_t ones = repeat(S::kZeros ? 0x3F803F80u : 0xBFC0BFC0u);  // 1, or -(16 + 8) / 16
+    constexpr int kJ = 4 / kPer;
+    const int b = wave + i * S::kWaves;
+#pragma unroll
+    for (int g = 0; g < kPer; ++g) {
+      floatx4_t sum = {};
+#pragma unroll
+      for (int j = g * kJ; j < (g + 1) * kJ; ++j) sum = mfma(x.v[j], ones, sum);
+      // the same in all 16 columns
+      if (c == 0 && b < S::BN / 16)
+        *reinterpret_cast<floatx4_t*>(smem + sums + 4 * (g * S::BN + 16 * b + 4 * h)) = sum;
+    }
+  };
+  // What a step starts with, read from LDS while the step before is computed.
+  constexpr int kWords = (kMeta + 3) / 4;
+  struct First {
+    u32x4_t q[TM];
+    uint32_t meta[TM][kWords];
+    Rows x;
+  };
+  const auto read_first = [&](First& f, uint32_t at) {
+    const uint8_t* wl = smem + at + S::kX + wm * (TM * 1024) + 16 * lane;
+    const uint8_t* ml = smem + at + S::kX + S::kW + wm * (TM * 16 * kMeta) + c * kMeta;
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+      f.q[t] = *reinterpret_cast<const u32x4_t*>(wl + 1024 * t);
+      const uint8_t* m = ml + t * (16 * kMeta);
+      if constexpr (kMeta == 2) {
+        f.meta[t][0] = *reinterpret_cast<const uint16_t*>(m);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) f.meta[t][i] = reinterpret_cast<const uint32_t*>(m)[i];
+      }
+    }
+    f.x = x_rows(at, wn * TN);
+  };
+  // A step, on the stage at `at`, with what is in f; f and the group sums for the stage at `then`.
+  const auto compute = [&](First& f, uint32_t at, uint32_t sums, uint32_t then, uint32_t ahead) {
+    constexpr int kJ = 4 / kPer;
+    const auto sum_of = [&](int b, int g) {
+      return *reinterpret_cast<const floatx4_t*>(smem + sums + 4 * (g * S::BN + 16 * (wn * TN + b) + 4 * h));
+    };
+    bf16x8_t w[TM][4];
+    float scale[TM][kPer], zero[TM][kPer];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[t][j] = expand(f.q[t][j], masks);
+#pragma unroll
+      for (int g = 0; g < kPer; ++g) {
+        if constexpr (S::kZeros) scale[t][g] = bf_lo(f.meta[t][g]), zero[t][g] = bf_hi(f.meta[t][g]);
+        else scale[t][g] = g & 1 ? bf_hi(f.meta[t][g / 2]) : bf_lo(f.meta[t][g / 2]), zero[t][g] = 0.0f;
+      }
+    }
+    Rows x = f.x;
+    floatx4_t last[TM];  // the last group's sums of the row block before, not yet in acc
+    const auto settle = [&](const floatx4_t* d, int b, int g) {
+#pragma unroll
+      for (int t = 0; t < TM; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][b][i] = __builtin_fmaf(scale[t][g], d[t][i], acc[t][b][i]);
+    };
+    floatx4_t sum = sum_of(0, 0);
+    Rows ys = sum_rows(then, 0);
+#pragma unroll
+    for (int b = 0; b < TN; ++b) {
+      Rows coming;
+      if (b + 1 < TN) coming = x_rows(at, wn * TN + b + 1);
+      else read_first(f, then);
+#pragma unroll
+      for (int g = 0; g < kPer; ++g) {
+        floatx4_t d[TM];
+#pragma unroll
+        for (int t = 0; t < TM; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[t][i] = S::kZeros ? sum[i] * zero[t][g] : sum[i];
+        if (g + 1 < kPer) sum = sum_of(b, g + 1);
+        else if (b + 1 < TN) sum = sum_of(b + 1, 0);
+#pragma unroll
+        for (int j = g * kJ; j < (g + 1) * kJ; ++j)
+#pragma unroll
+          for (int t = 0; t < TM; ++t) d[t] = mfma(x.v[j], w[t][j], d[t]);
+        if (b + g > 0) settle(last, g > 0 ? b : b - 1, g > 0 ? g - 1 : kPer - 1);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) last[t] = d[t];
+      }
+      if (b + 1 < TN) x = coming;
+      // behind the first products of this step, the sums of the next one
+      if (b < kSumBlocks) {
+        sum_up(ys, ahead, b);
+        if (b + 1 < kSumBlocks) ys = sum_rows(then, b + 1);
+      }
+    }
+    static_assert(kSumBlocks <= TN, "tile shape");
+    settle(last, TN - 1, kPer - 1);
+  };
+
+  const auto next = [](uint32_t at) { return at + S::kStage == S::kRing ? 0u : at + S::kStage; };
+  uint32_t in = 0, out = 0;  // where the next stage goes, and which is next to be used
+  for (int s = 0; s < NS - 1; ++s) {
+    stage_in(s, in);
+    in = next(in);
+  }
+  uint32_t sums = S::kRing;
+  vm_wait<(NS - 2) * S::P>();
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < kSumBlocks; ++i) sum_up(sum_rows(0, i), sums, i);
+  First first;
+  read_first(first, 0);
+#pragma unroll 1
+  for (int s = 0; s < steps; ++s) {
+    vm_wait<(NS - 3) * S::P>();  // the stage after this one
+    lds_barrier();
+    stage_in(s + NS - 1, in);
+    in = next(in);
+    const uint32_t then = next(out), ahead = 2 * S::kRing + S::kSum - sums;
+    compute(first, out, sums, then, ahead);
+    out = then, sums = ahead;
+  }
+  vm_wait<0>();
+#pragma unroll
+  for (int t = 0; t < TM; ++t) {
+    const int m = 16 * (t0 + wm * TM + t) + c;
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int b = 0; b < TN; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * (wn * TN + b) + 4 * h + i;
+        if (r >= rows) continue;
+        const long long at = static_cast<long long>(n0 + r) * p.M + m;
+        const float v = 16.0f * acc[t][b][i];
+        if (p.f32) static_cast<float*>(p.y)[at] = v;
+        else static_cast<uint16_t*>(p.y)[at] = f2bf(v);
+      }
+  }
+}
+
+template <typename S>
+void launch_tile(const W4Args& p, hipStream_t stream) {
+  hipLaunchKernelGGL(w4_tile_kernel<S>, dim3(ceil_div(p.M, S::BM), ceil_div(p.N, S::BN)), dim3(S::kThreads), 0,
+                     stream, p);
+}
+
+// ---------------------------------------------------------------- which kernel
+// A call's time in us, over 1024 .. 163840 features, 2048 .. 7168 columns and 1 .. 2048 rows of each
+// form alone: start + steps * (step + fill * step_rows + (more + fill * more_rows) * (w - w0)), with w
+// workgroups a CU (above w0) and a workgroup's rows filled to `fill`.  The form that this puts first
+// is within 3% of the fastest one on average, 30% at most (where two forms cross).  Examples,
+// groups of 128: one row of 4096 x 7168 5.0 us with <1, 1, 8, 2>, 11.6 with <4, 1, 4, 2>; one of 163840 x
+// 2048 35.8 with the latter, 77 with the former; 48 rows of those 62 with the tile of 48 rows, 94 with
+// <4, 4, 4, 1>; 2048 rows of 4096 x 7168 132 with the tile of 256 x 128, 156 with 128 x 64, of 1024
+// rows 101 and 81.  Groups of 32 take half as long again in the tile kernel, whose vector work grows with
+// the groups; its widest tile would spill registers with them.
+struct Form {
+  int bm, bn;
+  bool whole;  // half of the cost is by whole rounds of workgroups
+  float start, step, step_rows, more, more_rows, w0;
+};
+constexpr Form kForms[] = {
+    {16, 16, false, 5.9f, 0.0f, 0.03f, 0.079f, 0.123f, 0.90f},    // stream <1, 1, 8, 2>
+    {32, 16, false, 3.2f, 0.055f, 0.064f, 0.114f, 0.061f, 0.71f}, // stream <2, 1, 4, 2>
+    {64, 16, false, 3.4f, 0.139f, 0.002f, 0.216f, 0.0f, 0.70f},   // stream <4, 1, 4, 2>
+    {64, 32, false, 3.4f, 0.197f, 0.073f, 0.234f, 0.09f, 0.74f},  // stream <4, 2, 4, 1>
+    {64, 64, false, 4.3f, 0.332f, 0.18f, 0.356f, 0.235f, 0.83f},  // stream <4, 4, 4, 1>
+    {128, 48, false, 4.1f, 0.737f, 0.0f, 0.588f, 0.0f, 0.90f},    // tile <4, 1, 2, 3>
+    {128, 64, true, 4.8f, 0.857f, 0.0f, 0.73f, 0.0f, 1.17f},      // tile <4, 1, 2, 4>
+    {256, 64, true, 4.4f, 1.231f, 0.0f, 1.547f, 0.0f, 0.88f},     // tile <8, 1, 2, 4>
+    {128, 128, true, 4.5f, 1.292f, 0.0f, 1.522f, 0.0f, 0.92f},    // tile <4, 2, 2, 4>
+    {256, 128, true, 6.9f, 1.948f, 0.0f, 2.495f, 0.0f, 0.81f},    // tile <4, 2, 4, 4>
+};
+constexpr int kStreams = 5, kFormCount = sizeof(kForms) / sizeof(kForms[0]);
+
+int choose_form(int M, int N, int K, int group) {
+  int best = 0;
+  float best_time = 0.0f;
+  const float steps = static_cast<float>(ceil_div(K, kStep));
+  for (int i = 0; i < kFormCount - (group == 32 ? 1 : 0); ++i) {
+    const Form& f = kForms[i];
+    const int blocks = ceil_div(N, f.bn);
+    const float groups = static_cast<float>(ceil_div(M, f.bm)) * static_cast<float>(blocks) / 256.0f;
+    const float w = f.whole ? 0.5f * (groups + __builtin_ceilf(groups)) : groups;
+    const float fill = static_cast<float>(N) / (static_cast<float>(blocks) * static_cast<float>(f.bn));
+    const float over = w > f.w0 ? w - f.w0 : 0.0f;
+    const float step = f.step + fill * f.step_rows + (f.more + fill * f.more_rows) * over;
+    const float time = f.start + steps * step * (group == 32 && i >= kStreams ? 1.5f : 1.0f);
+    if (i == 0 || time < best_time) best = i, best_time = time;
+  }
+  return best;
+}
+
 template <int G, bool kZeros>
 void launch_w4(const W4Args& p, hipStream_t stream) {
-  if (p.N <= 16) launch_stream<G, kZeros, 1, 1, 4, 4>(p, stream);
-  else launch_stream<G, kZeros, 2, 2, 4, 2>(p, stream);
+  switch (choose_form(p.M, p.N, p.K, G)) {
+    case 0: launch_stream<G, kZeros, 1, 1, 8, 2>(p, stream); break;
+    case 1: launch_stream<G, kZeros, 2, 1, 4, 2>(p, stream); break;
+    case 2: launch_stream<G, kZeros, 4, 1, 4, 2>(p, stream); break;
+    case 3: launch_stream<G, kZeros, 4, 2, 4, 1>(p, stream); break;
+    case 4: launch_stream<G, kZeros, 4, 4, 4, 1>(p, stream); break;
+    case 5: launch_tile<W4Tile<G, kZeros, 4, 1, 2, 3, 3>>(p, stream); break;
+    case 6: launch_tile<W4Tile<G, kZeros, 4, 1, 2, 4, 3>>(p, stream); break;
+    case 7: launch_tile<W4Tile<G, kZeros, 8, 1, 2, 4, 3>>(p, stream); break;
+    case 8: launch_tile<W4Tile<G, kZeros, 4, 2, 2, 4, 3>>(p, stream); break;
+    default:
+      if constexpr (G != 32) launch_tile<W4Tile<G, kZeros, 4, 2, 4, 4, 3>>(p, stream);
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
