@@ -25,14 +25,16 @@
 namespace pega {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kBins = 1024;
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kBins = kThreads;        // one a thread
 constexpr int kList = 4096;            // elements of the cuts' bins kept in LDS
 constexpr int kMaxSplit = 16;          // workgroups of a row
 constexpr int kMaxParts = 256;         // of a row, whose masses the draw goes over first (a multiple of kMaxSplit)
 constexpr int kFlight = 4;              // vectors of a thread in flight
-constexpr int kPairs = 256;            // candidates that are compared with each other
-constexpr int kWorkgroups = 512;       // two a CU
+constexpr int kMaxFew = 1024;          // so few fit the list with room for what shares the last one's bin
+constexpr int kPairs = kThreads / 4;   // candidates that are compared with each other
+constexpr int kWorkgroups = 2048;      // eight a CU
+constexpr int kMaxRows = 256;          // of a round of launches, which bounds the workspace
 constexpr int kMaxVocab = 1 << 19;     // sums of weights stay below 2^63
 constexpr double kRange = 28.0;        // smaller weights than e^-28 are zero
 constexpr double kLog2e = 1.4426950408889634;
@@ -50,6 +52,7 @@ struct SampleArgs {
   const int32_t* top_k;
   int32_t* tokens;
   float* logprobs;
+  bool has_temperature, has_top_p, has_min_p, has_top_k;
 };
 
 __device__ __forceinline__ float clean(float l) { return l == l ? l + 0.0f : -__builtin_inff(); }  // -0 is 0
@@ -66,16 +69,16 @@ __device__ __forceinline__ u64 place(float l, int i) {
 }
 
 // A row as vectors of 16 bytes, wherever it starts (the loads need no alignment); the last one reaches back to
-// end with the row.  kTiny: rows shorter than a vector.
-template <typename T, bool kTiny = false>
+// end with the row.  Rows shorter than a vector go element by element.
+template <typename T>
 struct Row {
-  static constexpr int kVec = kTiny ? 4 : 16 / static_cast<int>(sizeof(T));
+  static constexpr int kVec = 16 / static_cast<int>(sizeof(T));
   const T* p;
   int n, vecs;  // elements, vectors
 
   __device__ __forceinline__ Row(const T* row, int size) : p(row), n(size), vecs(ceil_div(size, kVec)) {}
   static __device__ __forceinline__ float value(uint4 q, int e) {
-    if constexpr (sizeof(T) == 4 || kTiny)
+    if constexpr (sizeof(T) == 4)
       return clean(__builtin_bit_cast(float, e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w));
     const uint32_t w = (e >> 1) == 0 ? q.x : (e >> 1) == 1 ? q.y : (e >> 1) == 2 ? q.z : q.w;
     return clean(e & 1 ? bf_hi(w) : bf_lo(w));
@@ -84,46 +87,52 @@ struct Row {
     if constexpr (sizeof(T) == 4) return clean(p[i]);
     else return clean(bf2f(p[i]));
   }
-  __device__ __forceinline__ int start(int v) const { return kTiny ? v * kVec : min(v * kVec, n - kVec); }
+  __device__ __forceinline__ int start(int v) const { return min(v * kVec, n - kVec); }
   __device__ __forceinline__ uint4 load(int v) const {  // past the last: the last
-    const int from = start(min(v, vecs - 1));
     uint4 q;
-    if constexpr (kTiny) {
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = __builtin_bit_cast(uint32_t, at(min(from + e, n - 1)));
-      q = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      __builtin_memcpy(&q, p + from, 16);
-    }
+    __builtin_memcpy(&q, p + start(min(v, vecs - 1)), 16);
     return q;
   }
   // The largest place of the vectors in [from, to), over `threads` threads.
   __device__ __forceinline__ u64 best(int from, int to, int tid, int threads) const {
     u64 best = 0;
+    if (n < kVec) {
+      if (from == 0 && tid < n) best = place(at(tid), tid);
+      return best;
+    }
     for (int v = from + tid; v < to; v += kFlight * threads) {
       uint4 q[kFlight];
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) q[j] = load(v + j * threads);
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        const int i = start(min(v + j * threads, vecs - 1));
+        // each element once: the threads' largest are of disjoint elements
+        const int vec = v + j * threads, i = start(min(vec, vecs - 1));
 #pragma unroll
-        for (int e = 0; e < kVec; ++e)  // (a tiny row's last one several times over: the first of them counts)
-          best = max(best, place(value(q[j], e), min(i + e, n - 1)));
+        for (int e = 0; e < kVec; ++e)
+          if (vec < to && i + e >= vec * kVec) best = max(best, place(value(q[j], e), i + e));
       }
     }
     return best;
   }
   // f(i, l[i]) for the vectors' elements with l >= low, over `threads` threads with kFlight loads in flight
   // each.  Few copies of f: the passes are short enough for a CU's instruction fetches to show.
-  template <typename F>
-  __device__ __forceinline__ void each(int from, int to, int tid, int threads, float low, F f) const {
+  // after(base): once for each round of vectors base .. base + threads - 1, by all threads.
+  template <typename F, typename A>
+  __device__ __forceinline__ void each(int from, int to, int tid, int threads, float low, F f, A after) const {
+    if (n < kVec) {
+      if (from == 0 && from < to) {
+        each_plain(tid, threads, low, f);
+        after(from);
+      }
+      return;
+    }
     uint4 q[kFlight];
 #pragma unroll
     for (int j = 0; j < kFlight; ++j) q[j] = load(from + tid + j * threads);
 #pragma unroll 1
-    for (int v = from + tid; v < to; v += threads) {
+    for (int base = from; base < to; base += threads) {
+      const int v = base + tid;
       uint4 now = q[0];
 #pragma unroll
       for (int j = 0; j + 1 < kFlight; ++j) q[j] = q[j + 1];
@@ -131,18 +140,20 @@ struct Row {
       float most = value(now, 0);
 #pragma unroll
       for (int e = 1; e < kVec; ++e) most = fmaxf(most, value(now, e));
-      if (most < low) continue;
-      int i = start(v);
+      if (v < to && most >= low) {
+        int i = start(v);
 #pragma unroll 1
-      for (int w = 0; w < kVec; w += 4) {
+        for (int w = 0; w < kVec; w += 4) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float l = value(now, e);
-          if (l >= low && i + e >= v * kVec && (!kTiny || i + e < n)) f(i + e, l);
+          for (int e = 0; e < 4; ++e) {
+            const float l = value(now, e);
+            if (l >= low && i + e >= v * kVec) f(i + e, l);
+          }
+          i += 4;
+          now = make_uint4(now.z, now.w, now.x, now.y);
         }
-        i += 4;
-        now = make_uint4(now.z, now.w, now.x, now.y);
       }
+      after(base);
     }
   }
   // The same, element by element: where speed does not count.
@@ -187,9 +198,8 @@ struct Scale {
     return __builtin_bit_cast(u64, whole) & 0xfffffffffffffull;
   }
   // bins of equal width in the logarithm, the largest weights in bin 0
-  __device__ __forceinline__ int bin(double d) const {
-    return min(kBins - 1, static_cast<int>(-d * per * kBinsPerOctave));
-  }
+  __device__ __forceinline__ double position(double d) const { return -d * per * kBinsPerOctave; }
+  __device__ __forceinline__ int bin(double d) const { return min(kBins - 1, static_cast<int>(position(d))); }
   // below every d of a bin
   __device__ __forceinline__ double edge(int b) const { return -(b + 1) / (per * kBinsPerOctave) * (1 + 0x1p-30); }
   // a float below every logit that lies d or less below the maximum
@@ -203,13 +213,13 @@ struct Scale {
 struct Shared {
   u64 mass[kBins];  // the row's histogram
   uint32_t count[kBins];
-  u64 fine_mass[kBins];  // a narrower one inside a bin of it
+  __align__(16) u64 fine_mass[kBins];  // a narrower one inside a bin of it
   uint32_t fine_count[kBins];
   u64 part[kMaxParts];  // masses of the row's parts
   uint32_t key[kList];  // elements of the bins in which the cuts fall
   int32_t index[kList];
-  u64 wave_mass[kWaves];
-  uint32_t wave_count[kWaves];
+  u64 wave_mass[16];
+  uint32_t wave_count[16];
   u64 found_mass;
   uint32_t found_count;
   int found, last, listed;
@@ -281,7 +291,7 @@ __device__ __forceinline__ u64 block_max(Shared& s, u64 v, int tid) {
   __syncthreads();
   if ((tid & 63) == 0) s.wave_mass[tid >> 6] = v;
   __syncthreads();
-  return lane64(max16(s.wave_mass[tid & 15]), 0);
+  return lane64(max16(s.wave_mass[tid & (kWaves - 1)]), 0);
 }
 
 // A cut of the order: the first `count` elements, or those with less than `mass` before them,
@@ -338,25 +348,28 @@ struct Request {
   int k;        // 0: all
   bool none;    // no logit above -inf
   bool first;   // the first of the order alone
-  bool few;     // k fits the list: all that the k cut leaves is listed, and has weights only then
+  bool few;     // a small k: all that its cut leaves is listed without a histogram of the row
   __device__ __forceinline__ bool cuts() const { return k > 0 || top_p < 1.0f; }
+  __device__ __forceinline__ bool settled() const { return none || first; }
 };
 
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-__device__ __forceinline__ Request request(const SampleArgs& p, int row, u64 best) {
+// splits: of the row
+__device__ __forceinline__ Request request(const SampleArgs& p, int row, u64 best, int splits) {
   Request q;
   const float top = value_of(static_cast<uint32_t>(best >> 32));
-  const float temp = p.temperature ? p.temperature[row] : 1.0f;
-  const float min_p = p.min_p ? p.min_p[row] : 0.0f;
+  // (loads side by side: a missing one's pointer is u's)
+  const float temp = p.has_temperature ? p.temperature[row] : 1.0f;
+  const float min_p = p.has_min_p ? p.min_p[row] : 0.0f;
   const bool greedy = !(temp > 0.0f);
-  q.k = greedy ? 1 : p.top_k ? max(p.top_k[row], 0) : 0;
+  q.k = greedy ? 1 : p.has_top_k ? max(p.top_k[row], 0) : 0;
   q.first = q.k == 1;
-  q.few = q.k > 0 && q.k <= kList / 2;
+  q.few = q.k > 0 && q.k <= min(kMaxFew, splits * (kThreads / 2));
   q.none = top == -__builtin_inff();
-  q.top_p = p.top_p ? p.top_p[row] : 1.0f;
+  q.top_p = p.has_top_p ? p.top_p[row] : 1.0f;
   q.u = p.u[row];
   q.temp = greedy ? 1.0 : static_cast<double>(fminf(temp, 3.40282347e38f));
   q.scale.max = top;
@@ -374,22 +387,22 @@ __device__ __forceinline__ void write(const SampleArgs& p, int row, int token, f
 }
 
 // One element's share of the histogram.
-__device__ __forceinline__ void count_in(Shared& s, const Scale& scale, bool masses, float l) {
+__device__ __forceinline__ void count_in(Shared& s, const Scale& scale, float l) {
   const double d = scale.below(l);
   if (!scale.live(d)) return;
   const int b = scale.bin(d);
   atomicAdd(&s.count[b], 1u);
-  if (masses) atomicAdd(&s.mass[b], scale.weight(d));
+  atomicAdd(&s.mass[b], scale.weight(d));
 }
 
-// The histogram of vectors [from, to): counts, and masses unless few will have weight.
+// The histogram of vectors [from, to).
 template <typename R>
-__device__ __forceinline__ void histogram(Shared& s, const R& row, const Scale& scale, bool masses,
-                                          int from, int to, int tid) {
+__device__ __forceinline__ void histogram(Shared& s, const R& row, const Scale& scale, int from,
+                                          int to, int tid) {
   s.count[tid] = 0, s.mass[tid] = 0;
   __syncthreads();
   row.each(from, to, tid, kThreads, scale.bound(scale.least),
-           [&](int, float l) { count_in(s, scale, masses, l); });
+           [&](int, float l) { count_in(s, scale, l); }, [](int) {});
   __syncthreads();
 }
 
@@ -401,18 +414,19 @@ struct Plan {
   int sure;         // bins before it are kept whole
   int k_bin, p_first, p_last;  // of the cuts, -1 without one; the p cut's within a range
   uint32_t candidates;         // elements of those bins
+  uint32_t k_before, p_before;  // elements and masses ahead of k_bin and of p_last
+  u64 k_mass, p_mass;
   __device__ __forceinline__ bool has(int b) const { return b == k_bin || (b >= p_first && b <= p_last); }
 };
 
-__device__ __forceinline__ Plan no_plan() { return Plan{0, 0, false, false, kBins, -1, -1, -2, 0}; }
+__device__ __forceinline__ Plan no_plan() { return Plan{0, 0, false, false, kBins, -1, -1, -2, 0, 0, 0, 0, 0}; }
 
-__device__ __forceinline__ u64 p_mass(float p, u64 total) {
+__device__ __forceinline__ u64 p_target(float p, u64 total) {
   const double want = static_cast<double>(fmaxf(p, 0.0f)) * static_cast<double>(total);
   return min(max(static_cast<u64>(__builtin_ceil(want)), u64{1}), total);
 }
 
-// few: as in Request (the row's masses are not known then).
-__device__ __forceinline__ Plan make_plan(Shared& s, const Request& q, bool few, const Bin& bin, int tid) {
+__device__ __forceinline__ Plan make_plan(Shared& s, const Request& q, const Bin& bin, int tid) {
   Plan plan = no_plan();
   __syncthreads();
   if (tid == kThreads - 1) s.found_count = bin.count, s.found_mass = bin.mass;
@@ -426,27 +440,48 @@ __device__ __forceinline__ Plan make_plan(Shared& s, const Request& q, bool few,
     least = 0;
     plan.k_bin = find_bin(s, bin, Target{static_cast<uint32_t>(q.k), kNoMass}, before, least, tid);
     most = least + s.mass[plan.k_bin];
+    plan.k_before = before, plan.k_mass = least;
     plan.sure = plan.k_bin;
     plan.candidates = s.count[plan.k_bin];
   }
-  if (few) {
-    plan.p_first = 0, plan.p_last = plan.by_k ? plan.k_bin : kBins - 1;
-    plan.sure = 0;
-    plan.candidates = plan.by_k ? before + s.count[plan.k_bin] : plan.live;
-  } else if (plan.by_p) {
+  if (plan.by_p) {
     before = 0;
     u64 mass_before = 0;
-    plan.p_last = find_bin(s, bin, Target{kNoCount, p_mass(q.top_p, most)}, before, mass_before, tid);
+    plan.p_last = find_bin(s, bin, Target{kNoCount, p_target(q.top_p, most)}, before, mass_before, tid);
     const uint32_t until = before + s.count[plan.p_last];
+    plan.p_before = before, plan.p_mass = mass_before;
     if (plan.by_k) {
       before = 0, mass_before = 0;
-      plan.p_first = find_bin(s, bin, Target{kNoCount, p_mass(q.top_p, max(least, u64{1}))}, before, mass_before, tid);
+      plan.p_first = find_bin(s, bin, Target{kNoCount, p_target(q.top_p, max(least, u64{1}))}, before, mass_before, tid);
     } else {
       plan.p_first = plan.p_last;
     }
     plan.sure = plan.p_first;
     plan.candidates = until - before + (plan.k_bin > plan.p_last ? s.count[plan.k_bin] : 0u);
   }
+  return plan;
+}
+
+// The plan of a row with a small k.  `keys(i)` for i < n are the largest of disjoint parts of the row, so the
+// k-th largest of them is no larger than the k-th largest logit: all bins down to its bin are listed.
+template <typename K>
+__device__ __forceinline__ Plan few_plan(Shared& s, const Request& q, int n, const K& keys, int tid) {
+  s.count[tid] = 0, s.mass[tid] = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const double d = q.scale.below(value_of(keys(i)));
+    if (q.scale.live(d)) atomicAdd(&s.count[q.scale.bin(d)], 1u);
+  }
+  __syncthreads();
+  uint32_t before = 0;
+  u64 none = 0;
+  const int b = find_bin(s, scan_bins(s, s.count, s.mass, tid), Target{static_cast<uint32_t>(q.k), kNoMass}, before,
+                         none, tid);
+  Plan plan = no_plan();
+  plan.by_p = q.top_p < 1.0f;
+  plan.sure = 0;
+  plan.p_first = 0, plan.p_last = b < 0 ? kBins - 1 : b;  // fewer than k parts with weight: everything that has any
   return plan;
 }
 
@@ -462,82 +497,123 @@ __device__ __forceinline__ void pick(Shared& s, const R& row, const Scale& scale
   const bool gather = plan.candidates <= kList;
   const int lowest = plan.sure == kBins ? kBins - 1 : max(plan.k_bin, plan.p_last);
   const float low = fmaxf(scale.bound(scale.least), scale.bound(scale.edge(lowest)));
-  for (int i = first + wave; i < end; i += kWaves) {
-    u64 m = 0;
-    const int from = i * part, to = min(from + part, row.vecs);
-    row.each(from, to, lane, 64, low, [&](int at, float l) {
-      const double d = scale.below(l);
-      if (!scale.live(d)) return;
-      const int b = scale.bin(d);
-      if (b < plan.sure) {
-        m += scale.weight(d);
-      } else if (gather && plan.has(b)) {
-        const int to_list = atomicAdd(&s.listed, 1);
-        if (to_list < kList) s.key[to_list] = key_of(l), s.index[to_list] = at;
-      }
-    });
-    m = scan64(m);
-    if (lane == 63) s.part[i] = m;
-  }
+  // a wave's parts in one run, so that its loads stay in flight from one to the next
+  const int each_wave = ceil_div(end - first, kWaves), mine = first + wave * each_wave;
+  const int from = mine * part, to = min(min(mine + each_wave, end) * part, row.vecs);
+  if (lane < each_wave && mine + lane < end) s.part[mine + lane] = 0;
+  u64 m = 0;
+  row.each(from, to, lane, 64, low, [&](int at, float l) {
+    const double d = scale.below(l);
+    if (!scale.live(d)) return;
+    const int b = scale.bin(d);
+    if (b < plan.sure) {
+      m += scale.weight(d);
+    } else if (gather && plan.has(b)) {
+      const int to_list = atomicAdd(&s.listed, 1);
+      if (to_list < kList) s.key[to_list] = key_of(l), s.index[to_list] = at;
+    }
+  }, [&](int base) {
+    if ((base + 64 - from) % part != 0 && base + 64 < to) return;
+    const u64 sum = scan64(m);
+    if (lane == 63) s.part[base / part] = sum;
+    m = 0;
+  });
   __syncthreads();
 }
 
-// Where a cut falls in bin `bin`, of which before and mass_before lie ahead.  each(f) calls f(key, index)
+// Where a cut falls among n <= kPairs elements of which mine() are meant: each against all others, four
+// threads to one, a fourth of them each.
+template <typename M>
+__device__ __forceinline__ Cut resolve_pairs(Shared& s, const uint32_t* key, const int32_t* index, int n, const M& mine,
+                                             const Scale& scale, const Target& t, uint32_t before, u64 mass_before,
+                                             int tid) {
+  const int own = tid >> 2, quarter = tid & 3;
+  const uint32_t k = key[min(own, n - 1)];
+  const int i = index[min(own, n - 1)];
+  const bool ours = own < n && mine(k, i);
+  const u64 at = ours ? place(value_of(k), i) : 0;  // 0: not meant, or past the last: ahead of nothing
+  const u64 w = ours ? scale.weight(scale.below(value_of(k))) : 0;
+  __syncthreads();
+  if (quarter == 0) s.fine_mass[2 * own] = at, s.fine_mass[2 * own + 1] = w;
+  __syncthreads();
+  uint32_t c = 0;
+  u64 m = 0;
+  const int n4 = (n + 3) >> 2;
+#pragma unroll 8
+  for (int j = 0; j < n4; ++j) {
+    const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&s.fine_mass[2 * (4 * j + quarter)]);
+    const bool ahead = other.x > at;
+    c += ahead ? 1u : 0u, m += ahead ? other.y : 0;
+  }
+  c += dpp<0xB1, 0xF>(c), m += dpp64<0xB1>(m);
+  c += dpp<0x4E, 0xF>(c), m += dpp64<0x4E>(m);
+  before += c, mass_before += m;
+  if (ours && quarter == 0 && before < t.count && mass_before < t.mass &&
+      (before + 1 >= t.count || mass_before + w >= t.mass))
+    s.found = own, s.found_mass = mass_before + w;
+  __syncthreads();
+  const Cut cut{key[s.found], index[s.found], s.found_mass};
+  __syncthreads();
+  return cut;
+}
+
+// Where a cut falls in bin `bin` (-1: among all candidates), of which before and mass_before lie ahead.  each(f) calls f(key, index)
 // for the candidates, `listed` of them from the list (more than it holds: from the row).
 template <typename E>
 __device__ Cut resolve(Shared& s, const E& each, int listed, const Scale& scale, const Target& t, int bin,
                        uint32_t before, u64 mass_before, const Cut& inside, int tid) {
   const auto mine = [&](uint32_t k, int i) {
-    return scale.bin(scale.below(value_of(k))) == bin && inside.keeps(k, i);
+    return (bin < 0 || scale.bin(scale.below(value_of(k))) == bin) && inside.keeps(k, i);
   };
-  Cut cut;
-  if (listed <= kPairs) {
-    // each element against all others, four threads to one: a fourth of them each
-    const int own = tid >> 2, quarter = tid & 3;
-    const uint32_t k = s.key[min(own, listed - 1)];
-    const int i = s.index[min(own, listed - 1)];
-    const bool ours = own < listed && mine(k, i);
-    const u64 w = ours ? scale.weight(scale.below(value_of(k))) : 0;
+  if (listed <= kPairs)
+    return resolve_pairs(s, s.key, s.index, listed, mine, scale, t, before, mass_before, tid);
+  // the bin in 512 steps of its logarithm (all candidates: by their bins), and the elements of the one step
+  const auto step_of = [&](uint32_t k) {
+    const double d = scale.below(value_of(k));
+    return bin < 0 ? scale.bin(d) : min(kBins - 1, max(0, static_cast<int>((scale.position(d) - bin) * kBins)));
+  };
+  __syncthreads();
+  s.fine_count[tid] = 0, s.fine_mass[tid] = 0;
+  if (tid == 0) s.last = 0;
+  __syncthreads();
+  each([&](uint32_t k, int i) {
+    if (!mine(k, i)) return;
+    const int b = step_of(k);
+    atomicAdd(&s.fine_count[b], 1u);
+    atomicAdd(&s.fine_mass[b], scale.weight(scale.below(value_of(k))));
+  });
+  __syncthreads();
+  const int step = find_bin(s, scan_bins(s, s.fine_count, s.fine_mass, tid), t, before, mass_before, tid);
+  const int left = static_cast<int>(s.fine_count[step]);
+  __syncthreads();
+  if (left <= kPairs) {
+    uint32_t* key = s.fine_count;
+    int32_t* index = reinterpret_cast<int32_t*>(s.fine_count + kPairs);
+    each([&](uint32_t k, int i) {
+      if (!mine(k, i) || step_of(k) != step) return;
+      const int at = atomicAdd(&s.last, 1);
+      key[at] = k, index[at] = i;
+    });
     __syncthreads();
-    if (quarter == 0) s.fine_mass[own] = w;  // 0: not in this bin, or past the last
-    __syncthreads();
-    uint32_t c = 0;
-    u64 m = 0;
-    const int n4 = (listed + 3) >> 2;
-#pragma unroll 4
-    for (int j = 0; j < n4; ++j) {
-      const int at = 4 * j + quarter;  // below kPairs, where the list has places
-      const uint32_t kj = s.key[at];
-      const u64 wj = s.fine_mass[at];
-      const bool ahead = wj && (kj > k || (kj == k && s.index[at] < i));
-      c += ahead ? 1u : 0u, m += ahead ? wj : 0;
-    }
-    c += dpp<0xB1, 0xF>(c), m += dpp64<0xB1>(m);
-    c += dpp<0x4E, 0xF>(c), m += dpp64<0x4E>(m);
-    before += c, mass_before += m;
-    if (ours && quarter == 0 && before < t.count && mass_before < t.mass &&
-        (before + 1 >= t.count || mass_before + w >= t.mass))
-      s.found = own, s.found_mass = mass_before + w;
-    __syncthreads();
-    cut.key = s.key[s.found], cut.index = s.index[s.found], cut.mass = s.found_mass;
-    __syncthreads();
-    return cut;
+    return resolve_pairs(s, key, index, left, [](uint32_t, int) { return true; }, scale, t, before, mass_before, tid);
   }
+  // many equal or nearly so
+  Cut cut;
   u64 up = 0, down = 0;
   each([&](uint32_t k, int i) {
-    if (mine(k, i)) up = max(up, static_cast<u64>(k)), down = max(down, static_cast<u64>(~k));
+    if (mine(k, i) && step_of(k) == step) up = max(up, static_cast<u64>(k)), down = max(down, static_cast<u64>(~k));
   });
   uint32_t hi = static_cast<uint32_t>(block_max(s, up, tid));
   uint32_t lo = ~static_cast<uint32_t>(block_max(s, down, tid));
   uint32_t ties = 0;
-  while (true) {  // the range falls to a 1024th each time
+  while (true) {  // the range falls to a 512th each time
     int shift = 0;
     while (((hi - lo) >> shift) >= kBins) ++shift;
     __syncthreads();
     s.fine_count[tid] = 0, s.fine_mass[tid] = 0;
     __syncthreads();
     each([&](uint32_t k, int i) {
-      if (k < lo || k > hi || !mine(k, i)) return;
+      if (k < lo || k > hi || !mine(k, i)) return;  // (of this step: lo and hi are)
       const uint32_t b = (hi - k) >> shift;
       atomicAdd(&s.fine_count[b], 1u);
       atomicAdd(&s.fine_mass[b], scale.weight(scale.below(value_of(k))));
@@ -589,10 +665,10 @@ __device__ __forceinline__ void again(Shared& s, const R& row, const Request& q,
   s.count[tid] = 0, s.mass[tid] = 0;
   if (tid < parts) s.part[tid] = 0;
   __syncthreads();
-  row.each_plain(tid, kThreads, low, [&](int, float l) { count_in(s, q.scale, true, l); });
+  row.each_plain(tid, kThreads, low, [&](int, float l) { count_in(s, q.scale, l); });
   __syncthreads();
   bin = scan_bins(s, s.count, s.mass, tid);
-  plan = make_plan(s, q, false, bin, tid);
+  plan = make_plan(s, q, bin, tid);
   if (tid == 0) s.listed = 0;
   __syncthreads();
   row.each_plain(tid, kThreads, low, [&](int i, float l) {
@@ -615,7 +691,9 @@ __device__ __forceinline__ void finish(Shared& s, const SampleArgs& p, int row_i
                                        Plan plan, Bin bin, int part, int parts, int tid) {
   const Scale& scale = q.scale;
   const bool few = q.few && plan.candidates <= kList;
-  if (q.few && !few) again(s, row, q, plan, bin, part, parts, tid);
+  // (fewer than k listed are all that have weight; k or more may not be)
+  if (few) plan.by_k = plan.candidates >= static_cast<uint32_t>(q.k);
+  else if (q.few) again(s, row, q, plan, bin, part, parts, tid);
   const int listed = static_cast<int>(plan.candidates);
   const auto each = [&](auto f) {
     // one loop for both, so that f is there once
@@ -638,12 +716,13 @@ __device__ __forceinline__ void finish(Shared& s, const SampleArgs& p, int row_i
   Cut cut{0, 0x7fffffff, plan.total};
 #pragma unroll 1
   for (int which = plan.by_k ? 0 : 1; which < (plan.by_p ? 2 : 1); ++which) {  // the k cut, the p cut
-    if (which == 1 && few) {  // the masses of what is left
+    const bool pairs = few && plan.by_k && listed <= kPairs;  // the k cut has summed up what it leaves
+    if (which == 1 && few && !pairs) {  // the masses of what is left
       __syncthreads();
       s.count[tid] = 0, s.mass[tid] = 0;
       __syncthreads();
       each([&](uint32_t k, int i) {
-        if (cut.keeps(k, i)) count_in(s, scale, true, value_of(k));
+        if (cut.keeps(k, i)) count_in(s, scale, value_of(k));
       });
       __syncthreads();
       bin = scan_bins(s, s.count, s.mass, tid);
@@ -651,10 +730,14 @@ __device__ __forceinline__ void finish(Shared& s, const SampleArgs& p, int row_i
       __syncthreads();
       cut.mass = s.found_mass;
     }
-    const Target t = which == 0 ? Target{static_cast<uint32_t>(q.k), kNoMass} : Target{kNoCount, p_mass(q.top_p, cut.mass)};
-    uint32_t before = 0;
-    u64 mass_before = 0;
-    const int b = find_bin(s, bin, t, before, mass_before, tid);
+    const Target t = which == 0 ? Target{static_cast<uint32_t>(q.k), kNoMass} : Target{kNoCount, p_target(q.top_p, cut.mass)};
+    uint32_t before = which == 0 ? plan.k_before : plan.p_before;
+    u64 mass_before = which == 0 ? plan.k_mass : plan.p_mass;
+    int b = which == 0 ? plan.k_bin : plan.p_last;  // (few: -1, nothing ahead)
+    if (which == 1 && (few || plan.by_k)) {
+      before = 0, mass_before = 0;
+      b = pairs ? -1 : find_bin(s, bin, t, before, mass_before, tid);
+    }
     cut = resolve(s, each, listed, scale, t, b, before, mass_before, cut, tid);
   }
   if (plan.sure < kBins) {
@@ -711,65 +794,35 @@ __device__ __forceinline__ void finish(Shared& s, const SampleArgs& p, int row_i
   }
 }
 
-template <typename T, bool kTiny = false>
-__device__ __forceinline__ Row<T, kTiny> row_of(const SampleArgs& p, int row) {
-  return Row<T, kTiny>(static_cast<const T*>(p.logits) + row * p.stride, p.vocab);
+template <typename T>
+__device__ __forceinline__ Row<T> row_of(const SampleArgs& p, int row) {
+  return Row<T>(static_cast<const T*>(p.logits) + row * p.stride, p.vocab);
 }
 
-template <typename R>
-__device__ __forceinline__ u64 best_of(Shared& s, const R& row, int from, int to, int tid) {
-  return block_max(s, row.best(from, to, tid, kThreads), tid);
+__device__ __forceinline__ void write_settled(const SampleArgs& p, const Request& q, int row, u64 best) {
+  if (q.none) write(p, row, -1, -__builtin_inff());
+  else write(p, row, static_cast<int>(0xffffffffu - static_cast<uint32_t>(best)), 0.0f);
 }
 
-__device__ __forceinline__ bool settled(const SampleArgs& p, const Request& q, int row, u64 best, bool writes) {
-  if (!q.none && !q.first) return false;
-  if (writes) write(p, row, q.none ? -1 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(best)), q.none ? -__builtin_inff() : 0.0f);
-  return true;
-}
-
-// A workgroup a row.
-template <typename T, bool kTiny>
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs p, int part, int parts) {
-  __shared__ Shared s;
-  const int tid = threadIdx.x, row_id = blockIdx.x;
-  const auto row = row_of<T, kTiny>(p, row_id);
-  const u64 best = best_of(s, row, 0, row.vecs, tid);
-  const Request q = request(p, row_id, best);
-  if (settled(p, q, row_id, best, tid == 0)) return;
-  Plan plan = no_plan();
-  Bin bin{};
-  if (q.cuts()) {
-    histogram(s, row, q.scale, !q.few, 0, row.vecs, tid);
-    bin = scan_bins(s, s.count, s.mass, tid);
-    plan = make_plan(s, q, q.few, bin, tid);
-  }
-  pick(s, row, q.scale, plan, part, 0, parts, tid);
-  finish(s, p, row_id, row, q, plan, bin, part, parts, tid);
-}
-
-// Few rows: several workgroups a row, and three launches.  What they hand on, for each row:
+// Four launches, of several workgroups (splits) a row where there are few rows:
+//   best       the first of the order in each split, and each thread's largest
+//   scan       rows with a small k: the list; rows without cuts: the parts' masses; others: the histogram
+//   pick       those others: the list and the parts' masses
+//   finish     the cuts and the draw, a workgroup a row
+// What they hand on, for each row:
 struct Hand {
-  u64 best[kMaxSplit];        // launch 1: the first of the order in each split
-  uint32_t listed, done;      // launch 3: elements in the list, workgroups that have ended
+  u64 best[kMaxSplit];
+  Request request;  // from scan on
+  Plan plan;
+  uint32_t listed;
   u64 part[kMaxParts];
   uint32_t key[kList];
   int32_t index[kList];
 };
-struct Histogram {  // launch 2, of each split
+struct Histogram {  // of each split; before scan its threads' largest keys
   u64 mass[kBins];
   uint32_t count[kBins];
 };
-
-// Between workgroups of a launch: device-coherent (the L2 is per XCD).
-template <typename V>
-__device__ __forceinline__ void store_coherent(V* p, V v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-template <typename V>
-__device__ __forceinline__ V load_coherent(const V* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 struct SplitArgs {
   SampleArgs p;
   Hand* hand;
@@ -784,11 +837,13 @@ __global__ __launch_bounds__(kThreads) void sample_best_kernel(SplitArgs a) {
   const Row<T> row = row_of<T>(a.p, row_id);
   const int per = a.parts / a.splits * a.part;
   const int from = split * per, to = min(from + per, row.vecs);
-  const u64 best = best_of(s, row, from, to, tid);
+  const u64 own = row.best(from, to, tid, kThreads);
+  a.hist[static_cast<long long>(row_id) * a.splits + split].count[tid] = static_cast<uint32_t>(own >> 32);
+  const u64 best = block_max(s, own, tid);
   Hand& h = a.hand[row_id];
   if (tid == 0) {
     h.best[split] = best;
-    if (split == 0) h.listed = 0, h.done = 0;
+    if (split == 0) h.listed = 0;
   }
 }
 
@@ -799,81 +854,115 @@ __device__ __forceinline__ u64 best_of(const Hand& h, int splits) {
   return best;
 }
 
+// A split's share of the list and of the parts' masses.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_histogram_kernel(SplitArgs a) {
-  __shared__ Shared s;
-  const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
-  const Row<T> row = row_of<T>(a.p, row_id);
-  const u64 best = best_of(a.hand[row_id], a.splits);
-  const Request q = request(a.p, row_id, best);
-  if (settled(a.p, q, row_id, best, split == 0 && tid == 0) || !q.cuts()) return;
-  const int per = a.parts / a.splits * a.part;
-  const int from = split * per, to = min(from + per, row.vecs);
-  histogram(s, row, q.scale, !q.few, from, to, tid);
-  Histogram& h = a.hist[static_cast<long long>(row_id) * a.splits + split];
-  h.count[tid] = s.count[tid];
-  if (!q.few) h.mass[tid] = s.mass[tid];
+__device__ __forceinline__ void hand_over(Shared& s, const SplitArgs& a, Hand& hand, const Row<T>& row, const Request& q,
+                                          const Plan& plan, int split, int tid) {
+  const int per = a.parts / a.splits, first = split * per;
+  pick(s, row, q.scale, plan, a.part, first, first + per, tid);
+  if (tid < per) hand.part[first + tid] = s.part[first + tid];
+  const int listed = s.listed;
+  if (listed == 0) return;
+  if (tid == 0) s.last = static_cast<int>(atomicAdd(&hand.listed, static_cast<uint32_t>(listed)));
+  __syncthreads();
+  for (int i = tid; i < min(listed, kList) && s.last + i < kList; i += kThreads)
+    hand.key[s.last + i] = s.key[i], hand.index[s.last + i] = s.index[i];
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SplitArgs a) {
+__global__ __launch_bounds__(kThreads) void sample_scan_kernel(SplitArgs a) {
   __shared__ Shared s;
   const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
   const Row<T> row = row_of<T>(a.p, row_id);
   Hand& hand = a.hand[row_id];
   const u64 best = best_of(hand, a.splits);
-  const Request q = request(a.p, row_id, best);
-  if (settled(a.p, q, row_id, best, false)) return;  // launch 2 has written it
-  Plan plan = no_plan();
+  const Request q = request(a.p, row_id, best, a.splits);
+  const bool writes = split == 0 && tid == 0;
+  if (writes) hand.request = q;
+  if (q.settled()) {
+    if (writes) write_settled(a.p, q, row_id, best);
+    return;
+  }
+  Histogram* h = a.hist + static_cast<long long>(row_id) * a.splits;
+  if (q.cuts() && !q.few) {
+    const int per = a.parts / a.splits * a.part;
+    const int from = split * per, to = min(from + per, row.vecs);
+    histogram(s, row, q.scale, from, to, tid);
+    h[split].count[tid] = s.count[tid], h[split].mass[tid] = s.mass[tid];
+    return;
+  }
+  const Plan plan = q.few ? few_plan(s, q, a.splits, [&](int i) { return h[i].count[tid]; }, tid) : no_plan();
+  if (writes) hand.plan = plan;
+  hand_over(s, a, hand, row, q, plan, split, tid);
+}
+
+// The row's histogram, and the plan that follows from it.
+__device__ __forceinline__ Plan planned(Shared& s, const SplitArgs& a, int row_id, const Request& q, Bin& bin,
+                                        int tid) {
+  const Histogram* h = a.hist + static_cast<long long>(row_id) * a.splits;
+  uint32_t c = 0;
+  u64 m = 0;
+#pragma unroll 1
+  for (int i = 0; i < a.splits; i += 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // four in flight
+      const Histogram& from = h[min(i + j, a.splits - 1)];
+      const uint32_t count = from.count[tid];
+      const u64 mass = from.mass[tid];
+      if (i + j < a.splits) c += count, m += mass;
+    }
+  }
+  s.count[tid] = c, s.mass[tid] = m;
+  __syncthreads();
+  bin = scan_bins(s, s.count, s.mass, tid);
+  return make_plan(s, q, bin, tid);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_pick_kernel(SplitArgs a) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
+  const Row<T> row = row_of<T>(a.p, row_id);
+  Hand& hand = a.hand[row_id];
+  const Request q = hand.request;
+  if (q.settled() || !q.cuts() || q.few) return;
   Bin bin{};
-  if (q.cuts()) {
-    const Histogram* h = a.hist + static_cast<long long>(row_id) * a.splits;
-    uint32_t c[kMaxSplit];
-    u64 m[kMaxSplit];
+  const Plan plan = planned(s, a, row_id, q, bin, tid);
+  if (split == 0 && tid == 0) hand.plan = plan;
+  hand_over(s, a, hand, row, q, plan, split, tid);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SplitArgs a) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, row_id = blockIdx.x;
+  const Row<T> row = row_of<T>(a.p, row_id);
+  const Hand& hand = a.hand[row_id];
+  const Request q = hand.request;
+  if (q.settled()) return;
+  Plan plan = hand.plan;
+  if (q.few) plan.candidates = hand.listed;
+  Bin bin{};
+  if (plan.by_k && plan.by_p && !q.few) planned(s, a, row_id, q, bin, tid);  // the p cut's bin follows from the k cut
+  if (tid < a.parts) s.part[tid] = hand.part[tid];
+  if (plan.candidates <= kList) {
+    const int n = static_cast<int>(plan.candidates);
+#pragma unroll 1
+    for (int i = tid; i < n; i += 4 * kThreads) {
+      uint32_t k[4];
+      int32_t at[4];
 #pragma unroll
-    for (int i = 0; i < kMaxSplit; ++i)  // all in flight
-      if (i < a.splits) c[i] = h[i].count[tid], m[i] = q.few ? 0 : h[i].mass[tid];
-      else c[i] = 0, m[i] = 0;
+      for (int j = 0; j < 4; ++j) k[j] = hand.key[min(i + j * kThreads, n - 1)], at[j] = hand.index[min(i + j * kThreads, n - 1)];
 #pragma unroll
-    for (int i = 1; i < kMaxSplit; ++i) c[0] += c[i], m[0] += m[i];
-    s.count[tid] = c[0], s.mass[tid] = m[0];
-    __syncthreads();
-    bin = scan_bins(s, s.count, s.mass, tid);
-    plan = make_plan(s, q, q.few, bin, tid);
-  }
-  const int per = a.parts / a.splits, first = split * per;
-  pick(s, row, q.scale, plan, a.part, first, first + per, tid);
-  if (tid < per) store_coherent(&hand.part[first + tid], s.part[first + tid]);
-  const int listed = min(s.listed, kList);
-  if (listed > 0) {
-    if (tid == 0)
-      s.last = static_cast<int>(__hip_atomic_fetch_add(&hand.listed, static_cast<uint32_t>(listed),
-                                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    __syncthreads();
-    for (int i = tid; i < listed && s.last + i < kList; i += kThreads) {
-      store_coherent(&hand.key[s.last + i], s.key[i]);
-      store_coherent(&hand.index[s.last + i], s.index[i]);
+      for (int j = 0; j < 4; ++j)
+        if (i + j * kThreads < n) s.key[i + j * kThreads] = k[j], s.index[i + j * kThreads] = at[j];
     }
   }
-  // every store has completed before the workgroup counts itself in; the row's last one goes on
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (tid == 0)
-    s.found = __hip_atomic_fetch_add(&hand.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u ==
-              static_cast<uint32_t>(a.splits);
-  __syncthreads();
-  if (!s.found) return;
-  if (tid < a.parts) s.part[tid] = load_coherent(&hand.part[tid]);
-  if (plan.candidates <= kList)
-    for (int i = tid; i < static_cast<int>(plan.candidates); i += kThreads) {
-      s.key[i] = load_coherent(&hand.key[i]);
-      s.index[i] = load_coherent(&hand.index[i]);
-    }
   __syncthreads();
   finish(s, a.p, row_id, row, q, plan, bin, a.part, a.parts, tid);
 }
 
-// Workgroups a row: rows that fill the card by themselves take one.
+// Workgroups a row.
 int splits_of(int rows, int vocab) {
   int n = 1;
   while (n < kMaxSplit && 2 * n * rows <= kWorkgroups && vocab / (2 * n) >= kThreads) n *= 2;
@@ -881,24 +970,26 @@ int splits_of(int rows, int vocab) {
 }
 
 template <typename T>
-void launch(const SampleArgs& p, void* workspace, hipStream_t stream) {
-  const int splits = splits_of(p.rows, p.vocab);
-  const dim3 grid(splits, p.rows), block(kThreads);
-  const bool tiny = p.vocab < Row<T>::kVec;
-  // parts of whole rounds of a wave's loads, a multiple of `splits` in number
-  const int vecs = ceil_div(p.vocab, tiny ? Row<T, true>::kVec : Row<T>::kVec), round = 64 * kFlight;
-  const int part = round * ceil_div(vecs, round * kMaxParts);
-  const int parts = splits * ceil_div(ceil_div(vecs, part), splits);
-  if (splits == 1) {
-    const auto kernel = tiny ? sample_row_kernel<T, true> : sample_row_kernel<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(p.rows), block, 0, stream, p, part, parts);
-    return;
+void launch(SampleArgs p, void* workspace, hipStream_t stream) {
+  for (int left = p.rows; left > 0; left -= kMaxRows) {
+    p.rows = left < kMaxRows ? left : kMaxRows;
+    const int splits = splits_of(p.rows, p.vocab);
+    // parts of whole rounds of a wave, a multiple of `splits` in number
+    const int vecs = ceil_div(p.vocab, Row<T>::kVec), round = 64;
+    const int part = round * ceil_div(vecs, round * kMaxParts);
+    const int parts = splits * ceil_div(ceil_div(vecs, part), splits);
+    const dim3 grid(splits, p.rows), block(kThreads);
+    Hand* hand = static_cast<Hand*>(workspace);
+    const SplitArgs a{p, hand, reinterpret_cast<Histogram*>(hand + p.rows), splits, part, parts};
+    hipLaunchKernelGGL(sample_best_kernel<T>, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(sample_scan_kernel<T>, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(sample_pick_kernel<T>, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(sample_finish_kernel<T>, dim3(p.rows), block, 0, stream, a);
+    p.logits = static_cast<const T*>(p.logits) + kMaxRows * p.stride;
+    p.u += kMaxRows, p.temperature += kMaxRows, p.top_p += kMaxRows, p.min_p += kMaxRows, p.top_k += kMaxRows;
+    p.tokens += kMaxRows;
+    if (p.logprobs) p.logprobs += kMaxRows;
   }
-  const SplitArgs a{p, static_cast<Hand*>(workspace),
-                    reinterpret_cast<Histogram*>(static_cast<Hand*>(workspace) + p.rows), splits, part, parts};
-  hipLaunchKernelGGL(sample_best_kernel<T>, grid, block, 0, stream, a);
-  hipLaunchKernelGGL(sample_histogram_kernel<T>, grid, block, 0, stream, a);
-  hipLaunchKernelGGL(sample_draw_kernel<T>, grid, block, 0, stream, a);
 }
 
 }  // namespace
@@ -908,8 +999,8 @@ using namespace pega;
 
 PEGA_API long long pega_sample_workspace_bytes(int rows, int vocab) {
   if (rows <= 0 || vocab <= 0) return 0;
-  // of the batches up to `rows` that are split, the most rows and the most splits
-  const long long most = rows < kWorkgroups / 2 ? rows : kWorkgroups / 2;
+  // for any batch up to `rows`: the most rows, and the most histograms
+  const long long most = rows < kMaxRows ? rows : kMaxRows;
   const long long hists = most * kMaxSplit < kWorkgroups ? most * kMaxSplit : kWorkgroups;
   return most * static_cast<long long>(sizeof(Hand)) + hists * static_cast<long long>(sizeof(Histogram));
 }
@@ -944,7 +1035,10 @@ PEGA_API int pega_sample_tokens(const void* logits, bool logits_bf16, long long 
       if (overlap(outs[o].p, outs[o].bytes, outs[i].p, outs[i].bytes))
         return fail(kInvalidValue, "sample_tokens: two outputs overlap");
   }
-  const SampleArgs p{logits, row_stride, rows, vocab, uniform, temperature, top_p, min_p, top_k, tokens, logprobs};
+  const auto there = [&](const float* v) { return v ? v : uniform; };
+  const SampleArgs p{logits, row_stride, rows, vocab, uniform, there(temperature), there(top_p), there(min_p),
+                     top_k ? top_k : reinterpret_cast<const int32_t*>(uniform), tokens, logprobs,
+                     temperature != nullptr, top_p != nullptr, min_p != nullptr, top_k != nullptr};
   if (logits_bf16) launch<uint16_t>(p, workspace, stream);
   else launch<float>(p, workspace, stream);
   return launch_status("sample_tokens");
