@@ -321,7 +321,7 @@ __global__ __launch_bounds__(S::kThreads) void w4_tile_kernel(W4Args p) {
 #pragma unroll
   for (int j = 0; j < S::PX; ++j) {
     const int i = min(wave * S::PX + j, S::kXLoads - 1);
-    const int r = 4 * i + (lane >> 4), piece = (lane & 15) ^ (r & 7);
+    const int r = 4 * i + (lane >> 4), piece = (lane & 15) ^ (r & 15);
     x_dst[j] = lds0 + 1024u * static_cast<uint32_t>(i);
     x_col[j] = 8 * piece;
     x_voff[j] = static_cast<uint32_t>(r) * x_row + 16u * static_cast<uint32_t>(piece);
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(S::kThreads) void w4_tile_kernel(W4Args p) {
     Rows x;
     const uint8_t* xl = smem + at + (16 * b + c) * 256;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x.v[j] = *reinterpret_cast<const u32x4_t*>(xl + 16 * ((4 * j + h) ^ (c & 7)));
+    for (int j = 0; j < 4; ++j) x.v[j] = *reinterpret_cast<const u32x4_t*>(xl + 16 * ((4 * j + h) ^ c));
     return x;
   };
   // a step's group sums of X, row blocks in turn by wave: block `wave` + i kWaves
