@@ -381,8 +381,8 @@ __global__ __launch_bounds__(S::kThreads) void w4_tile_kernel(W4Args p) {
       floatx4_t sum = {};
 #pragma unroll
       for (int j = g * kJ; j < (g + 1) * kJ; ++j) sum = mfma(x.v[j], ones, sum);
-      // the same in all 16 columns
-      if (c == 0 && b < S::BN / 16)
+      // the same in all 16 columns, which all write it: no branch cuts the step in two
+      if (S::BN / 16 % S::kWaves == 0 || b < S::BN / 16)
         *reinterpret_cast<floatx4_t*>(smem + sums + 4 * (g * S::BN + 16 * b + 4 * h)) = sum;
     }
   };
