@@ -983,7 +983,7 @@ void launch(SampleArgs p, void* workspace, hipStream_t stream) {
     const SplitArgs a{p, hand, reinterpret_cast<Histogram*>(hand + p.rows), splits, part, parts};
     hipLaunchKernelGGL(sample_best_kernel<T>, grid, block, 0, stream, a);
     hipLaunchKernelGGL(sample_scan_kernel<T>, grid, block, 0, stream, a);
-    hipLaunchKernelGGL(sample_pick_kernel<T>, grid, block, 0, stream, a);
+    if (p.has_top_k || p.has_top_p) hipLaunchKernelGGL(sample_pick_kernel<T>, grid, block, 0, stream, a);
     hipLaunchKernelGGL(sample_finish_kernel<T>, dim3(p.rows), block, 0, stream, a);
     p.logits = static_cast<const T*>(p.logits) + kMaxRows * p.stride;
     p.u += kMaxRows, p.temperature += kMaxRows, p.top_p += kMaxRows, p.min_p += kMaxRows, p.top_k += kMaxRows;

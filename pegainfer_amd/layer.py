@@ -226,24 +226,37 @@ class KimiSharedExpert:
     (dense_w13_swiglu, the same bits as the reference's two calls); from
     PREFILL_TOKENS tokens the reference's prefill sequence runs instead
     (moe_nccl.rs:266-275): the gate/up GEMM into [T, 2I] (gemm_graphsafe, which
-    takes hipBLASLt at those sizes), the SwiGLU kernel, the down GEMM."""
+    takes hipBLASLt at those sizes), the SwiGLU kernel, the down GEMM.
+    With 4-bit projections (a pair of ops.W4Weight, no reference counterpart) every
+    size runs that sequence on ops.w4_gemm."""
 
     PREFILL_TOKENS = 256
 
-    def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, *, max_tokens: int,
-                 device="cuda"):
-        assert gate_up.dim() == 2 and down.dim() == 2
-        self.gate_up, self.down = gate_up.contiguous(), down.contiguous()
-        self.I = gate_up.shape[0] // 2
-        self.H = gate_up.shape[1]
-        assert tuple(down.shape) == (self.H, self.I)
+    def __init__(self, gate_up, down, *, max_tokens: int, device="cuda"):
+        self.w4 = isinstance(gate_up, ops.W4Weight)
+        if self.w4:
+            if not isinstance(down, ops.W4Weight):
+                raise ValueError("a 4-bit gate/up projection needs a 4-bit down projection")
+            self.gate_up, self.down = gate_up, down
+            (two_i, self.H), down_shape = ((w.out_dim, w.in_dim) for w in (gate_up, down))
+        else:
+            assert gate_up.dim() == 2 and down.dim() == 2
+            self.gate_up, self.down = gate_up.contiguous(), down.contiguous()
+            (two_i, self.H), down_shape = gate_up.shape, tuple(down.shape)
+        self.I = two_i // 2
+        assert two_i % 2 == 0 and down_shape == (self.H, self.I)
         bf = dict(dtype=torch.bfloat16, device=device)
         self.act = torch.zeros(max_tokens, self.I, **bf)
         self.h13 = (torch.zeros(max_tokens, 2 * self.I, **bf)
-                    if max_tokens >= self.PREFILL_TOKENS else None)
+                    if self.w4 or max_tokens >= self.PREFILL_TOKENS else None)
 
     def forward(self, normed: torch.Tensor, projected: torch.Tensor) -> torch.Tensor:
         T = normed.shape[0]
+        if self.w4:
+            ops.w4_gemm(self.gate_up, normed, self.h13[:T])
+            ops.kimi_marlin_w13_swiglu(self.h13[:T], self.act[:T], T, self.I)
+            ops.w4_gemm(self.down, self.act[:T], projected)
+            return projected
         if T >= self.PREFILL_TOKENS:
             ops.gemm_graphsafe(self.gate_up, normed, self.h13[:T])
             ops.kimi_marlin_w13_swiglu(self.h13[:T], self.act[:T], T, self.I)
@@ -284,12 +297,15 @@ class KimiMoeDecodeLayer:
     few_tokens: batches of up to that many tokens (at most ops.FEW_TOKENS_MAX) take the
     two-launch form instead, ops.moe_few_tokens, which rounds less in between (the INT4
     weights' products, the routed rows and the joins stay fp32), so its bits differ.  Sizes
-    that it does not take (ops.FewTokensWorkspace) are refused here."""
+    that it does not take (ops.FewTokensWorkspace) and a shared expert of ops.W4Weight
+    projections are refused here."""
 
     def __init__(self, routed: RoutedExperts, shared: KimiSharedExpert, *, n_experts: int = 384,
                  device="cuda", few_tokens: int = 0):
         self.routed, self.shared = routed, shared
         T, H = routed.max_tokens, routed.H
+        if few_tokens and shared.w4:
+            raise ValueError("the two-launch form takes no shared expert of W4Weight projections")
         self.few_ws = few_workspace(routed, shared.I, few_tokens, device)
         self.projected = torch.zeros(T, H, dtype=torch.bfloat16, device=device)
         self.routed_f32 = torch.zeros(T, H, dtype=torch.float32, device=device)
@@ -313,6 +329,42 @@ class KimiMoeDecodeLayer:
         ops.kimi_residual_add_scaled_f32(hidden, projected, routed_f32, ops.KIMI_K2_ROUTER_SCALE,
                                          out)
         return out
+
+
+class TokenHead:
+    """The end of a decode step (no reference counterpart here): the last block's output joins the
+    residual between its two norms (ops.sandwich_rmsnorm), the normed sum goes through a head
+    with 4-bit weights into fp32 logits (ops.w4_gemm), and a token of each row is drawn
+    (ops.sample_tokens).  Every buffer is allocated in the constructor; `forward` only enqueues
+    kernels on the current stream."""
+
+    def __init__(self, head: ops.W4Weight, final_norm: torch.Tensor, *, max_rows: int, eps: float,
+                 post_norm: torch.Tensor = None, unit_offset: bool = False, device="cuda"):
+        """final_norm: the norm in front of the head; post_norm: the one behind the last block, if
+        the model has it; unit_offset: both are stored less one."""
+        if final_norm.numel() != head.in_dim:
+            raise ValueError(f"the head takes rows of {head.in_dim}, the norm has {final_norm.numel()}")
+        self.head, self.final_norm, self.post_norm = head, final_norm, post_norm
+        self.max_rows, self.eps, self.unit_offset = max_rows, eps, unit_offset
+        self.normed = torch.zeros(max_rows, head.in_dim, dtype=torch.bfloat16, device=device)
+        self.logits = torch.zeros(max_rows, head.out_dim, dtype=torch.float32, device=device)
+        self.sample_ws = ops.SampleWorkspace(max_rows, head.out_dim, device=device)
+
+    def forward(self, x: torch.Tensor, residual, uniform: torch.Tensor, tokens: torch.Tensor, *,
+                gate: torch.Tensor = None, residual_scale: float = 1.0,
+                logprobs: torch.Tensor = None, **draw) -> torch.Tensor:
+        """tokens[r] for the rows of x (the last block's output).  draw: temperature, top_k, top_p,
+        min_p as ops.sample_tokens takes them.  The logits stay in self.logits[:rows]."""
+        rows = x.shape[0]
+        if rows > self.max_rows:
+            raise ValueError(f"{rows} rows exceed the head's {self.max_rows}")
+        normed, logits = self.normed[:rows], self.logits[:rows]
+        ops.sandwich_rmsnorm(x, residual, self.final_norm, self.eps, post_weight=self.post_norm,
+                             gate=gate, residual_scale=residual_scale,
+                             unit_offset=self.unit_offset, normed=normed)
+        ops.w4_gemm(self.head, normed, logits)
+        ops.sample_tokens(self.sample_ws, logits, uniform, tokens, logprobs=logprobs, **draw)
+        return tokens
 
 
 class ExpertFFN:
