@@ -163,3 +163,41 @@ def test_captured_on_another_stream():
         torch.cuda.synchronize()
         eager = _run(xd, w, True)
         assert torch.equal(y, eager)
+
+
+# sizes that take each form of the kernels (five streaming ones, then tiles from narrow to wide), with an odd
+# number of features and, where the group allows it, a last step that is not whole
+FORMS = {
+    32: [(1, 2051, 7136), (1, 1000, 448), (3, 33001, 448), (17, 12003, 448), (40, 20011, 1376), (130, 33001, 1376),
+         (1500, 4083, 448), (420, 8200, 448), (600, 12003, 1376)],
+    64: [(1, 2051, 7104), (1, 1000, 448), (3, 33001, 448), (17, 12003, 448), (40, 20011, 1344), (40, 33001, 448),
+         (900, 2051, 1344), (3000, 1000, 448), (600, 12003, 448), (300, 20011, 1344)],
+    128: [(1, 2051, 7168), (1, 1000, 384), (1, 33001, 1408), (17, 12003, 384), (40, 20011, 1408), (40, 33001, 384),
+          (1500, 4083, 384), (3000, 1000, 384), (768, 5001, 7168), (600, 33001, 384)],
+}
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group,rows,n,k", [(g, *c) for g, cs in FORMS.items() for c in cs])
+def test_every_form(group, rows, n, k, zeros):
+    """The reference in float64 on the GPU, features in blocks."""
+    from pegainfer_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    packed = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=g)
+    s = (torch.randn(n, k // group, device="cuda", generator=g) * 0.01).to(torch.bfloat16)
+    z = torch.randint(0, 17, (n, k // group), dtype=torch.uint8, device="cuda", generator=g) if zeros else None
+    y = _run(x, ops.w4_pack(packed, s, z, group=group), True)
+    q = torch.stack((packed & 15, packed >> 4), -1).reshape(n, k).double()
+    zr = 8.0 if z is None else z.double().repeat_interleave(group, 1)
+    sr = s.double().repeat_interleave(group, 1)
+    for at in range(0, n, 4096):
+        part = slice(at, at + 4096)
+        qp, zp = q[part], zr if z is None else zr[part]
+        want = x.double() @ ((qp - zp) * sr[part]).T
+        mag = x.double().abs() @ ((32 + qp + zp) * sr[part].abs()).T
+        bound = (2 * group + k // group + 18) * 2.0 ** -23 * mag + want.abs() * 2.0 ** -24  # w4_bound
+        bad = (y[:, part].double() - want).abs() > bound
+        assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist())
+        # and far inside it for most: a wrong scale, code or row would not be
+        assert ((y[:, part].double() - want).abs() <= 1e-5 * mag).float().mean() > 0.999
