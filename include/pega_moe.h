@@ -418,7 +418,8 @@ int pega_sandwich_rmsnorm(const void* x, bool x_is_f32, const uint16_t* residual
  * packed [out_dim][in_dim / 2] bytes, the even column in the low nibble; scales bf16
  * [out_dim][in_dim / group_size]; zeros bytes of the same shape, 0 to 127, or NULL.  codes takes
  * ceil(out_dim / 16) * ceil(in_dim / 128) * 1024 bytes, meta the same number of units of
- * 16 * 128 / group_size * (zeros ? 4 : 2) bytes.  in_dim is whole groups, at most 2^20.  packed is
+ * 16 * 128 / group_size * (zeros ? 4 : 2) bytes.  in_dim is whole groups, at most 2^20, out_dim at most
+ * 2^26.  packed is
  * 4-byte aligned, codes and meta 16-byte (801 otherwise). */
 int pega_w4_pack(const uint8_t* packed, const uint16_t* scales, const uint8_t* zeros,
                  uint8_t* codes, uint8_t* meta, int out_dim, int in_dim, int group_size,
@@ -427,8 +428,9 @@ int pega_w4_pack(const uint8_t* packed, const uint16_t* scales, const uint8_t* z
 /* No reference counterpart: Y[n][m] = sum_k X[n][k] * (q[m][k] - z[m][k / g]) * s[m][k / g], X [N][K]
  * bf16, Y [N][M] bf16 or, with y_is_f32, fp32; any M, N and whole groups of K.  No weight is
  * rounded: products with the codes' integers are exact, group sums and their products with the scales
- * fp32.  A row of X with an infinity or a NaN gives NaN.  A row's result does not depend on the other
- * rows' values.  No workspace.  16-byte aligned buffers (801 otherwise); Y overlaps no input. */
+ * fp32.  A row of X with an infinity or a NaN gives NaN, one with 2^119 and more may.  A row's result
+ * does not depend on the other rows' values.  No workspace.  At most 2^20 columns, 2^26 features and
+ * 1048560 rows; X, codes and meta 16-byte aligned, Y by its type (801 otherwise); Y overlaps no input. */
 int pega_w4_gemm(const uint8_t* codes, const uint8_t* meta, bool has_zeros, int group_size,
                  const uint16_t* X, void* Y, bool y_is_f32, int M, int N, int K,
                  hipStream_t stream);

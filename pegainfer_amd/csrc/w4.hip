@@ -10,7 +10,8 @@
 // group is a chain of v_mfma_f32_16x16x32_bf16, the second sum with a constant operand, and
 // 16 s d is the group's share of Y: products of bf16 with exact integers, fp32 sums, one scale an
 // fp32 group sum.  No weight is rounded.  (16 + q and 16 + z cancel to at most two bits of the
-// fp32 sums.)  An infinite or NaN activation gives NaN in its whole row.
+// fp32 sums.)  An infinite or NaN activation gives NaN in its whole row, and so may one of 2^119 and more,
+// with which a group's two sums pass fp32's range.
 //
 // Device layout, for tiles of 16 features (the last one padded) and steps of 128 columns (the last
 // one padded): per tile and step 64 lanes' 16 bytes, lane (c, h) = (lane % 16, lane / 16) holding
@@ -589,8 +590,8 @@ int check_sizes(const char* name, int M, int K, int group) {
   if (group != 32 && group != 64 && group != 128)
     return fail(kNotSupported, "%s: groups of 32, 64 or 128 columns, got %d", name, group);
   if (K % group != 0) return fail(kInvalidValue, "%s: %d columns are not whole groups of %d", name, K, group);
-  if (K > (1 << 20) || M > (1 << 28))
-    return fail(kNotSupported, "%s: at most 2^20 columns and 2^28 features, got %d x %d", name, M, K);
+  if (K > (1 << 20) || M > (1 << 26))
+    return fail(kNotSupported, "%s: at most 2^20 columns and 2^26 features, got %d x %d", name, M, K);
   return kSuccess;
 }
 
@@ -634,8 +635,9 @@ PEGA_API int pega_w4_gemm(const uint8_t* codes, const uint8_t* meta, bool has_ze
   if (N < 0) return fail(kInvalidValue, "w4_gemm: %d rows", N);
   if (N == 0) return kSuccess;  // empty tensors have no address
   if (!codes || !meta || !X || !Y) return fail(kInvalidValue, "w4_gemm: null pointer");
-  if (!aligned16(codes) || !aligned16(meta) || !aligned16(X) || !aligned16(Y))
-    return fail(kNotSupported, "w4_gemm: buffers must be 16-byte aligned");
+  if (!aligned16(codes) || !aligned16(meta) || !aligned16(X) ||
+      (reinterpret_cast<uintptr_t>(Y) & (y_is_f32 ? 3u : 1u)))
+    return fail(kNotSupported, "w4_gemm: X and the weight must be 16-byte aligned, Y by its type");
   if (N > 16 * 65535) return fail(kNotSupported, "w4_gemm: at most %d rows, got %d", 16 * 65535, N);
   const long long units = 1LL * ceil_div(M, 16) * ceil_div(K, kStep);
   const long long y_bytes = (y_is_f32 ? 4LL : 2LL) * N * M;

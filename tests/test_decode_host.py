@@ -54,7 +54,7 @@ PACK = [A, A << 1, A << 2, A << 3, A << 4, 20, 256, 64, None]
 
 @pytest.mark.parametrize("at,value,code", [
     (0, None, 1), (1, None, 1), (3, None, 1), (4, None, 1), (5, 0, 1), (5, -3, 1), (6, 0, 1), (6, 96, 1),
-    (6, -64, 1), (7, 16, 801), (7, 0, 801), (7, 256, 801), (6, 1 << 21, 801), (5, (1 << 28) + 1, 801),
+    (6, -64, 1), (7, 16, 801), (7, 0, 801), (7, 256, 801), (6, 1 << 21, 801), (5, (1 << 26) + 1, 801),
     (0, A + 2, 801), (1, (A << 1) + 1, 801), (3, (A << 3) + 8, 801), (4, (A << 4) + 4, 801),
     (3, A, 1), (4, A << 1, 1), (3, A << 2, 1), (4, (A << 3) + 1024, 1)])
 def test_pack_refuses(at, value, code):
@@ -69,7 +69,7 @@ GEMM = [A, A << 2, True, 64, A << 4, A << 6, True, 20, 3, 256, None]
 @pytest.mark.parametrize("at,value,code", [
     (0, None, 1), (1, None, 1), (4, None, 1), (5, None, 1), (7, 0, 1), (8, -1, 1), (9, 0, 1), (9, 100, 1),
     (3, 48, 801), (9, 1 << 21, 801), (8, 16 * 65535 + 1, 801),
-    (0, A + 8, 801), (1, (A << 2) + 4, 801), (4, (A << 4) + 2, 801), (5, (A << 6) + 4, 801),
+    (0, A + 8, 801), (1, (A << 2) + 4, 801), (4, (A << 4) + 2, 801), (5, (A << 6) + 2, 801), (7, (1 << 26) + 1, 801),
     (5, A, 1), (5, A << 2, 1), (5, (A << 4) + 16, 1)])
 def test_gemm_refuses(at, value, code):
     args = list(GEMM)

@@ -81,6 +81,20 @@ def test_many_equal_or_close(rows, vocab, sigma, bf16):
            top_p=np.tile([0.37, 0.5], n // 2), temperature=np.tile([1.0, 2.5], n // 2))
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows", [1, 5, 300])
+@pytest.mark.parametrize("k", [2, 50, 1024, 1025])
+def test_small_k_among_more_equal_logits_than_are_listed(rows, k, bf16):
+    """A few tokens ahead, then thousands that share the k-th place: cut by index."""
+    v = 20000
+    l = torch.full((rows, v), 1.25, device="cuda")
+    l[:, 9::5000] = 1.5
+    l[:, 3] = float("nan")
+    l = l.to(torch.bfloat16) if bf16 else l
+    g = np.random.default_rng(k)
+    _check(l, u=g.random(rows, dtype=np.float32), top_k=[k] * rows, top_p=[0.9] * rows)
+
+
 def test_equal_logits_in_closed_form():
     """V equal logits, top-k k: k equal weights; a draw with u is token floor(u k)."""
     v, k = 100000, 6250

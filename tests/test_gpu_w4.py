@@ -98,6 +98,10 @@ def test_repeats_and_writes_nothing_else(rows):
         ops.w4_gemm(w, xd, out)
         assert torch.equal(out, first)
     assert (big[:32] == 3).all() and (big[32 + rows * 77:] == 3).all()
+    odd = torch.full((rows * 77 + 3,), 3.0, device="cuda")  # a result that starts and ends anywhere
+    part = odd[1:1 + rows * 77].view(rows, 77)
+    ops.w4_gemm(w, xd, part)
+    assert torch.equal(part, first) and odd[0] == 3 and (odd[-2:] == 3).all()
     ops.w4_gemm(w, xd[:0], out[:0])  # no rows: nothing to do
 
 
