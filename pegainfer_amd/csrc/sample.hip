@@ -33,7 +33,8 @@ constexpr int kMaxParts = 256;         // of a row, whose masses the draw goes o
 constexpr int kFlight = 4;              // vectors of a thread in flight
 constexpr int kMaxFew = 1024;          // so few fit the list with room for what shares the last one's bin
 constexpr int kPairs = kThreads / 4;   // candidates that are compared with each other
-constexpr int kWorkgroups = 2048;      // eight a CU
+constexpr int kWorkgroups = 1024;      // four a CU
+constexpr int kFewWorkgroups = 256;    // no more than one a CU
 constexpr int kMaxRows = 256;          // of a round of launches, which bounds the workspace
 constexpr int kMaxVocab = 1 << 19;     // sums of weights stay below 2^63
 constexpr double kRange = 28.0;        // smaller weights than e^-28 are zero
@@ -55,11 +56,11 @@ struct SampleArgs {
   bool has_temperature, has_top_p, has_min_p, has_top_k;
 };
 
-__device__ __forceinline__ float clean(float l) { return l == l ? l + 0.0f : -__builtin_inff(); }  // -0 is 0
+__device__ __forceinline__ float clean(float l) { return l == l ? l : -__builtin_inff(); }
 
 // Floats in the order of their values.
 __device__ __forceinline__ uint32_t key_of(float l) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, l);
+  const uint32_t b = __builtin_bit_cast(uint32_t, l + 0.0f);  // -0 is 0
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
@@ -79,9 +80,9 @@ struct Row {
   __device__ __forceinline__ Row(const T* row, int size) : p(row), n(size), vecs(ceil_div(size, kVec)) {}
   static __device__ __forceinline__ float value(uint4 q, int e) {
     if constexpr (sizeof(T) == 4)
-      return clean(__builtin_bit_cast(float, e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w));
+      return __builtin_bit_cast(float, e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w);
     const uint32_t w = (e >> 1) == 0 ? q.x : (e >> 1) == 1 ? q.y : (e >> 1) == 2 ? q.z : q.w;
-    return clean(e & 1 ? bf_hi(w) : bf_lo(w));
+    return e & 1 ? bf_hi(w) : bf_lo(w);
   }
   __device__ __forceinline__ float at(int i) const {
     if constexpr (sizeof(T) == 4) return clean(p[i]);
@@ -93,12 +94,14 @@ struct Row {
     __builtin_memcpy(&q, p + start(min(v, vecs - 1)), 16);
     return q;
   }
-  // The largest place of the vectors in [from, to), over `threads` threads.
+  // The place of this thread's first in the order among the vectors in [from, to), over `threads` threads,
+  // each element once.
   __device__ __forceinline__ u64 best(int from, int to, int tid, int threads) const {
-    u64 best = 0;
+    float top = -__builtin_inff();
+    int at = -1;
     if (n < kVec) {
-      if (from == 0 && tid < n) best = place(at(tid), tid);
-      return best;
+      if (from == 0 && tid < n) top = this->at(tid), at = tid;
+      return place(top, at);
     }
     for (int v = from + tid; v < to; v += kFlight * threads) {
       uint4 q[kFlight];
@@ -106,16 +109,19 @@ struct Row {
       for (int j = 0; j < kFlight; ++j) q[j] = load(v + j * threads);
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        // each element once: the threads' largest are of disjoint elements
-        const int vec = v + j * threads, i = start(min(vec, vecs - 1));
+        float most = value(q[j], 0);
+#pragma unroll
+        for (int e = 1; e < kVec; ++e) most = fmaxf(most, value(q[j], e));  // (NaNs left out)
+        if (!(most > top)) continue;  // seldom passed: later elements of one value are behind it
+        const int vec = v + j * threads, i = start(min(vec, vecs - 1)), own = vec * kVec - i;
 #pragma unroll
         for (int e = 0; e < kVec; ++e)
-          if (vec < to && i + e >= vec * kVec) best = max(best, place(value(q[j], e), i + e));
+          if (vec < to && e >= own && value(q[j], e) > top) top = value(q[j], e), at = i + e;
       }
     }
-    return best;
+    return place(top, at);
   }
-  // f(i, l[i]) for the vectors' elements with l >= low, over `threads` threads with kFlight loads in flight
+  // f(i, l[i]) for the vectors' elements with l >= low (a NaN has not), over `threads` threads with kFlight loads in flight
   // each.  Few copies of f: the passes are short enough for a CU's instruction fetches to show.
   // after(base): once for each round of vectors base .. base + threads - 1, by all threads.
   template <typename F, typename A>
@@ -139,15 +145,18 @@ struct Row {
       q[kFlight - 1] = load(v + kFlight * threads);
       float most = value(now, 0);
 #pragma unroll
-      for (int e = 1; e < kVec; ++e) most = fmaxf(most, value(now, e));
+      for (int e = 1; e < kVec; ++e) most = fmaxf(most, value(now, e));  // (NaNs left out)
       if (v < to && most >= low) {
-        int i = start(v);
+        const int first = start(v);
+        // the last vector may reach back over the one before, whose elements are not its own
+        const int own = v * kVec - first;
+        int i = first;
 #pragma unroll 1
         for (int w = 0; w < kVec; w += 4) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float l = value(now, e);
-            if (l >= low && i + e >= v * kVec) f(i + e, l);
+            if (l >= low && i + e - first >= own) f(i + e, l);
           }
           i += 4;
           now = make_uint4(now.z, now.w, now.x, now.y);
@@ -167,41 +176,50 @@ struct Row {
   }
 };
 
+// 2^r = sum of (r ln 2)^k / k!, for |r| <= 1/2; what follows k = 12 is 2^-52 of the sum.  The
+// coefficients stand in scalar registers, made in front of a loop: from vector registers each would be
+// moved in front of its product (78 against 98 us for 256 rows of 163840 weights).
+struct Powers {
+  double c[12] = {0x1.c3bd650fc2986p-36, 0x1.e8cac7351bb25p-32, 0x1.e4cf5158b8ecap-28,
+                  0x1.b5253d395e7c4p-24, 0x1.62c0223a5c824p-20, 0x1.ffcbfc588b0c7p-17,
+                  0x1.430912f86c787p-13, 0x1.5d87fe78a6731p-10, 0x1.3b2ab6fba4e77p-7,
+                  0x1.c6b08d704a0c0p-5, 0x1.ebfbdff82c58fp-3, 0x1.62e42fefa39efp-1};
+  __device__ __forceinline__ Powers() {
+#pragma unroll
+    for (int i = 0; i < 12; ++i) asm("" : "+s"(c[i]));
+  }
+  __device__ __forceinline__ double of(double r) const {
+    double e = c[0];
+#pragma unroll
+    for (int i = 1; i < 12; ++i) e = __builtin_fma(e, r, c[i]);
+    return __builtin_fma(e, r, 1.0);
+  }
+};
+
 // What turns a logit into a weight.
 struct Scale {
-  double max, least, per;  // the row's maximum, the least l - max that has weight, log2(e) / T
+  // the row's maximum, the least l - max that has weight, log2(e) / T, and bins for a unit of l
+  double max, least, per, bins;
   bool infinite;           // the maximum is +inf
 
   __device__ __forceinline__ double below(float l) const {
     if (infinite) return l == __builtin_inff() ? 0.0 : -__builtin_inf();
     return static_cast<double>(l) - max;
   }
-  __device__ __forceinline__ bool live(double d) const { return d >= least && d != -__builtin_inf(); }
+  __device__ __forceinline__ bool live(double d) const { return d >= least; }  // (least is finite)
   // 2^(d per + 44), rounded to a whole number
-  __device__ __forceinline__ u64 weight(double d) const {
-    const double x = d * per, n = __builtin_rint(x), r = (x - n) * 0.6931471805599453;
-    double e = 1.0 / 479001600.0;  // 1/12!; what follows is 2^-52 of the sum at |r| <= ln 2 / 2
-    e = __builtin_fma(e, r, 1.0 / 39916800.0);
-    e = __builtin_fma(e, r, 1.0 / 3628800.0);
-    e = __builtin_fma(e, r, 1.0 / 362880.0);
-    e = __builtin_fma(e, r, 1.0 / 40320.0);
-    e = __builtin_fma(e, r, 1.0 / 5040.0);
-    e = __builtin_fma(e, r, 1.0 / 720.0);
-    e = __builtin_fma(e, r, 1.0 / 120.0);
-    e = __builtin_fma(e, r, 1.0 / 24.0);
-    e = __builtin_fma(e, r, 1.0 / 6.0);
-    e = __builtin_fma(e, r, 0.5);
-    e = __builtin_fma(e, r, 1.0);
-    e = __builtin_fma(e, r, 1.0);
+  __device__ __forceinline__ u64 weight(double d, const Powers& powers = Powers()) const {
+    const double x = d * per, n = __builtin_rint(x), r = x - n;
+    const double e = powers.of(r);
     const u64 pow = static_cast<u64>(static_cast<int>(n) + 44 + 1023) << 52;
     const double whole = __builtin_fma(e, __builtin_bit_cast(double, pow), 0x1p52);
     return __builtin_bit_cast(u64, whole) & 0xfffffffffffffull;
   }
   // bins of equal width in the logarithm, the largest weights in bin 0
-  __device__ __forceinline__ double position(double d) const { return -d * per * kBinsPerOctave; }
+  __device__ __forceinline__ double position(double d) const { return -d * bins; }
   __device__ __forceinline__ int bin(double d) const { return min(kBins - 1, static_cast<int>(position(d))); }
   // below every d of a bin
-  __device__ __forceinline__ double edge(int b) const { return -(b + 1) / (per * kBinsPerOctave) * (1 + 0x1p-30); }
+  __device__ __forceinline__ double edge(int b) const { return -(b + 1) / bins * (1 + 0x1p-30); }
   // a float below every logit that lies d or less below the maximum
   __device__ __forceinline__ float bound(double d) const {
     if (infinite) return __builtin_inff();
@@ -351,6 +369,8 @@ struct Request {
   bool few;     // a small k: all that its cut leaves is listed without a histogram of the row
   __device__ __forceinline__ bool cuts() const { return k > 0 || top_p < 1.0f; }
   __device__ __forceinline__ bool settled() const { return none || first; }
+  // whether scan leaves nothing but the draw
+  __device__ __forceinline__ bool scanned() const { return settled() || few || !cuts(); }
 };
 
 __device__ __forceinline__ float value_of(uint32_t k) {
@@ -375,6 +395,7 @@ __device__ __forceinline__ Request request(const SampleArgs& p, int row, u64 bes
   q.scale.max = top;
   q.scale.infinite = top == __builtin_inff();
   q.scale.per = kLog2e / q.temp;
+  q.scale.bins = q.scale.per * kBinsPerOctave;
   q.scale.least = -kRange * q.temp;
   if (min_p > 0.0f)
     q.scale.least = fmax(q.scale.least, q.temp * ::log(static_cast<double>(fminf(min_p, 1.0f))));
@@ -387,12 +408,12 @@ __device__ __forceinline__ void write(const SampleArgs& p, int row, int token, f
 }
 
 // One element's share of the histogram.
-__device__ __forceinline__ void count_in(Shared& s, const Scale& scale, float l) {
+__device__ __forceinline__ void count_in(Shared& s, const Scale& scale, float l, const Powers& powers) {
   const double d = scale.below(l);
   if (!scale.live(d)) return;
   const int b = scale.bin(d);
   atomicAdd(&s.count[b], 1u);
-  atomicAdd(&s.mass[b], scale.weight(d));
+  atomicAdd(&s.mass[b], scale.weight(d, powers));
 }
 
 // The histogram of vectors [from, to).
@@ -401,8 +422,9 @@ __device__ __forceinline__ void histogram(Shared& s, const R& row, const Scale& 
                                           int to, int tid) {
   s.count[tid] = 0, s.mass[tid] = 0;
   __syncthreads();
+  const Powers powers;
   row.each(from, to, tid, kThreads, scale.bound(scale.least),
-           [&](int, float l) { count_in(s, scale, l); }, [](int) {});
+           [&](int, float l) { count_in(s, scale, l, powers); }, [](int) {});
   __syncthreads();
 }
 
@@ -468,10 +490,16 @@ template <typename K>
 __device__ __forceinline__ Plan few_plan(Shared& s, const Request& q, int n, const K& keys, int tid) {
   s.count[tid] = 0, s.mass[tid] = 0;
   __syncthreads();
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const double d = q.scale.below(value_of(keys(i)));
-    if (q.scale.live(d)) atomicAdd(&s.count[q.scale.bin(d)], 1u);
+#pragma unroll 1
+  for (int i = 0; i < n; i += 8) {
+    uint32_t k[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k[j] = keys(min(i + j, n - 1));  // in flight together
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const double d = q.scale.below(value_of(k[j]));
+      if (i + j < n && q.scale.live(d)) atomicAdd(&s.count[q.scale.bin(d)], 1u);
+    }
   }
   __syncthreads();
   uint32_t before = 0;
@@ -494,20 +522,21 @@ __device__ __forceinline__ void pick(Shared& s, const R& row, const Scale& scale
   __syncthreads();
   if (tid == 0) s.listed = 0;
   __syncthreads();
-  const bool gather = plan.candidates <= kList;
-  const int lowest = plan.sure == kBins ? kBins - 1 : max(plan.k_bin, plan.p_last);
+  const bool gather = plan.candidates <= kList, all = plan.sure == kBins;
+  const int lowest = all ? kBins - 1 : max(plan.k_bin, plan.p_last);
   const float low = fmaxf(scale.bound(scale.least), scale.bound(scale.edge(lowest)));
   // a wave's parts in one run, so that its loads stay in flight from one to the next
   const int each_wave = ceil_div(end - first, kWaves), mine = first + wave * each_wave;
   const int from = mine * part, to = min(min(mine + each_wave, end) * part, row.vecs);
   if (lane < each_wave && mine + lane < end) s.part[mine + lane] = 0;
   u64 m = 0;
+  const Powers powers;
   row.each(from, to, lane, 64, low, [&](int at, float l) {
     const double d = scale.below(l);
     if (!scale.live(d)) return;
-    const int b = scale.bin(d);
+    const int b = all ? 0 : scale.bin(d);
     if (b < plan.sure) {
-      m += scale.weight(d);
+      m += scale.weight(d, powers);
     } else if (gather && plan.has(b)) {
       const int to_list = atomicAdd(&s.listed, 1);
       if (to_list < kList) s.key[to_list] = key_of(l), s.index[to_list] = at;
@@ -665,7 +694,7 @@ __device__ __forceinline__ void again(Shared& s, const R& row, const Request& q,
   s.count[tid] = 0, s.mass[tid] = 0;
   if (tid < parts) s.part[tid] = 0;
   __syncthreads();
-  row.each_plain(tid, kThreads, low, [&](int, float l) { count_in(s, q.scale, l); });
+  row.each_plain(tid, kThreads, low, [&](int, float l) { count_in(s, q.scale, l, Powers()); });
   __syncthreads();
   bin = scan_bins(s, s.count, s.mass, tid);
   plan = make_plan(s, q, bin, tid);
@@ -722,7 +751,7 @@ __device__ __forceinline__ void finish(Shared& s, const SampleArgs& p, int row_i
       s.count[tid] = 0, s.mass[tid] = 0;
       __syncthreads();
       each([&](uint32_t k, int i) {
-        if (cut.keeps(k, i)) count_in(s, scale, value_of(k));
+        if (cut.keeps(k, i)) count_in(s, scale, value_of(k), Powers());
       });
       __syncthreads();
       bin = scan_bins(s, s.count, s.mass, tid);
@@ -804,17 +833,17 @@ __device__ __forceinline__ void write_settled(const SampleArgs& p, const Request
   else write(p, row, static_cast<int>(0xffffffffu - static_cast<uint32_t>(best)), 0.0f);
 }
 
-// Four launches, of several workgroups (splits) a row where there are few rows:
-//   best       the first of the order in each split, and each thread's largest
-//   scan       rows with a small k: the list; rows without cuts: the parts' masses; others: the histogram
-//   pick       those others: the list and the parts' masses
-//   finish     the cuts and the draw, a workgroup a row
+// Several workgroups (splits) a row, in three launches or four:
+//   best   the first of the order in each split, and each thread's largest
+//   scan   rows with a small k: the list; rows without cuts: the parts' masses; others: the histogram
+//   pick   those others: the list and the parts' masses
+//   draw   a workgroup a row: the cuts and the draw
 // What they hand on, for each row:
 struct Hand {
   u64 best[kMaxSplit];
   Request request;  // from scan on
   Plan plan;
-  uint32_t listed;
+  uint32_t listed, done;  // elements in the list, workgroups of the draw that have listed theirs
   u64 part[kMaxParts];
   uint32_t key[kList];
   int32_t index[kList];
@@ -843,7 +872,7 @@ __global__ __launch_bounds__(kThreads) void sample_best_kernel(SplitArgs a) {
   Hand& h = a.hand[row_id];
   if (tid == 0) {
     h.best[split] = best;
-    if (split == 0) h.listed = 0;
+    if (split == 0) h.listed = 0, h.done = 0;
   }
 }
 
@@ -854,19 +883,31 @@ __device__ __forceinline__ u64 best_of(const Hand& h, int splits) {
   return best;
 }
 
+// Between workgroups of a launch: device-coherent (the L2 is per XCD).
+template <typename V>
+__device__ __forceinline__ void store_coherent(V* p, V v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename V>
+__device__ __forceinline__ V load_coherent(const V* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // A split's share of the list and of the parts' masses.
 template <typename T>
 __device__ __forceinline__ void hand_over(Shared& s, const SplitArgs& a, Hand& hand, const Row<T>& row, const Request& q,
                                           const Plan& plan, int split, int tid) {
   const int per = a.parts / a.splits, first = split * per;
   pick(s, row, q.scale, plan, a.part, first, first + per, tid);
-  if (tid < per) hand.part[first + tid] = s.part[first + tid];
+  if (tid < per) store_coherent(&hand.part[first + tid], s.part[first + tid]);
   const int listed = s.listed;
   if (listed == 0) return;
   if (tid == 0) s.last = static_cast<int>(atomicAdd(&hand.listed, static_cast<uint32_t>(listed)));
   __syncthreads();
-  for (int i = tid; i < min(listed, kList) && s.last + i < kList; i += kThreads)
-    hand.key[s.last + i] = s.key[i], hand.index[s.last + i] = s.index[i];
+  for (int i = tid; i < min(listed, kList) && s.last + i < kList; i += kThreads) {
+    store_coherent(&hand.key[s.last + i], s.key[i]);
+    store_coherent(&hand.index[s.last + i], s.index[i]);
+  }
 }
 
 template <typename T>
@@ -925,26 +966,40 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SplitArgs a) {
   const Row<T> row = row_of<T>(a.p, row_id);
   Hand& hand = a.hand[row_id];
   const Request q = hand.request;
-  if (q.settled() || !q.cuts() || q.few) return;
+  if (q.scanned()) return;
   Bin bin{};
   const Plan plan = planned(s, a, row_id, q, bin, tid);
   if (split == 0 && tid == 0) hand.plan = plan;
   hand_over(s, a, hand, row, q, plan, split, tid);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SplitArgs a) {
+// kPicks: with pick's work in front, and the row's last workgroup to go on.
+template <typename T, bool kPicks>
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SplitArgs a) {
   __shared__ Shared s;
-  const int tid = threadIdx.x, row_id = blockIdx.x;
+  const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
   const Row<T> row = row_of<T>(a.p, row_id);
-  const Hand& hand = a.hand[row_id];
+  Hand& hand = a.hand[row_id];
   const Request q = hand.request;
-  if (q.settled()) return;
-  Plan plan = hand.plan;
-  if (q.few) plan.candidates = hand.listed;
+  if (q.settled() || (q.scanned() && split > 0)) return;
   Bin bin{};
-  if (plan.by_k && plan.by_p && !q.few) planned(s, a, row_id, q, bin, tid);  // the p cut's bin follows from the k cut
-  if (tid < a.parts) s.part[tid] = hand.part[tid];
+  Plan plan;
+  if (kPicks && !q.scanned()) {
+    plan = planned(s, a, row_id, q, bin, tid);
+    hand_over(s, a, hand, row, q, plan, split, tid);
+    // every store has completed before the workgroup counts itself in
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) s.found = atomicAdd(&hand.done, 1u) + 1u == static_cast<uint32_t>(a.splits);
+    __syncthreads();
+    if (!s.found) return;
+  } else {
+    plan = hand.plan;
+    // the p cut's bin follows from the k cut
+    if (!kPicks && plan.by_k && plan.by_p && !q.few) planned(s, a, row_id, q, bin, tid);
+  }
+  if (q.few) plan.candidates = load_coherent(&hand.listed);
+  if (tid < a.parts) s.part[tid] = load_coherent(&hand.part[tid]);
   if (plan.candidates <= kList) {
     const int n = static_cast<int>(plan.candidates);
 #pragma unroll 1
@@ -952,7 +1007,10 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SplitArgs a) {
       uint32_t k[4];
       int32_t at[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) k[j] = hand.key[min(i + j * kThreads, n - 1)], at[j] = hand.index[min(i + j * kThreads, n - 1)];
+      for (int j = 0; j < 4; ++j) {
+        k[j] = load_coherent(&hand.key[min(i + j * kThreads, n - 1)]);
+        at[j] = load_coherent(&hand.index[min(i + j * kThreads, n - 1)]);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (i + j * kThreads < n) s.key[i + j * kThreads] = k[j], s.index[i + j * kThreads] = at[j];
@@ -983,8 +1041,14 @@ void launch(SampleArgs p, void* workspace, hipStream_t stream) {
     const SplitArgs a{p, hand, reinterpret_cast<Histogram*>(hand + p.rows), splits, part, parts};
     hipLaunchKernelGGL(sample_best_kernel<T>, grid, block, 0, stream, a);
     hipLaunchKernelGGL(sample_scan_kernel<T>, grid, block, 0, stream, a);
-    if (p.has_top_k || p.has_top_p) hipLaunchKernelGGL(sample_pick_kernel<T>, grid, block, 0, stream, a);
-    hipLaunchKernelGGL(sample_finish_kernel<T>, dim3(p.rows), block, 0, stream, a);
+    // Few rows gain from one launch less (one row 24 us of kernels against 28); with many, pick's share is faster
+    // in a kernel of fewer registers, and idle workgroups in one of fewer launches (256 rows 130 against 147).
+    if (splits * p.rows <= kFewWorkgroups) {
+      hipLaunchKernelGGL((sample_draw_kernel<T, true>), grid, block, 0, stream, a);
+    } else {
+      hipLaunchKernelGGL(sample_pick_kernel<T>, grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sample_draw_kernel<T, false>), dim3(1, p.rows), block, 0, stream, a);
+    }
     p.logits = static_cast<const T*>(p.logits) + kMaxRows * p.stride;
     p.u += kMaxRows, p.temperature += kMaxRows, p.top_p += kMaxRows, p.min_p += kMaxRows, p.top_k += kMaxRows;
     p.tokens += kMaxRows;
