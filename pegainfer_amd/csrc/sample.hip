@@ -202,10 +202,8 @@ struct Scale {
   double max, least, per, bins;
   bool infinite;           // the maximum is +inf
 
-  __device__ __forceinline__ double below(float l) const {
-    if (infinite) return l == __builtin_inff() ? 0.0 : -__builtin_inf();
-    return static_cast<double>(l) - max;
-  }
+  // l - max; of an infinite maximum 0 and, for all else, -inf
+  __device__ __forceinline__ double below(float l) const { return __builtin_fmin(static_cast<double>(l) - max, 0.0); }
   __device__ __forceinline__ bool live(double d) const { return d >= least; }  // (least is finite)
   // 2^(d per + 44), rounded to a whole number
   __device__ __forceinline__ u64 weight(double d, const Powers& powers = Powers()) const {
@@ -218,13 +216,19 @@ struct Scale {
   // bins of equal width in the logarithm, the largest weights in bin 0
   __device__ __forceinline__ double position(double d) const { return -d * bins; }
   __device__ __forceinline__ int bin(double d) const { return min(kBins - 1, static_cast<int>(position(d))); }
-  // below every d of a bin
+  // above every d of a bin, below every one
+  __device__ __forceinline__ double inner(int b) const { return -b / bins * (1 - 0x1p-30); }
   __device__ __forceinline__ double edge(int b) const { return -(b + 1) / bins * (1 + 0x1p-30); }
-  // a float below every logit that lies d or less below the maximum
+  // a float below every logit that lies d or less below the maximum, and one above all that lie d or more
+  // below it
   __device__ __forceinline__ float bound(double d) const {
     if (infinite) return __builtin_inff();
     const float f = static_cast<float>(max + d);
     return f - __builtin_fabsf(f) * 0x1p-22f - 0x1p-126f;
+  }
+  __device__ __forceinline__ float over(double d) const {
+    const float f = static_cast<float>(max + d);
+    return f + __builtin_fabsf(f) * 0x1p-22f + 0x1p-126f;
   }
 };
 
@@ -529,12 +533,18 @@ __device__ __forceinline__ void pick(Shared& s, const R& row, const Scale& scale
   const int each_wave = ceil_div(end - first, kWaves), mine = first + wave * each_wave;
   const int from = mine * part, to = min(min(mine + each_wave, end) * part, row.vecs);
   if (lane < each_wave && mine + lane < end) s.part[mine + lane] = 0;
+  // from here on a logit is surely in the bins that are kept whole
+  const float whole = all ? scale.over(scale.least) : plan.sure == 0 ? __builtin_nanf("") : scale.over(scale.inner(plan.sure));
   u64 m = 0;
   const Powers powers;
   row.each(from, to, lane, 64, low, [&](int at, float l) {
     const double d = scale.below(l);
+    if (l >= whole) {
+      m += scale.weight(d, powers);
+      return;
+    }
     if (!scale.live(d)) return;
-    const int b = all ? 0 : scale.bin(d);
+    const int b = scale.bin(d);
     if (b < plan.sure) {
       m += scale.weight(d, powers);
     } else if (gather && plan.has(b)) {
