@@ -906,8 +906,8 @@ __device__ __forceinline__ V load_coherent(const V* p) {
 // A split's share of the list and of the parts' masses.
 template <typename T>
 __device__ __forceinline__ void hand_over(Shared& s, const SplitArgs& a, Hand& hand, const Row<T>& row, const Request& q,
-                                          const Plan& plan, int split, int tid) {
-  const int per = a.parts / a.splits, first = split * per;
+                                          const Plan& plan, int split, int splits, int tid) {
+  const int per = a.parts / splits, first = split * per;
   pick(s, row, q.scale, plan, a.part, first, first + per, tid);
   if (tid < per) store_coherent(&hand.part[first + tid], s.part[first + tid]);
   const int listed = s.listed;
@@ -944,7 +944,7 @@ __global__ __launch_bounds__(kThreads) void sample_scan_kernel(SplitArgs a) {
   }
   const Plan plan = q.few ? few_plan(s, q, a.splits, [&](int i) { return h[i].count[tid]; }, tid) : no_plan();
   if (writes) hand.plan = plan;
-  hand_over(s, a, hand, row, q, plan, split, tid);
+  hand_over(s, a, hand, row, q, plan, split, a.splits, tid);
 }
 
 // The row's histogram, and the plan that follows from it.
@@ -980,7 +980,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SplitArgs a) {
   Bin bin{};
   const Plan plan = planned(s, a, row_id, q, bin, tid);
   if (split == 0 && tid == 0) hand.plan = plan;
-  hand_over(s, a, hand, row, q, plan, split, tid);
+  hand_over(s, a, hand, row, q, plan, split, gridDim.x, tid);
 }
 
 // kPicks: with pick's work in front, and the row's last workgroup to go on.
@@ -996,7 +996,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SplitArgs a) {
   Plan plan;
   if (kPicks && !q.scanned()) {
     plan = planned(s, a, row_id, q, bin, tid);
-    hand_over(s, a, hand, row, q, plan, split, tid);
+    hand_over(s, a, hand, row, q, plan, split, a.splits, tid);
     // every store has completed before the workgroup counts itself in
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -1045,7 +1045,8 @@ void launch(SampleArgs p, void* workspace, hipStream_t stream) {
     // parts of whole rounds of a wave, a multiple of `splits` in number
     const int vecs = ceil_div(p.vocab, Row<T>::kVec), round = 64;
     const int part = round * ceil_div(vecs, round * kMaxParts);
-    const int parts = splits * ceil_div(ceil_div(vecs, part), splits);
+    const int picks = splits * 2 < kMaxSplit ? splits * 2 : kMaxSplit;
+    const int parts = picks * ceil_div(ceil_div(vecs, part), picks);
     const dim3 grid(splits, p.rows), block(kThreads);
     Hand* hand = static_cast<Hand*>(workspace);
     const SplitArgs a{p, hand, reinterpret_cast<Histogram*>(hand + p.rows), splits, part, parts};
@@ -1056,7 +1057,7 @@ void launch(SampleArgs p, void* workspace, hipStream_t stream) {
     if (splits * p.rows <= kFewWorkgroups) {
       hipLaunchKernelGGL((sample_draw_kernel<T, true>), grid, block, 0, stream, a);
     } else {
-      hipLaunchKernelGGL(sample_pick_kernel<T>, grid, block, 0, stream, a);
+      hipLaunchKernelGGL(sample_pick_kernel<T>, dim3(picks, p.rows), block, 0, stream, a);
       hipLaunchKernelGGL((sample_draw_kernel<T, false>), dim3(1, p.rows), block, 0, stream, a);
     }
     p.logits = static_cast<const T*>(p.logits) + kMaxRows * p.stride;
