@@ -54,7 +54,8 @@ _BF16 = torch.bfloat16
 
 
 def _is_bf16(t: torch.Tensor) -> bool:
-    return t.dtype is _BF16 or t.dtype in (torch.uint16, torch.int16)
+    dtype = t.dtype
+    return dtype is _BF16 or dtype in (torch.uint16, torch.int16)
 
 
 # --------------------------------------------------------------------------
@@ -1020,30 +1021,29 @@ def sandwich_rmsnorm(x: torch.Tensor, residual, pre_weight, eps: float, *,
     a row) or [rows, hidden].  unit_offset: weights are stored less one.  pre_weight may be None
     where residual_out alone is asked for.  Outputs, their places and their rounding as
     add_rmsnorm's: each is the formula's value rounded once, an output may be x or residual itself."""
-    if x.dim() != 2 or not (x.dtype == torch.float32 or _is_bf16(x)):
+    shape = x.shape
+    x32 = x.dtype is torch.float32
+    if len(shape) != 2 or not (x32 or _is_bf16(x)):
         raise ValueError("x must be bf16 or float32 [rows, hidden]")
-    rows, hidden = x.shape
-    for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
-        if w is not None and (not _is_bf16(w) or w.numel() != hidden):
-            raise ValueError(f"{name} must be bf16 [{hidden}]")
+    rows, hidden = shape
+    # (one look at each tensor, messages on failure only: a step of one row waits for its host)
+    if pre_weight is not None and (not _is_bf16(pre_weight) or pre_weight.numel() != hidden):
+        raise ValueError(f"pre_weight must be bf16 [{hidden}]")
+    if post_weight is not None and (not _is_bf16(post_weight) or post_weight.numel() != hidden):
+        raise ValueError(f"post_weight must be bf16 [{hidden}]")
     kind = 0
     if gate is not None:
         if not _is_bf16(gate):
             raise ValueError("gate must be bf16")
-        shape = tuple(gate.shape)
-        if shape == (hidden,):
-            kind = 1
-        elif shape == (rows, 1):
-            kind = 2
-        elif shape == (rows, hidden):
-            kind = 3
-        else:
-            raise ValueError(f"gate must be [{hidden}], [{rows}, 1] or [{rows}, {hidden}], got {list(shape)}")
-    if residual is not None:
+        of = gate.shape
+        kind = 1 if of == (hidden,) else 2 if of == (rows, 1) else 3 if of == shape else 0
+        if kind == 0:
+            raise ValueError(f"gate must be [{hidden}], [{rows}, 1] or [{rows}, {hidden}], got {list(of)}")
+    if residual is not None and (residual.shape != shape or not _is_bf16(residual)):
         _mx_rows("residual", residual, rows, hidden)
-    if residual_out is not None:
+    if residual_out is not None and (residual_out.shape != shape or not _is_bf16(residual_out)):
         _mx_rows("residual_out", residual_out, rows, hidden)
-    if normed is not None:
+    if normed is not None and (normed.shape != shape or not _is_bf16(normed)):
         _mx_rows("normed", normed, rows, hidden)
     codes = scales = None
     if quantized is not None:
@@ -1060,8 +1060,8 @@ def sandwich_rmsnorm(x: torch.Tensor, residual, pre_weight, eps: float, *,
         raise ValueError("residual_out and normed must be different buffers")
     px, pr, pp, pg, pw, ps, pn, pc, psc, stream = _ptrs_here(
         x, residual, post_weight, gate, pre_weight, residual_out, normed, codes, scales)
-    _lib.call("pega_sandwich_rmsnorm", px, x.dtype == torch.float32, pr, residual_scale, pp, pg, kind,
-              pw, bool(unit_offset), eps, ps, pn, pc, psc, rows, hidden, stream)
+    _lib.call("pega_sandwich_rmsnorm", px, x32, pr, residual_scale, pp, pg, kind, pw, unit_offset,
+              eps, ps, pn, pc, psc, rows, hidden, stream)
 
 
 # --------------------------------------------------------------------------
@@ -1125,13 +1125,15 @@ def w4_pack(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor = No
 def w4_gemm(w: W4Weight, x: torch.Tensor, y: torch.Tensor) -> None:
     """Y[n][m] = sum_k X[n][k] * (q[m][k] - z[m][k / group]) * s[m][k / group]: x bf16 [N, in], y bf16
     or float32 [N, out].  No weight is rounded; sums are fp32 (gemm_graphsafe on 4-bit weights)."""
-    if x.dim() != 2 or x.shape[1] != w.in_dim or not _is_bf16(x):
-        raise ValueError(f"x must be bf16 [rows, {w.in_dim}], got {x.dtype} {tuple(x.shape)}")
-    f32 = y.dtype == torch.float32
-    if tuple(y.shape) != (x.shape[0], w.out_dim) or not (f32 or _is_bf16(y)):
-        raise ValueError(f"y must be bf16 or float32 [{x.shape[0]}, {w.out_dim}], got {y.dtype} {tuple(y.shape)}")
+    of, dtype = x.shape, y.dtype
+    if len(of) != 2 or of[1] != w.in_dim or not _is_bf16(x):
+        raise ValueError(f"x must be bf16 [rows, {w.in_dim}], got {x.dtype} {tuple(of)}")
+    rows = of[0]
+    f32 = dtype is torch.float32
+    if y.shape != (rows, w.out_dim) or not (f32 or _is_bf16(y)):
+        raise ValueError(f"y must be bf16 or float32 [{rows}, {w.out_dim}], got {dtype} {tuple(y.shape)}")
     pc, pm, px, py, stream = _ptrs_here(w.codes, w.meta, x, y)
-    _lib.call("pega_w4_gemm", pc, pm, w.with_zeros, w.group, px, py, f32, w.out_dim, x.shape[0],
+    _lib.call("pega_w4_gemm", pc, pm, w.with_zeros, w.group, px, py, f32, w.out_dim, rows,
               w.in_dim, stream)
 
 
@@ -1171,28 +1173,31 @@ def sample_tokens(workspace: SampleWorkspace, logits: torch.Tensor, uniform: tor
     uniform, temperature, top_p, min_p float32, top_k int32, one value a row; None leaves a step out
     (as do top_k 0, top_p 1, min_p 0), temperature 0 takes the largest logit.  tokens int32,
     logprobs float32 or None.  NaN logits count as -inf; a row of nothing else gives token -1."""
-    if logits.dim() != 2 or not (logits.dtype == torch.float32 or logits.dtype is _BF16):
+    of, dtype = logits.shape, logits.dtype
+    if len(of) != 2 or not (dtype is torch.float32 or dtype is _BF16):
         raise ValueError("logits must be float32 or bf16 [rows, vocab]")
-    rows, vocab = logits.shape
+    rows, vocab = of
     if rows > workspace.max_rows or vocab > workspace.max_vocab:
         raise ValueError(f"{rows} x {vocab} logits exceed the workspace's "
                          f"{workspace.max_rows} x {workspace.max_vocab}")
-    if vocab == 0 or (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+    stride, step = logits.stride()
+    if vocab == 0 or (vocab > 1 and step != 1) or (rows > 1 and stride < vocab):
         raise ValueError("logits must have rows of adjacent values that do not overlap")
-    for name, t, dtype in (("uniform", uniform, torch.float32), ("tokens", tokens, torch.int32),
-                           ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
-                           ("logprobs", logprobs, torch.float32)):
-        if t is None and name not in ("uniform", "tokens"):
-            continue
-        if t.dtype != dtype or tuple(t.shape) != (rows,):
-            raise ValueError(f"{name} must be {dtype} [{rows}], got {t.dtype} {tuple(t.shape)}")
+    each = (rows,)
+    for t, want in ((uniform, torch.float32), (tokens, torch.int32), (temperature, torch.float32),
+                    (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32),
+                    (logprobs, torch.float32)):
+        if t is not None and (t.dtype is not want or t.shape != each):
+            raise ValueError(f"uniform, temperature, top_p, min_p and logprobs must be float32 [{rows}], "
+                             f"tokens and top_k int32 [{rows}], got {t.dtype} {tuple(t.shape)}")
+    if uniform is None or tokens is None:
+        raise ValueError("sample_tokens needs uniform and tokens")
     pu, pt, ptemp, pk, pp, pm, pl, pw, stream = _ptrs_here(
         uniform, tokens, temperature, top_k, top_p, min_p, logprobs, workspace.buffer)
-    if logits.device != tokens.device:
+    if logits.get_device() != tokens.get_device():
         raise ValueError(f"tensor must live on the current GPU, got {logits.device}")
-    _lib.call("pega_sample_tokens", logits.data_ptr(), logits.dtype is _BF16,
-              max(logits.stride(0), vocab), rows, vocab, pu, ptemp, pk, pp, pm, pt, pl, pw,
+    _lib.call("pega_sample_tokens", logits.data_ptr(), dtype is _BF16,
+              stride if stride > vocab else vocab, rows, vocab, pu, ptemp, pk, pp, pm, pt, pl, pw,
               workspace.buffer.numel(), stream)
 
 
