@@ -194,7 +194,11 @@ __global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) voi
 //
 // with a gate for each column, each row, each value, or none, and weights that are stored less one
 // (`one` = 1) or as they are (0).  One pass as above with two sums; all loads of a row are in flight
-// before the first sum.
+// before the first sum, and the row stays in registers until its last output is stored, so that
+// each value is read and written once.  Sums, norms and s are in 64 bits.
+// One row is bound by its latency, of the loads and of two sums over the workgroup one after the
+// other: 6.0 us for 7168 columns.  Many bf16 rows are bound by memory: 4096 x 7168 with a gate for
+// each value, bf16 and MXFP8 outputs 66 us, 4.9 TB/s.
 struct SandwichArgs {
   const void* x;
   const uint16_t *residual, *post, *pre, *gate;
@@ -207,7 +211,7 @@ struct SandwichArgs {
 };
 
 template <int CH, bool kX32>
-__global__ __launch_bounds__(CH == 1 ? 256 : CH == 2 ? 512 : 64 * kMaxWaves) void sandwich_rmsnorm_kernel(
+__global__ __launch_bounds__(64 * kMaxWaves) void sandwich_rmsnorm_kernel(
     SandwichArgs p) {
   __shared__ double s_sum[2][kMaxWaves];
   const int lanes = blockDim.x, lane = threadIdx.x;
@@ -456,8 +460,15 @@ PEGA_API int pega_sandwich_rmsnorm(const void* x, bool x_is_f32, const uint16_t*
                  eps, residual ? residual_scale : 1.0, unit_offset ? 1.0 : 0.0, residual_out, normed,
                  mxfp8_codes, mxfp8_scales, rows, hidden_dim};
   const int vecs = hidden_dim / 8;
-  if (vecs <= 4 * 64) launch_sandwich<1>(p, x_is_f32, stream);
-  else if (vecs <= 8 * 2 * 64 && (vecs <= 8 * 64 || rows <= 1024)) launch_sandwich<2>(p, x_is_f32, stream);
+  // Vectors a lane, in us without MXFP8, a gate for each row (bf16 x unless fp32 is said).  More of
+  // them take fewer waves to a row and more registers to a lane; with fp32 rows four spill.
+  //   one or two:  4096 columns, 1 row 4.3 and 4.8; 4096 rows 38.8 and 33.8, fp32 58.3 and 61.3;
+  //                7168 columns, 1024 rows 25.5 and 20.2, fp32 37.8 and 32.0; 2048 columns, 1 row 3.5 and 4.3
+  //   two or four: 7168 columns, 1 row 6.0 and 7.3; 4096 fp32 rows 104 and 150; 8192 columns, 4096 rows
+  //                57.9 and 55.0; 16384 columns, 1 row 9.7 and 10.1, 1024 rows 46 and 37, fp32 69 and 81
+  if (vecs <= 256 || (vecs <= 640 && (x_is_f32 || rows <= 256))) launch_sandwich<1>(p, x_is_f32, stream);
+  else if (vecs <= 512 || (vecs <= 1024 && rows <= 1024) || (vecs <= 2048 && x_is_f32))
+    launch_sandwich<2>(p, x_is_f32, stream);
   else launch_sandwich<4>(p, x_is_f32, stream);
   return launch_status("sandwich_rmsnorm");
 }

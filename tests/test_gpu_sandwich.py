@@ -74,6 +74,19 @@ def test_formula(gate, rows, cols, x32, post, residual, offset, scale):
     ref.assert_rounded(_bits(y), wz, "normed")
 
 
+@pytest.mark.parametrize("rows,cols,x32", [
+    (2, 5120, True), (2, 5128, True), (256, 4104, False), (257, 4104, False), (3, 5120, False), (2, 5128, False),
+    (1024, 8192, False), (1025, 8192, False), (3, 8200, True), (3, 8200, False), (2, 16384, True), (2, 16384, False),
+    (2, 16392, False), (1030, 5120, True)])
+def test_borders_of_forms(rows, cols, x32):
+    """Either side of each border in rows, columns and type between the kernel's forms."""
+    v = _inputs(rows * 7 + cols, rows, cols, x32, "row")
+    s, y, _ = _run(v, scale=0.5)
+    ws, wz = _want(v, 0.5)
+    ref.assert_rounded(_bits(s), ws, "sum")
+    ref.assert_rounded(_bits(y), wz, "normed")
+
+
 @pytest.mark.parametrize("gate", ["none", "col", "row", "full"])
 @pytest.mark.parametrize("rows,cols", [(1, 32), (3, 96), (5, 2048), (2, 7168), (4, 8224)])
 def test_quantized(gate, rows, cols):
