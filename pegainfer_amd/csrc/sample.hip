@@ -17,8 +17,20 @@
 //
 // No sort.  A histogram of the weights' logarithms (counts and masses in LDS) finds the bin in which
 // each cut falls; its elements are listed, and compared with each other or, where they are many,
-// narrowed down by histograms of their keys; equal keys are cut by index.  Three passes over the
-// row: its maximum, the histogram, and the list with the masses of what is kept whole.
+// narrowed down by histograms of their keys; equal keys are cut by index.  A row is read two or three
+// times: for its largest logit, then for the histogram, then for the list and the masses of what is
+// kept whole.  Where k is small (its bound: the threads of the first pass) the histogram falls away:
+// each thread of the first pass leaves its own largest, the k-th largest of these is a bound below
+// which nothing is kept, and what lies above it is listed at once.
+//
+// What bounds it: the first pass, memory (256 rows of 163840 fp32 logits, 168 MB, 34 us, 4.9 TB/s).
+// The others read what the first left in the caches and are bound by the vector units, a chain of 12
+// products in 64 bits for each weight (the histogram 39 us of those rows, the third pass 26 us; 13 us
+// for the cuts; together 113).  One row is bound by latency alone: launches of 4.3, 9.1 and 7.9 us.
+// So a row is split over up to 16 workgroups, of 512 threads as there are bins (of 1024 threads with
+// more than 64 registers one fitted a CU).  One workgroup a row for everything took 268 us for one row
+// and 317 for 256.  The passes' bodies are loops of few instructions, not unrolled: these kernels are
+// short enough for a CU's instruction fetches to show.
 #include "common.h"
 #include "pega_moe.h"
 
@@ -27,13 +39,15 @@ namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kBins = kThreads;        // one a thread
-constexpr int kList = 4096;            // elements of the cuts' bins kept in LDS
+// Elements of the cuts' bins kept in LDS.  With 4096 three workgroups fit a CU; with 3200 four do, which is no
+// faster (256 rows 112.5 and 113.7 us), and with 2048 some rows are over it (233).
+constexpr int kList = 4096;
 constexpr int kMaxSplit = 16;          // workgroups of a row
 constexpr int kMaxParts = 256;         // of a row, whose masses the draw goes over first (a multiple of kMaxSplit)
-constexpr int kFlight = 4;              // vectors of a thread in flight
+constexpr int kFlight = 4;             // vectors of a thread in flight
 constexpr int kMaxFew = 1024;          // so few fit the list with room for what shares the last one's bin
-constexpr int kPairs = kThreads / 4;   // candidates that are compared with each other
-constexpr int kWorkgroups = 1024;      // four a CU
+constexpr int kPairs = kThreads / 4;   // candidates that are compared with each other, by four threads each
+constexpr int kWorkgroups = 1024;      // of a launch, where rows are fewer
 constexpr int kFewWorkgroups = 256;    // no more than one a CU
 constexpr int kMaxRows = 256;          // of a round of launches, which bounds the workspace
 constexpr int kMaxVocab = 1 << 19;     // sums of weights stay below 2^63
@@ -121,8 +135,8 @@ struct Row {
     }
     return place(top, at);
   }
-  // f(i, l[i]) for the vectors' elements with l >= low (a NaN has not), over `threads` threads with kFlight loads in flight
-  // each.  Few copies of f: the passes are short enough for a CU's instruction fetches to show.
+  // f(i, l[i]) for the vectors' elements with l >= low (a NaN has not), over `threads` threads with
+  // kFlight loads in flight each.  f is there four times, not once for each element in flight.
   // after(base): once for each round of vectors base .. base + threads - 1, by all threads.
   template <typename F, typename A>
   __device__ __forceinline__ void each(int from, int to, int tid, int threads, float low, F f, A after) const {
@@ -301,7 +315,7 @@ __device__ __forceinline__ void block_scan(Shared& s, uint32_t& count, u64& mass
 }
 
 // The largest over the workgroup, in each thread.
-__device__ __forceinline__ u64 block_max(Shared& s, u64 v, int tid) {
+__device__ __forceinline__ u64 block_max(u64* wave_max, u64 v, int tid) {
   const auto max16 = [](u64 x) {
     x = max(x, dpp64<0xB1>(x));     // quad_perm [1,0,3,2]
     x = max(x, dpp64<0x4E>(x));     // quad_perm [2,3,0,1]
@@ -311,9 +325,9 @@ __device__ __forceinline__ u64 block_max(Shared& s, u64 v, int tid) {
   v = max16(v);
   v = max(max(lane64(v, 0), lane64(v, 16)), max(lane64(v, 32), lane64(v, 48)));
   __syncthreads();
-  if ((tid & 63) == 0) s.wave_mass[tid >> 6] = v;
+  if ((tid & 63) == 0) wave_max[tid >> 6] = v;
   __syncthreads();
-  return lane64(max16(s.wave_mass[tid & (kWaves - 1)]), 0);
+  return lane64(max16(wave_max[tid & (kWaves - 1)]), 0);
 }
 
 // A cut of the order: the first `count` elements, or those with less than `mass` before them,
@@ -642,8 +656,8 @@ __device__ Cut resolve(Shared& s, const E& each, int listed, const Scale& scale,
   each([&](uint32_t k, int i) {
     if (mine(k, i) && step_of(k) == step) up = max(up, static_cast<u64>(k)), down = max(down, static_cast<u64>(~k));
   });
-  uint32_t hi = static_cast<uint32_t>(block_max(s, up, tid));
-  uint32_t lo = ~static_cast<uint32_t>(block_max(s, down, tid));
+  uint32_t hi = static_cast<uint32_t>(block_max(s.wave_mass, up, tid));
+  uint32_t lo = ~static_cast<uint32_t>(block_max(s.wave_mass, down, tid));
   uint32_t ties = 0;
   while (true) {  // the range falls to a 512th each time
     int shift = 0;
@@ -871,14 +885,14 @@ struct SplitArgs {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_best_kernel(SplitArgs a) {
-  __shared__ Shared s;
+  __shared__ u64 wave_max[kWaves];  // (all that it needs: with Shared 114.4 us for 256 rows, without 112.5)
   const int tid = threadIdx.x, row_id = blockIdx.y, split = blockIdx.x;
   const Row<T> row = row_of<T>(a.p, row_id);
   const int per = a.parts / a.splits * a.part;
   const int from = split * per, to = min(from + per, row.vecs);
   const u64 own = row.best(from, to, tid, kThreads);
   a.hist[static_cast<long long>(row_id) * a.splits + split].count[tid] = static_cast<uint32_t>(own >> 32);
-  const u64 best = block_max(s, own, tid);
+  const u64 best = block_max(wave_max, own, tid);
   Hand& h = a.hand[row_id];
   if (tid == 0) {
     h.best[split] = best;

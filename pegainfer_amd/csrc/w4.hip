@@ -121,6 +121,10 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* __restrict_
 // A workgroup per 16 MR features and 16 RB rows; its waves share K's steps.  x is the
 // instruction's first operand, so a lane's sums are of its own feature and it needs that feature's
 // scales alone.  D steps are in flight.
+// Bound by the weights' stream from memory: a lane's 16 bytes are all it needs of a step's codes, read once and
+// never staged.  One row of 163840 x 7168 (606 MB): 101 us, 6.0 TB/s.  One of 4096 x 7168 (16.5 MB): 5.6 us of
+// kernel, one round trip of the loads and the join, which is why eight waves share K there and few features go to a
+// workgroup; with many features more of them to a workgroup read each row of X less often.
 template <int G, bool kZeros, int MR, int RB>
 struct W4Step {
   static constexpr int kWords = (meta_bytes(G, kZeros) + 3) / 4;
@@ -272,6 +276,11 @@ void launch_stream(const W4Args& p, hipStream_t stream) {
 // piece ^ (row % 8), which spreads eight lanes' fragment reads over all banks.
 // sum_k x over a group (times -24 / 16 without zero points) is one more chain a row block, with a
 // constant operand, which the waves share out a step ahead; its features' chains start from it.
+// (A chain in every wave instead of the shared sums: 9% slower.)
+// Bound by instruction issue: each code is expanded by every wave that has its features, so wide tiles, whose waves
+// take many rows, spread that over more products.  4096 rows of 4096 x 7168, groups of 128, zero points: 253 us, 950
+// TFLOP/s, matrix cores busy 43% and vector units 49% of the cycles.  333 rows of 9728 x 2560: 31 us, one workgroup a CU
+// that reads LDS and multiplies in turn; 48 rows of 163840 x 2048: 62 us, 3.3 TB/s, two workgroups a CU.
 template <int G_, bool kZeros_, int WM_, int WN_, int TM_, int TN_, int NS_>
 struct W4Tile {
   static constexpr int G = G_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, NS = NS_;
