@@ -210,11 +210,21 @@ struct SandwichArgs {
   int rows, hidden;
 };
 
+// What a wave's lanes have written to LDS before, its lanes read behind it (a wave's own accesses go in order).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A lane's 8 columns of an fp32 row are two loads' worth.  Taken as they lie, each load of a wave would touch
+// half of every line; so a wave loads its 128 pieces of 16 bytes in order, and its lanes exchange them
+// (4096 rows of 7168 columns 104 us without, 69 with; 333 of 2048 6.2 and 5.3).
 template <int CH, bool kX32>
 __global__ __launch_bounds__(64 * kMaxWaves) void sandwich_rmsnorm_kernel(
     SandwichArgs p) {
   __shared__ double s_sum[2][kMaxWaves];
-  const int lanes = blockDim.x, lane = threadIdx.x;
+  const int lanes = blockDim.x, lane = threadIdx.x, in_wave = lane & 63;
   const int row = blockIdx.x * blockDim.y + threadIdx.y;
   const int vecs = p.hidden >> 3;
   const bool in = row < p.rows;
@@ -234,10 +244,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) void sandwich_rmsnorm_kernel(
     const int v = lane + c * lanes;
     const bool ok = in && v < vecs;
     const long long at = base + 8LL * v;
-    if constexpr (kX32) {
-      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + at);
-      xr[c][0] = ok ? q[0] : zero;
-      xr[c][1] = ok ? q[1] : zero;
+    if constexpr (kX32) {  // pieces of 4 columns, each load's side by side
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + base);
+      const int piece = 2 * (v - in_wave) + in_wave;
+      xr[c][0] = in && piece < 2 * vecs ? q[piece] : zero;
+      xr[c][1] = in && piece + 64 < 2 * vecs ? q[piece + 64] : zero;
     } else {
       xr[c][0] = ok ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + at) : zero;
     }
@@ -249,6 +260,20 @@ __global__ __launch_bounds__(64 * kMaxWaves) void sandwich_rmsnorm_kernel(
     if (v < vecs && p.post) pw[c] = *reinterpret_cast<const uint4*>(p.post + 8 * v);
     nw[c] = zero;
     if (v < vecs && p.pre) nw[c] = *reinterpret_cast<const uint4*>(p.pre + 8 * v);
+  }
+  if constexpr (kX32) {  // a lane's two pieces, by way of its wave's part of LDS
+    extern __shared__ uint4 s_x[];
+    uint4* part = s_x + 128 * ((threadIdx.y * blockDim.x + threadIdx.x) >> 6);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      // (even pieces in one half, odd ones in the other, so that the reads meet no bank twice)
+      part[(in_wave >> 1) + 64 * (in_wave & 1)] = xr[c][0];
+      part[(in_wave >> 1) + 64 * (in_wave & 1) + 32] = xr[c][1];
+      wave_sync();
+      xr[c][0] = part[in_wave];
+      xr[c][1] = part[in_wave + 64];
+      wave_sync();
+    }
   }
   const auto x_at = [&](int c, int i) {
     if constexpr (kX32) {
@@ -327,7 +352,8 @@ void launch_sandwich(SandwichArgs p, bool x32, hipStream_t stream) {
   const int most = (1 << 25) / waves;  // rows a launch, as launch_norm's
   for (int rows = p.rows;; rows -= most) {
     p.rows = rows < most ? rows : most;
-    hipLaunchKernelGGL(kernel, dim3(ceil_div(p.rows, per)), dim3(64 * waves, per), 0, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(ceil_div(p.rows, per)), dim3(64 * waves, per), x32 ? 2048 * waves * per : 0, stream,
+                       p);
     if (rows <= most) return;
     const long long at = static_cast<long long>(most) * p.hidden;
     p.x = static_cast<const uint8_t*>(p.x) + (x32 ? 4 : 2) * at;
@@ -462,10 +488,10 @@ PEGA_API int pega_sandwich_rmsnorm(const void* x, bool x_is_f32, const uint16_t*
   const int vecs = hidden_dim / 8;
   // Vectors a lane, in us without MXFP8, a gate for each row (bf16 x unless fp32 is said).  More of
   // them take fewer waves to a row and more registers to a lane; with fp32 rows four spill.
-  //   one or two:  4096 columns, 1 row 4.3 and 4.8; 4096 rows 38.8 and 33.8, fp32 58.3 and 61.3;
-  //                7168 columns, 1024 rows 25.5 and 20.2, fp32 37.8 and 32.0; 2048 columns, 1 row 3.5 and 4.3
-  //   two or four: 7168 columns, 1 row 6.0 and 7.3; 4096 fp32 rows 104 and 150; 8192 columns, 4096 rows
-  //                57.9 and 55.0; 16384 columns, 1 row 9.7 and 10.1, 1024 rows 46 and 37, fp32 69 and 81
+  //   one or two:  4096 columns, 1 row 4.3 and 4.8; 4096 rows 37.0 and 33.6, fp32 39.6 and 38.7;
+  //                7168 columns, 1024 rows 25.4 and 19.2, fp32 27.3 and 23.2; 2048 columns, 1 row 3.6 and 4.4
+  //   two or four: 7168 columns, 1 row 6.0 and 7.3; 4096 fp32 rows 71 and 150; 8192 columns, 4096 rows
+  //                56.5 and 54.4; 16384 columns, 1 row 9.7 and 10.0, 1024 rows 46 and 35, fp32 56 and 83
   if (vecs <= 256 || (vecs <= 640 && (x_is_f32 || rows <= 256))) launch_sandwich<1>(p, x_is_f32, stream);
   else if (vecs <= 512 || (vecs <= 1024 && rows <= 1024) || (vecs <= 2048 && x_is_f32))
     launch_sandwich<2>(p, x_is_f32, stream);
