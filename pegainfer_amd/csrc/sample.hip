@@ -23,10 +23,10 @@
 // each thread of the first pass leaves its own largest, the k-th largest of these is a bound below
 // which nothing is kept, and what lies above it is listed at once.
 //
-// What bounds it: the first pass, memory (256 rows of 163840 fp32 logits, 168 MB, 34 us, 4.9 TB/s).
+// What bounds it: the first pass, memory (256 rows of 163840 fp32 logits, 168 MB, 32 us, 5.2 TB/s).
 // The others read what the first left in the caches and are bound by the vector units, a chain of 12
-// products in 64 bits for each weight (the histogram 39 us of those rows, the third pass 26 us; 13 us
-// for the cuts; together 113).  One row is bound by latency alone: launches of 4.3, 9.1 and 7.9 us.
+// products in 64 bits for each weight (the histogram 40 us of those rows, the third pass 26 us; 13 us
+// for the cuts; together 113).  One row is bound by latency alone: launches of 4.2, 9.4 and 7.6 us.
 // So a row is split over up to 16 workgroups, of 512 threads as there are bins (of 1024 threads with
 // more than 64 registers one fitted a CU).  One workgroup a row for everything took 268 us for one row
 // and 317 for 256.  The passes' bodies are loops of few instructions, not unrolled: these kernels are
