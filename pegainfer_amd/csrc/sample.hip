@@ -98,6 +98,16 @@ struct Row {
     const uint32_t w = (e >> 1) == 0 ? q.x : (e >> 1) == 1 ? q.y : (e >> 1) == 2 ? q.z : q.w;
     return e & 1 ? bf_hi(w) : bf_lo(w);
   }
+  // Whether a comparison holds for an element of one of the wave's vectors.  By comparisons, which no NaN passes, and
+  // by their lane masks: the maximum of a number and a signaling NaN is a NaN, which would hide the numbers beside it,
+  // and the compiler makes such a maximum out of comparisons that are joined in a lane.
+  template <typename C>
+  static __device__ __forceinline__ bool any(uint4 q, C holds) {
+    u64 found = 0;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) found |= __builtin_amdgcn_ballot_w64(holds(value(q, e)));
+    return found != 0;
+  }
   __device__ __forceinline__ float at(int i) const {
     if constexpr (sizeof(T) == 4) return clean(p[i]);
     else return clean(bf2f(p[i]));
@@ -123,10 +133,7 @@ struct Row {
       for (int j = 0; j < kFlight; ++j) q[j] = load(v + j * threads);
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        float most = value(q[j], 0);
-#pragma unroll
-        for (int e = 1; e < kVec; ++e) most = fmaxf(most, value(q[j], e));  // (NaNs left out)
-        if (!(most > top)) continue;  // seldom passed: later elements of one value are behind it
+        if (!any(q[j], [&](float l) { return l > top; })) continue;  // seldom passed: later elements of one value are behind it
         const int vec = v + j * threads, i = start(min(vec, vecs - 1)), own = vec * kVec - i;
 #pragma unroll
         for (int e = 0; e < kVec; ++e)
@@ -157,10 +164,7 @@ struct Row {
 #pragma unroll
       for (int j = 0; j + 1 < kFlight; ++j) q[j] = q[j + 1];
       q[kFlight - 1] = load(v + kFlight * threads);
-      float most = value(now, 0);
-#pragma unroll
-      for (int e = 1; e < kVec; ++e) most = fmaxf(most, value(now, e));  // (NaNs left out)
-      if (v < to && most >= low) {
+      if (v < to && any(now, [&](float l) { return l >= low; })) {
         const int first = start(v);
         // the last vector may reach back over the one before, whose elements are not its own
         const int own = v * kVec - first;

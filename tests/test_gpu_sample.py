@@ -211,3 +211,26 @@ def test_captured(rows):
         torch.cuda.synchronize()
         want = _draw(logits, u.cpu().numpy(), **{k: v.cpu().numpy() for k, v in dev.items()})
         assert (tokens.cpu().numpy() == want[0]).all() and (logprobs.cpu().numpy() == want[1]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 80])  # of each kind: few rows, many
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("kw", [{}, {"top_k": 3}, {"top_k": 2000}, {"top_p": 0.9}, {"temperature": 0.0},
+                                {"top_k": 40, "top_p": 0.8}, {"top_p": 0.9, "min_p": 0.01}])
+def test_signaling_nans_hide_nothing_beside_them(kw, bf16, rows):
+    """In every place of every vector of 16 bytes, the largest logit's among them."""
+    vec, v = (8, 3001) if bf16 else (4, 3001)
+    patterns = [0x7F81, 0xFF81, 0x7FBF] if bf16 else [0x7F800001, 0xFF800001, 0x7FBFFFFF]
+    kind = np.uint16 if bf16 else np.uint32
+    for e in range(vec):
+        plain = _logits(e, rows, v, 1.0, bf16)
+        bits = plain.view(torch.int16 if bf16 else torch.int32).cpu().numpy().view(kind).copy()
+        top = np.array([1496 + (e + 1 + r % (vec - 1)) % vec for r in range(rows)])  # 1496: a vector's first
+        for r in range(rows):
+            bits[r, e::vec] = patterns[(r + e) % 3]
+            bits[r, top[r]] = 0x40E0 if bf16 else 0x40E00000  # 7
+        logits = torch.from_numpy(bits.view(np.int16 if bf16 else np.int32)).cuda().view(plain.dtype)
+        g = np.random.default_rng(e)
+        _check(logits, u=g.random(rows, dtype=np.float32), **{k: [x] * rows for k, x in kw.items()})
+        greedy = _draw(logits, [0.5] * rows, temperature=[0.0] * rows)[0]
+        assert (greedy == top).all()
