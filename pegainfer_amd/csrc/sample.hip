@@ -237,11 +237,12 @@ struct Scale {
   // above every d of a bin, below every one
   __device__ __forceinline__ double inner(int b) const { return -b / bins * (1 - 0x1p-30); }
   __device__ __forceinline__ double edge(int b) const { return -(b + 1) / bins * (1 + 0x1p-30); }
-  // a float below every logit that lies d or less below the maximum, and one above all that lie d or more
-  // below it
+  // A float below every logit l with below(l) >= d, so that what it leaves out is never live, and one above all with
+  // below(l) <= d.  The first leaves room for the rounding of l - max, up to 2^-53 |d|, beside which max + d may be next
+  // to nothing; the sum's own rounding is relative to it.
   __device__ __forceinline__ float bound(double d) const {
     if (infinite) return __builtin_inff();
-    const float f = static_cast<float>(max + d);
+    const float f = static_cast<float>(max + d - (__builtin_fabs(max) + __builtin_fabs(d)) * 0x1p-50);
     return f - __builtin_fabsf(f) * 0x1p-22f - 0x1p-126f;
   }
   __device__ __forceinline__ float over(double d) const {

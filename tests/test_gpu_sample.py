@@ -234,3 +234,21 @@ def test_signaling_nans_hide_nothing_beside_them(kw, bf16, rows):
         _check(logits, u=g.random(rows, dtype=np.float32), **{k: [x] * rows for k, x in kw.items()})
         greedy = _draw(logits, [0.5] * rows, temperature=[0.0] * rows)[0]
         assert (greedy == top).all()
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 0.5])
+@pytest.mark.parametrize("kw", [{}, {"top_k": 2}, {"top_k": 4000}, {"top_p": 1 - 2.0 ** -24}])
+@pytest.mark.parametrize("vocab", [2, 5, 5000])
+def test_weights_on_the_border_of_the_range(vocab, kw, temperature, bf16, rows):
+    """The largest logit is 28 T, all others are all but zero: in 64 bits they lie 28 T below it, the
+    smallest weight that there is, and the sum of the two in fp32 is lost."""
+    g = np.random.default_rng(vocab)
+    l = torch.zeros(rows, vocab)
+    l[:, 1::3], l[:, 2::3] = -1e-20, -1e-38
+    l[:, vocab // 2] = 28 * temperature
+    l = (l.to(torch.bfloat16) if bf16 else l).cuda()
+    for u in (0.0, 0.5, 1 - 2.0 ** -24, 1.0, 3.0):
+        _check(l, u=[u] * rows, temperature=[temperature] * rows, **{k: [x] * rows for k, x in kw.items()})
+    _check(l, u=g.random(rows, dtype=np.float32), temperature=[temperature] * rows)
