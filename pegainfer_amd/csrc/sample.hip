@@ -13,7 +13,9 @@
 //
 // Weights are whole multiples of 2^-44, rounded once from 64 bits, and their sums are of 64-bit
 // integers: exact in any order, so that a row's token depends on nothing but its inputs, and every
-// comparison is of exact sums (the weights' rounding moves a border by 10^-11 at most).
+// comparison is of exact sums with a share of the whole in 64-bit floating point.  The weights' rounding,
+// 2^-45 each, moves a border by V 2^-45 of the sum at most: where nearly all are equal and small, by
+// 4.7e-9 with 163840 of them.
 //
 // No sort.  A histogram of the weights' logarithms (counts and masses in LDS) finds the bin in which
 // each cut falls; its elements are listed, and compared with each other or, where they are many,
@@ -50,13 +52,15 @@ constexpr int kPairs = kThreads / 4;   // candidates that are compared with each
 constexpr int kWorkgroups = 1024;      // of a launch, where rows are fewer
 constexpr int kFewWorkgroups = 256;    // no more than one a CU
 constexpr int kMaxRows = 256;          // of a round of launches, which bounds the workspace
-constexpr int kMaxVocab = 1 << 19;     // sums of weights stay below 2^63
+constexpr int kMaxVocab = 1 << 19;     // sums of weights: at most 2^63
 constexpr double kRange = 28.0;        // smaller weights than e^-28 are zero
 constexpr double kLog2e = 1.4426950408889634;
 constexpr double kBinsPerOctave = kBins / (kRange * kLog2e + 0.01);
 
 typedef unsigned long long u64;
-constexpr u64 kNoMass = u64{1} << 63;  // more than any sum of weights, less than 2^64 by more than a weight
+constexpr u64 kOne = u64{1} << 44;              // the largest logit's weight
+constexpr u64 kNoMass = (u64{1} << 63) + kOne;  // more than any sum of weights; one more weight fits on top
+static_assert(kNoMass > kMaxVocab * kOne && kNoMass + kOne > kNoMass, "sums of weights");
 constexpr uint32_t kNoCount = 0xffffffffu;
 
 struct SampleArgs {

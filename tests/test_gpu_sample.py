@@ -252,3 +252,19 @@ def test_weights_on_the_border_of_the_range(vocab, kw, temperature, bf16, rows):
     for u in (0.0, 0.5, 1 - 2.0 ** -24, 1.0, 3.0):
         _check(l, u=[u] * rows, temperature=[temperature] * rows, **{k: [x] * rows for k, x in kw.items()})
     _check(l, u=g.random(rows, dtype=np.float32), temperature=[temperature] * rows)
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_the_largest_sum_of_weights(rows):
+    """2^19 equal logits, whose weights add up to 2^63: cut by count, by mass, by both, or not at all."""
+    v = 1 << 19
+    logits = torch.full((rows, v), 2.5, dtype=torch.bfloat16, device="cuda")
+    u = np.resize(np.array([0.0, 0.25, 0.5, 0.7503, 1 - 2.0 ** -24], np.float32), rows)
+    p = np.float32(0.3)
+    for kept, kw in ((v, {}), (v, {"top_k": v}), (v - 1, {"top_k": v - 1}), (6250, {"top_k": 6250}), (3, {"top_k": 3}),
+                     (int(np.ceil(float(p) * v)), {"top_p": p}), (v, {"top_p": 1 - 2.0 ** -24}),
+                     (int(np.ceil(float(p) * (v - 1))), {"top_k": v - 1, "top_p": p})):
+        tokens, logprobs = _draw(logits, u, **{k: [x] * rows for k, x in kw.items()})
+        # a uniform number of 24 bits times a count of 20: exact in 64 bits
+        assert tokens.tolist() == [int(float(x) * kept) for x in u], kw
+        assert np.abs(logprobs + np.log(kept)).max() <= 2.0 ** -24 * (1 + np.log(kept)), kw
