@@ -428,8 +428,9 @@ int pega_w4_pack(const uint8_t* packed, const uint16_t* scales, const uint8_t* z
 /* No reference counterpart: Y[n][m] = sum_k X[n][k] * (q[m][k] - z[m][k / g]) * s[m][k / g], X [N][K]
  * bf16, Y [N][M] bf16 or, with y_is_f32, fp32; any M, N and whole groups of K.  No weight is
  * rounded: products with the codes' integers are exact, group sums and their products with the scales
- * fp32.  A row of X with an infinity or a NaN gives NaN, one with 2^119 and more may.  A row's result
- * does not depend on the other rows' values.  No workspace.  At most 2^20 columns, 2^26 features and
+ * fp32: the error is relative to sum |x| (16 + q + 16 + z) |s|.  A row of X with an infinity or a NaN
+ * gives NaN; one with finite values of 2^117 and more may (2^119 where no zero point is above 15).  A
+ * row's result does not depend on the other rows' values.  No workspace.  At most 2^20 columns, 2^26 features and
  * 1048560 rows; X, codes and meta 16-byte aligned, Y by its type (801 otherwise); Y overlaps no input. */
 int pega_w4_gemm(const uint8_t* codes, const uint8_t* meta, bool has_zeros, int group_size,
                  const uint16_t* X, void* Y, bool y_is_f32, int M, int N, int K,

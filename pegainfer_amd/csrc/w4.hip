@@ -9,9 +9,10 @@
 // 1.0 are the number (16 + q) / 16.  So d = sum_k x (16 + q) / 16 - sum_k x (16 + z) / 16 over a
 // group is a chain of v_mfma_f32_16x16x32_bf16, the second sum with a constant operand, and
 // 16 s d is the group's share of Y: products of bf16 with exact integers, fp32 sums, one scale an
-// fp32 group sum.  No weight is rounded.  (16 + q and 16 + z cancel to at most two bits of the
-// fp32 sums.)  An infinite or NaN activation gives NaN in its whole row, and so may one of 2^119 and more,
-// with which a group's two sums pass fp32's range.
+// fp32 group sum.  No weight is rounded.  What is rounded are sums of x (16 + q) and x (16 + z), so the error is
+// relative to sum |x| (16 + q + 16 + z) |s|: a group whose codes all are its zero point gives about 2^-23 of that
+// and not zero.  An infinite or NaN activation gives NaN in its whole row.  So may finite ones of 2^117 and more
+// (2^119 where no zero point is above 15), with which sums of up to 128 |x| (16 + z) / 16 pass fp32's range.
 //
 // Device layout, for tiles of 16 features (the last one padded) and steps of 128 columns (the last
 // one padded): per tile and step 64 lanes' 16 bytes, lane (c, h) = (lane % 16, lane / 16) holding

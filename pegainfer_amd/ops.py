@@ -1124,7 +1124,8 @@ def w4_pack(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor = No
 
 def w4_gemm(w: W4Weight, x: torch.Tensor, y: torch.Tensor) -> None:
     """Y[n][m] = sum_k X[n][k] * (q[m][k] - z[m][k / group]) * s[m][k / group]: x bf16 [N, in], y bf16
-    or float32 [N, out].  No weight is rounded; sums are fp32 (gemm_graphsafe on 4-bit weights)."""
+    or float32 [N, out].  No weight is rounded; sums are fp32 (gemm_graphsafe on 4-bit weights).  A row
+    with an infinity or a NaN gives NaN; finite values of 2^117 and more may."""
     of, dtype = x.shape, y.dtype
     if len(of) != 2 or of[1] != w.in_dim or not _is_bf16(x):
         raise ValueError(f"x must be bf16 [rows, {w.in_dim}], got {x.dtype} {tuple(of)}")

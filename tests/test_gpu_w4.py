@@ -205,3 +205,33 @@ def test_every_form(group, rows, n, k, zeros):
         assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist())
         # and far inside it for most: a wrong scale, code or row would not be
         assert ((y[:, part].double() - want).abs() <= 1e-5 * mag).float().mean() > 0.999
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group,rows,n,k", [(g, *c) for g, cs in FORMS.items() for c in cs])
+def test_every_form_bit_for_bit(group, rows, n, k, zeros):
+    """Whole activations up to 3, scales of 2^-20 to 2^-18: in units of the smallest scale every sum of a row is a
+    whole number below 3 * 127 * 4 * 7168 < 2^24, so the result is exact in any order.  Then the same with the
+    activations just below the largest that rows of finite values may have: 3 * 2^115 < 2^117 with zero points up
+    to 127, 3 * 2^117 < 2^119 without.  The first row has the largest value everywhere."""
+    from pegainfer_amd import ops
+    assert 3 * 127 * 4 * k < 2 ** 24
+    g = torch.Generator(device="cuda").manual_seed(rows * 3 + n)
+    x = torch.randint(-3, 4, (rows, k), device="cuda", generator=g).to(torch.bfloat16)
+    x[0] = 3
+    packed = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=g)
+    s = torch.exp2(torch.randint(-20, -17, (n, k // group), device="cuda", generator=g).float()).to(torch.bfloat16)
+    z = torch.randint(0, 128, (n, k // group), dtype=torch.uint8, device="cuda", generator=g) if zeros else None
+    if zeros:
+        z[0], z[-1] = 127, 127
+    w = ops.w4_pack(packed, s, z, group=group)
+    up = 2.0 ** (115 if zeros else 117)
+    y, high = _run(x, w, True), _run(x * up, w, True)
+    q = torch.stack((packed & 15, packed >> 4), -1).reshape(n, k).double()
+    zr = 8.0 if z is None else z.double().repeat_interleave(group, 1)
+    sr = s.double().repeat_interleave(group, 1)
+    for at in range(0, n, 4096):
+        part = slice(at, at + 4096)
+        want = x.double() @ ((q[part] - (zr if z is None else zr[part])) * sr[part]).T
+        assert torch.equal(y[:, part].double(), want)
+        assert torch.equal(high[:, part].double(), want * up)
