@@ -487,7 +487,9 @@ PEGA_API int pega_sandwich_rmsnorm(const void* x, bool x_is_f32, const uint16_t*
                  mxfp8_codes, mxfp8_scales, rows, hidden_dim};
   const int vecs = hidden_dim / 8;
   // Vectors a lane, in us without MXFP8, a gate for each row (bf16 x unless fp32 is said).  More of
-  // them take fewer waves to a row and more registers to a lane; with fp32 rows four spill.
+  // them take fewer waves to a row and more registers to a lane; with fp32 rows four spill 69, and are taken
+  // above 16384 columns alone, where two would need more waves than a workgroup has (1024 rows of 32768 columns
+  // 167 us, bf16 82).
   //   one or two:  4096 columns, 1 row 4.3 and 4.8; 4096 rows 37.0 and 33.6, fp32 39.6 and 38.7;
   //                7168 columns, 1024 rows 25.4 and 19.2, fp32 27.3 and 23.2; 2048 columns, 1 row 3.6 and 4.4
   //   two or four: 7168 columns, 1 row 6.0 and 7.3; 4096 fp32 rows 71 and 150; 8192 columns, 4096 rows

@@ -27,8 +27,8 @@
 //
 // What bounds it: the first pass, memory (256 rows of 163840 fp32 logits, 168 MB, 32 us, 5.2 TB/s).
 // The others read what the first left in the caches and are bound by the vector units, a chain of 12
-// products in 64 bits for each weight (the histogram 40 us of those rows, the third pass 26 us; 13 us
-// for the cuts; together 113).  One row is bound by latency alone: launches of 4.2, 9.4 and 7.6 us.
+// products in 64 bits for each weight (the histogram 40 us of those rows, the third pass 27 us; 14 us
+// for the cuts; together 116).  One row is bound by latency alone: launches of 4.3, 9.5 and 7.8 us.
 // So a row is split over up to 16 workgroups, of 512 threads as there are bins (of 1024 threads with
 // more than 64 registers one fitted a CU).  One workgroup a row for everything took 268 us for one row
 // and 317 for 256.  The passes' bodies are loops of few instructions, not unrolled: these kernels are
@@ -42,7 +42,9 @@ namespace {
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kBins = kThreads;        // one a thread
 // Elements of the cuts' bins kept in LDS.  With 4096 three workgroups fit a CU; with 3200 four do, which is no
-// faster (256 rows 112.5 and 113.7 us), and with 2048 some rows are over it (233).
+// faster (256 rows 112.5 and 113.7 us), and with 2048 some rows are over it (233).  A row over it is gone over by one
+// workgroup, element by element: with top-p 0.9 over 163840 normal logits of sigma / T = 0.75 and less, one row takes
+// 398 to 441 us (38 with 2.2), 256 rows 721 to 737 (180), and 256 rows with one such among them 621.
 constexpr int kList = 4096;
 constexpr int kMaxSplit = 16;          // workgroups of a row
 constexpr int kMaxParts = 256;         // of a row, whose masses the draw goes over first (a multiple of kMaxSplit)

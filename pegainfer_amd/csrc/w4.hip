@@ -72,6 +72,8 @@ __device__ __forceinline__ floatx4_t mfma(u32x4_t a, bf16x8_t b, floatx4_t c) {
 }
 
 // ---------------------------------------------------------------- device layout
+// Once, at load time.  A load of a wave takes 16 bytes of each of 16 features: 163840 x 7168 in 339 us, 1.4 times a
+// copy of its bytes.
 __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* __restrict__ packed,
                                                       const uint16_t* __restrict__ scales,
                                                       const uint8_t* __restrict__ zeros,
@@ -274,13 +276,13 @@ void launch_stream(const W4Args& p, hipStream_t stream) {
 // A workgroup of WM x WN waves owns 16 TM WM features x 16 TN WN rows, each wave 16 TM of the features and
 // 16 TN of the rows, for all of K; a stage of the ring in LDS holds a step of X, codes and scales,
 // brought in by loads straight to LDS, one barrier a step.  A row of X has its 16-byte pieces at slot
-// piece ^ (row % 8), which spreads eight lanes' fragment reads over all banks.
+// piece ^ (row % 16), which spreads sixteen lanes' fragment reads over all 64 banks.
 // sum_k x over a group (times -24 / 16 without zero points) is one more chain a row block, with a
 // constant operand, which the waves share out a step ahead; its features' chains start from it.
 // (A chain in every wave instead of the shared sums: 9% slower.)
 // Bound by instruction issue: each code is expanded by every wave that has its features, so wide tiles, whose waves
 // take many rows, spread that over more products.  4096 rows of 4096 x 7168, groups of 128, zero points: 253 us, 950
-// TFLOP/s, matrix cores busy 43% and vector units 49% of the cycles.  333 rows of 9728 x 2560: 31 us, one workgroup a CU
+// TFLOP/s, matrix cores busy 42% and vector units 55% of the cycles.  333 rows of 9728 x 2560: 31 us, one workgroup a CU
 // that reads LDS and multiplies in turn; 48 rows of 163840 x 2048: 62 us, 3.3 TB/s, two workgroups a CU.
 template <int G_, bool kZeros_, int WM_, int WN_, int TM_, int TN_, int NS_>
 struct W4Tile {
@@ -533,12 +535,15 @@ void launch_tile(const W4Args& p, hipStream_t stream) {
 // A call's time in us, over 1024 .. 163840 features, 2048 .. 7168 columns and 1 .. 2048 rows of each
 // form alone: start + steps * (step + fill * step_rows + (more + fill * more_rows) * (w - w0)), with w
 // workgroups a CU (above w0) and a workgroup's rows filled to `fill`.  The form that this puts first
-// is within 3% of the fastest one on average, 30% at most (where two forms cross).  Examples,
+// is within 3% of the fastest one on average, 34% at most (one row of 1024 x 2048, groups of 32 with zero
+// points: 4.3 us where the first form takes 3.2; the streaming forms have one set of costs for all groups).  Examples,
 // groups of 128: one row of 4096 x 7168 5.0 us with <1, 1, 8, 2>, 11.6 with <4, 1, 4, 2>; one of 163840 x
 // 2048 35.8 with the latter, 77 with the former; 48 rows of those 62 with the tile of 48 rows, 94 with
 // <4, 4, 4, 1>; 2048 rows of 4096 x 7168 132 with the tile of 256 x 128, 156 with 128 x 64, of 1024
 // rows 101 and 81.  Groups of 32 take half as long again in the tile kernel, whose vector work grows with
-// the groups; its widest tile would spill registers with them.
+// the groups; its widest tile would spill registers with them (with groups of 64 and zero points it spills one).
+// Two streaming forms have one wave a SIMD with groups of 32, of 256 registers and a few more: <4, 1, 4, 2> with
+// zero points (one row of 32768 x 2048 12.7 us, with groups of 128 10.2) and <4, 4, 4, 1> without.
 struct Form {
   int bm, bn;
   bool whole;  // half of the cost is by whole rounds of workgroups
