@@ -139,7 +139,8 @@ struct Row {
       for (int j = 0; j < kFlight; ++j) q[j] = load(v + j * threads);
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        if (!any(q[j], [&](float l) { return l > top; })) continue;  // seldom passed: later elements of one value are behind it
+        // seldom passed: later elements of one value are behind it
+        if (!any(q[j], [&](float l) { return l > top; })) continue;
         const int vec = v + j * threads, i = start(min(vec, vecs - 1)), own = vec * kVec - i;
 #pragma unroll
         for (int e = 0; e < kVec; ++e)
@@ -244,7 +245,7 @@ struct Scale {
   __device__ __forceinline__ double inner(int b) const { return -b / bins * (1 - 0x1p-30); }
   __device__ __forceinline__ double edge(int b) const { return -(b + 1) / bins * (1 + 0x1p-30); }
   // A float below every logit l with below(l) >= d, so that what it leaves out is never live, and one above all with
-  // below(l) <= d.  The first leaves room for the rounding of l - max, up to 2^-53 |d|, beside which max + d may be next
+  // below(l) < d.  The first leaves room for the rounding of l - max, up to 2^-53 |d|, beside which max + d may be next
   // to nothing; the sum's own rounding is relative to it.
   __device__ __forceinline__ float bound(double d) const {
     if (infinite) return __builtin_inff();
